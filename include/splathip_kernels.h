@@ -106,6 +106,101 @@ int splat_kernel_reconstruct(splat_ctx* ctx, int V, int H, int W, const float* d
                              const float* conf, const uint8_t* mask, const uint8_t* foreground, double* cameras,
                              float* points, float* conf_out);
 
+/* --- a paged cache of keys and values ------------------------------------------------------------
+ * For scenes that grow: the keys and values of the tokens that are there stay in pages, and what is new
+ * attends to them. No counterpart in the reference, whose models see every view in every call. Heads of 64
+ * channels, as in splat_kernel_attention.
+ *
+ * Position p of sequence i lies in row p % page_size of page table[i * width + p / page_size]; a slot is
+ * page * page_size + row. Lengths, tables and slots are device arrays: nothing here waits for the host. Table entries
+ * outside [0, pages) hold no keys (their positions are left out), slots outside [0, pages * page_size) are not
+ * written, lengths are clamped to what the table's row and max_len hold, negative ones to 0.
+ *
+ * These calls allocate nothing and wait for nothing, so they may be captured into a HIP graph on the context's
+ * stream. Calls that may run at the same time need workspaces of their own. */
+
+/* The pools [pages][kv_heads][page_size][64] in `dtype`, 16-byte aligned; page_stride elements from one page to
+ * the next in both (at least kv_heads * page_size * 64, a multiple of 8; 0: exactly that). page_size is a power
+ * of two from 8 to 256, pages * page_size below 2^31. */
+typedef struct splat_kv_cache {
+  int32_t dtype;
+  int32_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int64_t page_stride;
+  void* k;
+  void* v;
+} splat_kv_cache;
+
+/* Status that splat_kernel_block_tables leaves on the device. */
+typedef enum splat_table_status {
+  SPLAT_TABLE_OK = 0,
+  SPLAT_TABLE_BAD_LENGTH = 1, /* a negative length, one past the table's width, or `used` outside the pool */
+  SPLAT_TABLE_POOL_EMPTY = 2, /* the pool holds fewer pages than are needed */
+  SPLAT_TABLE_SLOTS_FULL = 3  /* more than `cap` new tokens */
+} splat_table_status;
+
+/* Block tables and slot maps of n requests that hold past[i] positions and get add[i] new ones. The pages that
+ * request i lacks are the next of pool [pool_size] behind the *used that are taken, requests in order; they go
+ * into table [n, width] behind its ceil(past[i] / page_size) pages. Out: lens[i] = past[i] + add[i]; starts [n + 1],
+ * the first new token of each request and their number; slots [cap] and positions [cap] (NULL: not wanted) of the new
+ * tokens, requests in order, -1 and 0 behind the last; *used_out = pages taken now. lens may be past and used_out
+ * used; other outputs overlap nothing. If *status is not SPLAT_TABLE_OK nothing was taken: the table, lens and
+ * used stay, starts are 0 and slots -1. An entry of the pool or table below 0 gives slots of -1. n up to 2^20. */
+int splat_kernel_block_tables(splat_ctx* ctx, int n, const int32_t* past, const int32_t* add, int page_size,
+                              const int32_t* pool, int pool_size, const int32_t* used, int32_t* table, int width,
+                              int32_t* lens, int32_t* starts, int32_t* slots, int32_t* positions, int cap,
+                              int32_t* used_out, int32_t* status);
+
+/* Norms of the queries' and keys' heads and the position rotation in one pass over qkv [tokens, (heads + 2 *
+ * kv_heads) * 64] (q | k | v, row stride ld) in `dtype`; statistics and angles in fp32 or more, rounded once.
+ * norm: per head over its 64 channels, SPLAT_NORM_LAYER (x - mean) / sqrt(var + eps) * w + b (biased variance) or
+ * SPLAT_NORM_RMS x / sqrt(mean(x^2) + eps) * w + b, with w and b fp32 [64] (qw, qb for queries, kw, kb for keys; NULL:
+ * left out). rope: SPLAT_ROPE_LINE turns channels (c, c + 32) by positions[t] * rope_base^(-c / 32); SPLAT_ROPE_GRID
+ * turns (c, c + 16) of channels 0-31 by positions[t][0] and of channels 32-63 by positions[t][1], times
+ * rope_base^(-c / 16) (depthanything3-rs/src/rope.rs:57-73, with base 100). q_out [tokens, heads * 64] and k_out
+ * [tokens, kv_heads * 64] (NULL: not wanted) have row strides ldq and ldk; they may be qkv's own q and k blocks, and
+ * overlap it nowhere else. With cache and slots [tokens] (both or neither) keys and values also go to the cache;
+ * a slot outside the pool (-1: padding) stores nothing. The slots of one call are distinct. Row strides are multiples
+ * of 8 elements, rows 16-byte aligned. */
+typedef enum splat_norm { SPLAT_NORM_NONE = 0, SPLAT_NORM_LAYER = 1, SPLAT_NORM_RMS = 2 } splat_norm;
+typedef enum splat_rope { SPLAT_ROPE_NONE = 0, SPLAT_ROPE_LINE = 1, SPLAT_ROPE_GRID = 2 } splat_rope;
+int splat_kernel_qk_norm_rope(splat_ctx* ctx, int dtype, const void* qkv, int64_t ld, int tokens, int heads,
+                              int kv_heads, int norm, const float* qw, const float* qb, const float* kw,
+                              const float* kb, float eps, int rope, double rope_base, const int32_t* positions,
+                              void* q_out, int64_t ldq, void* k_out, int64_t ldk, const splat_kv_cache* cache,
+                              const int32_t* slots);
+
+/* Per page and head the lowest and the highest key of each channel, bounds [pages][kv_heads][2][64] in the cache's
+ * dtype, over the page's positions below lens[i]: of the pages that hold the last add[i] positions of each
+ * sequence (add NULL: all of its pages). max_add: about the largest add, which sizes the launch; any value is
+ * right. NaN in a channel gives NaN. A page that two tables share has to be full, or as full in both. */
+int splat_kernel_page_bounds(splat_ctx* ctx, const splat_kv_cache* cache, int n, const int32_t* table, int width,
+                             const int32_t* lens, const int32_t* add, int max_add, void* bounds);
+
+/* Attention of one token a sequence over its lens[i] cached positions: out[i, h] = softmax(scale q[i, h] K^T) V with
+ * the keys and values of head h / (heads / kv_heads); zeros for a sequence without keys. q and out [n, heads * 64] in the
+ * cache's dtype, row strides ldq and ldo (multiples of 8 elements, rows 16-byte aligned, not overlapping). max_len: an
+ * upper bound of the lengths that the host knows, for the launch (longer ones are cut there). In bf16 and f16 the
+ * weights go to the matrix cores rounded to that type, as in splat_kernel_attention.
+ * workspace: device memory of at least splat_paged_attention_workspace's bytes, 16-byte aligned. */
+int splat_paged_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, size_t* bytes);
+int splat_kernel_paged_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* q, int64_t ldq, int n,
+                                 int heads, const int32_t* table, int width, const int32_t* lens, int max_len,
+                                 float scale, void* out, int64_t ldo, void* workspace, size_t workspace_bytes);
+
+/* splat_kernel_paged_attention over the topk pages of each (sequence, key head) with the largest scores, the newest
+ * page always among them. A page's score is the most that the dot products of the group's queries with a key between
+ * the page's bounds (splat_kernel_page_bounds) can sum to, in 64 bits; the lower page first where scores are equal, NaN
+ * above all. selected [n, kv_heads, topk]: the pages' places in the table's row, ascending, -1 behind the last.
+ * scale must be positive. */
+int splat_sparse_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, int topk,
+                                     size_t* bytes);
+int splat_kernel_sparse_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* bounds, const void* q,
+                                  int64_t ldq, int n, int heads, const int32_t* table, int width,
+                                  const int32_t* lens, int max_len, int topk, float scale, void* out, int64_t ldo,
+                                  int32_t* selected, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

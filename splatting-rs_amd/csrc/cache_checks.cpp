@@ -1,0 +1,212 @@
+// Checks and launch rules of the paged cache's operators (cache.h).
+#include "cache.h"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+namespace splat {
+
+namespace {
+
+long type_size(int dt) { return dt == 0 ? 4 : 2; }
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+void check_page_size(int page_size) {
+  SPLAT_CHECK(page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0, BAD_ARGUMENT,
+              "page_size must be a power of two from 8 to 256");
+}
+
+void check_width(int width, int page_size) {
+  SPLAT_CHECK(width >= 1 && long(width) * page_size <= 0x7fffffffL, BAD_ARGUMENT,
+              "a table's row must hold 1 to 2^31 - 1 positions");
+}
+
+void check_sizes(const KvCache& c) {
+  SPLAT_CHECK(c.dt >= 0 && c.dt <= 2, BAD_ARGUMENT, "cache: unknown dtype");
+  check_page_size(c.page_size);
+  SPLAT_CHECK(c.pages >= 1 && long(c.pages) * c.page_size <= 0x7fffffffL, BAD_ARGUMENT,
+              "cache: pages times page_size must be 1 to 2^31 - 1");
+  SPLAT_CHECK(c.kv_heads >= 1 && c.kv_heads <= 4096, BAD_ARGUMENT, "cache: kv_heads must be 1 to 4096");
+}
+
+void check_cache(KvCache& c) {
+  check_sizes(c);
+  SPLAT_CHECK(c.page_stride >= long(c.kv_heads) * c.page_size * 64 && c.page_stride % 8 == 0 && c.page_stride <= (1L << 31),
+              BAD_ARGUMENT, "cache: page_stride must hold a page, be a multiple of 8 elements and at most 2^31");
+  SPLAT_CHECK(c.k && c.v && aligned16(c.k) && aligned16(c.v), BAD_ARGUMENT, "cache: k and v must be 16-byte aligned");
+  c.shift = __builtin_ctz(c.page_size);
+}
+
+// Whether rows of `wa` bytes every `sa` and rows of `wb` bytes every `sb` share memory. Rows of one stride may
+// lie side by side, as the column blocks of one matrix do.
+bool rows_meet(const void* a, long sa, long wa, const void* b, long sb, long wb, long rows) {
+  if (!a || !b || rows <= 0) return false;
+  const intptr_t pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+  if (pa + (rows - 1) * sa + wa <= pb || pb + (rows - 1) * sb + wb <= pa) return false;
+  if (sa != sb || sa <= 0) return true;
+  long d = (pb - pa) % sa;
+  if (d < 0) d += sa;
+  return d < wa || d + wb > sa;
+}
+bool meet(const void* a, long wa, const void* b, long wb) {
+  return wa > 0 && wb > 0 && rows_meet(a, 0, wa, b, 0, wb, 1);
+}
+
+long pool_bytes(const KvCache& c) {
+  return ((c.pages - 1L) * c.page_stride + long(c.kv_heads) * c.page_size * 64) * type_size(c.dt);
+}
+bool meets_pools(const KvCache& c, const void* p, long bytes) {
+  return meet(c.k, pool_bytes(c), p, bytes) || meet(c.v, pool_bytes(c), p, bytes);
+}
+
+// What attention over the cache needs, whichever pages it takes.
+void check_attention(PagedArgs& a) {
+  check_cache(a.cache);
+  SPLAT_CHECK(a.n >= 0 && a.heads >= 1 && a.heads <= 65536 && a.heads % a.cache.kv_heads == 0, BAD_ARGUMENT,
+              "attention: heads must be a multiple of the cache's kv_heads");
+  SPLAT_CHECK(long(a.n) * a.heads <= (1 << 24), BAD_ARGUMENT, "attention: more than 2^24 query rows");
+  check_width(a.width, a.cache.page_size);
+  SPLAT_CHECK(a.max_len >= 0, BAD_ARGUMENT, "attention: max_len is negative");
+  SPLAT_CHECK(std::isfinite(a.scale), BAD_ARGUMENT, "attention: scale is not finite");
+  if (a.n == 0) return;
+  SPLAT_CHECK(a.q && a.table && a.lens && a.out, BAD_ARGUMENT, "attention: a required pointer is NULL");
+  const long es = type_size(a.cache.dt), w = a.heads * 64L;
+  SPLAT_CHECK(aligned16(a.q) && aligned16(a.out) && a.ldq % 8 == 0 && a.ldo % 8 == 0 && a.ldq >= w && a.ldo >= w, BAD_ARGUMENT,
+              "attention: rows of q and out must be 16-byte aligned, heads * 64 wide and a multiple of 8 elements apart");
+  SPLAT_CHECK(!rows_meet(a.q, a.ldq * es, w * es, a.out, a.ldo * es, w * es, a.n), BAD_ARGUMENT, "attention: out overlaps q");
+  SPLAT_CHECK(!meets_pools(a.cache, a.out, ((a.n - 1L) * a.ldo + w) * es), BAD_ARGUMENT, "attention: out overlaps the cache");
+}
+
+void check_workspace(const void* workspace, size_t bytes, size_t need) {
+  SPLAT_CHECK(need == 0 || (workspace && aligned16(workspace) && bytes >= need), BAD_ARGUMENT,
+              "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+}
+
+}  // namespace
+
+void check_block_tables(BlockTableArgs& a) {
+  check_page_size(a.page_size);
+  check_width(a.width, a.page_size);
+  SPLAT_CHECK(a.n >= 0 && a.n <= (1 << 20), BAD_ARGUMENT, "block tables: n must be 0 to 2^20");
+  SPLAT_CHECK(a.pool_size >= 0 && a.cap >= 0, BAD_ARGUMENT, "block tables: pool_size or cap is negative");
+  SPLAT_CHECK(a.used && a.starts && a.used_out && a.status && (a.n == 0 || (a.past && a.add && a.table && a.lens)) &&
+                  (a.pool_size == 0 || a.pool) && (a.cap == 0 || a.slots),
+              BAD_ARGUMENT, "block tables: a required pointer is NULL");
+  struct Range { const void* at; long bytes; };
+  const Range in[] = {{a.past, a.n * 4L}, {a.add, a.n * 4L}, {a.pool, a.pool_size * 4L}, {a.used, 4}};
+  const Range out[] = {{a.lens, a.n * 4L}, {a.used_out, 4}, {a.table, 4L * a.n * a.width}, {a.starts, 4L * (a.n + 1L)},
+                       {a.slots, a.cap * 4L}, {a.positions, a.cap * 4L}, {a.status, 4}};
+  for (int o = 0; o < 7; ++o) {
+    for (int i = 0; i < 4; ++i) {
+      if ((o == 0 && i == 0 && a.lens == a.past) || (o == 1 && i == 3 && a.used_out == a.used)) continue;
+      SPLAT_CHECK(!meet(out[o].at, out[o].bytes, in[i].at, in[i].bytes), BAD_ARGUMENT, "block tables: an output overlaps an input");
+    }
+    for (int i = 0; i < o; ++i)
+      SPLAT_CHECK(!meet(out[o].at, out[o].bytes, out[i].at, out[i].bytes), BAD_ARGUMENT, "block tables: two outputs overlap");
+  }
+  a.shift = __builtin_ctz(a.page_size);
+}
+
+void check_qk_norm_rope(QkArgs& a, double base) {
+  SPLAT_CHECK(a.dt >= 0 && a.dt <= 2, BAD_ARGUMENT, "unknown dtype");
+  SPLAT_CHECK(a.tokens >= 0 && a.heads >= 1 && a.kv_heads >= 1 && a.heads <= 65536 && a.kv_heads <= 4096, BAD_ARGUMENT,
+              "qk norm: tokens, heads or kv_heads");
+  SPLAT_CHECK(a.norm >= NORM_NONE && a.norm <= NORM_RMS, BAD_ARGUMENT, "qk norm: unknown norm");
+  SPLAT_CHECK(a.rope >= ROPE_NONE && a.rope <= ROPE_GRID, BAD_ARGUMENT, "qk norm: unknown rotation");
+  SPLAT_CHECK(a.norm == NORM_NONE || (std::isfinite(a.eps) && a.eps >= 0.f), BAD_ARGUMENT, "qk norm: eps must be finite and not negative");
+  SPLAT_CHECK(a.rope == ROPE_NONE || (std::isfinite(base) && base >= 1.0), BAD_ARGUMENT, "qk norm: rope_base must be at least 1");
+  SPLAT_CHECK(a.has_cache == (a.slots != nullptr), BAD_ARGUMENT, "qk norm: a cache needs slots, and slots a cache");
+  if (a.has_cache) {
+    check_cache(a.cache);
+    SPLAT_CHECK(a.cache.dt == a.dt && a.cache.kv_heads == a.kv_heads, BAD_ARGUMENT,
+                "qk norm: the cache has another dtype or other kv_heads");
+  }
+  if (a.tokens == 0) return;
+  SPLAT_CHECK(a.qkv && a.q_out && (a.rope == ROPE_NONE || a.positions), BAD_ARGUMENT, "qk norm: a required pointer is NULL");
+  const long es = type_size(a.dt), cols = (a.heads + 2L * a.kv_heads) * 64, wq = a.heads * 64L, wk = a.kv_heads * 64L;
+  SPLAT_CHECK(aligned16(a.qkv) && aligned16(a.q_out) && aligned16(a.k_out) && a.ld % 8 == 0 && a.ldq % 8 == 0 && a.ld >= cols &&
+                  a.ldq >= wq && (!a.k_out || (a.ldk % 8 == 0 && a.ldk >= wk)),
+              BAD_ARGUMENT, "qk norm: rows must be 16-byte aligned, as wide as their heads and a multiple of 8 elements apart");
+  const char* in = static_cast<const char*>(a.qkv);
+  SPLAT_CHECK((a.q_out == in && a.ldq == a.ld) || !rows_meet(in, a.ld * es, cols * es, a.q_out, a.ldq * es, wq * es, a.tokens),
+              BAD_ARGUMENT, "qk norm: q_out overlaps qkv and is not its query block");
+  SPLAT_CHECK((a.k_out == in + wq * es && a.ldk == a.ld) || !rows_meet(in, a.ld * es, cols * es, a.k_out, a.ldk * es, wk * es, a.tokens),
+              BAD_ARGUMENT, "qk norm: k_out overlaps qkv and is not its key block");
+  SPLAT_CHECK(!rows_meet(a.q_out, a.ldq * es, wq * es, a.k_out, a.ldk * es, wk * es, a.tokens), BAD_ARGUMENT, "qk norm: q_out overlaps k_out");
+  if (a.has_cache) {
+    const long before = a.tokens - 1L;
+    SPLAT_CHECK(!meets_pools(a.cache, in, (before * a.ld + cols) * es) && !meets_pools(a.cache, a.q_out, (before * a.ldq + wq) * es) &&
+                    (!a.k_out || !meets_pools(a.cache, a.k_out, (before * a.ldk + wk) * es)),
+                BAD_ARGUMENT, "qk norm: the cache overlaps the rows");
+    const long stride = a.cache.page_stride * es, page = wk * a.cache.page_size * es;  // k and v may share pages
+    SPLAT_CHECK(!rows_meet(a.cache.k, stride, page, a.cache.v, stride, page, a.cache.pages), BAD_ARGUMENT,
+                "qk norm: the cache's keys and values overlap");
+  }
+}
+
+void check_page_bounds(BoundsArgs& a) {
+  check_cache(a.cache);
+  SPLAT_CHECK(a.n >= 0 && a.max_add >= 0, BAD_ARGUMENT, "page bounds: n or max_add is negative");
+  check_width(a.width, a.cache.page_size);
+  if (a.n == 0) return;
+  SPLAT_CHECK(a.table && a.lens && a.bounds && aligned16(a.bounds), BAD_ARGUMENT,
+              "page bounds: a required pointer is NULL, or bounds not 16-byte aligned");
+  SPLAT_CHECK(!meets_pools(a.cache, a.bounds, long(a.cache.pages) * a.cache.kv_heads * 128 * type_size(a.cache.dt)), BAD_ARGUMENT,
+              "page bounds: bounds overlap the cache");
+  // add positions that end anywhere lie in one page more than they fill
+  a.per_seq = int(std::min<long>(a.width, a.add ? (long(a.max_add) + a.cache.page_size - 1) / a.cache.page_size + 1 : a.width));
+  SPLAT_CHECK(long(a.n) * a.per_seq * a.cache.kv_heads <= (1L << 32), BAD_ARGUMENT, "page bounds: more than 2^32 pages and heads");
+}
+
+void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes) {
+  check_attention(a);
+  if (a.n > 0) check_workspace(workspace, bytes, paged_attention_bytes(a.cache, a.n, a.heads, a.max_len));
+}
+
+void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) {
+  check_attention(a.at);
+  SPLAT_CHECK(a.topk >= 1, BAD_ARGUMENT, "sparse attention: topk must be at least 1");
+  SPLAT_CHECK(a.at.scale > 0.f, BAD_ARGUMENT, "sparse attention: scale must be positive");
+  if (a.at.n == 0) return;
+  SPLAT_CHECK(a.bounds && aligned16(a.bounds) && a.selected, BAD_ARGUMENT,
+              "sparse attention: a required pointer is NULL, or bounds not 16-byte aligned");
+  SPLAT_CHECK(!meets_pools(a.at.cache, a.selected, 4L * a.at.n * a.at.cache.kv_heads * a.topk), BAD_ARGUMENT,
+              "sparse attention: selected overlaps the cache");
+  check_workspace(workspace, bytes, sparse_attention_bytes(a.at.cache, a.at.n, a.at.heads, a.at.max_len, a.topk));
+}
+
+namespace {
+void check_workspace_sizes(const KvCache& c, int n, int heads, int max_len) {
+  check_sizes(c);
+  SPLAT_CHECK(n >= 0 && max_len >= 0 && heads >= 1 && heads % c.kv_heads == 0 && long(n) * heads <= (1 << 24), BAD_ARGUMENT,
+              "workspace: n, heads or max_len");
+}
+}  // namespace
+
+size_t paged_attention_bytes(const KvCache& c, int n, int heads, int max_len) {
+  check_workspace_sizes(c, n, heads, max_len);
+  return 0;
+}
+
+size_t sparse_attention_bytes(const KvCache& c, int n, int heads, int max_len, int topk) {
+  check_workspace_sizes(c, n, heads, max_len);
+  SPLAT_CHECK(topk >= 1, BAD_ARGUMENT, "sparse attention: topk must be at least 1");
+  return size_t(n) * c.kv_heads * ((long(max_len) + c.page_size - 1) / c.page_size) * 8;
+}
+
+void rope_turns(int rope, double base, double (&freq)[32]) {
+  // products of powers of two of the step: at most five roundings each
+  const int h = rope == ROPE_LINE ? 32 : 16;
+  double step[5];
+  for (int b = 0; b < 5; ++b) step[b] = std::pow(base, -double(1 << b) / h);
+  for (int i = 0; i < 32; ++i) {
+    double f = 0.15915494309189535;  // 1 / (2 pi)
+    for (int b = 0; b < 5; ++b)
+      if (i >> b & 1) f *= step[b];
+    freq[i] = f;
+  }
+}
+
+}  // namespace splat

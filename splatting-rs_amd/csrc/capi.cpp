@@ -150,6 +150,37 @@ AttnArgs attention_args(int dtype, const void* qkv, void* out, int S, int L, int
   a.seq_stride = L;
   return a;
 }
+// splat_kv_cache -> the library's description (the launchers check its sizes)
+KvCache kv_cache(const splat_kv_cache* c) {
+  SPLAT_CHECK(c != nullptr, BAD_ARGUMENT, "cache is NULL");
+  KvCache k;
+  k.dt = model_dtype(c->dtype);
+  k.pages = c->pages;
+  k.page_size = c->page_size;
+  k.kv_heads = c->kv_heads;
+  k.page_stride = c->page_stride ? c->page_stride : int64_t(c->kv_heads) * c->page_size * 64;
+  k.k = c->k;
+  k.v = c->v;
+  return k;
+}
+
+PagedArgs paged_args(const splat_kv_cache* cache, const void* q, int64_t ldq, int n, int heads, const int32_t* table,
+                     int width, const int32_t* lens, int max_len, float scale, void* out, int64_t ldo) {
+  PagedArgs a;
+  a.cache = kv_cache(cache);
+  a.q = q;
+  a.ldq = ldq;
+  a.n = n;
+  a.heads = heads;
+  a.table = table;
+  a.width = width;
+  a.lens = lens;
+  a.max_len = max_len;
+  a.scale = scale;
+  a.out = out;
+  a.ldo = ldo;
+  return a;
+}
 template <typename T>
 void d2h(Context* ctx, T* host, const void* dev, size_t count) {
   if (host) SPLAT_HIP(hipMemcpyAsync(host, dev, count * sizeof(T), hipMemcpyDeviceToHost, ctx->stream));
@@ -466,6 +497,118 @@ int splat_kernel_attention(splat_ctx* ctx, int dtype, const void* qkv, void* out
     attention(dry, a);
     if (c->reserve_workspace()) c->clear_graphs();
     attention(c->ex, a);
+  });
+}
+
+int splat_kernel_block_tables(splat_ctx* ctx, int n, const int32_t* past, const int32_t* add, int page_size,
+                              const int32_t* pool, int pool_size, const int32_t* used, int32_t* table, int width,
+                              int32_t* lens, int32_t* starts, int32_t* slots, int32_t* positions, int cap,
+                              int32_t* used_out, int32_t* status) {
+  return guard(C(ctx), [&] {
+    BlockTableArgs a;
+    a.n = n;
+    a.past = past;
+    a.add = add;
+    a.page_size = page_size;
+    a.pool = pool;
+    a.pool_size = pool_size;
+    a.used = used;
+    a.table = table;
+    a.width = width;
+    a.lens = lens;
+    a.starts = starts;
+    a.slots = slots;
+    a.positions = positions;
+    a.cap = cap;
+    a.used_out = used_out;
+    a.status = status;
+    block_tables(C(ctx)->ex, a);
+  });
+}
+
+int splat_kernel_qk_norm_rope(splat_ctx* ctx, int dtype, const void* qkv, int64_t ld, int tokens, int heads,
+                              int kv_heads, int norm, const float* qw, const float* qb, const float* kw,
+                              const float* kb, float eps, int rope, double rope_base, const int32_t* positions,
+                              void* q_out, int64_t ldq, void* k_out, int64_t ldk, const splat_kv_cache* cache,
+                              const int32_t* slots) {
+  return guard(C(ctx), [&] {
+    QkArgs a;
+    a.dt = model_dtype(dtype);
+    a.qkv = qkv;
+    a.ld = ld;
+    a.tokens = tokens;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.norm = norm;
+    a.qw = qw;
+    a.qb = qb;
+    a.kw = kw;
+    a.kb = kb;
+    a.eps = eps;
+    a.rope = rope;
+    a.positions = positions;
+    a.q_out = q_out;
+    a.ldq = ldq;
+    a.k_out = k_out;
+    a.ldk = ldk;
+    a.has_cache = cache != nullptr;
+    if (cache) a.cache = kv_cache(cache);
+    a.slots = slots;
+    qk_norm_rope(C(ctx)->ex, a, rope_base);
+  });
+}
+
+int splat_kernel_page_bounds(splat_ctx* ctx, const splat_kv_cache* cache, int n, const int32_t* table, int width,
+                             const int32_t* lens, const int32_t* add, int max_add, void* bounds) {
+  return guard(C(ctx), [&] {
+    BoundsArgs a;
+    a.cache = kv_cache(cache);
+    a.n = n;
+    a.table = table;
+    a.width = width;
+    a.lens = lens;
+    a.add = add;
+    a.max_add = max_add;
+    a.bounds = bounds;
+    page_bounds(C(ctx)->ex, a);
+  });
+}
+
+int splat_paged_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, size_t* bytes) {
+  return guard_free([&] {
+    SPLAT_CHECK(bytes != nullptr, BAD_ARGUMENT, "bytes is NULL");
+    *bytes = paged_attention_bytes(kv_cache(cache), n, heads, max_len);
+  });
+}
+
+int splat_kernel_paged_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* q, int64_t ldq, int n,
+                                 int heads, const int32_t* table, int width, const int32_t* lens, int max_len,
+                                 float scale, void* out, int64_t ldo, void* workspace, size_t workspace_bytes) {
+  return guard(C(ctx), [&] {
+    paged_attention(C(ctx)->ex, paged_args(cache, q, ldq, n, heads, table, width, lens, max_len, scale, out, ldo),
+                    workspace, workspace_bytes);
+  });
+}
+
+int splat_sparse_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, int topk,
+                                     size_t* bytes) {
+  return guard_free([&] {
+    SPLAT_CHECK(bytes != nullptr, BAD_ARGUMENT, "bytes is NULL");
+    *bytes = sparse_attention_bytes(kv_cache(cache), n, heads, max_len, topk);
+  });
+}
+
+int splat_kernel_sparse_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* bounds, const void* q,
+                                  int64_t ldq, int n, int heads, const int32_t* table, int width,
+                                  const int32_t* lens, int max_len, int topk, float scale, void* out, int64_t ldo,
+                                  int32_t* selected, void* workspace, size_t workspace_bytes) {
+  return guard(C(ctx), [&] {
+    SparseArgs a;
+    a.at = paged_args(cache, q, ldq, n, heads, table, width, lens, max_len, scale, out, ldo);
+    a.bounds = bounds;
+    a.topk = topk;
+    a.selected = selected;
+    sparse_attention(C(ctx)->ex, a, workspace, workspace_bytes);
   });
 }
 

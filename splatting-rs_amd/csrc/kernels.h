@@ -4,6 +4,7 @@
 #pragma once
 
 #include <functional>
+#include "cache.h"
 #include "common.h"
 
 namespace splat {
@@ -228,5 +229,13 @@ void mean_rows(const Exec& ex, int dt, const void* in, int groups, int P, int C,
 void exp_clamp(const Exec& ex, float* x, int count, float lo);
 void normalize_rows(const Exec& ex, float* x, int rows, int dim, float min_norm);
 void scale_rows(const Exec& ex, const float* x, int rows, int dim, const float* scale, float* out);
+
+// --- paged cache of keys and values (cache.hip; arguments and their checks: cache.h) -------------
+
+void block_tables(const Exec& ex, const BlockTableArgs& a);
+void qk_norm_rope(const Exec& ex, const QkArgs& a, double base);
+void page_bounds(const Exec& ex, const BoundsArgs& a);
+void paged_attention(const Exec& ex, const PagedArgs& a, void* workspace, size_t bytes);
+void sparse_attention(const Exec& ex, const SparseArgs& a, void* workspace, size_t bytes);
 
 }  // namespace splat

@@ -25,6 +25,9 @@ LIB_PATH = os.path.join(os.path.dirname(_HERE), "libsplathip.so")
 OK, BAD_ARGUMENT, BAD_SHAPE, MISSING_KEY, SHAPE_MISMATCH, HIP_ERROR, NONFINITE, IO_ERROR, NOT_LOADED = range(9)
 F32, BF16, F16 = 0, 1, 2
 DTYPES = {"f32": F32, "fp32": F32, "bf16": BF16, "f16": F16}
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
+ROPE_NONE, ROPE_LINE, ROPE_GRID = 0, 1, 2
+TABLE_OK, TABLE_BAD_LENGTH, TABLE_POOL_EMPTY, TABLE_SLOTS_FULL = 0, 1, 2, 3
 STAGE_BLOCK, STAGE_DENSE_HEAD, STAGE_CAMERA_HEAD = 0, 1, 2
 FILTER_TRIANGLE, FILTER_CATMULLROM, FILTER_LANCZOS3 = 1, 2, 3   # image 0.25.10 imageops::FilterType
 
@@ -67,6 +70,15 @@ class ReconOutC(C.Structure):
 class KernelStatC(C.Structure):
     _fields_ = [("name", C.c_char * 32), ("launches", C.c_int), ("ms", C.c_double), ("flops", C.c_double),
                 ("bytes", C.c_double)]
+
+
+class KvCache(C.Structure):
+    """splat_kv_cache: the pools of a paged cache (k and v are device pointers)."""
+    _fields_ = [("dtype", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32),
+                ("page_stride", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+    def __init__(self, dtype: int, k: int, v: int, pages: int, page_size: int, kv_heads: int, page_stride: int = 0):
+        super().__init__(dtype, pages, page_size, kv_heads, page_stride, k, v)
 
 
 PROGRESS_FN = C.CFUNCTYPE(None, C.c_int, C.c_int, C.c_void_p)
@@ -112,6 +124,26 @@ SIGNATURES = {
     "splat_kernel_attention": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),
     "splat_kernel_attention_noalloc": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                                  C.c_int]),
+    "splat_kernel_block_tables": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                            C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                            C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    "splat_kernel_qk_norm_rope": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                            C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_float,
+                                            C.c_int, C.c_double, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+                                            C.c_int64, C.POINTER(KvCache), C.c_void_p]),
+    "splat_kernel_page_bounds": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.c_int, C.c_void_p, C.c_int, C.c_void_p,
+                                           C.c_void_p, C.c_int, C.c_void_p]),
+    "splat_paged_attention_workspace": (C.c_int, [C.POINTER(KvCache), C.c_int, C.c_int, C.c_int,
+                                                  C.POINTER(C.c_size_t)]),
+    "splat_kernel_paged_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.c_void_p, C.c_int64, C.c_int, C.c_int,
+                                               C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_float, C.c_void_p,
+                                               C.c_int64, C.c_void_p, C.c_size_t]),
+    "splat_sparse_attention_workspace": (C.c_int, [C.POINTER(KvCache), C.c_int, C.c_int, C.c_int, C.c_int,
+                                                   C.POINTER(C.c_size_t)]),
+    "splat_kernel_sparse_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_int64,
+                                                C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int,
+                                                C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                                C.c_size_t]),
     "splat_profile_begin": (C.c_int, [C.c_void_p]),
     "splat_profile_end": (C.c_int, [C.c_void_p, C.POINTER(KernelStatC), C.c_int, C.POINTER(C.c_int)]),
     "splat_kernel_conv2d": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
@@ -422,6 +454,39 @@ class Context:
         self.check(self._lib.splat_kernel_attention_noalloc(self.handle, dtype, C.c_void_p(qkv), C.c_void_p(out), S, L,
                                                             heads))
 
+    # The paged cache's operators (device pointers as ints, 0 for NULL; cache: a KvCache).
+    def kernel_block_tables(self, n: int, past: int, add: int, page_size: int, pool: int, pool_size: int, used: int,
+                            table: int, width: int, lens: int, starts: int, slots: int, positions: int, cap: int,
+                            used_out: int, status: int):
+        self.check(self._lib.splat_kernel_block_tables(self.handle, n, past, add, page_size, pool, pool_size, used,
+                                                       table, width, lens, starts, slots, positions, cap, used_out,
+                                                       status))
+
+    def kernel_qk_norm_rope(self, dtype: int, qkv: int, ld: int, tokens: int, heads: int, kv_heads: int, norm: int,
+                            qw: int, qb: int, kw: int, kb: int, eps: float, rope: int, rope_base: float,
+                            positions: int, q_out: int, ldq: int, k_out: int = 0, ldk: int = 0,
+                            cache: Optional[KvCache] = None, slots: int = 0):
+        self.check(self._lib.splat_kernel_qk_norm_rope(self.handle, dtype, qkv, ld, tokens, heads, kv_heads, norm, qw,
+                                                       qb, kw, kb, eps, rope, rope_base, positions, q_out, ldq, k_out,
+                                                       ldk, cache, slots))
+
+    def kernel_page_bounds(self, cache: KvCache, n: int, table: int, width: int, lens: int, add: int, max_add: int,
+                           bounds: int):
+        self.check(self._lib.splat_kernel_page_bounds(self.handle, cache, n, table, width, lens, add, max_add, bounds))
+
+    def kernel_paged_attention(self, cache: KvCache, q: int, ldq: int, n: int, heads: int, table: int, width: int,
+                               lens: int, max_len: int, scale: float, out: int, ldo: int, workspace: int,
+                               workspace_bytes: int):
+        self.check(self._lib.splat_kernel_paged_attention(self.handle, cache, q, ldq, n, heads, table, width, lens,
+                                                          max_len, scale, out, ldo, workspace, workspace_bytes))
+
+    def kernel_sparse_attention(self, cache: KvCache, bounds: int, q: int, ldq: int, n: int, heads: int, table: int,
+                                width: int, lens: int, max_len: int, topk: int, scale: float, out: int, ldo: int,
+                                selected: int, workspace: int, workspace_bytes: int):
+        self.check(self._lib.splat_kernel_sparse_attention(self.handle, cache, bounds, q, ldq, n, heads, table, width,
+                                                           lens, max_len, topk, scale, out, ldo, selected, workspace,
+                                                           workspace_bytes))
+
     def kernel_conv2d(self, dtype, inp, V, H, W, Cin, w, Cout, ldw, ks, stride, bias, relu_in, act, res, out):
         self.check(self._lib.splat_kernel_conv2d(self.handle, dtype, C.c_void_p(inp), V, H, W, Cin, C.c_void_p(w), Cout,
                                                  ldw, ks, stride, C.c_void_p(bias), relu_in, act, C.c_void_p(res),
@@ -453,6 +518,20 @@ def reference_ma_spec() -> dict:
 def _check_free(rc: int):
     if rc != OK:
         raise SplatError(rc, lib().splat_last_error(None).decode())
+
+
+def paged_attention_workspace(cache: KvCache, n: int, heads: int, max_len: int) -> int:
+    """Bytes of device memory that kernel_paged_attention needs for these sizes."""
+    b = C.c_size_t()
+    _check_free(lib().splat_paged_attention_workspace(cache, n, heads, max_len, C.byref(b)))
+    return b.value
+
+
+def sparse_attention_workspace(cache: KvCache, n: int, heads: int, max_len: int, topk: int) -> int:
+    """Bytes of device memory that kernel_sparse_attention needs for these sizes."""
+    b = C.c_size_t()
+    _check_free(lib().splat_sparse_attention_workspace(cache, n, heads, max_len, topk, C.byref(b)))
+    return b.value
 
 
 def da3_model_input_size(width: int, height: int):
