@@ -74,6 +74,16 @@ void check_qk_norm_rope(QkArgs& a, double base);
 void check_page_bounds(BoundsArgs& a);
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes);
 void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes);
+
+// How attention over the cache is launched: `cols` groups of up to 16 query heads of one key head, and for long
+// sequences `workers` waves for each, which leave parts to join; 0: one block a sequence and group. topk 0: all
+// pages.
+constexpr int PART_HEAD = 68;  // floats of one head in one part
+struct PagedPlan {
+  int cols = 0, workers = 0;
+  size_t before_bytes = 0, bytes = 0;  // of the workspace: the sequences' tile counts, and all of it
+};
+PagedPlan paged_plan(const KvCache& c, int n, int heads, int max_len, int topk);
 size_t paged_attention_bytes(const KvCache& c, int n, int heads, int max_len);
 size_t sparse_attention_bytes(const KvCache& c, int n, int heads, int max_len, int topk);
 

@@ -8,6 +8,7 @@
 #include "kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace splat {
 
@@ -273,61 +274,513 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs p) {
 }
 
 // --- attention of one token over the cache ------------------------------------------------------
+//
+// S^T = K Q^T and O^T = V^T P^T on the 16x16 matrix instructions, the query heads that share a key head as the
+// 16 columns (fewer: columns of zeros, which cost nothing, since the bytes of K and V bound the kernel).
+// The scores come out with a lane holding one head (lane % 16) and keys 4 (lane / 16) + r, which is the
+// operand layout of the second product as it stands; V is read transposed from LDS.
+//
+// A wave works alone: tiles of 32 keys (16 in fp32: 4 KB of K and 4 KB of V in every type) stream into its own
+// ring in LDS, four loads of 1 KB for each, that many bytes ahead, and no barrier holds it up. A load covers 8
+// rows (4 in fp32) of one page, and the rows that are not there (past the length, a missing page) lie outside
+// its buffer, so that they arrive as zeros whatever memory holds.
 
-// One wave a (sequence, query head): 8 lanes a key row, 8 keys at a time, a running maximum and sum for
-// each of the 8 groups of lanes, joined at the end. `sel` != null: only the pages that it lists.
-template <typename T>
-__global__ void __launch_bounds__(64) paged_attention_kernel(const PagedArgs p, const int* sel, int topk) {
-  const int lane = threadIdx.x, g = lane >> 3, j = lane & 7;
-  const int h = blockIdx.x % p.heads, i = blockIdx.x / p.heads, kh = h / (p.heads / p.cache.kv_heads);
-  const KvCache& c = p.cache;
-  const int ps = 1 << c.shift;
-  const int len = length_of(p.lens[i], p.width, c.shift, p.max_len);
-  float q[8], o[8] = {};
-  load8(static_cast<const T*>(p.q) + i * p.ldq + h * 64 + j * 8, q);
-  const float scale = p.scale * 1.44269504088896341f;
-  float m = -INFINITY, l = 0.f;
-  bool some = false;
-  const int count = sel ? topk : (len + ps - 1) >> c.shift;
-  for (int a = 0; a < count; ++a) {
-    const int pi = sel ? sel[(long(i) * c.kv_heads + kh) * topk + a] : a;
-    if (pi < 0) break;
-    const int page = p.table[long(i) * p.width + pi];
-    if (!page_ok(page, c.pages)) continue;
-    const int rows = min(ps, len - (pi << c.shift));
-    const long at = page_at(c, page, kh) + j * 8;
-    for (int r = g; r < rows; r += 8) {
-      float x[8], s = 0.f;
-      load8(static_cast<const T*>(c.k) + at + r * 64, x);
+typedef __bf16 bf16x8_v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int int32x4_v __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(3))) char* lds_cptr;
+
+// A wave-uniform load of memory that the launch only reads.
+__device__ inline int uload(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// 16 bytes a lane from `base + off` into LDS at lds + 16 * lane; offsets from `bytes` on read as zeros.
+__device__ inline void load_lds(const void* base, uint32_t bytes, uint32_t off, uint32_t lds) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  const int32x4_v r = {uniform(int(uint32_t(a))), uniform(int(uint32_t(a >> 32))), uniform(int(bytes)), 0x00020000};
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(uniform(int(lds))), "v"(off), "s"(r)
+               : "memory");
+}
+template <int N> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// Maximum (sum) over lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ inline float max_groups(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float sum_groups(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The two products on a tile in LDS. KEYS keys in T16 groups of 16; PIECE rows to a load.
+template <typename T> struct TileOps {  // bf16, f16: rows of 128 bytes
+  static constexpr int KEYS = 32, T16 = 2, PIECE = 8;
+  // f16 weights below 2^-14 lose bits: the largest one is 2^12, so that they do so from 2^-26 of it on.
+  static constexpr float TOP = std::is_same<T, f16>::value ? 12.f : 0.f;
+  uint4 q[2];
+  __device__ inline void load_q(const T* row, int g, bool in) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += q[e] * x[e];
-      s = sum8(s) * scale;
-      const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-      const float keep = exp2f(m - ref), w = exp2f(s - ref);
-      load8(static_cast<const T*>(c.v) + at + r * 64, x);
+    for (int s = 0; s < 2; ++s)
+      q[s] = in ? *reinterpret_cast<const uint4*>(row + 32 * s + 8 * g) : make_uint4(0, 0, 0, 0);
+  }
+  // Takes the loads as done here: inside the loop the compiler's wait for them would be one for every tile in flight.
+  __device__ inline void pin_q() {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = o[e] * keep + w * x[e];
-      l = l * keep + w;
-      m = mn;
-      some = true;
+    for (int s = 0; s < 2; ++s) asm volatile("" : "+v"(q[s].x), "+v"(q[s].y), "+v"(q[s].z), "+v"(q[s].w));
+  }
+  // Offset of this lane's 16 bytes within piece `p` (1 KB, 8 rows): chunk c of row r lies in slot c ^ ((r / 2) & 7)
+  // for keys, c ^ 2 ((r / 2) & 3) for values, so that the rows that a read takes lie in different banks.
+  __device__ static inline uint32_t k_off(int lane, int p) { return (lane >> 3) * 128 + (((lane & 7) ^ (((lane >> 4) + 4 * p) & 7)) * 16); }
+  __device__ static inline uint32_t v_off(int lane, int) { return (lane >> 3) * 128 + (((lane & 7) ^ (2 * ((lane >> 4) & 3))) * 16); }
+  __device__ static inline f32x4 mma(const uint4& a, const uint4& b, const f32x4& c) {
+    if constexpr (std::is_same<T, bf16>::value)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_v, a), __builtin_bit_cast(f16x8_v, b), c, 0, 0, 0);
+  }
+  __device__ inline void scores(const char* kt, int lane, f32x4 (&x)[T16]) const {
+    const int row = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        a = mma(*reinterpret_cast<const uint4*>(kt + (16 * t + row) * 128 + (((4 * s + g) ^ ((row >> 1) & 7)) * 16)), q[s], a);
+      x[t] = a;
     }
   }
+  __device__ static inline void weigh(const char* vt, int lane, const f32x4 (&w)[T16], f32x4 (&o)[4]) {
+    const int g = lane >> 4, j = (lane >> 2) & 3, cc = lane & 3;
+    const uint4 p = make_uint4(pack2<T>(w[0][0], w[0][1]), pack2<T>(w[0][2], w[0][3]), pack2<T>(w[1][0], w[1][1]),
+                               pack2<T>(w[1][2], w[1][3]));
+    const int row = 4 * g + j;  // and 16 + row, whose chunks lie alike
 #pragma unroll
-  for (int d = 8; d < 64; d <<= 1) {
-    const float om = __shfl_xor(m, d), ol = __shfl_xor(l, d);
-    const bool os = __shfl_xor(int(some), d);
-    const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
-    // a side without keys has no part, whatever the other holds
-    const float a = some ? exp2f(m - ref) : 0.f, b = os ? exp2f(om - ref) : 0.f;
-    l = l * a + ol * b;
+    for (int d = 0; d < 4; ++d) {
+      typedef short v4s __attribute__((ext_vector_type(4)));
+      const char* at = vt + row * 128 + (((2 * d + (cc >> 1)) ^ (2 * ((row >> 1) & 3))) * 16) + (cc & 1) * 8;
+      uint32_t f[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = o[e] * a + __shfl_xor(o[e], d) * b;
-    m = mn;
-    some |= os;
+      for (int t = 0; t < 2; ++t) {
+        const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)((lds_cptr)(at + t * 2048)));
+        const uint2 u = __builtin_bit_cast(uint2, r);
+        f[2 * t] = u.x;
+        f[2 * t + 1] = u.y;
+      }
+      o[d] = mma(make_uint4(f[0], f[1], f[2], f[3]), p, o[d]);
+    }
   }
+};
+template <> struct TileOps<float> {  // rows of 256 bytes
+  static constexpr int KEYS = 16, T16 = 1, PIECE = 4;
+  static constexpr float TOP = 0.f;
+  float4 q[4];
+  __device__ inline void load_q(const float* row, int g, bool in) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = some ? o[e] / l : 0.f;
-  if (lane < 8) store8(static_cast<T*>(p.out) + i * p.ldo + h * 64 + j * 8, o);
+    for (int b = 0; b < 4; ++b)
+      q[b] = in ? *reinterpret_cast<const float4*>(row + 16 * b + 4 * g) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ inline void pin_q() {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) asm volatile("" : "+v"(q[b].x), "+v"(q[b].y), "+v"(q[b].z), "+v"(q[b].w));
+  }
+  // chunk c of row r in slot c ^ r for keys, c ^ 4 (r / 4) for values
+  __device__ static inline uint32_t k_off(int lane, int p) { return (lane >> 4) * 256 + (((lane & 15) ^ (4 * p + (lane >> 4))) * 16); }
+  __device__ static inline uint32_t v_off(int lane, int p) { return (lane >> 4) * 256 + (((lane & 15) ^ (4 * p)) * 16); }
+  __device__ inline void scores(const char* kt, int lane, f32x4 (&x)[T16]) const {
+    const int row = lane & 15, g = lane >> 4;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float4 k = *reinterpret_cast<const float4*>(kt + row * 256 + (((4 * b + g) ^ row) * 16));
+      a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.x, q[b].x, a, 0, 0, 0);
+      a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.y, q[b].y, a, 0, 0, 0);
+      a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.z, q[b].z, a, 0, 0, 0);
+      a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.w, q[b].w, a, 0, 0, 0);
+    }
+    x[0] = a;
+  }
+  __device__ static inline void weigh(const char* vt, int lane, const f32x4 (&w)[T16], f32x4 (&o)[4]) {
+    const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = *reinterpret_cast<const float*>(vt + (4 * g + r) * 256 + (((4 * d + (c >> 2)) ^ (4 * g)) * 16) + (c & 3) * 4);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[0][r], o[d], 0, 0, 0);
+      }
+  }
+};
+
+constexpr int TILE_BYTES = 8192;  // K, then V
+constexpr int STAGES = 2;
+
+// Where a wave stands: sequence i holds tiles [base, next) of the launch's row of tiles.
+struct Cursor {
+  int i;
+  long base, next;
+};
+
+// Tiles of sequence i: of its positions, or of the pages that were selected.
+template <int KEYS> __device__ inline int tiles_of(const PagedArgs& p, int i, int topk) {
+  const int len = length_of(p.lens[i], p.width, p.cache.shift, p.max_len);
+  if (!topk) return int((long(len) + KEYS - 1) / KEYS);
+  const int held = int((long(len) + p.cache.page_size - 1) >> p.cache.shift);
+  return int(((long(min(held, topk)) << p.cache.shift) + KEYS - 1) / KEYS);
+}
+
+// One wave: the running softmax of one group of heads over tiles [t, end), which may cross sequences.
+// finish(cursor, first tile, state) is called at the end of each sequence's part.
+template <typename T> struct PagedWave {
+  using Ops = TileOps<T>;
+  static constexpr int KEYS = Ops::KEYS, PIECE = Ops::PIECE;
+  const PagedArgs& p;
+  const int* sel;  // [n, kv_heads, topk] or null
+  const int topk, kh, lane;
+  const uint32_t lds;   // of the wave's ring
+  const char* ring;
+  Ops ops;
+  f32x4 o[4];
+  float m, l;
+  int some;  // keys were there
+
+  __device__ inline void clear() {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+    some = 0;
+  }
+
+  // Loads local tile t of sequence i into slot b of the ring; the rows of each piece that are there, 8 bits a piece.
+  __device__ inline uint32_t issue(int i, int t, int b) {
+    const KvCache& c = p.cache;
+    const int len = uniform(length_of(uload(p.lens + i), p.width, c.shift, p.max_len)), ps = c.page_size;
+    const int held = int((long(len) + ps - 1) >> c.shift), count = topk ? min(held, topk) : held;
+    const int* row = p.table + long(i) * p.width;
+    uint32_t there = 0;
+    int entry[4], rows[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int pos = t * KEYS + k * PIECE, e = pos >> c.shift;
+      int j = min(e, count - 1);
+      if (topk) j = uload(sel + (long(i) * c.kv_heads + kh) * topk + j);
+      entry[k] = uload(row + max(j, 0));
+      const int left = len - int(long(j) << c.shift) - (pos & (ps - 1));
+      rows[k] = e < count && j >= 0 ? max(0, min(PIECE, left)) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool ok = page_ok(entry[k], c.pages);
+      const int r = ok ? rows[k] : 0;
+      there |= uint32_t(r) << (8 * k);
+      const long at = (ok ? page_at(c, entry[k], kh) : 0) + long((t * KEYS + k * PIECE) & (ps - 1)) * 64;
+      const uint32_t bytes = uint32_t(r) * 64 * sizeof(T), to = lds + b * TILE_BYTES + k * 1024;
+      load_lds(static_cast<const T*>(c.k) + at, bytes, Ops::k_off(lane, k), to);
+      load_lds(static_cast<const T*>(c.v) + at, bytes, Ops::v_off(lane, k), to + TILE_BYTES / 2);
+    }
+    return uniform(int(there));
+  }
+
+  __device__ inline void tile(int b, uint32_t there, float scale) {
+    constexpr uint32_t ALL = PIECE * 0x01010101u;
+    const char* kt = ring + b * TILE_BYTES;
+    f32x4 x[Ops::T16];
+    ops.scores(kt, lane, x);
+    const int g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < Ops::T16; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[t][r] *= scale;
+    if (there != ALL) {
+#pragma unroll
+      for (int t = 0; t < Ops::T16; ++t) {
+        const int key = 16 * t + 4 * g, rows = int((there >> (8 * (key / PIECE))) & 255u) - key % PIECE;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r >= rows) x[t][r] = -INFINITY;
+      }
+    }
+    some |= there != 0;
+    float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
+    if constexpr (Ops::T16 == 2) mx = fmaxf(mx, fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    const float mn = fmaxf(m, max_groups(mx));
+    const float ref = mn == -INFINITY ? 0.f : mn - Ops::TOP;
+    // the weights are 2^(x - ref); what was summed against another reference moves along
+    const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[d][r] *= keep;
+#pragma unroll
+    for (int t = 0; t < Ops::T16; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - ref);
+        l += x[t][r];
+      }
+    Ops::weigh(kt + TILE_BYTES / 2, lane, x, o);
+  }
+
+  // Local tiles [t, end) of one sequence with nothing in flight before or after.
+  __device__ inline void run(int i, int t, int end, float scale) {
+    uint32_t there[STAGES];
+#pragma unroll
+    for (int b = 0; b < STAGES; ++b) there[b] = t + b < end ? issue(i, t + b, b) : 0;
+    ops.pin_q();
+    while (t < end) {
+#pragma unroll
+      for (int b = 0; b < STAGES; ++b) {
+        if (t + b >= end) break;
+        if (t + b + 1 < end) wait_loads<8 * (STAGES - 1)>();
+        else wait_loads<0>();
+        tile(b, there[b], scale);
+        if (t + b + STAGES < end) there[b] = issue(i, t + b + STAGES, b);
+      }
+      t += STAGES;
+    }
+  }
+
+  // The normalised result, or zeros where no key was there.
+  __device__ inline void store(int i, int head, float sum) const {
+    const float inv = 1.f / sum;
+    T* out = static_cast<T*>(p.out) + i * p.ldo + long(head) * 64 + 4 * (lane >> 4);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = some ? o[d][r] * inv : 0.f;
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out + 16 * d) = make_float4(v[0], v[1], v[2], v[3]);
+      else *reinterpret_cast<uint2*>(out + 16 * d) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    }
+  }
+};
+
+constexpr int PAGED_WAVES = 4;
+
+// One block a (sequence, group of up to 16 heads of one key head): its waves take a quarter of the tiles each
+// and join their sums in LDS.
+template <typename T>
+__global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const PagedArgs p, const int* sel, int topk, float scale) {
+  using Wave = PagedWave<T>;
+  __shared__ __attribute__((aligned(1024))) char smem[PAGED_WAVES * STAGES * TILE_BYTES];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int G = p.heads / p.cache.kv_heads, parts = (G + 15) / 16;
+  const int i = blockIdx.x, kh = int(blockIdx.y) / parts, g0 = int(blockIdx.y) % parts * 16;
+  const int col = lane & 15, head = kh * G + g0 + col;
+  char* ring = smem + wave * STAGES * TILE_BYTES;
+  Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
+  w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
+  w.clear();
+  const int nt = uniform(tiles_of<Wave::KEYS>(p, i, topk));
+  w.run(i, int(long(nt) * wave / PAGED_WAVES), int(long(nt) * (wave + 1) / PAGED_WAVES), scale);
+  w.l = sum_groups(w.l);
+  // the join: every wave's m, l and whether it had keys, then the sums moved to the common reference
+  float* ml = reinterpret_cast<float*>(smem);
+  __syncthreads();
+  if (lane < 16) {
+    float* at = ml + (wave * 16 + lane) * 4;
+    at[0] = w.m;
+    at[1] = w.l;
+    at[2] = __int_as_float(w.some);
+  }
+  __syncthreads();
+  float mn = -INFINITY;
+  for (int k = 0; k < PAGED_WAVES; ++k) mn = fmaxf(mn, ml[(k * 16 + col) * 4]);
+  float sum = 0.f;
+  int some = 0;
+  for (int k = 0; k < PAGED_WAVES; ++k) {
+    const float* at = ml + (k * 16 + col) * 4;
+    if (!__float_as_int(at[2])) continue;
+    some = 1;
+    sum += at[1] * (at[0] == -INFINITY ? 0.f : exp2f(at[0] - mn));
+  }
+  const float keep = !w.some ? 0.f : w.m == -INFINITY ? 0.f : exp2f(w.m - mn);
+  float* os = ml + 1024;  // [wave][d][r][lane]
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) os[((wave * 4 + d) * 4 + r) * 64 + lane] = w.some ? w.o[d][r] * keep : 0.f;
+  __syncthreads();
+  if (g0 + col >= G) return;
+  // wave d writes channels 16 d + 4 (lane / 16) + (0..3)
+  float v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float a = 0.f;
+    for (int k = 0; k < PAGED_WAVES; ++k) a += os[((k * 4 + wave) * 4 + r) * 64 + lane];
+    v[r] = some ? a / sum : 0.f;
+  }
+  T* out = static_cast<T*>(p.out) + i * p.ldo + long(head) * 64 + 16 * wave + 4 * (lane >> 4);
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+}
+
+// Long or uneven sequences: the tiles of all sequences in a row, cut into one equal part a wave. A sequence that
+// lies within one part is written at once; of the others each wave leaves its part's sums, unnormalised, for
+// paged_join_kernel: slot 0 for the sequence that the part begins in, slot 1 for one that it ends in.
+constexpr int SCAN_MAX = 1024;
+
+
+// before[i]: tiles of the sequences before i, for i in [0, n]. By one block of NT threads.
+template <int KEYS, int NT> __device__ inline void scan_tiles(const PagedArgs& p, int topk, long* before) {
+  __shared__ long wsum[NT / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  long base = 0;
+  for (int i0 = 0; i0 <= p.n; i0 += NT) {
+    const int i = i0 + tid;
+    const long c = i < p.n ? tiles_of<KEYS>(p, i, topk) : 0;
+    long inc = c;
+    for (int m = 1; m < 64; m <<= 1) {
+      const long o = __shfl_up(inc, m);
+      if (lane >= m) inc += o;
+    }
+    if (lane == 63) wsum[wave] = inc;
+    __syncthreads();
+    long at = base + inc - c;
+    for (int k = 0; k < NT / 64; ++k) {
+      if (k < wave) at += wsum[k];
+      base += wsum[k];
+    }
+    if (i <= p.n) before[i] = at;
+    __syncthreads();
+  }
+}
+
+template <int KEYS> __global__ void __launch_bounds__(1024) paged_scan_kernel(const PagedArgs p, int topk, long* before) {
+  scan_tiles<KEYS, 1024>(p, topk, before);
+}
+
+// A part: `heads` (up to 16) times 64 sums, then (m, l) of each head; l is -1 where no key was there. PART_HEAD
+// floats a head keep the parts 16-byte aligned.
+struct Part {
+  const int heads;
+  __device__ inline explicit Part(int G) : heads(min(G, 16)) {}
+  __device__ inline long size() const { return heads * long(PART_HEAD); }
+  __device__ inline int ml(int g) const { return heads * 64 + g * 2; }
+};
+
+template <typename T, bool SCAN>
+__global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const PagedArgs p, const int* sel, int topk, float scale,
+                                                                          int workers, long* before, float* parts) {
+  using Wave = PagedWave<T>;
+  __shared__ __attribute__((aligned(1024))) char smem[PAGED_WAVES * STAGES * TILE_BYTES];
+  __shared__ long own[SCAN ? SCAN_MAX + 1 : 1];
+  const long* pre = before;
+  if constexpr (SCAN) {  // few sequences: every block counts for itself, one leaves the counts for the join
+    scan_tiles<Wave::KEYS, PAGED_WAVES * 64>(p, topk, own);
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+      for (int i = threadIdx.x; i <= p.n; i += PAGED_WAVES * 64) before[i] = own[i];
+    pre = own;
+  }
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int G = p.heads / p.cache.kv_heads, groups = (G + 15) / 16, cols = p.cache.kv_heads * groups;
+  const int kh = int(blockIdx.y) / groups, g0 = int(blockIdx.y) % groups * 16;
+  const int col = lane & 15, head = kh * G + g0 + col;
+  const long worker = long(blockIdx.x) * PAGED_WAVES + wave, total = pre[p.n];
+  const long W = min(long(workers), total);  // each has a tile at least
+  if (worker >= W) return;
+  long t = total * worker / W;
+  const long end = total * (worker + 1) / W;
+  const Part part(G);
+  char* ring = smem + wave * STAGES * TILE_BYTES;
+  Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
+  int lo = 0, hi = p.n;  // the sequence that tile t belongs to
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const long first = t;
+  for (int i = uniform(lo); t < end; i = uniform(i + 1)) {
+    const long b0 = pre[i], b1 = pre[i + 1];
+    const long stop = min(end, b1);
+    if (stop <= t) continue;
+    w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
+    w.clear();
+    w.run(i, uniform(int(t - b0)), uniform(int(stop - b0)), scale);
+    w.l = sum_groups(w.l);
+    if (g0 + col < G) {
+      if (t == b0 && stop == b1) {
+        w.store(i, head, w.l);
+      } else {
+        float* at = parts + ((worker * cols + blockIdx.y) * 2 + (t == first ? 0 : 1)) * part.size();
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          *reinterpret_cast<float4*>(at + col * 64 + 16 * d + 4 * (lane >> 4)) = make_float4(w.o[d][0], w.o[d][1], w.o[d][2], w.o[d][3]);
+        if (lane < 16) *reinterpret_cast<float2*>(at + part.ml(col)) = make_float2(w.m, w.some ? w.l : -1.f);
+      }
+    }
+    t = stop;
+  }
+}
+
+// One block a (sequence, head): the parts of a sequence that several waves had. Every wave finds the common
+// reference from all parts' (m, l), then sums every JOIN_WAVES-th part, a channel a lane.
+constexpr int JOIN_WAVES = 8;
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const PagedArgs p, int workers, const long* before, const float* parts) {
+  const int i = blockIdx.x, head = blockIdx.y, G = p.heads / p.cache.kv_heads, groups = (G + 15) / 16, cols = p.cache.kv_heads * groups;
+  const int col = head / G * groups + head % G / 16, g = head % G % 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long b0 = before[i], b1 = before[i + 1], total = before[p.n];
+  T* out = static_cast<T*>(p.out) + i * p.ldo + long(head) * 64;
+  if (b0 == b1) {
+    if (threadIdx.x < 64) out[threadIdx.x] = from_f<T>(0.f);
+    return;
+  }
+  // the last worker that begins at or before tile b: begin(w) = floor(total w / W)
+  const long W = min(long(workers), total);
+  auto holder = [&](long b) { return ((b + 1) * W - 1) / total; };
+  const long w0 = holder(b0), w1 = holder(b1 - 1);
+  if (w0 == w1) return;  // written whole
+  const long count = w1 - w0 + 1;
+  const Part layout(G);
+  auto part = [&](long k) {
+    const long w = w0 + k;
+    return parts + ((w * cols + col) * 2 + (total * w / W >= b0 ? 0 : 1)) * layout.size();
+  };
+  float mx = -INFINITY;
+  int some = 0;
+  for (long k = lane; k < count; k += 64) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(k) + layout.ml(g));
+    if (ml.y < 0.f) continue;  // NaN stays
+    mx = fmaxf(mx, ml.x);
+    some = 1;
+  }
+  for (int d = 1; d < 64; d <<= 1) {
+    mx = fmaxf(mx, __shfl_xor(mx, d));
+    some |= __shfl_xor(some, d);
+  }
+  float acc = 0.f, sum = 0.f;
+#pragma unroll 8
+  for (long k = wave; k < count; k += JOIN_WAVES) {
+    const float* at = part(k);
+    const float2 ml = *reinterpret_cast<const float2*>(at + layout.ml(g));
+    const float o = at[g * 64 + lane];
+    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+    if (ml.y < 0.f) continue;
+    acc += o * f;
+    sum += ml.y * f;
+  }
+  __shared__ float accs[JOIN_WAVES][64], sums[JOIN_WAVES];
+  accs[wave][lane] = acc;
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  if (wave) return;
+  acc = sum = 0.f;
+  for (int k = 0; k < JOIN_WAVES; ++k) {
+    acc += accs[k][lane];
+    sum += sums[k];
+  }
+  out[lane] = from_f<T>(some ? acc / sum : 0.f);
 }
 
 // --- selection of pages -------------------------------------------------------------------------
@@ -454,15 +907,36 @@ void page_bounds(const Exec& ex, const BoundsArgs& args) {
   SPLAT_HIP(hipGetLastError());
 }
 
+// The launches of attention over the cache. topk: 0, or the pages that sel lists.
+void attend(const Exec& ex, const PagedArgs& a, const int* sel, int topk, char* workspace) {
+  const PagedPlan plan = paged_plan(a.cache, a.n, a.heads, a.max_len, topk);
+  const float scale = a.scale * 1.44269504088896341f;  // scores as exponents of 2
+  long* before = reinterpret_cast<long*>(workspace);
+  float* parts = reinterpret_cast<float*>(workspace + plan.before_bytes);
+  by_type(a.cache.dt, [&](auto t) {
+    using T = decltype(t);
+    if (!plan.workers) {
+      paged_whole_kernel<T><<<dim3(a.n, plan.cols), PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale);
+      return;
+    }
+    const dim3 grid(plan.workers / PAGED_WAVES, plan.cols);
+    if (a.n <= SCAN_MAX) {
+      paged_parts_kernel<T, true><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
+    } else {
+      paged_scan_kernel<TileOps<T>::KEYS><<<1, 1024, 0, ex.stream>>>(a, topk, before);
+      paged_parts_kernel<T, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
+    }
+    paged_join_kernel<T><<<dim3(a.n, a.heads), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.workers, before, parts);
+  });
+}
+
 void paged_attention(const Exec& ex, const PagedArgs& args, void* workspace, size_t bytes) {
   PagedArgs a = args;
   check_paged_attention(a, workspace, bytes);
   if (a.n == 0 || ex.dry) return;
   const double keys = double(a.n) * a.max_len;
   ProfScope prof(ex, "paged_attention", 256 * keys * a.heads, 128 * keys * a.cache.kv_heads * dtype_size(a.cache.dt));
-  by_type(a.cache.dt, [&](auto t) {
-    paged_attention_kernel<decltype(t)><<<a.n * a.heads, 64, 0, ex.stream>>>(a, nullptr, 0);
-  });
+  attend(ex, a, nullptr, 0, static_cast<char*>(workspace));
   SPLAT_HIP(hipGetLastError());
 }
 
@@ -475,13 +949,14 @@ void sparse_attention(const Exec& ex, const SparseArgs& args, void* workspace, s
   const double rows = 2.0 * maxp + 2.0 * std::min(s.topk, maxp) * a.cache.page_size;
   ProfScope prof(ex, "sparse_attention", 256.0 * a.n * a.heads * std::min(s.topk, maxp) * a.cache.page_size,
                  pairs * rows * 64 * dtype_size(a.cache.dt));
-  uint64_t* keys = static_cast<uint64_t*>(workspace);
+  char* ws = static_cast<char*>(workspace);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(ws + paged_plan(a.cache, a.n, a.heads, a.max_len, s.topk).bytes);
   by_type(a.cache.dt, [&](auto t) {
     using T = decltype(t);
     page_score_kernel<T><<<pairs, 256, 0, ex.stream>>>(a, static_cast<const T*>(s.bounds), maxp, keys);
     page_select_kernel<<<pairs, 256, 0, ex.stream>>>(keys, maxp, s.topk, s.selected);
-    paged_attention_kernel<T><<<a.n * a.heads, 64, 0, ex.stream>>>(a, s.selected, s.topk);
   });
+  attend(ex, a, s.selected, s.topk, ws);
   SPLAT_HIP(hipGetLastError());
 }
 

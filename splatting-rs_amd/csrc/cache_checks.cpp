@@ -64,7 +64,7 @@ bool meets_pools(const KvCache& c, const void* p, long bytes) {
 // What attention over the cache needs, whichever pages it takes.
 void check_attention(PagedArgs& a) {
   check_cache(a.cache);
-  SPLAT_CHECK(a.n >= 0 && a.heads >= 1 && a.heads <= 65536 && a.heads % a.cache.kv_heads == 0, BAD_ARGUMENT,
+  SPLAT_CHECK(a.n >= 0 && a.heads >= 1 && a.heads <= 32768 && a.heads % a.cache.kv_heads == 0, BAD_ARGUMENT,
               "attention: heads must be a multiple of the cache's kv_heads");
   SPLAT_CHECK(long(a.n) * a.heads <= (1 << 24), BAD_ARGUMENT, "attention: more than 2^24 query rows");
   check_width(a.width, a.cache.page_size);
@@ -180,20 +180,35 @@ void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) 
 namespace {
 void check_workspace_sizes(const KvCache& c, int n, int heads, int max_len) {
   check_sizes(c);
-  SPLAT_CHECK(n >= 0 && max_len >= 0 && heads >= 1 && heads % c.kv_heads == 0 && long(n) * heads <= (1 << 24), BAD_ARGUMENT,
+  SPLAT_CHECK(n >= 0 && max_len >= 0 && heads >= 1 && heads <= 32768 && heads % c.kv_heads == 0 && long(n) * heads <= (1 << 24), BAD_ARGUMENT,
               "workspace: n, heads or max_len");
 }
 }  // namespace
 
+PagedPlan paged_plan(const KvCache& c, int n, int heads, int max_len, int topk) {
+  const int G = heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;  // positions of a tile
+  PagedPlan plan;
+  plan.cols = c.kv_heads * ((G + 15) / 16);
+  const long most = topk ? std::min<long>(max_len, long(topk) * c.page_size) : max_len;
+  if (most <= 1024) return plan;
+  // eight waves on each of 256 CUs, but two tiles at least for each where all sequences are as long as may be
+  const long tiles = n * ((most + keys - 1) / keys);
+  const long workers = std::min<long>(2048 / plan.cols, (tiles + 1) / 2);
+  plan.workers = int(std::max<long>(4, workers / 4 * 4));
+  plan.before_bytes = ((n + 1) * 8L + 15) / 16 * 16;
+  plan.bytes = plan.before_bytes + size_t(plan.workers) * plan.cols * 2 * std::min(G, 16) * PART_HEAD * 4;
+  return plan;
+}
+
 size_t paged_attention_bytes(const KvCache& c, int n, int heads, int max_len) {
   check_workspace_sizes(c, n, heads, max_len);
-  return 0;
+  return paged_plan(c, n, heads, max_len, 0).bytes;
 }
 
 size_t sparse_attention_bytes(const KvCache& c, int n, int heads, int max_len, int topk) {
   check_workspace_sizes(c, n, heads, max_len);
   SPLAT_CHECK(topk >= 1, BAD_ARGUMENT, "sparse attention: topk must be at least 1");
-  return size_t(n) * c.kv_heads * ((long(max_len) + c.page_size - 1) / c.page_size) * 8;
+  return paged_plan(c, n, heads, max_len, topk).bytes + size_t(n) * c.kv_heads * ((long(max_len) + c.page_size - 1) / c.page_size) * 8;
 }
 
 void rope_turns(int rope, double base, double (&freq)[32]) {

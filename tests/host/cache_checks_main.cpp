@@ -236,6 +236,19 @@ int main() {
   P("paged out over q", [](auto& a) { a.out = const_cast<void*>(a.q); });
   P("paged out over cache", [](auto& a) { a.out = a.cache.k; });
 
+  say("paged workspace odd", [] {
+    PagedArgs a = paged();
+    a.max_len = 1 << 20;
+    a.width = 1 << 16;
+    check_paged_attention(a, at(4), size_t(1) << 40);
+  });
+  say("paged workspace small", [] {
+    PagedArgs a = paged();
+    a.max_len = 1 << 20;
+    a.width = 1 << 16;
+    check_paged_attention(a, at(64 * MB), paged_attention_bytes(a.cache, a.n, a.heads, a.max_len) - 1);
+  });
+
   auto S = [&](const char* n, const std::function<void(SparseArgs&)>& f) { on<SparseArgs>(n, sparse(), check_sparse, f); };
   S("sparse ok", [](auto&) {});
   S("sparse ok topk 2^30", [](auto& a) { a.topk = 1 << 20; });
