@@ -785,78 +785,187 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const Paged
 
 // --- selection of pages -------------------------------------------------------------------------
 
-// Scores as whole numbers in the order of the scores, NaN above all; 0: not a page of the sequence.
+// Scores as whole numbers in the order of the scores, NaN above all; 0: no page there.
 __device__ inline uint64_t order_of(double s) {
-  if (s != s) return ~0ull - 1;
+  if (s != s) return ~0ull;
   const uint64_t b = __double_as_longlong(s);
   return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
 
-// One block a (sequence, key head). The most that q k can be for a key between the page's bounds, summed
-// over the group's heads, is sum_c hi_c A_c + lo_c B_c with A and B the sums of the positive and the negative
-// parts of the heads' queries. In 64 bits: a page next to the border is chosen or not by less than 32 bits
-// hold.
+// The most that q k can be for a key between the page's bounds, summed over the group's heads, is
+// sum_c hi_c A_c + lo_c B_c, with A and B the sums of the positive and the negative parts of the heads' queries:
+// 128 products a page, however many heads share it. In 64 bits: which of two pages next to the border is
+// taken can hang on less than 32 bits hold. 16 lanes a page, 8 products each, 16 pages a wave whose loads fly
+// together; bound by its two dependent loads (the table's entry, the bounds).
+constexpr int SCORE_PAGES = 64;  // a block
 template <typename T>
 __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, const T* bounds, int maxp, uint64_t* keys) {
-  __shared__ double A[64], B[64];
   const KvCache& c = p.cache;
-  const int i = blockIdx.x / c.kv_heads, kh = blockIdx.x % c.kv_heads, G = p.heads / c.kv_heads;
-  if (threadIdx.x < 64) {
-    double a = 0, b = 0;
-    for (int g = 0; g < G; ++g) {
-      const double x = to_f<T>(static_cast<const T*>(p.q)[i * p.ldq + (kh * G + g) * 64 + threadIdx.x]);
-      if (x > 0) a += x;
-      else b += x;
-    }
-    A[threadIdx.x] = a;
-    B[threadIdx.x] = b;
+  const int chunks = (maxp + SCORE_PAGES - 1) / SCORE_PAGES, chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks;
+  const int i = pair / c.kv_heads, kh = pair % c.kv_heads, G = p.heads / c.kv_heads;
+  const int lane = threadIdx.x & 63, sub = lane & 15, hi = sub >> 3, j = sub & 7;
+  const int held = int((long(length_of(p.lens[i], p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
+  const int p0 = chunk * SCORE_PAGES + (threadIdx.x >> 6) * 16 + (lane >> 4);
+  if (chunk * SCORE_PAGES >= held) return;
+  int page[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) page[k] = p0 + 4 * k < held ? p.table[long(i) * p.width + p0 + 4 * k] : -1;
+  double cf[8] = {};
+  for (int g = 0; g < G; ++g) {
+    float x[8];
+    load8(static_cast<const T*>(p.q) + i * p.ldq + (long(kh) * G + g) * 64 + j * 8, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cf[e] += (x[e] > 0.f) == (hi != 0) ? double(x[e]) : 0.0;
   }
-  __syncthreads();
-  const int ps = 1 << c.shift;
-  const int len = length_of(p.lens[i], p.width, c.shift, p.max_len);
-  const int held = (len + ps - 1) >> c.shift;
-  for (int j = threadIdx.x; j < maxp; j += 256) {
-    uint64_t key = 0;
-    const int page = j < held ? p.table[long(i) * p.width + j] : -1;
-    if (page_ok(page, c.pages)) {
-      const T* lo = bounds + (long(page) * c.kv_heads + kh) * 128;
-      double s = 0;
-      for (int d = 0; d < 64; ++d) s += double(to_f<T>(lo[d])) * B[d] + double(to_f<T>(lo[64 + d])) * A[d];
-      key = j == held - 1 ? ~0ull : order_of(s);
-    }
-    keys[(long(i) * c.kv_heads + kh) * maxp + j] = key;
+  float v[4][8] = {};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (page_ok(page[k], c.pages)) load8(bounds + (long(page[k]) * c.kv_heads + kh) * 128 + sub * 8, v[k]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    double s = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += double(v[k][e]) * cf[e];
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) s += __shfl_xor(s, m);
+    if (sub == 0 && p0 + 4 * k < held)
+      keys[long(pair) * maxp + p0 + 4 * k] = page_ok(page[k], c.pages) ? order_of(s) : 0;
   }
 }
 
-// The topk largest keys' places in ascending order, the lowest place first among equal keys, -1 behind them.
-__global__ void __launch_bounds__(256) page_select_kernel(const uint64_t* keys, int maxp, int topk, int* sel) {
-  const uint64_t* k = keys + long(blockIdx.x) * maxp;
-  int* out = sel + long(blockIdx.x) * topk;
-  __shared__ int total;
-  if (threadIdx.x == 0) total = 0;
-  __syncthreads();
-  for (int b = 0; b < maxp; b += 256) {
-    const int j = b + threadIdx.x;
-    bool take = false;
-    if (j < maxp && k[j] != 0) {
-      int ahead = 0;
-      for (int o = 0; o < maxp; ++o) ahead += k[o] > k[j] || (k[o] == k[j] && o < j);
-      take = ahead < topk;
-    }
-    __shared__ int flags[256];
-    flags[threadIdx.x] = take;
-    __syncthreads();
-    int at = total, all = 0;
-    for (int o = 0; o < 256; ++o) {
-      if (o < int(threadIdx.x)) at += flags[o];
-      all += flags[o];
-    }
-    if (take) out[at] = j;
-    __syncthreads();
-    if (threadIdx.x == 0) total += all;
-    __syncthreads();
+// Exclusive sum over the block's threads; `total` gets all of it. `room`: one int a wave and one.
+constexpr int SELECT_THREADS = 1024, SELECT_BINS = 2048;
+__device__ inline int scan_block(int v, int* room, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int inc = v;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int o = __shfl_up(inc, m);
+    if (lane >= m) inc += o;
   }
-  for (int a = total + threadIdx.x; a < topk; a += 256) out[a] = -1;
+  __syncthreads();  // the room's last readers
+  if (lane == 63) room[wave] = inc;
+  __syncthreads();
+  int before = inc - v;
+  total = 0;
+#pragma unroll
+  for (int k = 0; k < SELECT_THREADS / 64; ++k) {
+    const int r = room[k];
+    if (k < wave) before += r;
+    total += r;
+  }
+  return before;
+}
+
+// One block a (sequence, key head): the topk largest keys' places, ascending, the lowest place first among equal
+// keys, -1 behind them; the newest page is taken first. The keys that are still undecided lie in [lo, hi]; they
+// are counted into up to 2048 equal bins of that range, the bins above the border's are taken, and its bin is the
+// next range: two rounds for most scores, six at most. Counts do not hang on the order of the atomic adds.
+// Thread t holds keys [t K, (t + 1) K) in registers (K > 0), or reads them every round (K = 0, `k` each).
+template <int K>
+__global__ void __launch_bounds__(SELECT_THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, int maxp, int k,
+                                                                     int topk, int* sel) {
+  __shared__ int bins[SELECT_BINS], room[SELECT_THREADS / 64], found[3];
+  __shared__ uint64_t ends[2][SELECT_THREADS / 64];
+  const KvCache& c = p.cache;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = blockIdx.x / c.kv_heads;
+  const int held = int((long(length_of(p.lens[i], p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
+  const uint64_t* in = keys + long(blockIdx.x) * maxp;
+  int* out = sel + long(blockIdx.x) * topk;
+  if (K > 0) k = K;
+  uint64_t mine[K > 0 ? K : 1];
+  if constexpr (K > 0) {
+#pragma unroll
+    for (int e = 0; e < K; ++e) mine[e] = tid * K + e < held ? in[tid * K + e] : 0;
+  }
+  auto each = [&](auto&& fn) {
+    if constexpr (K > 0) {
+#pragma unroll
+      for (int e = 0; e < K; ++e) fn(tid * K + e, mine[e]);
+    } else {
+      for (int e = 0; e < k; ++e) {
+        const long at = long(tid) * k + e;
+        if (at < held) fn(int(at), in[at]);
+      }
+    }
+  };
+  // the newest page aside: how many there are, and their range
+  const int newest = held - 1;
+  uint64_t lo = ~0ull, hi = 0;
+  int mycount = 0, there, first = 0;
+  each([&](int at, uint64_t key) {
+    if (key == 0) return;
+    if (at == newest) {
+      first = 1;
+      return;
+    }
+    ++mycount;
+    lo = min(lo, key);
+    hi = max(hi, key);
+  });
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    lo = min(lo, uint64_t(__shfl_xor((unsigned long long)lo, m)));
+    hi = max(hi, uint64_t(__shfl_xor((unsigned long long)hi, m)));
+  }
+  if (lane == 0) {
+    ends[0][wave] = lo;
+    ends[1][wave] = hi;
+  }
+  scan_block(mycount, room, there);
+#pragma unroll
+  for (int w = 0; w < SELECT_THREADS / 64; ++w) {
+    lo = min(lo, ends[0][w]);
+    hi = max(hi, ends[1][w]);
+  }
+  const bool newest_there = __syncthreads_or(first);
+  int need = min(topk - int(newest_there), there), inside = there;  // to take from [lo, hi], and how many lie in it
+  while (need < inside && need > 0 && lo < hi) {
+    const int shift = max(0, 53 - __clzll(hi - lo));  // (hi - lo) >> shift < 2048
+    for (int b = tid; b < SELECT_BINS; b += SELECT_THREADS) bins[b] = 0;
+    __syncthreads();
+    each([&](int at, uint64_t key) {
+      if (key >= lo && key <= hi && at != newest) atomicAdd(&bins[int((key - lo) >> shift)], 1);
+    });
+    __syncthreads();
+    // thread t has the t-th pair of bins from above
+    const int b1 = bins[SELECT_BINS - 1 - 2 * tid], b0 = bins[SELECT_BINS - 2 - 2 * tid];
+    int all;
+    const int above = scan_block(b1 + b0, room, all);
+    if (above < need && need <= above + b1 + b0) {
+      const bool up = need <= above + b1;
+      found[0] = SELECT_BINS - 1 - 2 * tid - (up ? 0 : 1);
+      found[1] = up ? above : above + b1;
+      found[2] = up ? b1 : b0;
+    }
+    __syncthreads();
+    need -= found[1];
+    inside = found[2];
+    const uint64_t at = lo + (uint64_t(found[0]) << shift);
+    const uint64_t last = (1ull << shift) - 1;
+    if (hi - at > last) hi = at + last;
+    lo = at;
+    __syncthreads();  // found and bins are written again
+  }
+  // taken: the newest, what lies above the range, and of the range all or (equal keys) the first `need`
+  const bool all = need == inside;
+  int equal = 0, eq_total;
+  if (!all && need > 0) each([&](int at, uint64_t key) { equal += key >= lo && key <= hi && at != newest; });
+  int eq_before = scan_block(equal, room, eq_total);
+  auto takes = [&](int at, uint64_t key, int& eq) {
+    if (key == 0) return false;
+    if (at == newest || key > hi) return true;
+    if (key < lo || need == 0) return false;
+    return all || eq++ < need;
+  };
+  int count = 0, total, eq = eq_before;
+  each([&](int at, uint64_t key) { count += takes(at, key, eq); });
+  int to = scan_block(count, room, total);
+  eq = eq_before;
+  each([&](int at, uint64_t key) {
+    if (takes(at, key, eq)) out[to++] = at;
+  });
+  for (int e = total + tid; e < topk; e += SELECT_THREADS) out[e] = -1;
 }
 
 // Runs fn with the storage type dt as a value.
@@ -953,9 +1062,15 @@ void sparse_attention(const Exec& ex, const SparseArgs& args, void* workspace, s
   uint64_t* keys = reinterpret_cast<uint64_t*>(ws + paged_plan(a.cache, a.n, a.heads, a.max_len, s.topk).bytes);
   by_type(a.cache.dt, [&](auto t) {
     using T = decltype(t);
-    page_score_kernel<T><<<pairs, 256, 0, ex.stream>>>(a, static_cast<const T*>(s.bounds), maxp, keys);
-    page_select_kernel<<<pairs, 256, 0, ex.stream>>>(keys, maxp, s.topk, s.selected);
+    if (maxp > 0)
+      page_score_kernel<T><<<pairs * cdiv(maxp, SCORE_PAGES), 256, 0, ex.stream>>>(a, static_cast<const T*>(s.bounds), maxp, keys);
   });
+  const int each = cdiv(maxp, SELECT_THREADS);
+  auto select = [&](auto kernel) { kernel<<<pairs, SELECT_THREADS, 0, ex.stream>>>(a, keys, maxp, each, s.topk, s.selected); };
+  if (each <= 1) select(page_select_kernel<1>);
+  else if (each <= 4) select(page_select_kernel<4>);
+  else if (each <= 16) select(page_select_kernel<16>);
+  else select(page_select_kernel<0>);
   attend(ex, a, s.selected, s.topk, ws);
   SPLAT_HIP(hipGetLastError());
 }

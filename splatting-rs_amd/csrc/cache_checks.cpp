@@ -174,6 +174,8 @@ void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) 
               "sparse attention: a required pointer is NULL, or bounds not 16-byte aligned");
   SPLAT_CHECK(!meets_pools(a.at.cache, a.selected, 4L * a.at.n * a.at.cache.kv_heads * a.topk), BAD_ARGUMENT,
               "sparse attention: selected overlaps the cache");
+  SPLAT_CHECK(long(a.at.n) * a.at.cache.kv_heads * ((long(a.at.max_len) + a.at.cache.page_size - 1) / a.at.cache.page_size + 63) < (1L << 37),
+              BAD_ARGUMENT, "sparse attention: more than 2^37 pages and heads");
   check_workspace(workspace, bytes, sparse_attention_bytes(a.at.cache, a.at.n, a.at.heads, a.at.max_len, a.topk));
 }
 
