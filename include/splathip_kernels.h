@@ -146,7 +146,7 @@ typedef enum splat_table_status {
  * the first new token of each request and their number; slots [cap] and positions [cap] (NULL: not wanted) of the new
  * tokens, requests in order, -1 and 0 behind the last; *used_out = pages taken now. lens may be past and used_out
  * used; other outputs overlap nothing. If *status is not SPLAT_TABLE_OK nothing was taken: the table, lens and
- * used stay, starts are 0 and slots -1. An entry of the pool or table below 0 gives slots of -1. n up to 2^20. */
+ * used stay, starts are 0 and slots -1. An entry of the pool or table below 0 gives slots of -1. n up to 65536. */
 int splat_kernel_block_tables(splat_ctx* ctx, int n, const int32_t* past, const int32_t* add, int page_size,
                               const int32_t* pool, int pool_size, const int32_t* used, int32_t* table, int width,
                               int32_t* lens, int32_t* starts, int32_t* slots, int32_t* positions, int cap,
@@ -155,8 +155,8 @@ int splat_kernel_block_tables(splat_ctx* ctx, int n, const int32_t* past, const 
 /* Norms of the queries' and keys' heads and the position rotation in one pass over qkv [tokens, (heads + 2 *
  * kv_heads) * 64] (q | k | v, row stride ld) in `dtype`; statistics and angles in fp32 or more, rounded once.
  * norm: per head over its 64 channels, SPLAT_NORM_LAYER (x - mean) / sqrt(var + eps) * w + b (biased variance) or
- * SPLAT_NORM_RMS x / sqrt(mean(x^2) + eps) * w + b, with w and b fp32 [64] (qw, qb for queries, kw, kb for keys; NULL:
- * left out). rope: SPLAT_ROPE_LINE turns channels (c, c + 32) by positions[t] * rope_base^(-c / 32); SPLAT_ROPE_GRID
+ * SPLAT_NORM_RMS x / sqrt(mean(x^2) + eps) * w + b, with w and b fp32 [64] (qw, qb for queries, kw, kb for keys, 16-byte
+ * aligned; NULL: left out). rope: SPLAT_ROPE_LINE turns channels (c, c + 32) by positions[t] * rope_base^(-c / 32); SPLAT_ROPE_GRID
  * turns (c, c + 16) of channels 0-31 by positions[t][0] and of channels 32-63 by positions[t][1], times
  * rope_base^(-c / 16) (depthanything3-rs/src/rope.rs:57-73, with base 100). q_out [tokens, heads * 64] and k_out
  * [tokens, kv_heads * 64] (NULL: not wanted) have row strides ldq and ldk; they may be qkv's own q and k blocks, and

@@ -14,11 +14,59 @@ namespace splat {
 
 namespace {
 
-// Sum over the 8 lanes of a head row; every lane gets it.
-__device__ inline float sum8(float v) {
-#pragma unroll
-  for (int m = 1; m < 8; m <<= 1) v += __shfl_xor(v, m);
-  return v;
+// The value of the lane that CTRL names (a DPP control), `old` in the rows that ROWS leaves out and for lanes without one.
+template <int CTRL, int ROWS> __device__ inline int from_lane(int old, int v) {
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> __device__ inline uint64_t from_lane(uint64_t old, uint64_t v) {
+  const uint32_t l = from_lane<CTRL, ROWS>(int(uint32_t(old)), int(uint32_t(v))), h = from_lane<CTRL, ROWS>(int(old >> 32), int(v >> 32));
+  return uint64_t(h) << 32 | l;
+}
+template <int CTRL, int ROWS> __device__ inline float from_lane(float old, float v) {
+  return __int_as_float(from_lane<CTRL, ROWS>(__float_as_int(old), __float_as_int(v)));
+}
+template <int CTRL, int ROWS> __device__ inline double from_lane(double old, double v) {
+  return __longlong_as_double(from_lane<CTRL, ROWS>(uint64_t(__double_as_longlong(old)), uint64_t(__double_as_longlong(v))));
+}
+// Combines every lane with those before it: 1, 2, 4 and 8 to the left in its row of 16, then the rows'
+// last lanes (0x142 and 0x143 hand lane 15 of a row and lane 31 on). Lane 63 ends with all 64.
+template <typename V, typename F> __device__ inline V scan_wave(V v, V none, F&& fn) {
+  v = fn(v, from_lane<0x111, 0xf>(none, v));
+  v = fn(v, from_lane<0x112, 0xf>(none, v));
+  v = fn(v, from_lane<0x114, 0xf>(none, v));
+  v = fn(v, from_lane<0x118, 0xf>(none, v));
+  v = fn(v, from_lane<0x142, 0xa>(none, v));
+  return fn(v, from_lane<0x143, 0xc>(none, v));
+}
+__device__ inline int sum_wave(int v) {
+  return scan_wave(v, 0, [](int a, int b) { return a + b; });
+}
+
+// Sum over the 8 lanes of a head row; every lane gets it (lanes l ^ 1, l ^ 2, then the other quad's mirror).
+template <typename V> __device__ inline V sum8(V v) {
+  v += from_lane<0xB1, 0xf>(v, v);
+  v += from_lane<0x4E, 0xf>(v, v);
+  return v + from_lane<0x141, 0xf>(v, v);
+}
+
+// A wave-uniform load of memory that the launch only reads.
+__device__ inline int uload(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// a / b for a, b >= 0, in 32 bits where they fit: the 64-bit division is a hundred instructions.
+__device__ inline long quotient(long a, long b) {
+  return (uint64_t(a) | uint64_t(b)) >> 32 ? a / b : long(uint32_t(a) / uint32_t(b));
+}
+
+// fn over lanes l, l ^ 16, l ^ 32, l ^ 48 (over_rows) and l, l ^ 8, ... (over_halves, then over_rows).
+template <typename F> __device__ inline float over_rows(float v, F&& fn) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fn(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fn(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+template <typename F> __device__ inline float over_halves(float v, F&& fn) {
+  return over_rows(fn(v, from_lane<0x128, 0xf>(v, v)), fn);
 }
 
 // 8 consecutive channels.
@@ -47,93 +95,90 @@ template <> __device__ inline void store8<float>(float* p, const float (&x)[8]) 
 
 // --- block tables and slot maps -----------------------------------------------------------------
 
-constexpr int TABLE_THREADS = 1024;
-
 // Request i holds past[i] positions in ceil(past / ps) pages; its add[i] new ones take the next pages of
 // the pool, requests in order. Every block sums the requests up again (thread t its k of them, then one scan
 // over the threads), so that a token finds its request and its page without a pass before: a binary search
-// over the threads' sums, then a walk over at most k requests. A new page begins with a new token, whose
-// thread writes the table's entry.
+// over the threads' sums for four tokens at a time, then a walk over at most k requests. A new page begins with
+// a new token, whose thread writes the table's entry.
 // The call takes effect whole or not at all: the status is known before anything is written.
 // FILL writes the table, slots and positions, COMMIT lens, starts, used and status, which may lie over
 // past and used: with several blocks it runs as a second launch.
-template <bool FILL, bool COMMIT>
-__global__ void __launch_bounds__(TABLE_THREADS) block_tables_kernel(const BlockTableArgs p) {
-  __shared__ long tok[TABLE_THREADS + 1], pag[TABLE_THREADS + 1];
-  __shared__ long wtok[16], wpag[16];
-  __shared__ int bad_any;
-  const int tid = threadIdx.x, k = (p.n + TABLE_THREADS - 1) / TABLE_THREADS;
+template <int THREADS, bool FILL, bool COMMIT>
+__global__ void __launch_bounds__(THREADS) block_tables_kernel(const BlockTableArgs p, bool vec) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ long tok[THREADS], pag[THREADS], wtok[WAVES], wpag[WAVES];
+  const int tid = threadIdx.x, k = (p.n + THREADS - 1) / THREADS;
   const int i0 = int(min(long(tid) * k, long(p.n))), i1 = int(min(long(i0) + k, long(p.n)));
   const int ps = 1 << p.shift;
   const long most = long(p.width) << p.shift;
-  if (tid == 0) bad_any = 0;
   const int used = *p.used;
   long nt = 0, np = 0;
-  bool bad = false;
+  bool bad = used < 0 || used > p.pool_size;
   for (int i = i0; i < i1; ++i) {
     const long a = p.past[i], d = p.add[i];
     bad |= a < 0 || d < 0 || a + d > most;
     nt += d;
     np += ((a + d + ps - 1) >> p.shift) - ((a + ps - 1) >> p.shift);
   }
-  __syncthreads();
-  if (bad) bad_any = 1;
-  long st = nt, sp = np;  // inclusive scan over the wave, then over the waves
+  const auto plus = [](uint64_t a, uint64_t b) { return a + b; };
+  const long st = long(scan_wave(uint64_t(nt), uint64_t(0), plus)), sp = long(scan_wave(uint64_t(np), uint64_t(0), plus));
   const int lane = tid & 63, wave = tid >> 6;
-  for (int m = 1; m < 64; m <<= 1) {
-    const long ot = __shfl_up(st, m), op = __shfl_up(sp, m);
-    if (lane >= m) { st += ot; sp += op; }
-  }
   if (lane == 63) { wtok[wave] = st; wpag[wave] = sp; }
-  __syncthreads();
-  long bt = 0, bp = 0, total = 0, pages = 0;
-  for (int w = 0; w < 16; ++w) {
-    if (w < wave) { bt += wtok[w]; bp += wpag[w]; }
+  const bool broken = __syncthreads_or(bad);
+  long et = st - nt, ep = sp - np, total = 0, pages = 0;  // exclusive sums and all
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) { et += wtok[w]; ep += wpag[w]; }
     total += wtok[w];
     pages += wpag[w];
   }
-  const long et = bt + st - nt, ep = bp + sp - np;  // exclusive
-  tok[tid] = et;
-  pag[tid] = ep;
-  const bool broken = bad_any != 0 || used < 0 || used > p.pool_size;
   const int status = broken ? TABLE_BAD_LENGTH : pages > long(p.pool_size) - used ? TABLE_POOL_EMPTY
                      : total > p.cap ? TABLE_SLOTS_FULL : TABLE_OK;
-  __syncthreads();
   if constexpr (FILL) {
+    tok[tid] = et;
+    pag[tid] = ep;
+    __syncthreads();
     const long count = status == TABLE_OK ? total : 0;
-    for (long t = long(blockIdx.x) * TABLE_THREADS + tid; t < p.cap; t += long(gridDim.x) * TABLE_THREADS) {
-      int slot = -1, pos = 0;
+    for (long t = (long(blockIdx.x) * THREADS + tid) * 4; t < p.cap; t += long(gridDim.x) * THREADS * 4) {
+      int slot[4] = {-1, -1, -1, -1}, pos[4] = {};
       if (t < count) {
-        int lo = 0, hi = TABLE_THREADS;  // the last thread whose sum is at most t
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (tok[mid] <= t) lo = mid;
-          else hi = mid;
-        }
+        int lo = 0;  // the last thread whose sum is at most t
+#pragma unroll
+        for (int half = THREADS / 2; half; half >>= 1)
+          if (tok[lo + half] <= t) lo += half;
         long r = t - tok[lo], pg = pag[lo];
-        int i = int(min(long(lo) * k, long(p.n)));
-        int a = p.past[i], d = p.add[i];
-        while (r >= d) {  // ends: the thread's requests hold more than r tokens
-          r -= d;
-          pg += ((long(a) + d + ps - 1) >> p.shift) - ((long(a) + ps - 1) >> p.shift);
-          ++i;
-          a = p.past[i];
-          d = p.add[i];
+        int i = lo * k, a = p.past[i], d = p.add[i], held = -1, page = -1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u, ++r) {
+          if (t + u >= count) break;
+          while (r >= d) {  // ends: token t + u belongs to a request
+            r -= d;
+            pg += ((long(a) + d + ps - 1) >> p.shift) - ((long(a) + ps - 1) >> p.shift);
+            ++i;
+            a = p.past[i];
+            d = p.add[i];
+            held = -1;
+          }
+          pos[u] = a + int(r);
+          const int j = pos[u] >> p.shift, have = int((long(a) + ps - 1) >> p.shift);
+          if (j != held) {
+            held = j;
+            page = j < have ? p.table[long(i) * p.width + j] : p.pool[used + pg + (j - have)];
+          }
+          if (j >= have && (pos[u] & (ps - 1)) == 0) p.table[long(i) * p.width + j] = page;
+          const long s = (long(page) << p.shift) + (pos[u] & (ps - 1));
+          slot[u] = page < 0 || s > 0x7fffffffL ? -1 : int(s);
         }
-        pos = a + int(r);
-        const int j = pos >> p.shift, have = int((long(a) + ps - 1) >> p.shift);
-        int page;
-        if (j < have) {
-          page = p.table[long(i) * p.width + j];
-        } else {
-          page = p.pool[used + pg + (j - have)];
-          if ((pos & (ps - 1)) == 0) p.table[long(i) * p.width + j] = page;
-        }
-        const long s = (long(page) << p.shift) + (pos & (ps - 1));
-        slot = page < 0 || s > 0x7fffffffL ? -1 : int(s);
       }
-      p.slots[t] = slot;
-      if (p.positions) p.positions[t] = pos;
+      if (vec && t + 4 <= p.cap) {
+        *reinterpret_cast<int4*>(p.slots + t) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        if (p.positions) *reinterpret_cast<int4*>(p.positions + t) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        continue;
+      }
+      for (int u = 0; u < 4 && t + u < p.cap; ++u) {
+        p.slots[t + u] = slot[u];
+        if (p.positions) p.positions[t + u] = pos[u];
+      }
     }
   }
   if constexpr (COMMIT) {
@@ -155,118 +200,169 @@ __global__ void __launch_bounds__(TABLE_THREADS) block_tables_kernel(const Block
 
 // --- norms of queries and keys with the rotation ------------------------------------------------
 
-// One wave a token: 8 lanes hold a head row (8 channels each), 8 rows at a time. Lane l < 32 takes
-// frequency l's angle once for all heads, in 64 bits up to the fraction of a turn.
-template <typename T>
+// 4 consecutive channels, as they lie in memory and as floats.
+template <typename T> struct Quad {
+  using Raw = uint2;
+  __device__ static inline void get(const uint2& w, float* x) {
+    x[0] = u16f<T>(w.x);
+    x[1] = u16f<T>(w.x >> 16);
+    x[2] = u16f<T>(w.y);
+    x[3] = u16f<T>(w.y >> 16);
+  }
+  __device__ static inline uint2 put(const float* x) { return make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])); }
+};
+template <> struct Quad<float> {
+  using Raw = float4;
+  __device__ static inline void get(const float4& w, float* x) { x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w; }
+  __device__ static inline float4 put(const float* x) { return make_float4(x[0], x[1], x[2], x[3]); }
+};
+
+// A wave takes one token and up to IT steps of 8 head rows, 8 lanes a row; a step's rows are all queries, keys
+// or values. A lane holds the two quads of channels that turn together, (c, c + 32) on a line and (c, c + 16)
+// in each half on a grid, so that no value crosses lanes but in the sums. Lane l < 32 takes frequency l's angle
+// once for all heads, in 64 bits up to the fraction of a turn; all loads are under way before it.
+template <typename T, int IT, int ROPE>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs p) {
-  __shared__ float2 turn[4][32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long t = long(blockIdx.x) * 4 + wave;
+  using Raw = typename Quad<T>::Raw;
+  __shared__ __attribute__((aligned(16))) float turn[4][2][32];  // cosines, sines
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), j = lane & 7, in_step = lane >> 3;
+  const int t = blockIdx.x * 4 + wave;
   if (t >= p.tokens) return;
-  const int j = lane & 7;
-  if (p.rope != ROPE_NONE) {
+  constexpr int SPAN = ROPE == ROPE_GRID ? 16 : 32;
+  const int c0 = ROPE == ROPE_GRID ? (j >> 2) * 32 + (j & 3) * 4 : j * 4;
+  const int nq = (p.heads + 7) >> 3, nk = (p.kv_heads + 7) >> 3, steps = nq + (p.slots ? 2 : 1) * nk, s0 = blockIdx.y * IT;
+  // the step's kind (0 queries, 1 keys, 2 values) and this lane's head
+  auto kind_of = [&](int s) { return s < nq ? 0 : s < nq + nk ? 1 : 2; };
+  auto head_of = [&](int s, int kind) { return (kind == 0 ? s : kind == 1 ? s - nq : s - nq - nk) * 8 + in_step; };
+  auto heads_of = [&](int kind) { return kind == 0 ? p.heads : p.kv_heads; };
+  Raw raw[IT][2];
+  const T* row = static_cast<const T*>(p.qkv) + t * p.ld + c0;
+#pragma unroll
+  for (int s = 0; s < IT; ++s) {
+    if (s0 + s >= steps) break;
+    const int kind = kind_of(s0 + s), h = head_of(s0 + s, kind);
+    if (h >= heads_of(kind)) continue;
+    const T* at = row + ((kind == 0 ? 0 : kind == 1 ? p.heads : p.heads + p.kv_heads) + h) * 64L;
+    raw[s][0] = *reinterpret_cast<const Raw*>(at);
+    raw[s][1] = *reinterpret_cast<const Raw*>(at + SPAN);
+  }
+  const int slot = p.slots ? uload(p.slots + t) : -1;
+  const bool cached = p.slots && slot_ok(slot, p.cache);
+  float cs[4], sn[4];
+  if constexpr (ROPE != ROPE_NONE) {
     if (lane < 32) {
-      const int pos = p.rope == ROPE_LINE ? p.positions[t] : p.positions[2 * t + (lane >> 4)];
-      const double x = double(pos) * p.freq[p.rope == ROPE_LINE ? lane : lane & 15];
+      const int pos = ROPE == ROPE_LINE ? p.positions[t] : p.positions[2L * t + (lane >> 4)];
+      const double x = double(pos) * p.freq[ROPE == ROPE_LINE ? lane : lane & 15];
       float s, c;
       sincospif(float(2.0 * (x - rint(x))), &s, &c);
-      turn[wave][lane] = make_float2(c, s);
+      turn[wave][0][lane] = c;
+      turn[wave][1][lane] = s;
     }
-    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_wave_barrier();  // the wave's own rows: its LDS operations stay in order
+    *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(&turn[wave][0][4 * j]);
+    *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(&turn[wave][1][4 * j]);
   }
-  const int slot = p.slots ? p.slots[t] : -1;
-  const bool cached = p.slots && slot_ok(slot, p.cache);
-  const int R = p.heads + (p.slots ? 2 : 1) * p.kv_heads;
-  for (int r0 = 0; r0 < R; r0 += 8) {
-    const int r = r0 + (lane >> 3);
-    const bool in = r < R;
-    float x[8] = {};
-    if (in) load8(static_cast<const T*>(p.qkv) + t * p.ld + r * 64 + j * 8, x);
-    const bool isq = r < p.heads, isk = !isq && r < p.heads + p.kv_heads;
-    if (isq || isk) {
-      const float* w = isq ? p.qw : p.kw;
-      const float* b = isq ? p.qb : p.kb;
+#pragma unroll
+  for (int s = 0; s < IT; ++s) {
+    if (s0 + s >= steps) break;
+    const int kind = kind_of(s0 + s), h = head_of(s0 + s, kind);
+    if (kind < 2) {
+      float x[8];
+      Quad<T>::get(raw[s][0], x);
+      Quad<T>::get(raw[s][1], x + 4);
       if (p.norm != NORM_NONE) {
-        float m = 0.f, v = 0.f;
         if (p.norm == NORM_LAYER) {
+          const float m = sum8(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) * (1.f / 64.f);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) m += x[e];
-          m = sum8(m) * (1.f / 64.f);
+          for (int e = 0; e < 8; ++e) x[e] -= m;
         }
+        float v = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { x[e] -= m; v += x[e] * x[e]; }
-        const float s = 1.f / sqrtf(sum8(v) * (1.f / 64.f) + p.eps);
+        for (int e = 0; e < 8; ++e) v += x[e] * x[e];
+        const float r = 1.f / sqrtf(sum8(v) * (1.f / 64.f) + p.eps);
+        const float* w = kind == 0 ? p.qw : p.kw;
+        const float* b = kind == 0 ? p.qb : p.kb;
+        float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] *= s;
-          if (w) x[e] *= w[j * 8 + e];
-          if (b) x[e] += b[j * 8 + e];
+        for (int e = 0; e < 8; ++e) x[e] *= r;
+        if (w) {
+          *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(w + c0);
+          *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(w + c0 + SPAN);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= f[e];
+        }
+        if (b) {
+          *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(b + c0);
+          *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(b + c0 + SPAN);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] += f[e];
         }
       }
-      if (p.rope != ROPE_NONE) {
-        const int span = p.rope == ROPE_LINE ? 4 : 2;  // the partner's lane, and this lane's first frequency
-        const int f0 = p.rope == ROPE_LINE ? (j & 3) * 8 : (j >> 2) * 16 + (j & 1) * 8;
-        const float sign = (j & span) ? 1.f : -1.f;
+      if constexpr (ROPE != ROPE_NONE) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 cs = turn[wave][f0 + e];
-          const float o = __shfl_xor(x[e], span);
-          x[e] = x[e] * cs.x + sign * o * cs.y;
+        for (int e = 0; e < 4; ++e) {
+          const float a = x[e], b = x[e + 4];
+          x[e] = a * cs[e] - b * sn[e];
+          x[e + 4] = b * cs[e] + a * sn[e];
         }
       }
+      raw[s][0] = Quad<T>::put(x);
+      raw[s][1] = Quad<T>::put(x + 4);
     }
-    if (!in) continue;
-    if (isq) {
-      store8(static_cast<T*>(p.q_out) + t * p.ldq + r * 64 + j * 8, x);
-      continue;
-    }
-    const int h = isk ? r - p.heads : r - p.heads - p.kv_heads;
-    if (isk && p.k_out) store8(static_cast<T*>(p.k_out) + t * p.ldk + h * 64 + j * 8, x);
-    if (cached) {
-      store8(static_cast<T*>(isk ? p.cache.k : p.cache.v) + slot_at(p.cache, slot, h) + j * 8, x);
-    }
+    if (h >= heads_of(kind)) continue;
+    auto put = [&](T* at) {
+      *reinterpret_cast<Raw*>(at) = raw[s][0];
+      *reinterpret_cast<Raw*>(at + SPAN) = raw[s][1];
+    };
+    if (kind == 0) put(static_cast<T*>(p.q_out) + t * p.ldq + h * 64L + c0);
+    if (kind == 1 && p.k_out) put(static_cast<T*>(p.k_out) + t * p.ldk + h * 64L + c0);
+    if (kind && cached) put(static_cast<T*>(kind == 1 ? p.cache.k : p.cache.v) + slot_at(p.cache, slot, h) + c0);
   }
 }
 
 // --- key bounds per page ------------------------------------------------------------------------
 
 // NaN in either operand gives NaN.
-__device__ inline float low(float a, float b) { return b < a || b != b ? b : a; }
-__device__ inline float high(float a, float b) { return b > a || b != b ? b : a; }
+__device__ inline float low(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ inline float high(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// One wave a (sequence, page, head), 8 lanes a row, 8 rows at a time.
+// One wave a (sequence, page, head), 8 lanes a row, 8 rows a load, 8 loads under way.
 template <typename T>
 __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs p) {
   const KvCache& c = p.cache;
-  const long unit = long(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const long unit = long(blockIdx.x) * 4 + uniform(threadIdx.x >> 6);
   if (unit >= long(p.n) * p.per_seq * c.kv_heads) return;
   const int lane = threadIdx.x & 63, j = lane & 7, ps = 1 << c.shift;
-  const int h = int(unit % c.kv_heads), first = int(unit / c.kv_heads % p.per_seq), i = int(unit / c.kv_heads / p.per_seq);
-  const int len = length_of(p.lens[i], p.width, c.shift, 0x7fffffff);
-  const int fresh = p.add ? min(max(p.add[i], 0), len) : len;
+  const uint32_t of_seq = uint32_t(p.per_seq) * c.kv_heads;
+  const int i = int(quotient(unit, of_seq)), rest = int(unit - long(i) * of_seq), h = rest % c.kv_heads, first = rest / c.kv_heads;
+  const int len = length_of(uload(p.lens + i), p.width, c.shift, 0x7fffffff);
+  const int fresh = p.add ? min(max(uload(p.add + i), 0), len) : len;
   if (fresh == 0) return;
-  const int last = (len + ps - 1) >> c.shift;
+  const int last = int((long(len) + ps - 1) >> c.shift);
   for (int g = ((len - fresh) >> c.shift) + first; g < last; g += p.per_seq) {
-    const int page = p.table[long(i) * p.width + g];
+    const int page = uload(p.table + long(i) * p.width + g);
     if (!page_ok(page, c.pages)) continue;
     const int rows = min(ps, len - (g << c.shift));
     const T* k = static_cast<const T*>(c.k) + page_at(c, page, h) + j * 8;
     float lo[8], hi[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
-    for (int r = lane >> 3; r < rows; r += 8) {
-      float x[8];
-      load8(k + r * 64, x);
+    for (int r0 = lane >> 3; r0 < rows; r0 += 64) {
+      float x[8][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { lo[e] = low(lo[e], x[e]); hi[e] = high(hi[e], x[e]); }
+      for (int u = 0; u < 8; ++u)
+        if (8 * u < rows) load8(k + min(r0 + 8 * u, rows - 1) * 64, x[u]);  // the last row again changes nothing
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (8 * u < rows)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) { lo[e] = low(lo[e], x[u][e]); hi[e] = high(hi[e], x[u][e]); }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-#pragma unroll
-      for (int m = 8; m < 64; m <<= 1) {
-        lo[e] = low(lo[e], __shfl_xor(lo[e], m));
-        hi[e] = high(hi[e], __shfl_xor(hi[e], m));
-      }
+    for (int e = 0; e < 8; ++e) {
+      lo[e] = over_halves(lo[e], low);
+      hi[e] = over_halves(hi[e], high);
+    }
     T* out = static_cast<T*>(p.bounds) + (long(page) * c.kv_heads + h) * 128 + j * 8;
     if (lane < 8) store8(out, lo);
     else if (lane < 16) store8(out + 64, hi);
@@ -291,10 +387,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int int32x4_v __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(3))) char* lds_cptr;
 
-// A wave-uniform load of memory that the launch only reads.
-__device__ inline int uload(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
-__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
 // 16 bytes a lane from `base + off` into LDS at lds + 16 * lane; offsets from `bytes` on read as zeros.
 __device__ inline void load_lds(const void* base, uint32_t bytes, uint32_t off, uint32_t lds) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
@@ -304,20 +396,8 @@ __device__ inline void load_lds(const void* base, uint32_t bytes, uint32_t off, 
 }
 template <int N> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// Maximum (sum) over lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ inline float max_groups(float v) {
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ inline float sum_groups(float v) {
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
+__device__ inline float max_groups(float v) { return over_rows(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ inline float sum_groups(float v) { return over_rows(v, [](float a, float b) { return a + b; }); }
 // The two products on a tile in LDS. KEYS keys in T16 groups of 16; PIECE rows to a load.
 template <typename T> struct TileOps {  // bf16, f16: rows of 128 bytes
   static constexpr int KEYS = 32, T16 = 2, PIECE = 8;
@@ -687,8 +767,8 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
   const long worker = long(blockIdx.x) * PAGED_WAVES + wave, total = pre[p.n];
   const long W = min(long(workers), total);  // each has a tile at least
   if (worker >= W) return;
-  long t = total * worker / W;
-  const long end = total * (worker + 1) / W;
+  long t = quotient(total * worker, W);
+  const long end = quotient(total * (worker + 1), W);
   const Part part(G);
   char* ring = smem + wave * STAGES * TILE_BYTES;
   Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
@@ -722,65 +802,91 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
   }
 }
 
-// One block a (sequence, head): the parts of a sequence that several waves had. Every wave finds the common
-// reference from all parts' (m, l), then sums every JOIN_WAVES-th part, a channel a lane.
-constexpr int JOIN_WAVES = 8;
+// One block a (sequence, group of heads): the parts of a sequence that several waves had. SPLIT waves share a head
+// (all eight where the group has one), each with every SPLIT-th part, a channel a lane, JOIN_PARTS parts under way.
+// Bound by its chain of loads (counts, then parts), not by their bytes.
+constexpr int JOIN_WAVES = 8, JOIN_PARTS = 12;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const PagedArgs p, int workers, const long* before, const float* parts) {
-  const int i = blockIdx.x, head = blockIdx.y, G = p.heads / p.cache.kv_heads, groups = (G + 15) / 16, cols = p.cache.kv_heads * groups;
-  const int col = head / G * groups + head % G / 16, g = head % G % 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float accs[JOIN_WAVES][64], sums[JOIN_WAVES], refs[JOIN_WAVES];
+  __shared__ int somes[JOIN_WAVES];
+  const int i = blockIdx.x, col = blockIdx.y, G = p.heads / p.cache.kv_heads, groups = (G + 15) / 16, cols = p.cache.kv_heads * groups;
+  const int head0 = col / groups * G + col % groups * 16, heads = min(16, G - col % groups * 16);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const long b0 = before[i], b1 = before[i + 1], total = before[p.n];
-  T* out = static_cast<T*>(p.out) + i * p.ldo + long(head) * 64;
+  T* out = static_cast<T*>(p.out) + i * p.ldo + long(head0) * 64;
   if (b0 == b1) {
-    if (threadIdx.x < 64) out[threadIdx.x] = from_f<T>(0.f);
+    for (int e = threadIdx.x; e < heads * 64; e += JOIN_WAVES * 64) out[e] = from_f<T>(0.f);
     return;
   }
   // the last worker that begins at or before tile b: begin(w) = floor(total w / W)
   const long W = min(long(workers), total);
-  auto holder = [&](long b) { return ((b + 1) * W - 1) / total; };
-  const long w0 = holder(b0), w1 = holder(b1 - 1);
+  const long w0 = quotient((b0 + 1) * W - 1, total), w1 = quotient(b1 * W - 1, total);
   if (w0 == w1) return;  // written whole
-  const long count = w1 - w0 + 1;
+  const int count = int(w1 - w0) + 1;
   const Part layout(G);
-  auto part = [&](long k) {
-    const long w = w0 + k;
-    return parts + ((w * cols + col) * 2 + (total * w / W >= b0 ? 0 : 1)) * layout.size();
-  };
-  float mx = -INFINITY;
-  int some = 0;
-  for (long k = lane; k < count; k += 64) {
-    const float2 ml = *reinterpret_cast<const float2*>(part(k) + layout.ml(g));
-    if (ml.y < 0.f) continue;  // NaN stays
-    mx = fmaxf(mx, ml.x);
-    some = 1;
+  // only the first part can be the second of its worker
+  const long step = 2 * cols * layout.size();
+  const float* at0 = parts + (w0 * cols + col) * 2 * layout.size();
+  const float* first = at0 + (quotient(total * w0, W) >= b0 ? 0 : layout.size());
+  auto part = [&](int k) { return k ? at0 + k * step : first; };
+  const int split = heads >= 5 ? 1 : JOIN_WAVES / heads, at_once = JOIN_WAVES / split;
+  for (int g0 = 0; g0 < heads; g0 += at_once) {
+    const int g = g0 + wave / split;
+    float acc = 0.f, sum = 0.f, m = -INFINITY;
+    int some = 0;
+    if (g < heads && wave < split * at_once)
+      for (int k0 = wave % split; k0 < count; k0 += JOIN_PARTS * split) {
+        float2 ml[JOIN_PARTS];
+        float o[JOIN_PARTS], mx = m;
+#pragma unroll
+        for (int u = 0; u < JOIN_PARTS; ++u) {
+          const int k = min(k0 + u * split, count - 1);
+          const float* at = part(k);
+          ml[u] = *reinterpret_cast<const float2*>(at + layout.ml(g));
+          o[u] = at[g * 64 + lane];
+        }
+#pragma unroll
+        for (int u = 0; u < JOIN_PARTS; ++u)
+          if (k0 + u * split < count && !(ml[u].y < 0.f)) {  // NaN stays
+            mx = fmaxf(mx, ml[u].x);
+            some = 1;
+          }
+        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+        acc *= keep;
+        sum *= keep;
+        m = mx;
+#pragma unroll
+        for (int u = 0; u < JOIN_PARTS; ++u)
+          if (k0 + u * split < count && !(ml[u].y < 0.f)) {
+            const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mx);
+            acc += o[u] * f;
+            sum += ml[u].y * f;
+          }
+      }
+    if (split > 1) {
+      accs[wave][lane] = acc;
+      if (lane == 0) {
+        sums[wave] = sum;
+        refs[wave] = m;
+        somes[wave] = some;
+      }
+      __syncthreads();
+      if (wave % split == 0) {
+        float mx = m;
+        for (int k = 1; k < split; ++k) mx = fmaxf(mx, refs[wave + k]);
+        acc = sum = 0.f;
+        for (int k = 0; k < split; ++k) {
+          if (!somes[wave + k]) continue;
+          some = 1;
+          const float f = refs[wave + k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(refs[wave + k] - mx);
+          acc += accs[wave + k][lane] * f;
+          sum += sums[wave + k] * f;
+        }
+      }
+    }
+    if (g < heads && wave % split == 0 && wave < split * at_once) out[g * 64 + lane] = from_f<T>(some ? acc / sum : 0.f);
   }
-  for (int d = 1; d < 64; d <<= 1) {
-    mx = fmaxf(mx, __shfl_xor(mx, d));
-    some |= __shfl_xor(some, d);
-  }
-  float acc = 0.f, sum = 0.f;
-#pragma unroll 8
-  for (long k = wave; k < count; k += JOIN_WAVES) {
-    const float* at = part(k);
-    const float2 ml = *reinterpret_cast<const float2*>(at + layout.ml(g));
-    const float o = at[g * 64 + lane];
-    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
-    if (ml.y < 0.f) continue;
-    acc += o * f;
-    sum += ml.y * f;
-  }
-  __shared__ float accs[JOIN_WAVES][64], sums[JOIN_WAVES];
-  accs[wave][lane] = acc;
-  if (lane == 0) sums[wave] = sum;
-  __syncthreads();
-  if (wave) return;
-  acc = sum = 0.f;
-  for (int k = 0; k < JOIN_WAVES; ++k) {
-    acc += accs[k][lane];
-    sum += sums[k];
-  }
-  out[lane] = from_f<T>(some ? acc / sum : 0.f);
 }
 
 // --- selection of pages -------------------------------------------------------------------------
@@ -795,7 +901,7 @@ __device__ inline uint64_t order_of(double s) {
 // The most that q k can be for a key between the page's bounds, summed over the group's heads, is
 // sum_c hi_c A_c + lo_c B_c, with A and B the sums of the positive and the negative parts of the heads' queries:
 // 128 products a page, however many heads share it. In 64 bits: which of two pages next to the border is
-// taken can hang on less than 32 bits hold. 16 lanes a page, 8 products each, 16 pages a wave whose loads fly
+// taken can hang on less than 32 bits hold. 8 lanes a page, 16 products each, 16 pages a wave whose loads fly
 // together; bound by its two dependent loads (the table's entry, the bounds).
 constexpr int SCORE_PAGES = 64;  // a block
 template <typename T>
@@ -803,53 +909,52 @@ __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, cons
   const KvCache& c = p.cache;
   const int chunks = (maxp + SCORE_PAGES - 1) / SCORE_PAGES, chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks;
   const int i = pair / c.kv_heads, kh = pair % c.kv_heads, G = p.heads / c.kv_heads;
-  const int lane = threadIdx.x & 63, sub = lane & 15, hi = sub >> 3, j = sub & 7;
-  const int held = int((long(length_of(p.lens[i], p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
-  const int p0 = chunk * SCORE_PAGES + (threadIdx.x >> 6) * 16 + (lane >> 4);
+  const int lane = threadIdx.x & 63, j = lane & 7;
+  const int held = int((long(length_of(uload(p.lens + i), p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
+  const int p0 = chunk * SCORE_PAGES + (threadIdx.x >> 6) * 16 + (lane >> 3);
   if (chunk * SCORE_PAGES >= held) return;
-  int page[4];
+  int page[2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) page[k] = p0 + 4 * k < held ? p.table[long(i) * p.width + p0 + 4 * k] : -1;
-  double cf[8] = {};
+  for (int k = 0; k < 2; ++k) page[k] = p0 + 8 * k < held ? p.table[long(i) * p.width + p0 + 8 * k] : -1;
+  double A[8] = {}, B[8] = {};
   for (int g = 0; g < G; ++g) {
     float x[8];
     load8(static_cast<const T*>(p.q) + i * p.ldq + (long(kh) * G + g) * 64 + j * 8, x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) cf[e] += (x[e] > 0.f) == (hi != 0) ? double(x[e]) : 0.0;
+    for (int e = 0; e < 8; ++e) {
+      A[e] += x[e] > 0.f ? double(x[e]) : 0.0;
+      B[e] += x[e] > 0.f ? 0.0 : double(x[e]);
+    }
   }
-  float v[4][8] = {};
+  float lo[2][8] = {}, hi[2][8] = {};
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (page_ok(page[k], c.pages)) load8(bounds + (long(page[k]) * c.kv_heads + kh) * 128 + sub * 8, v[k]);
+  for (int k = 0; k < 2; ++k)
+    if (page_ok(page[k], c.pages)) {
+      const T* at = bounds + (long(page[k]) * c.kv_heads + kh) * 128 + j * 8;
+      load8(at, lo[k]);
+      load8(at + 64, hi[k]);
+    }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 2; ++k) {
     double s = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += double(v[k][e]) * cf[e];
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) s += __shfl_xor(s, m);
-    if (sub == 0 && p0 + 4 * k < held)
-      keys[long(pair) * maxp + p0 + 4 * k] = page_ok(page[k], c.pages) ? order_of(s) : 0;
+    for (int e = 0; e < 8; ++e) s += double(lo[k][e]) * B[e] + double(hi[k][e]) * A[e];
+    s = sum8(s);
+    if (j == 0 && p0 + 8 * k < held) keys[long(pair) * maxp + p0 + 8 * k] = page_ok(page[k], c.pages) ? order_of(s) : 0;
   }
 }
 
-// Exclusive sum over the block's threads; `total` gets all of it. `room`: one int a wave and one.
-constexpr int SELECT_THREADS = 1024, SELECT_BINS = 2048;
-__device__ inline int scan_block(int v, int* room, int& total) {
+// Exclusive sum over the block's threads; `total` gets all of it. `room`: one int a wave.
+template <int THREADS> __device__ inline int scan_block(int v, int* room, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int inc = v;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int o = __shfl_up(inc, m);
-    if (lane >= m) inc += o;
-  }
+  const int inc = sum_wave(v);
   __syncthreads();  // the room's last readers
   if (lane == 63) room[wave] = inc;
   __syncthreads();
   int before = inc - v;
   total = 0;
 #pragma unroll
-  for (int k = 0; k < SELECT_THREADS / 64; ++k) {
+  for (int k = 0; k < THREADS / 64; ++k) {
     const int r = room[k];
     if (k < wave) before += r;
     total += r;
@@ -862,22 +967,24 @@ __device__ inline int scan_block(int v, int* room, int& total) {
 // are counted into up to 2048 equal bins of that range, the bins above the border's are taken, and its bin is the
 // next range: two rounds for most scores, six at most. Counts do not hang on the order of the atomic adds.
 // Thread t holds keys [t K, (t + 1) K) in registers (K > 0), or reads them every round (K = 0, `k` each).
-template <int K>
-__global__ void __launch_bounds__(SELECT_THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, int maxp, int k,
-                                                                     int topk, int* sel) {
-  __shared__ int bins[SELECT_BINS], room[SELECT_THREADS / 64], found[3];
-  __shared__ uint64_t ends[2][SELECT_THREADS / 64];
+constexpr int SELECT_BINS = 2048;
+template <int THREADS, int K>
+__global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, int maxp, int k, int topk, int* sel) {
+  constexpr int WAVES = THREADS / 64, EACH = SELECT_BINS / THREADS;
+  __shared__ int bins[SELECT_BINS], room[WAVES], found[3];
+  __shared__ uint64_t ends[2][WAVES];
   const KvCache& c = p.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = blockIdx.x / c.kv_heads;
-  const int held = int((long(length_of(p.lens[i], p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
   const uint64_t* in = keys + long(blockIdx.x) * maxp;
   int* out = sel + long(blockIdx.x) * topk;
-  if (K > 0) k = K;
   uint64_t mine[K > 0 ? K : 1];
-  if constexpr (K > 0) {
+  if constexpr (K > 0) {  // with the length, whatever it is
+    k = K;
 #pragma unroll
-    for (int e = 0; e < K; ++e) mine[e] = tid * K + e < held ? in[tid * K + e] : 0;
+    for (int e = 0; e < K; ++e) mine[e] = tid * K + e < maxp ? in[tid * K + e] : 0;
   }
+  const int held = int((long(length_of(p.lens[i], p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
+  const int newest = held - 1;
   auto each = [&](auto&& fn) {
     if constexpr (K > 0) {
 #pragma unroll
@@ -889,32 +996,35 @@ __global__ void __launch_bounds__(SELECT_THREADS) page_select_kernel(const Paged
       }
     }
   };
+  if constexpr (K > 0) {
+#pragma unroll
+    for (int e = 0; e < K; ++e)
+      if (tid * K + e >= held) mine[e] = 0;
+  }
   // the newest page aside: how many there are, and their range
-  const int newest = held - 1;
   uint64_t lo = ~0ull, hi = 0;
-  int mycount = 0, there, first = 0;
+  int count = 0, there, first = 0;
   each([&](int at, uint64_t key) {
     if (key == 0) return;
     if (at == newest) {
       first = 1;
       return;
     }
-    ++mycount;
+    ++count;
     lo = min(lo, key);
     hi = max(hi, key);
   });
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    lo = min(lo, uint64_t(__shfl_xor((unsigned long long)lo, m)));
-    hi = max(hi, uint64_t(__shfl_xor((unsigned long long)hi, m)));
-  }
-  if (lane == 0) {
+  lo = scan_wave(lo, ~uint64_t(0), [](uint64_t a, uint64_t b) { return min(a, b); });
+  hi = scan_wave(hi, uint64_t(0), [](uint64_t a, uint64_t b) { return max(a, b); });
+  if (lane == 63) {
     ends[0][wave] = lo;
     ends[1][wave] = hi;
   }
-  scan_block(mycount, room, there);
+  scan_block<THREADS>(count, room, there);
+  lo = ends[0][0];
+  hi = ends[1][0];
 #pragma unroll
-  for (int w = 0; w < SELECT_THREADS / 64; ++w) {
+  for (int w = 1; w < WAVES; ++w) {
     lo = min(lo, ends[0][w]);
     hi = max(hi, ends[1][w]);
   }
@@ -922,51 +1032,64 @@ __global__ void __launch_bounds__(SELECT_THREADS) page_select_kernel(const Paged
   int need = min(topk - int(newest_there), there), inside = there;  // to take from [lo, hi], and how many lie in it
   while (need < inside && need > 0 && lo < hi) {
     const int shift = max(0, 53 - __clzll(hi - lo));  // (hi - lo) >> shift < 2048
-    for (int b = tid; b < SELECT_BINS; b += SELECT_THREADS) bins[b] = 0;
+#pragma unroll
+    for (int b = 0; b < EACH; ++b) bins[tid + b * THREADS] = 0;
     __syncthreads();
     each([&](int at, uint64_t key) {
       if (key >= lo && key <= hi && at != newest) atomicAdd(&bins[int((key - lo) >> shift)], 1);
     });
     __syncthreads();
-    // thread t has the t-th pair of bins from above
-    const int b1 = bins[SELECT_BINS - 1 - 2 * tid], b0 = bins[SELECT_BINS - 2 - 2 * tid];
-    int all;
-    const int above = scan_block(b1 + b0, room, all);
-    if (above < need && need <= above + b1 + b0) {
-      const bool up = need <= above + b1;
-      found[0] = SELECT_BINS - 1 - 2 * tid - (up ? 0 : 1);
-      found[1] = up ? above : above + b1;
-      found[2] = up ? b1 : b0;
+    // thread t has the t-th EACH bins from above
+    const int top = SELECT_BINS - 1 - EACH * tid;
+    int mine_[EACH], sum = 0, all;
+#pragma unroll
+    for (int b = 0; b < EACH; ++b) sum += mine_[b] = bins[top - b];
+    int above = scan_block<THREADS>(sum, room, all);
+    if (above < need && need <= above + sum) {
+#pragma unroll
+      for (int b = 0; b < EACH; ++b) {
+        if (above < need && need <= above + mine_[b]) {
+          found[0] = top - b;
+          found[1] = above;
+          found[2] = mine_[b];
+        }
+        above += mine_[b];
+      }
     }
     __syncthreads();
     need -= found[1];
     inside = found[2];
-    const uint64_t at = lo + (uint64_t(found[0]) << shift);
-    const uint64_t last = (1ull << shift) - 1;
+    const uint64_t at = lo + (uint64_t(found[0]) << shift), last = (1ull << shift) - 1;
     if (hi - at > last) hi = at + last;
     lo = at;
     __syncthreads();  // found and bins are written again
   }
   // taken: the newest, what lies above the range, and of the range all or (equal keys) the first `need`
   const bool all = need == inside;
-  int equal = 0, eq_total;
-  if (!all && need > 0) each([&](int at, uint64_t key) { equal += key >= lo && key <= hi && at != newest; });
-  int eq_before = scan_block(equal, room, eq_total);
+  int eq_before = 0, total;
+  if (!all && need > 0) {
+    int equal = 0;
+    each([&](int at, uint64_t key) { equal += key >= lo && key <= hi && at != newest; });
+    eq_before = scan_block<THREADS>(equal, room, total);
+  }
   auto takes = [&](int at, uint64_t key, int& eq) {
     if (key == 0) return false;
     if (at == newest || key > hi) return true;
     if (key < lo || need == 0) return false;
     return all || eq++ < need;
   };
-  int count = 0, total, eq = eq_before;
+  count = 0;
+  int eq = eq_before;
   each([&](int at, uint64_t key) { count += takes(at, key, eq); });
-  int to = scan_block(count, room, total);
+  int to = scan_block<THREADS>(count, room, total);
   eq = eq_before;
   each([&](int at, uint64_t key) {
     if (takes(at, key, eq)) out[to++] = at;
   });
-  for (int e = total + tid; e < topk; e += SELECT_THREADS) out[e] = -1;
+  for (int e = total + tid; e < topk; e += THREADS) out[e] = -1;
 }
+
+constexpr long QK_WAVES = 8192;
 
 // Runs fn with the storage type dt as a value.
 template <typename F> void by_type(int dt, F&& fn) {
@@ -982,13 +1105,20 @@ void block_tables(const Exec& ex, const BlockTableArgs& args) {
   check_block_tables(a);
   if (ex.dry) return;
   ProfScope prof(ex, "block_tables", 4.0 * a.cap, 8.0 * a.cap + 16.0 * a.n);
-  const int blocks = std::min(cdiv(a.cap, TABLE_THREADS), 512);
-  if (blocks <= 1) {
-    block_tables_kernel<true, true><<<1, TABLE_THREADS, 0, ex.stream>>>(a);
-  } else {
-    block_tables_kernel<true, false><<<blocks, TABLE_THREADS, 0, ex.stream>>>(a);
-    block_tables_kernel<false, true><<<1, TABLE_THREADS, 0, ex.stream>>>(a);
-  }
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
+  // 256 threads a block where each has at most four requests to sum up
+  auto launch = [&](auto threads) {
+    constexpr int N = decltype(threads)::value;
+    const int blocks = int(std::min<long>((long(a.cap) + 4 * N - 1) / (4 * N), N == 256 ? 1024 : 256));
+    if (blocks <= 1) {
+      block_tables_kernel<N, true, true><<<1, N, 0, ex.stream>>>(a, vec);
+    } else {
+      block_tables_kernel<N, true, false><<<blocks, N, 0, ex.stream>>>(a, vec);
+      block_tables_kernel<N, false, true><<<1, N, 0, ex.stream>>>(a, vec);
+    }
+  };
+  if (a.n <= 1024) launch(std::integral_constant<int, 256>());
+  else launch(std::integral_constant<int, 1024>());
   SPLAT_HIP(hipGetLastError());
 }
 
@@ -1000,7 +1130,17 @@ void qk_norm_rope(const Exec& ex, const QkArgs& args, double base) {
   const double values = double(a.tokens) * (a.heads + (a.has_cache ? 2 : 1) * a.kv_heads) * 64;
   ProfScope prof(ex, "qk_norm_rope", 12 * values, 2 * values * dtype_size(a.dt));
   by_type(a.dt, [&](auto t) {
-    qk_norm_rope_kernel<decltype(t)><<<cdiv(a.tokens, 4), 256, 0, ex.stream>>>(a);
+    using T = decltype(t);
+    // a step of 8 head rows a wave while that leaves waves to spare, else five steps, whose angles are taken once
+    const int steps = cdiv(a.heads, 8) + (a.has_cache ? 2 : 1) * cdiv(a.kv_heads, 8), tokens = cdiv(a.tokens, 4);
+    auto launch = [&](auto rope) {
+      constexpr int R = decltype(rope)::value;
+      if (long(a.tokens) * steps <= QK_WAVES) qk_norm_rope_kernel<T, 1, R><<<dim3(tokens, steps), 256, 0, ex.stream>>>(a);
+      else qk_norm_rope_kernel<T, 5, R><<<dim3(tokens, cdiv(steps, 5)), 256, 0, ex.stream>>>(a);
+    };
+    if (a.rope == ROPE_NONE) launch(std::integral_constant<int, ROPE_NONE>());
+    else if (a.rope == ROPE_LINE) launch(std::integral_constant<int, ROPE_LINE>());
+    else launch(std::integral_constant<int, ROPE_GRID>());
   });
   SPLAT_HIP(hipGetLastError());
 }
@@ -1035,7 +1175,7 @@ void attend(const Exec& ex, const PagedArgs& a, const int* sel, int topk, char* 
       paged_scan_kernel<TileOps<T>::KEYS><<<1, 1024, 0, ex.stream>>>(a, topk, before);
       paged_parts_kernel<T, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
     }
-    paged_join_kernel<T><<<dim3(a.n, a.heads), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.workers, before, parts);
+    paged_join_kernel<T><<<dim3(a.n, plan.cols), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.workers, before, parts);
   });
 }
 
@@ -1065,12 +1205,13 @@ void sparse_attention(const Exec& ex, const SparseArgs& args, void* workspace, s
     if (maxp > 0)
       page_score_kernel<T><<<pairs * cdiv(maxp, SCORE_PAGES), 256, 0, ex.stream>>>(a, static_cast<const T*>(s.bounds), maxp, keys);
   });
-  const int each = cdiv(maxp, SELECT_THREADS);
-  auto select = [&](auto kernel) { kernel<<<pairs, SELECT_THREADS, 0, ex.stream>>>(a, keys, maxp, each, s.topk, s.selected); };
-  if (each <= 1) select(page_select_kernel<1>);
-  else if (each <= 4) select(page_select_kernel<4>);
-  else if (each <= 16) select(page_select_kernel<16>);
-  else select(page_select_kernel<0>);
+  auto select = [&](auto kernel, int threads) {
+    kernel<<<pairs, threads, 0, ex.stream>>>(a, keys, maxp, cdiv(maxp, threads), s.topk, s.selected);
+  };
+  if (maxp <= 1024) select(page_select_kernel<256, 4>, 256);
+  else if (maxp <= 4096) select(page_select_kernel<512, 8>, 512);
+  else if (maxp <= 16384) select(page_select_kernel<1024, 16>, 1024);
+  else select(page_select_kernel<1024, 0>, 1024);
   attend(ex, a, s.selected, s.topk, ws);
   SPLAT_HIP(hipGetLastError());
 }

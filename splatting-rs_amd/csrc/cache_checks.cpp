@@ -89,7 +89,7 @@ void check_workspace(const void* workspace, size_t bytes, size_t need) {
 void check_block_tables(BlockTableArgs& a) {
   check_page_size(a.page_size);
   check_width(a.width, a.page_size);
-  SPLAT_CHECK(a.n >= 0 && a.n <= (1 << 20), BAD_ARGUMENT, "block tables: n must be 0 to 2^20");
+  SPLAT_CHECK(a.n >= 0 && a.n <= 65536, BAD_ARGUMENT, "block tables: n must be 0 to 65536");
   SPLAT_CHECK(a.pool_size >= 0 && a.cap >= 0, BAD_ARGUMENT, "block tables: pool_size or cap is negative");
   SPLAT_CHECK(a.used && a.starts && a.used_out && a.status && (a.n == 0 || (a.past && a.add && a.table && a.lens)) &&
                   (a.pool_size == 0 || a.pool) && (a.cap == 0 || a.slots),
@@ -123,6 +123,8 @@ void check_qk_norm_rope(QkArgs& a, double base) {
     SPLAT_CHECK(a.cache.dt == a.dt && a.cache.kv_heads == a.kv_heads, BAD_ARGUMENT,
                 "qk norm: the cache has another dtype or other kv_heads");
   }
+  SPLAT_CHECK(aligned16(a.qw) && aligned16(a.qb) && aligned16(a.kw) && aligned16(a.kb), BAD_ARGUMENT,
+              "qk norm: qw, qb, kw and kb must be 16-byte aligned");
   if (a.tokens == 0) return;
   SPLAT_CHECK(a.qkv && a.q_out && (a.rope == ROPE_NONE || a.positions), BAD_ARGUMENT, "qk norm: a required pointer is NULL");
   const long es = type_size(a.dt), cols = (a.heads + 2L * a.kv_heads) * 64, wq = a.heads * 64L, wk = a.kv_heads * 64L;

@@ -142,7 +142,7 @@ int main() {
   T("tables ok no slots", [](auto& a) { a.cap = 0; a.slots = nullptr; a.positions = nullptr; });
   T("tables ok no pool", [](auto& a) { a.pool_size = 0; a.pool = nullptr; });
   T("tables n -1", [](auto& a) { a.n = -1; });
-  T("tables n 2^20 + 1", [](auto& a) { a.n = (1 << 20) + 1; });
+  T("tables n 65537", [](auto& a) { a.n = 65537; });
   T("tables page 4", [](auto& a) { a.page_size = 4; });
   T("tables page 24", [](auto& a) { a.page_size = 24; });
   T("tables page 512", [](auto& a) { a.page_size = 512; });
@@ -184,6 +184,8 @@ int main() {
   Q("qk qkv NULL", [](auto& a) { a.qkv = nullptr; });
   Q("qk positions NULL", [](auto& a) { a.positions = nullptr; });
   Q("qk odd qkv", [](auto& a) { a.qkv = at(8 * MB + 2); });
+  Q("qk odd qw", [](auto& a) { a.qw = reinterpret_cast<float*>(at(20 * MB + 4)); });
+  Q("qk odd kb", [](auto& a) { a.kb = reinterpret_cast<float*>(at(20 * MB + 8)); });
   Q("qk ld 1028", [](auto& a) { a.ld = 1028; });
   Q("qk ld short", [](auto& a) { a.ld = 15 * 64; });
   Q("qk ldq short", [](auto& a) { a.ldq = 7 * 64; });
