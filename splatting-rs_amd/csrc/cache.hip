@@ -101,8 +101,8 @@ template <> __device__ inline void store8<float>(float* p, const float (&x)[8]) 
 // over the threads' sums for four tokens at a time, then a walk over at most k requests. A new page begins with
 // a new token, whose thread writes the table's entry.
 // The call takes effect whole or not at all: the status is known before anything is written.
-// FILL writes the table, slots and positions, COMMIT lens, starts, used and status, which may lie over
-// past and used: with several blocks it runs as a second launch.
+// FILL writes the table, slots and positions, COMMIT (block 0) lens, starts, used and status; where those lie over
+// past and used and there are several blocks, it runs as a second launch.
 template <int THREADS, bool FILL, bool COMMIT>
 __global__ void __launch_bounds__(THREADS) block_tables_kernel(const BlockTableArgs p, bool vec) {
   constexpr int WAVES = THREADS / 64;
@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(THREADS) block_tables_kernel(const BlockTableA
     }
   }
   if constexpr (COMMIT) {
+    if (blockIdx.x != 0) return;
     if (FILL) __syncthreads();  // the block's tokens have read past
     long t = et;
     for (int i = i0; i < i1; ++i) {
@@ -348,15 +349,20 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
     for (int r0 = lane >> 3; r0 < rows; r0 += 64) {
-      float x[8][8];
+      uint4 raw[8][sizeof(T) / 2];  // as they lie in memory: the conversions would double the registers
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (8 * u < rows) load8(k + min(r0 + 8 * u, rows - 1) * 64, x[u]);  // the last row again changes nothing
+        if (8 * u < rows)  // the last row again changes nothing
+#pragma unroll
+          for (int w = 0; w < int(sizeof(T) / 2); ++w) raw[u][w] = reinterpret_cast<const uint4*>(k + min(r0 + 8 * u, rows - 1) * 64)[w];
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (8 * u < rows)
+        if (8 * u < rows) {
+          float x[8];
+          load8(reinterpret_cast<const T*>(raw[u]), x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) { lo[e] = low(lo[e], x[u][e]); hi[e] = high(hi[e], x[u][e]); }
+          for (int e = 0; e < 8; ++e) { lo[e] = low(lo[e], x[e]); hi[e] = high(hi[e], x[e]); }
+        }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -475,9 +481,12 @@ template <> struct TileOps<float> {  // rows of 256 bytes
   __device__ inline void scores(const char* kt, int lane, f32x4 (&x)[T16]) const {
     const int row = lane & 15, g = lane >> 4;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    float4 ks[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) ks[b] = *reinterpret_cast<const float4*>(kt + row * 256 + (((4 * b + g) ^ row) * 16));
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const float4 k = *reinterpret_cast<const float4*>(kt + row * 256 + (((4 * b + g) ^ row) * 16));
+      const float4& k = ks[b];
       a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.x, q[b].x, a, 0, 0, 0);
       a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.y, q[b].y, a, 0, 0, 0);
       a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.z, q[b].z, a, 0, 0, 0);
@@ -487,40 +496,35 @@ template <> struct TileOps<float> {  // rows of 256 bytes
   }
   __device__ static inline void weigh(const char* vt, int lane, const f32x4 (&w)[T16], f32x4 (&o)[4]) {
     const int g = lane >> 4, c = lane & 15;
+    float v[4][4];
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v = *reinterpret_cast<const float*>(vt + (4 * g + r) * 256 + (((4 * d + (c >> 2)) ^ (4 * g)) * 16) + (c & 3) * 4);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[0][r], o[d], 0, 0, 0);
-      }
+      for (int d = 0; d < 4; ++d)
+        v[r][d] = *reinterpret_cast<const float*>(vt + (4 * g + r) * 256 + (((4 * d + (c >> 2)) ^ (4 * g)) * 16) + (c & 3) * 4);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][d], w[0][r], o[d], 0, 0, 0);
   }
 };
 
 constexpr int TILE_BYTES = 8192;  // K, then V
-constexpr int STAGES = 2;
+constexpr int STAGES = 2;  // run() takes two
 
-// Where a wave stands: sequence i holds tiles [base, next) of the launch's row of tiles.
-struct Cursor {
-  int i;
-  long base, next;
-};
-
-// Tiles of sequence i: of its positions, or of the pages that were selected.
-template <int KEYS> __device__ inline int tiles_of(const PagedArgs& p, int i, int topk) {
-  const int len = length_of(p.lens[i], p.width, p.cache.shift, p.max_len);
+// Tiles of a sequence: of its positions, or of the pages that were selected.
+template <int KEYS> __device__ inline int tiles_in(int len, const KvCache& c, int topk) {
   if (!topk) return int((long(len) + KEYS - 1) / KEYS);
-  const int held = int((long(len) + p.cache.page_size - 1) >> p.cache.shift);
-  return int(((long(min(held, topk)) << p.cache.shift) + KEYS - 1) / KEYS);
+  const int held = int((long(len) + c.page_size - 1) >> c.shift);
+  return int(((long(min(held, topk)) << c.shift) + KEYS - 1) / KEYS);
 }
 
-// One wave: the running softmax of one group of heads over tiles [t, end), which may cross sequences.
-// finish(cursor, first tile, state) is called at the end of each sequence's part.
-template <typename T> struct PagedWave {
+// One wave: the running softmax of one group of heads over tiles of one sequence (SPARSE: of its selected pages).
+template <typename T, bool SPARSE> struct PagedWave {
   using Ops = TileOps<T>;
   static constexpr int KEYS = Ops::KEYS, PIECE = Ops::PIECE;
   const PagedArgs& p;
-  const int* sel;  // [n, kv_heads, topk] or null
+  const int* sel;  // [n, kv_heads, topk] (SPARSE)
   const int topk, kh, lane;
   const uint32_t lds;   // of the wave's ring
   const char* ring;
@@ -528,8 +532,14 @@ template <typename T> struct PagedWave {
   f32x4 o[4];
   float m, l;
   int some;  // keys were there
+  int len, held;
+  const int *row, *chosen;
 
-  __device__ inline void clear() {
+  __device__ inline void begin(int i) {
+    row = p.table + long(i) * p.width;
+    if (SPARSE) chosen = sel + (long(i) * p.cache.kv_heads + kh) * topk;
+    len = length_of(uload(p.lens + i), p.width, p.cache.shift, p.max_len);
+    held = int((long(len) + p.cache.page_size - 1) >> p.cache.shift);
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     m = -INFINITY;
@@ -537,30 +547,28 @@ template <typename T> struct PagedWave {
     some = 0;
   }
 
-  // Loads local tile t of sequence i into slot b of the ring; the rows of each piece that are there, 8 bits a piece.
-  __device__ inline uint32_t issue(int i, int t, int b) {
+  // Loads tile t into slot b of the ring; the rows of each piece that are there, 8 bits a piece. The table's entries
+  // are read whatever the length is, so that both loads are under way together.
+  __device__ inline uint32_t issue(int t, int b) {
     const KvCache& c = p.cache;
-    const int len = uniform(length_of(uload(p.lens + i), p.width, c.shift, p.max_len)), ps = c.page_size;
-    const int held = int((long(len) + ps - 1) >> c.shift), count = topk ? min(held, topk) : held;
-    const int* row = p.table + long(i) * p.width;
+    const int ps = c.page_size;
     uint32_t there = 0;
-    int entry[4], rows[4];
+    int place[4], entry[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int pos = t * KEYS + k * PIECE, e = pos >> c.shift;
-      int j = min(e, count - 1);
-      if (topk) j = uload(sel + (long(i) * c.kv_heads + kh) * topk + j);
-      entry[k] = uload(row + max(j, 0));
-      const int left = len - int(long(j) << c.shift) - (pos & (ps - 1));
-      rows[k] = e < count && j >= 0 ? max(0, min(PIECE, left)) : 0;
+      const int e = (t * KEYS + k * PIECE) >> c.shift;
+      place[k] = SPARSE ? e < topk ? uload(chosen + min(e, topk - 1)) : -1 : e;
     }
 #pragma unroll
+    for (int k = 0; k < 4; ++k) entry[k] = uload(row + (SPARSE ? max(min(place[k], p.width - 1), 0) : min(place[k], p.width - 1)));
+#pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const bool ok = page_ok(entry[k], c.pages);
-      const int r = ok ? rows[k] : 0;
-      there |= uint32_t(r) << (8 * k);
-      const long at = (ok ? page_at(c, entry[k], kh) : 0) + long((t * KEYS + k * PIECE) & (ps - 1)) * 64;
-      const uint32_t bytes = uint32_t(r) * 64 * sizeof(T), to = lds + b * TILE_BYTES + k * 1024;
+      const int in_page = (t * KEYS + k * PIECE) & (ps - 1);
+      const bool ok = place[k] >= 0 && place[k] < held && page_ok(entry[k], c.pages);
+      const int rows = ok ? max(0, min(PIECE, len - (place[k] << c.shift) - in_page)) : 0;
+      there |= uint32_t(rows) << (8 * k);
+      const long at = (ok ? page_at(c, entry[k], kh) : 0) + long(in_page) * 64;
+      const uint32_t bytes = uint32_t(rows) * 64 * sizeof(T), to = lds + b * TILE_BYTES + k * 1024;
       load_lds(static_cast<const T*>(c.k) + at, bytes, Ops::k_off(lane, k), to);
       load_lds(static_cast<const T*>(c.v) + at, bytes, Ops::v_off(lane, k), to + TILE_BYTES / 2);
     }
@@ -609,22 +617,22 @@ template <typename T> struct PagedWave {
     Ops::weigh(kt + TILE_BYTES / 2, lane, x, o);
   }
 
-  // Local tiles [t, end) of one sequence with nothing in flight before or after.
-  __device__ inline void run(int i, int t, int end, float scale) {
-    uint32_t there[STAGES];
-#pragma unroll
-    for (int b = 0; b < STAGES; ++b) there[b] = t + b < end ? issue(i, t + b, b) : 0;
+  // Tiles t, t + step, ... below end, two under way, none before or after.
+  __device__ inline void run(int t, int step, int end, float scale) {
+    uint32_t there = 0, next = 0;
+#pragma unroll 1
+    for (int b = 0; b < STAGES; ++b) {
+      there = next;
+      next = t + b * step < end ? issue(t + b * step, b) : 0;
+    }
     ops.pin_q();
-    while (t < end) {
-#pragma unroll
-      for (int b = 0; b < STAGES; ++b) {
-        if (t + b >= end) break;
-        if (t + b + 1 < end) wait_loads<8 * (STAGES - 1)>();
-        else wait_loads<0>();
-        tile(b, there[b], scale);
-        if (t + b + STAGES < end) there[b] = issue(i, t + b + STAGES, b);
-      }
-      t += STAGES;
+#pragma unroll 1
+    for (int b = 0; t < end; t += step, b ^= 1) {
+      if (t + step < end) wait_loads<8>();
+      else wait_loads<0>();
+      tile(b, there, scale);
+      there = next;
+      if (t + STAGES * step < end) next = issue(t + STAGES * step, b);
     }
   }
 
@@ -643,14 +651,14 @@ template <typename T> struct PagedWave {
   }
 };
 
-constexpr int PAGED_WAVES = 4;
+constexpr int PAGED_WAVES = 4, WHOLE_WAVES = 4;
 
-// One block a (sequence, group of up to 16 heads of one key head): its waves take a quarter of the tiles each
+// One block a (sequence, group of up to 16 heads of one key head): its waves take equal parts of the tiles
 // and join their sums in LDS.
-template <typename T>
-__global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const PagedArgs p, const int* sel, int topk, float scale) {
-  using Wave = PagedWave<T>;
-  __shared__ __attribute__((aligned(1024))) char smem[PAGED_WAVES * STAGES * TILE_BYTES];
+template <typename T, bool SPARSE>
+__global__ void __launch_bounds__(WHOLE_WAVES * 64, 8 / WHOLE_WAVES) paged_whole_kernel(const PagedArgs p, const int* sel, int topk, float scale) {
+  using Wave = PagedWave<T, SPARSE>;
+  __shared__ __attribute__((aligned(1024))) char smem[WHOLE_WAVES * STAGES * TILE_BYTES];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int G = p.heads / p.cache.kv_heads, parts = (G + 15) / 16;
   const int i = blockIdx.x, kh = int(blockIdx.y) / parts, g0 = int(blockIdx.y) % parts * 16;
@@ -658,9 +666,9 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const 
   char* ring = smem + wave * STAGES * TILE_BYTES;
   Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
   w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
-  w.clear();
-  const int nt = uniform(tiles_of<Wave::KEYS>(p, i, topk));
-  w.run(i, int(long(nt) * wave / PAGED_WAVES), int(long(nt) * (wave + 1) / PAGED_WAVES), scale);
+  w.begin(i);
+  // every fourth tile: the first ones do not hang on the length
+  w.run(wave, WHOLE_WAVES, tiles_in<Wave::KEYS>(w.len, p.cache, topk), scale);
   w.l = sum_groups(w.l);
   // the join: every wave's m, l and whether it had keys, then the sums moved to the common reference
   float* ml = reinterpret_cast<float*>(smem);
@@ -673,10 +681,12 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const 
   }
   __syncthreads();
   float mn = -INFINITY;
-  for (int k = 0; k < PAGED_WAVES; ++k) mn = fmaxf(mn, ml[(k * 16 + col) * 4]);
+#pragma unroll
+  for (int k = 0; k < WHOLE_WAVES; ++k) mn = fmaxf(mn, ml[(k * 16 + col) * 4]);
   float sum = 0.f;
   int some = 0;
-  for (int k = 0; k < PAGED_WAVES; ++k) {
+#pragma unroll
+  for (int k = 0; k < WHOLE_WAVES; ++k) {
     const float* at = ml + (k * 16 + col) * 4;
     if (!__float_as_int(at[2])) continue;
     some = 1;
@@ -689,13 +699,14 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const 
 #pragma unroll
     for (int r = 0; r < 4; ++r) os[((wave * 4 + d) * 4 + r) * 64 + lane] = w.some ? w.o[d][r] * keep : 0.f;
   __syncthreads();
-  if (g0 + col >= G) return;
+  if (g0 + col >= G || wave >= 4) return;
   // wave d writes channels 16 d + 4 (lane / 16) + (0..3)
   float v[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     float a = 0.f;
-    for (int k = 0; k < PAGED_WAVES; ++k) a += os[((k * 4 + wave) * 4 + r) * 64 + lane];
+#pragma unroll
+    for (int k = 0; k < WHOLE_WAVES; ++k) a += os[((k * 4 + wave) * 4 + r) * 64 + lane];
     v[r] = some ? a / sum : 0.f;
   }
   T* out = static_cast<T*>(p.out) + i * p.ldo + long(head) * 64 + 16 * wave + 4 * (lane >> 4);
@@ -716,7 +727,7 @@ template <int KEYS, int NT> __device__ inline void scan_tiles(const PagedArgs& p
   long base = 0;
   for (int i0 = 0; i0 <= p.n; i0 += NT) {
     const int i = i0 + tid;
-    const long c = i < p.n ? tiles_of<KEYS>(p, i, topk) : 0;
+    const long c = i < p.n ? tiles_in<KEYS>(length_of(p.lens[i], p.width, p.cache.shift, p.max_len), p.cache, topk) : 0;
     long inc = c;
     for (int m = 1; m < 64; m <<= 1) {
       const long o = __shfl_up(inc, m);
@@ -747,10 +758,10 @@ struct Part {
   __device__ inline int ml(int g) const { return heads * 64 + g * 2; }
 };
 
-template <typename T, bool SCAN>
+template <typename T, bool SPARSE, bool SCAN>
 __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const PagedArgs p, const int* sel, int topk, float scale,
                                                                           int workers, long* before, float* parts) {
-  using Wave = PagedWave<T>;
+  using Wave = PagedWave<T, SPARSE>;
   __shared__ __attribute__((aligned(1024))) char smem[PAGED_WAVES * STAGES * TILE_BYTES];
   __shared__ long own[SCAN ? SCAN_MAX + 1 : 1];
   const long* pre = before;
@@ -784,8 +795,8 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
     const long stop = min(end, b1);
     if (stop <= t) continue;
     w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
-    w.clear();
-    w.run(i, uniform(int(t - b0)), uniform(int(stop - b0)), scale);
+    w.begin(i);
+    w.run(uniform(int(t - b0)), 1, uniform(int(stop - b0)), scale);
     w.l = sum_groups(w.l);
     if (g0 + col < G) {
       if (t == b0 && stop == b1) {
@@ -912,19 +923,26 @@ __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, cons
   const int lane = threadIdx.x & 63, j = lane & 7;
   const int held = int((long(length_of(uload(p.lens + i), p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
   const int p0 = chunk * SCORE_PAGES + (threadIdx.x >> 6) * 16 + (lane >> 3);
+  int page[2];  // read together with the length, whatever it is
+#pragma unroll
+  for (int k = 0; k < 2; ++k) page[k] = p.table[long(i) * p.width + min(p0 + 8 * k, p.width - 1)];
   if (chunk * SCORE_PAGES >= held) return;
-  int page[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) page[k] = p0 + 8 * k < held ? p.table[long(i) * p.width + p0 + 8 * k] : -1;
+  for (int k = 0; k < 2; ++k)
+    if (p0 + 8 * k >= held) page[k] = -1;
   double A[8] = {}, B[8] = {};
-  for (int g = 0; g < G; ++g) {
-    float x[8];
-    load8(static_cast<const T*>(p.q) + i * p.ldq + (long(kh) * G + g) * 64 + j * 8, x);
+  for (int g0 = 0; g0 < G; g0 += 4) {  // four heads under way
+    float x[4][8] = {};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      A[e] += x[e] > 0.f ? double(x[e]) : 0.0;
-      B[e] += x[e] > 0.f ? 0.0 : double(x[e]);
-    }
+    for (int g = 0; g < 4; ++g)
+      if (g0 + g < G) load8(static_cast<const T*>(p.q) + i * p.ldq + (long(kh) * G + g0 + g) * 64 + j * 8, x[g]);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        A[e] += x[g][e] > 0.f ? double(x[g][e]) : 0.0;
+        B[e] += x[g][e] > 0.f ? 0.0 : double(x[g][e]);
+      }
   }
   float lo[2][8] = {}, hi[2][8] = {};
 #pragma unroll
@@ -944,35 +962,20 @@ __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, cons
   }
 }
 
-// Exclusive sum over the block's threads; `total` gets all of it. `room`: one int a wave.
-template <int THREADS> __device__ inline int scan_block(int v, int* room, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int inc = sum_wave(v);
-  __syncthreads();  // the room's last readers
-  if (lane == 63) room[wave] = inc;
-  __syncthreads();
-  int before = inc - v;
-  total = 0;
-#pragma unroll
-  for (int k = 0; k < THREADS / 64; ++k) {
-    const int r = room[k];
-    if (k < wave) before += r;
-    total += r;
-  }
-  return before;
-}
-
 // One block a (sequence, key head): the topk largest keys' places, ascending, the lowest place first among equal
 // keys, -1 behind them; the newest page is taken first. The keys that are still undecided lie in [lo, hi]; they
-// are counted into up to 2048 equal bins of that range, the bins above the border's are taken, and its bin is the
-// next range: two rounds for most scores, six at most. Counts do not hang on the order of the atomic adds.
+// are counted into up to 512 equal bins of that range, the bins above the border's are taken, and its bin is the
+// next range: two rounds for most scores, seven at most. Counts do not hang on the order of the atomic adds, and
+// every wave reads all bins for itself, so that a round has one barrier: of three sets of bins one is counted
+// into, one cleared, and one may still be read. What bounds the kernel is the chain of these steps.
 // Thread t holds keys [t K, (t + 1) K) in registers (K > 0), or reads them every round (K = 0, `k` each).
-constexpr int SELECT_BINS = 2048;
+constexpr int SELECT_BINS = 512;
 template <int THREADS, int K>
 __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, int maxp, int k, int topk, int* sel) {
-  constexpr int WAVES = THREADS / 64, EACH = SELECT_BINS / THREADS;
-  __shared__ int bins[SELECT_BINS], room[WAVES], found[3];
-  __shared__ uint64_t ends[2][WAVES];
+  constexpr int WAVES = THREADS / 64, EACH = SELECT_BINS / 64;
+  __shared__ __attribute__((aligned(16))) int bins[3][SELECT_BINS];
+  __shared__ int room[2][WAVES];
+  __shared__ uint32_t ends[2][WAVES];
   const KvCache& c = p.cache;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = blockIdx.x / c.kv_heads;
   const uint64_t* in = keys + long(blockIdx.x) * maxp;
@@ -983,8 +986,10 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
 #pragma unroll
     for (int e = 0; e < K; ++e) mine[e] = tid * K + e < maxp ? in[tid * K + e] : 0;
   }
-  const int held = int((long(length_of(p.lens[i], p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
+  const int held = int((long(length_of(uload(p.lens + i), p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
   const int newest = held - 1;
+  const bool newest_there = held > 0 && page_ok(uload(p.table + long(i) * p.width + max(newest, 0)), c.pages);
+  // fn(place, key) for this thread's places before the newest; 0: no page there
   auto each = [&](auto&& fn) {
     if constexpr (K > 0) {
 #pragma unroll
@@ -992,100 +997,111 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
     } else {
       for (int e = 0; e < k; ++e) {
         const long at = long(tid) * k + e;
-        if (at < held) fn(int(at), in[at]);
+        if (at < newest) fn(int(at), in[at]);
       }
     }
   };
   if constexpr (K > 0) {
 #pragma unroll
     for (int e = 0; e < K; ++e)
-      if (tid * K + e >= held) mine[e] = 0;
+      if (tid * K + e >= newest) mine[e] = 0;
   }
-  // the newest page aside: how many there are, and their range
-  uint64_t lo = ~0ull, hi = 0;
-  int count = 0, there, first = 0;
-  each([&](int at, uint64_t key) {
-    if (key == 0) return;
-    if (at == newest) {
-      first = 1;
-      return;
-    }
-    ++count;
-    lo = min(lo, key);
-    hi = max(hi, key);
+  for (int b = tid; b < SELECT_BINS; b += THREADS) bins[0][b] = 0;
+  // the range of the keys' upper halves
+  uint32_t low32 = ~0u, high32 = 0;
+  each([&](int, uint64_t key) {
+    if (key) low32 = min(low32, uint32_t(key >> 32));
+    high32 = max(high32, uint32_t(key >> 32));
   });
-  lo = scan_wave(lo, ~uint64_t(0), [](uint64_t a, uint64_t b) { return min(a, b); });
-  hi = scan_wave(hi, uint64_t(0), [](uint64_t a, uint64_t b) { return max(a, b); });
+  low32 = scan_wave(int(low32), -1, [](int a, int b) { return int(min(uint32_t(a), uint32_t(b))); });
+  high32 = scan_wave(int(high32), 0, [](int a, int b) { return int(max(uint32_t(a), uint32_t(b))); });
   if (lane == 63) {
-    ends[0][wave] = lo;
-    ends[1][wave] = hi;
+    ends[0][wave] = low32;
+    ends[1][wave] = high32;
   }
-  scan_block<THREADS>(count, room, there);
-  lo = ends[0][0];
-  hi = ends[1][0];
+  __syncthreads();
+  low32 = ends[0][0];
+  high32 = ends[1][0];
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) {
-    lo = min(lo, ends[0][w]);
-    hi = max(hi, ends[1][w]);
+    low32 = min(low32, ends[0][w]);
+    high32 = max(high32, ends[1][w]);
   }
-  const bool newest_there = __syncthreads_or(first);
-  int need = min(topk - int(newest_there), there), inside = there;  // to take from [lo, hi], and how many lie in it
-  while (need < inside && need > 0 && lo < hi) {
-    const int shift = max(0, 53 - __clzll(hi - lo));  // (hi - lo) >> shift < 2048
-#pragma unroll
-    for (int b = 0; b < EACH; ++b) bins[tid + b * THREADS] = 0;
-    __syncthreads();
-    each([&](int at, uint64_t key) {
-      if (key >= lo && key <= hi && at != newest) atomicAdd(&bins[int((key - lo) >> shift)], 1);
+  uint64_t lo = uint64_t(low32) << 32, hi = uint64_t(high32) << 32 | 0xffffffffu;
+  if (lo == 0) lo = 1;  // 0 is no key
+  int need = topk - int(newest_there), inside = -1;  // to take from [lo, hi], and how many lie in it: known from the first round on
+  for (int round = 0; need > 0 && need != inside && lo < hi; ++round) {
+    const int shift = max(0, 55 - __clzll(hi - lo));  // (hi - lo) >> shift < 512
+    int* now = bins[round % 3];
+    int* next = bins[(round + 1) % 3];
+    for (int b = tid; b < SELECT_BINS; b += THREADS) next[b] = 0;
+    each([&](int, uint64_t key) {
+      if (key >= lo && key <= hi) atomicAdd(&now[int((key - lo) >> shift)], 1);
     });
     __syncthreads();
-    // thread t has the t-th EACH bins from above
-    const int top = SELECT_BINS - 1 - EACH * tid;
-    int mine_[EACH], sum = 0, all;
+    // lane t has the t-th EACH bins from above
+    int cnt[EACH], sum = 0;
 #pragma unroll
-    for (int b = 0; b < EACH; ++b) sum += mine_[b] = bins[top - b];
-    int above = scan_block<THREADS>(sum, room, all);
-    if (above < need && need <= above + sum) {
+    for (int b = 0; b < EACH; b += 4) *reinterpret_cast<int4*>(cnt + b) = *reinterpret_cast<const int4*>(now + SELECT_BINS - EACH * (lane + 1) + b);
 #pragma unroll
-      for (int b = 0; b < EACH; ++b) {
-        if (above < need && need <= above + mine_[b]) {
-          found[0] = top - b;
-          found[1] = above;
-          found[2] = mine_[b];
-        }
-        above += mine_[b];
-      }
+    for (int b = 0; b < EACH; ++b) sum += cnt[b];
+    const int upto = sum_wave(sum), all = __builtin_amdgcn_readlane(upto, 63);
+    if (round == 0) need = min(need, all);
+    if (need == 0 || need == all) {
+      inside = all;
+      break;
     }
-    __syncthreads();
-    need -= found[1];
-    inside = found[2];
-    const uint64_t at = lo + (uint64_t(found[0]) << shift), last = (1ull << shift) - 1;
+    int above = upto - sum, bin = 0, got = 0, passed = 0;
+#pragma unroll
+    for (int b = EACH - 1; b >= 0; --b) {
+      if (above < need && need <= above + cnt[b]) {
+        bin = SELECT_BINS - EACH * (lane + 1) + b;
+        got = cnt[b];
+        passed = above;
+      }
+      above += cnt[b];
+    }
+    const int who = __builtin_ctzll(__ballot(got > 0));
+    need -= __builtin_amdgcn_readlane(passed, who);
+    inside = __builtin_amdgcn_readlane(got, who);
+    const uint64_t at = lo + (uint64_t(__builtin_amdgcn_readlane(bin, who)) << shift), last = (1ull << shift) - 1;
     if (hi - at > last) hi = at + last;
     lo = at;
-    __syncthreads();  // found and bins are written again
   }
   // taken: the newest, what lies above the range, and of the range all or (equal keys) the first `need`
-  const bool all = need == inside;
-  int eq_before = 0, total;
-  if (!all && need > 0) {
+  const bool some = need > 0 && need != inside;
+  int eq = 0, before = 0, total = 0;
+  if (some) {
     int equal = 0;
-    each([&](int at, uint64_t key) { equal += key >= lo && key <= hi && at != newest; });
-    eq_before = scan_block<THREADS>(equal, room, total);
+    each([&](int, uint64_t key) { equal += key >= lo && key <= hi; });
+    const int upto = sum_wave(equal);
+    if (lane == 63) room[1][wave] = upto;
+    __syncthreads();
+    eq = upto - equal;
+    for (int w = 0; w < wave; ++w) eq += room[1][w];
   }
-  auto takes = [&](int at, uint64_t key, int& eq) {
-    if (key == 0) return false;
-    if (at == newest || key > hi) return true;
-    if (key < lo || need == 0) return false;
-    return all || eq++ < need;
+  const int first = need > 0 ? need - eq : 0;  // of this thread's equal keys
+  int left = some ? first : need > 0 ? k : 0;
+  auto takes = [&](uint64_t key, int& left) {
+    if (key > hi) return true;
+    return key >= lo && key != 0 && left-- > 0;
   };
-  count = 0;
-  int eq = eq_before;
-  each([&](int at, uint64_t key) { count += takes(at, key, eq); });
-  int to = scan_block<THREADS>(count, room, total);
-  eq = eq_before;
+  int count = 0, l = left;
+  each([&](int, uint64_t key) { count += takes(key, l); });
+  const int upto = sum_wave(count);
+  if (lane == 63) room[0][wave] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) before += room[0][w];
+    total += room[0][w];
+  }
+  before += upto - count;
   each([&](int at, uint64_t key) {
-    if (takes(at, key, eq)) out[to++] = at;
+    if (takes(key, left)) out[before++] = at;
   });
+  if (tid == 0 && newest_there) out[total] = newest;
+  total += newest_there;
   for (int e = total + tid; e < topk; e += THREADS) out[e] = -1;
 }
 
@@ -1110,8 +1126,8 @@ void block_tables(const Exec& ex, const BlockTableArgs& args) {
   auto launch = [&](auto threads) {
     constexpr int N = decltype(threads)::value;
     const int blocks = int(std::min<long>((long(a.cap) + 4 * N - 1) / (4 * N), N == 256 ? 1024 : 256));
-    if (blocks <= 1) {
-      block_tables_kernel<N, true, true><<<1, N, 0, ex.stream>>>(a, vec);
+    if (blocks <= 1 || (a.lens != a.past && a.used_out != a.used)) {
+      block_tables_kernel<N, true, true><<<std::max(blocks, 1), N, 0, ex.stream>>>(a, vec);
     } else {
       block_tables_kernel<N, true, false><<<blocks, N, 0, ex.stream>>>(a, vec);
       block_tables_kernel<N, false, true><<<1, N, 0, ex.stream>>>(a, vec);
@@ -1162,20 +1178,25 @@ void attend(const Exec& ex, const PagedArgs& a, const int* sel, int topk, char* 
   const float scale = a.scale * 1.44269504088896341f;  // scores as exponents of 2
   long* before = reinterpret_cast<long*>(workspace);
   float* parts = reinterpret_cast<float*>(workspace + plan.before_bytes);
-  by_type(a.cache.dt, [&](auto t) {
+  auto launch = [&](auto t, auto sparse) {
     using T = decltype(t);
+    constexpr bool S = decltype(sparse)::value;
     if (!plan.workers) {
-      paged_whole_kernel<T><<<dim3(a.n, plan.cols), PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale);
+      paged_whole_kernel<T, S><<<dim3(a.n, plan.cols), WHOLE_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale);
       return;
     }
     const dim3 grid(plan.workers / PAGED_WAVES, plan.cols);
     if (a.n <= SCAN_MAX) {
-      paged_parts_kernel<T, true><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
+      paged_parts_kernel<T, S, true><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
     } else {
       paged_scan_kernel<TileOps<T>::KEYS><<<1, 1024, 0, ex.stream>>>(a, topk, before);
-      paged_parts_kernel<T, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
+      paged_parts_kernel<T, S, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
     }
     paged_join_kernel<T><<<dim3(a.n, plan.cols), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.workers, before, parts);
+  };
+  by_type(a.cache.dt, [&](auto t) {
+    if (topk) launch(t, std::true_type());
+    else launch(t, std::false_type());
   });
 }
 
