@@ -53,10 +53,9 @@ template <typename V> __device__ inline V sum8(V v) {
 __device__ inline int uload(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// a / b for a, b >= 0, in 32 bits where they fit: the 64-bit division is a hundred instructions.
-__device__ inline long quotient(long a, long b) {
-  return (uint64_t(a) | uint64_t(b)) >> 32 ? a / b : long(uint32_t(a) / uint32_t(b));
-}
+// floor(a / b) for 0 <= a < 2^52 and 0 < b < 2^52: a quotient below a whole number is so by more than the
+// rounding of the 64-bit float division. The integer division is a hundred instructions.
+__device__ inline long quotient(long a, long b) { return long(floor(double(a) / double(b))); }
 
 // fn over lanes l, l ^ 16, l ^ 32, l ^ 48 (over_rows) and l, l ^ 8, ... (over_halves, then over_rows).
 template <typename F> __device__ inline float over_rows(float v, F&& fn) {
@@ -617,22 +616,21 @@ template <typename T, bool SPARSE> struct PagedWave {
     Ops::weigh(kt + TILE_BYTES / 2, lane, x, o);
   }
 
-  // Tiles t, t + step, ... below end, two under way, none before or after.
+  // Tiles t, t + step, ... below end: tile k is asked for while tile k - 2 is used, in one copy of either's code (a
+  // launch begins with a cold instruction cache).
   __device__ inline void run(int t, int step, int end, float scale) {
-    uint32_t there = 0, next = 0;
-#pragma unroll 1
-    for (int b = 0; b < STAGES; ++b) {
-      there = next;
-      next = t + b * step < end ? issue(t + b * step, b) : 0;
-    }
+    const int count = t < end ? (end - t + step - 1) / step : 0;
+    uint32_t there = 0, next = 0;  // of tiles k - 2 and k - 1
     ops.pin_q();
 #pragma unroll 1
-    for (int b = 0; t < end; t += step, b ^= 1) {
-      if (t + step < end) wait_loads<8>();
-      else wait_loads<0>();
-      tile(b, there, scale);
+    for (int k = 0; k < count + 2; ++k) {
+      if (k >= 2) {
+        if (k - 1 < count) wait_loads<8>();
+        else wait_loads<0>();
+        tile(k & 1, there, scale);
+      }
       there = next;
-      if (t + STAGES * step < end) next = issue(t + STAGES * step, b);
+      if (k < count) next = issue(t + k * step, k & 1);
     }
   }
 
@@ -651,72 +649,111 @@ template <typename T, bool SPARSE> struct PagedWave {
   }
 };
 
-constexpr int PAGED_WAVES = 4, WHOLE_WAVES = 4;
+constexpr int PAGED_WAVES = 4;
+
+// A part: `heads` (up to 16) times 64 sums, then (m, l) of each head; l is -1 where no key was there. PART_HEAD
+// floats a head keep the parts 16-byte aligned.
+struct Part {
+  const int heads;
+  __device__ inline explicit Part(int G) : heads(min(G, 16)) {}
+  __device__ inline long size() const { return heads * long(PART_HEAD); }
+  __device__ inline int ml(int g) const { return heads * 64 + g * 2; }
+};
+
+// What the waves of a block ended with. Waves r, r + 1, ... whose last part is of one sequence, the later ones' only
+// part, join in LDS: wave d adds up channels 16 d + (0..15). The result is written normalised if the sequence lies in
+// them as a whole, else as one part in the place of the first of them.
+struct BlockEnds {
+  int seq[PAGED_WAVES];  // -1: nothing left to write
+  bool only[PAGED_WAVES], begins[PAGED_WAVES], ends[PAGED_WAVES];
+};
+template <typename T, typename Wave, typename Place>
+__device__ inline void join_block(const PagedArgs& p, const Wave& w, char* smem, BlockEnds& at, int wave, int head, bool in,
+                                  const Part& part, Place&& place) {
+  const int lane = w.lane, col = lane & 15, g = lane >> 4;
+  float* own = reinterpret_cast<float*>(smem + wave * STAGES * TILE_BYTES);  // its tiles are used up
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) own[(d * 4 + r) * 64 + lane] = w.o[d][r];
+  if (lane < 16) {
+    float* ml = own + 1024 + lane * 4;
+    ml[0] = w.m;
+    ml[1] = w.l;
+    ml[2] = __int_as_float(w.some);
+  }
+  __syncthreads();
+  for (int r = 0; r < PAGED_WAVES;) {
+    const int seq = at.seq[r];
+    int e = r + 1;
+    while (seq >= 0 && e < PAGED_WAVES && at.seq[e] == seq && at.only[e]) ++e;
+    if (seq >= 0) {
+      float mn = -INFINITY, sum = 0.f, f[PAGED_WAVES], v[4] = {};
+      int some = 0;
+      auto state = [&](int k) { return reinterpret_cast<const float*>(smem + k * STAGES * TILE_BYTES); };
+#pragma unroll
+      for (int k = 0; k < PAGED_WAVES; ++k)
+        if (k >= r && k < e) mn = fmaxf(mn, state(k)[1024 + col * 4]);
+#pragma unroll
+      for (int k = 0; k < PAGED_WAVES; ++k) {
+        if (k < r || k >= e) continue;
+        const float* ml = state(k) + 1024 + col * 4;
+        const int had = __float_as_int(ml[2]);
+        f[k] = !had || ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mn);
+        if (!had) continue;  // no key: its sums are zeros, whatever the others hold
+        some = 1;
+        sum += ml[1] * f[k];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] += state(k)[(wave * 4 + c) * 64 + lane] * f[k];
+      }
+      if (in) {
+        if (at.begins[r] && at.ends[e - 1]) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = some ? v[c] / sum : 0.f;
+          T* out = static_cast<T*>(p.out) + seq * p.ldo + long(head) * 64 + 16 * wave + 4 * g;
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+          else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        } else {
+          float* to = place(r, at.only[r]);
+          *reinterpret_cast<float4*>(to + col * 64 + 16 * wave + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
+          if (wave == 0 && g == 0) *reinterpret_cast<float2*>(to + part.ml(col)) = make_float2(mn, some ? sum : -1.f);
+        }
+      }
+    }
+    r = e;
+  }
+}
 
 // One block a (sequence, group of up to 16 heads of one key head): its waves take equal parts of the tiles
 // and join their sums in LDS.
 template <typename T, bool SPARSE>
-__global__ void __launch_bounds__(WHOLE_WAVES * 64, 8 / WHOLE_WAVES) paged_whole_kernel(const PagedArgs p, const int* sel, int topk, float scale) {
+__global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const PagedArgs p, const int* sel, int topk, float scale) {
   using Wave = PagedWave<T, SPARSE>;
-  __shared__ __attribute__((aligned(1024))) char smem[WHOLE_WAVES * STAGES * TILE_BYTES];
+  __shared__ __attribute__((aligned(1024))) char smem[PAGED_WAVES * STAGES * TILE_BYTES];
+  __shared__ BlockEnds ends;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int G = p.heads / p.cache.kv_heads, parts = (G + 15) / 16;
-  const int i = blockIdx.x, kh = int(blockIdx.y) / parts, g0 = int(blockIdx.y) % parts * 16;
+  const int G = p.heads / p.cache.kv_heads, groups = (G + 15) / 16;
+  const int i = blockIdx.x, kh = int(blockIdx.y) / groups, g0 = int(blockIdx.y) % groups * 16;
   const int col = lane & 15, head = kh * G + g0 + col;
   char* ring = smem + wave * STAGES * TILE_BYTES;
   Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
   w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
   w.begin(i);
+  if (threadIdx.x < PAGED_WAVES) {
+    ends.seq[threadIdx.x] = i;
+    ends.only[threadIdx.x] = ends.begins[threadIdx.x] = ends.ends[threadIdx.x] = true;
+  }
   // every fourth tile: the first ones do not hang on the length
-  w.run(wave, WHOLE_WAVES, tiles_in<Wave::KEYS>(w.len, p.cache, topk), scale);
+  w.run(wave, PAGED_WAVES, tiles_in<Wave::KEYS>(w.len, p.cache, topk), scale);
   w.l = sum_groups(w.l);
-  // the join: every wave's m, l and whether it had keys, then the sums moved to the common reference
-  float* ml = reinterpret_cast<float*>(smem);
-  __syncthreads();
-  if (lane < 16) {
-    float* at = ml + (wave * 16 + lane) * 4;
-    at[0] = w.m;
-    at[1] = w.l;
-    at[2] = __int_as_float(w.some);
-  }
-  __syncthreads();
-  float mn = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < WHOLE_WAVES; ++k) mn = fmaxf(mn, ml[(k * 16 + col) * 4]);
-  float sum = 0.f;
-  int some = 0;
-#pragma unroll
-  for (int k = 0; k < WHOLE_WAVES; ++k) {
-    const float* at = ml + (k * 16 + col) * 4;
-    if (!__float_as_int(at[2])) continue;
-    some = 1;
-    sum += at[1] * (at[0] == -INFINITY ? 0.f : exp2f(at[0] - mn));
-  }
-  const float keep = !w.some ? 0.f : w.m == -INFINITY ? 0.f : exp2f(w.m - mn);
-  float* os = ml + 1024;  // [wave][d][r][lane]
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) os[((wave * 4 + d) * 4 + r) * 64 + lane] = w.some ? w.o[d][r] * keep : 0.f;
-  __syncthreads();
-  if (g0 + col >= G || wave >= 4) return;
-  // wave d writes channels 16 d + 4 (lane / 16) + (0..3)
-  float v[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    float a = 0.f;
-#pragma unroll
-    for (int k = 0; k < WHOLE_WAVES; ++k) a += os[((k * 4 + wave) * 4 + r) * 64 + lane];
-    v[r] = some ? a / sum : 0.f;
-  }
-  T* out = static_cast<T*>(p.out) + i * p.ldo + long(head) * 64 + 16 * wave + 4 * (lane >> 4);
-  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
-  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+  join_block<T>(p, w, smem, ends, wave, head, g0 + col < G, Part(G), [](int, bool) { return static_cast<float*>(nullptr); });
 }
 
 // Long or uneven sequences: the tiles of all sequences in a row, cut into one equal part a wave. A sequence that
-// lies within one part is written at once; of the others each wave leaves its part's sums, unnormalised, for
-// paged_join_kernel: slot 0 for the sequence that the part begins in, slot 1 for one that it ends in.
+// lies within one part or one block's is written at once; of the others the parts' sums, unnormalised, are left
+// for paged_join_kernel: slot 0 for the sequence that a wave's part begins in, slot 1 for one that it ends in. With
+// span = PAGED_WAVES the parts that a block's waves end with are joined where they are of one sequence, so that a
+// long sequence leaves one part a block instead of one a wave (span = 1).
 constexpr int SCAN_MAX = 1024;
 
 
@@ -749,21 +786,13 @@ template <int KEYS> __global__ void __launch_bounds__(1024) paged_scan_kernel(co
   scan_tiles<KEYS, 1024>(p, topk, before);
 }
 
-// A part: `heads` (up to 16) times 64 sums, then (m, l) of each head; l is -1 where no key was there. PART_HEAD
-// floats a head keep the parts 16-byte aligned.
-struct Part {
-  const int heads;
-  __device__ inline explicit Part(int G) : heads(min(G, 16)) {}
-  __device__ inline long size() const { return heads * long(PART_HEAD); }
-  __device__ inline int ml(int g) const { return heads * 64 + g * 2; }
-};
-
 template <typename T, bool SPARSE, bool SCAN>
 __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const PagedArgs p, const int* sel, int topk, float scale,
-                                                                          int workers, long* before, float* parts) {
+                                                                          int workers, int span, long* before, float* parts) {
   using Wave = PagedWave<T, SPARSE>;
   __shared__ __attribute__((aligned(1024))) char smem[PAGED_WAVES * STAGES * TILE_BYTES];
   __shared__ long own[SCAN ? SCAN_MAX + 1 : 1];
+  __shared__ BlockEnds ends;
   const long* pre = before;
   if constexpr (SCAN) {  // few sequences: every block counts for itself, one leaves the counts for the join
     scan_tiles<Wave::KEYS, PAGED_WAVES * 64>(p, topk, own);
@@ -777,52 +806,75 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
   const int col = lane & 15, head = kh * G + g0 + col;
   const long worker = long(blockIdx.x) * PAGED_WAVES + wave, total = pre[p.n];
   const long W = min(long(workers), total);  // each has a tile at least
-  if (worker >= W) return;
-  long t = quotient(total * worker, W);
-  const long end = quotient(total * (worker + 1), W);
+  if (long(blockIdx.x) * PAGED_WAVES >= W) return;
   const Part part(G);
+  auto place = [&](long worker, bool only) { return parts + ((worker * cols + blockIdx.y) * 2 + (only ? 0 : 1)) * part.size(); };
   char* ring = smem + wave * STAGES * TILE_BYTES;
   Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
-  int lo = 0, hi = p.n;  // the sequence that tile t belongs to
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (pre[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  const long first = t;
-  for (int i = uniform(lo); t < end; i = uniform(i + 1)) {
-    const long b0 = pre[i], b1 = pre[i + 1];
-    const long stop = min(end, b1);
-    if (stop <= t) continue;
-    w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
-    w.begin(i);
-    w.run(uniform(int(t - b0)), 1, uniform(int(stop - b0)), scale);
-    w.l = sum_groups(w.l);
-    if (g0 + col < G) {
+  w.m = w.l = 0.f;
+  w.some = 0;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) w.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int last = -1;
+  bool only = false, begins = false, stops = false;
+  if (worker < W) {
+    long t = quotient(total * worker, W);
+    const long first = t, end = quotient(total * (worker + 1), W);
+    int lo = 0, hi = p.n;  // the sequence that tile t belongs to
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    for (int i = uniform(lo); t < end; i = uniform(i + 1)) {
+      const long b0 = pre[i], b1 = pre[i + 1];
+      const long stop = min(end, b1);
+      if (stop <= t) continue;
+      w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
+      w.begin(i);
+      w.run(uniform(int(t - b0)), 1, uniform(int(stop - b0)), scale);
+      w.l = sum_groups(w.l);
       if (t == b0 && stop == b1) {
-        w.store(i, head, w.l);
-      } else {
-        float* at = parts + ((worker * cols + blockIdx.y) * 2 + (t == first ? 0 : 1)) * part.size();
+        if (g0 + col < G) w.store(i, head, w.l);
+      } else if (stop == end && span > 1) {  // for the join with the next waves
+        last = i;
+        only = t == first;
+        begins = t == b0;
+        stops = stop == b1;
+      } else if (g0 + col < G) {
+        float* at = place(worker, t == first);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
           *reinterpret_cast<float4*>(at + col * 64 + 16 * d + 4 * (lane >> 4)) = make_float4(w.o[d][0], w.o[d][1], w.o[d][2], w.o[d][3]);
         if (lane < 16) *reinterpret_cast<float2*>(at + part.ml(col)) = make_float2(w.m, w.some ? w.l : -1.f);
       }
+      t = stop;
     }
-    t = stop;
   }
+  if (span == 1) return;
+  if (lane == 0) {
+    ends.seq[wave] = last;
+    ends.only[wave] = only;
+    ends.begins[wave] = begins;
+    ends.ends[wave] = stops;
+  }
+  const long worker0 = long(blockIdx.x) * PAGED_WAVES;
+  join_block<T>(p, w, smem, ends, wave, head, g0 + col < G, part, [&](int r, bool only) { return place(worker0 + r, only); });
 }
 
-// One block a (sequence, group of heads): the parts of a sequence that several waves had. SPLIT waves share a head
-// (all eight where the group has one), each with every SPLIT-th part, a channel a lane, JOIN_PARTS parts under way.
+// One block a (sequence, `per` heads of a group): the parts of a sequence that several waves had. SPLIT waves share a
+// head (all eight where the block has one), each with every SPLIT-th part, a channel a lane, JOIN_PARTS parts under way.
 // Bound by its chain of loads (counts, then parts), not by their bytes.
-constexpr int JOIN_WAVES = 8, JOIN_PARTS = 12;
+constexpr int JOIN_WAVES = 8, JOIN_PARTS = 8;
 template <typename T>
-__global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const PagedArgs p, int workers, const long* before, const float* parts) {
+__global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const PagedArgs p, int workers, int span, int per, const long* before, const float* parts) {
   __shared__ float accs[JOIN_WAVES][64], sums[JOIN_WAVES], refs[JOIN_WAVES];
   __shared__ int somes[JOIN_WAVES];
-  const int i = blockIdx.x, col = blockIdx.y, G = p.heads / p.cache.kv_heads, groups = (G + 15) / 16, cols = p.cache.kv_heads * groups;
-  const int head0 = col / groups * G + col % groups * 16, heads = min(16, G - col % groups * 16);
+  const int i = blockIdx.x, G = p.heads / p.cache.kv_heads, groups = (G + 15) / 16, cols = p.cache.kv_heads * groups;
+  const int blocks = (min(G, 16) + per - 1) / per, col = blockIdx.y / blocks, first_head = blockIdx.y % blocks * per;  // in the group
+  const int group = col % groups * 16, heads = min(per, min(16, G - group) - first_head);
+  if (heads <= 0) return;
+  const int head0 = col / groups * G + group + first_head;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const long b0 = before[i], b1 = before[i + 1], total = before[p.n];
   T* out = static_cast<T*>(p.out) + i * p.ldo + long(head0) * 64;
@@ -834,13 +886,18 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const Paged
   const long W = min(long(workers), total);
   const long w0 = quotient((b0 + 1) * W - 1, total), w1 = quotient(b1 * W - 1, total);
   if (w0 == w1) return;  // written whole
-  const int count = int(w1 - w0) + 1;
+  // Each `span` workers (one, or a block's) leave one part in the place of the first; the last worker's is one of its
+  // own where it went on to other sequences.
+  const bool went_on = quotient(total * (w1 + 1), W) != b1;
+  const long block0 = w0 / span, block1 = (went_on ? w1 - 1 : w1) / span;
+  if (!went_on && block0 == block1) return;  // written whole
+  const int joined = int(block1 - block0) + 1, count = joined + went_on;
   const Part layout(G);
-  // only the first part can be the second of its worker
-  const long step = 2 * cols * layout.size();
-  const float* at0 = parts + (w0 * cols + col) * 2 * layout.size();
-  const float* first = at0 + (quotient(total * w0, W) >= b0 ? 0 : layout.size());
-  auto part = [&](int k) { return k ? at0 + k * step : first; };
+  // floats from `parts`: below 2^31, as the plan's sizes are
+  const int size = int(layout.size()) * 2, step = span * cols * size, base = int(block0) * step + col * size;
+  const int first = int(w0) * cols * size + col * size + (quotient(total * w0, W) < b0 ? size / 2 : 0);  // w0's second part
+  const int last = int(w1) * cols * size + col * size;
+  auto part = [&](int k) { return parts + (k == 0 ? first : k < joined ? base + k * step : last); };
   const int split = heads >= 5 ? 1 : JOIN_WAVES / heads, at_once = JOIN_WAVES / split;
   for (int g0 = 0; g0 < heads; g0 += at_once) {
     const int g = g0 + wave / split;
@@ -854,8 +911,8 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const Paged
         for (int u = 0; u < JOIN_PARTS; ++u) {
           const int k = min(k0 + u * split, count - 1);
           const float* at = part(k);
-          ml[u] = *reinterpret_cast<const float2*>(at + layout.ml(g));
-          o[u] = at[g * 64 + lane];
+          ml[u] = *reinterpret_cast<const float2*>(at + layout.ml(first_head + g));
+          o[u] = at[(first_head + g) * 64 + lane];
         }
 #pragma unroll
         for (int u = 0; u < JOIN_PARTS; ++u)
@@ -1105,7 +1162,7 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
   for (int e = total + tid; e < topk; e += THREADS) out[e] = -1;
 }
 
-constexpr long QK_WAVES = 8192;
+constexpr long QK_WAVES = 8192, JOIN_BLOCKS = 256;
 
 // Runs fn with the storage type dt as a value.
 template <typename F> void by_type(int dt, F&& fn) {
@@ -1182,17 +1239,20 @@ void attend(const Exec& ex, const PagedArgs& a, const int* sel, int topk, char* 
     using T = decltype(t);
     constexpr bool S = decltype(sparse)::value;
     if (!plan.workers) {
-      paged_whole_kernel<T, S><<<dim3(a.n, plan.cols), WHOLE_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale);
+      paged_whole_kernel<T, S><<<dim3(a.n, plan.cols), PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale);
       return;
     }
     const dim3 grid(plan.workers / PAGED_WAVES, plan.cols);
+    const int span = plan.workers >= 128L * a.n ? PAGED_WAVES : 1;
     if (a.n <= SCAN_MAX) {
-      paged_parts_kernel<T, S, true><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
+      paged_parts_kernel<T, S, true><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, span, before, parts);
     } else {
       paged_scan_kernel<TileOps<T>::KEYS><<<1, 1024, 0, ex.stream>>>(a, topk, before);
-      paged_parts_kernel<T, S, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, before, parts);
+      paged_parts_kernel<T, S, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, span, before, parts);
     }
-    paged_join_kernel<T><<<dim3(a.n, plan.cols), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.workers, before, parts);
+    // a head a block, with eight waves on its parts, until there are blocks enough
+    const int most = std::min(a.heads / a.cache.kv_heads, 16), per = int(std::min<long>(most, std::max<long>(1, long(a.n) * a.heads / JOIN_BLOCKS)));
+    paged_join_kernel<T><<<dim3(a.n, plan.cols * cdiv(most, per)), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.workers, span, per, before, parts);
   };
   by_type(a.cache.dt, [&](auto t) {
     if (topk) launch(t, std::true_type());

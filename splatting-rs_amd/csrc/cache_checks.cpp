@@ -69,6 +69,9 @@ void check_attention(PagedArgs& a) {
   SPLAT_CHECK(long(a.n) * a.heads <= (1 << 24), BAD_ARGUMENT, "attention: more than 2^24 query rows");
   check_width(a.width, a.cache.page_size);
   SPLAT_CHECK(a.max_len >= 0, BAD_ARGUMENT, "attention: max_len is negative");
+  // the kernels divide tile counts times waves (up to 2^13) as 64-bit floats
+  SPLAT_CHECK(long(a.n) * std::min<long>(a.max_len, long(a.width) * a.cache.page_size) < (1L << 38), BAD_ARGUMENT,
+              "attention: more than 2^38 positions");
   SPLAT_CHECK(std::isfinite(a.scale), BAD_ARGUMENT, "attention: scale is not finite");
   if (a.n == 0) return;
   SPLAT_CHECK(a.q && a.table && a.lens && a.out, BAD_ARGUMENT, "attention: a required pointer is NULL");
