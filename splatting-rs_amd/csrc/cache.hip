@@ -969,54 +969,74 @@ __device__ inline uint64_t order_of(double s) {
 // The most that q k can be for a key between the page's bounds, summed over the group's heads, is
 // sum_c hi_c A_c + lo_c B_c, with A and B the sums of the positive and the negative parts of the heads' queries:
 // 128 products a page, however many heads share it. In 64 bits: which of two pages next to the border is
-// taken can hang on less than 32 bits hold. 8 lanes a page, 16 products each, 16 pages a wave whose loads fly
-// together; bound by its two dependent loads (the table's entry, the bounds).
+// taken can hang on less than 32 bits hold. 8 lanes a page, 16 products each.
+template <typename T> struct PageScore {
+  const PagedArgs& p;
+  const T* bounds;
+  const int kh, lane;
+  double A[8], B[8];
+  __device__ inline void load_q(int i) {
+    const int G = p.heads / p.cache.kv_heads, j = lane & 7;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) A[e] = B[e] = 0.0;
+    for (int g0 = 0; g0 < G; g0 += 4) {  // four heads under way
+      float x[4][8] = {};
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (g0 + g < G) load8(static_cast<const T*>(p.q) + i * p.ldq + (long(kh) * G + g0 + g) * 64 + j * 8, x[g]);
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          A[e] += x[g][e] > 0.f ? double(x[g][e]) : 0.0;
+          B[e] += x[g][e] > 0.f ? 0.0 : double(x[g][e]);
+        }
+    }
+  }
+  // 16 pages, two for each 8 lanes: page[k] is place + 8 k's (below 0: none); put(place, key) once for each place.
+  template <typename Put> __device__ inline void score(const int (&page)[2], int place, Put&& put) const {
+    const int j = lane & 7;
+    float lo[2][8] = {}, hi[2][8] = {};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (page_ok(page[k], p.cache.pages)) {
+        const T* at = bounds + (long(page[k]) * p.cache.kv_heads + kh) * 128 + j * 8;
+        load8(at, lo[k]);
+        load8(at + 64, hi[k]);
+      }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      double s = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += double(lo[k][e]) * B[e] + double(hi[k][e]) * A[e];
+      s = sum8(s);
+      if (j == 0) put(place + 8 * k, page_ok(page[k], p.cache.pages) ? order_of(s) : 0);
+    }
+  }
+};
+
+// A wave takes 16 pages of one (sequence, key head); bound by its two dependent loads (the table's entry with the
+// length, the bounds) and, in 64 bits, its products.
 constexpr int SCORE_PAGES = 64;  // a block
 template <typename T>
 __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, const T* bounds, int maxp, uint64_t* keys) {
   const KvCache& c = p.cache;
   const int chunks = (maxp + SCORE_PAGES - 1) / SCORE_PAGES, chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks;
-  const int i = pair / c.kv_heads, kh = pair % c.kv_heads, G = p.heads / c.kv_heads;
-  const int lane = threadIdx.x & 63, j = lane & 7;
+  const int i = pair / c.kv_heads, lane = threadIdx.x & 63;
   const int held = int((long(length_of(uload(p.lens + i), p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
   const int p0 = chunk * SCORE_PAGES + (threadIdx.x >> 6) * 16 + (lane >> 3);
   int page[2];  // read together with the length, whatever it is
 #pragma unroll
   for (int k = 0; k < 2; ++k) page[k] = p.table[long(i) * p.width + min(p0 + 8 * k, p.width - 1)];
   if (chunk * SCORE_PAGES >= held) return;
+  PageScore<T> score{p, bounds, pair % c.kv_heads, lane};
+  score.load_q(i);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if (p0 + 8 * k >= held) page[k] = -1;
-  double A[8] = {}, B[8] = {};
-  for (int g0 = 0; g0 < G; g0 += 4) {  // four heads under way
-    float x[4][8] = {};
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      if (g0 + g < G) load8(static_cast<const T*>(p.q) + i * p.ldq + (long(kh) * G + g0 + g) * 64 + j * 8, x[g]);
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        A[e] += x[g][e] > 0.f ? double(x[g][e]) : 0.0;
-        B[e] += x[g][e] > 0.f ? 0.0 : double(x[g][e]);
-      }
-  }
-  float lo[2][8] = {}, hi[2][8] = {};
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (page_ok(page[k], c.pages)) {
-      const T* at = bounds + (long(page[k]) * c.kv_heads + kh) * 128 + j * 8;
-      load8(at, lo[k]);
-      load8(at + 64, hi[k]);
-    }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    double s = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s += double(lo[k][e]) * B[e] + double(hi[k][e]) * A[e];
-    s = sum8(s);
-    if (j == 0 && p0 + 8 * k < held) keys[long(pair) * maxp + p0 + 8 * k] = page_ok(page[k], c.pages) ? order_of(s) : 0;
-  }
+  score.score(page, p0, [&](int at, uint64_t key) {
+    if (at < held) keys[long(pair) * maxp + at] = key;
+  });
 }
 
 // One block a (sequence, key head): the topk largest keys' places, ascending, the lowest place first among equal
@@ -1025,10 +1045,12 @@ __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, cons
 // next range: two rounds for most scores, seven at most. Counts do not hang on the order of the atomic adds, and
 // every wave reads all bins for itself, so that a round has one barrier: of three sets of bins one is counted
 // into, one cleared, and one may still be read. What bounds the kernel is the chain of these steps.
-// Thread t holds keys [t K, (t + 1) K) in registers (K > 0), or reads them every round (K = 0, `k` each).
+// Thread t holds keys [t K, (t + 1) K) in registers (K > 0), or reads them every round (K = 0, `k` each). FUSED (K = 1, a
+// wave for every 16 pages): the block scores the pages itself, a launch less for sequences of few pages.
 constexpr int SELECT_BINS = 512;
-template <int THREADS, int K>
-__global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, int maxp, int k, int topk, int* sel) {
+template <int THREADS, int K, typename T = void>
+__global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, const void* bounds, int maxp, int k, int topk, int* sel) {
+  constexpr bool FUSED = !std::is_void<T>::value;
   constexpr int WAVES = THREADS / 64, EACH = SELECT_BINS / 64;
   __shared__ __attribute__((aligned(16))) int bins[3][SELECT_BINS];
   __shared__ int room[2][WAVES];
@@ -1038,7 +1060,7 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
   const uint64_t* in = keys + long(blockIdx.x) * maxp;
   int* out = sel + long(blockIdx.x) * topk;
   uint64_t mine[K > 0 ? K : 1];
-  if constexpr (K > 0) {  // with the length, whatever it is
+  if constexpr (K > 0 && !FUSED) {  // with the length, whatever it is
     k = K;
 #pragma unroll
     for (int e = 0; e < K; ++e) mine[e] = tid * K + e < maxp ? in[tid * K + e] : 0;
@@ -1046,6 +1068,22 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
   const int held = int((long(length_of(uload(p.lens + i), p.width, c.shift, p.max_len)) + c.page_size - 1) >> c.shift);
   const int newest = held - 1;
   const bool newest_there = held > 0 && page_ok(uload(p.table + long(i) * p.width + max(newest, 0)), c.pages);
+  if constexpr (FUSED) {
+    static_assert(K == 1, "a key a thread");
+    __shared__ uint64_t scored[WAVES * 16];
+    PageScore<T> score{p, static_cast<const T*>(bounds), int(blockIdx.x % c.kv_heads), lane};
+    const int at = wave * 16 + (lane >> 3);
+    int page[2];  // read together with the length, whatever it is
+#pragma unroll
+    for (int e = 0; e < 2; ++e) page[e] = p.table[long(i) * p.width + min(at + 8 * e, p.width - 1)];
+    score.load_q(i);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (at + 8 * e >= held) page[e] = -1;
+    score.score(page, at, [&](int place, uint64_t key) { scored[place] = key; });
+    __syncthreads();
+    mine[0] = tid < WAVES * 16 ? scored[tid] : 0;
+  }
   // fn(place, key) for this thread's places before the newest; 0: no page there
   auto each = [&](auto&& fn) {
     if constexpr (K > 0) {
@@ -1163,6 +1201,7 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
 }
 
 constexpr long QK_WAVES = 8192, JOIN_BLOCKS = 256;
+constexpr int FUSE_MAX = 128;
 
 // Runs fn with the storage type dt as a value.
 template <typename F> void by_type(int dt, F&& fn) {
@@ -1283,16 +1322,21 @@ void sparse_attention(const Exec& ex, const SparseArgs& args, void* workspace, s
   uint64_t* keys = reinterpret_cast<uint64_t*>(ws + paged_plan(a.cache, a.n, a.heads, a.max_len, s.topk).bytes);
   by_type(a.cache.dt, [&](auto t) {
     using T = decltype(t);
-    if (maxp > 0)
-      page_score_kernel<T><<<pairs * cdiv(maxp, SCORE_PAGES), 256, 0, ex.stream>>>(a, static_cast<const T*>(s.bounds), maxp, keys);
+    auto select = [&](auto kernel, int threads) {
+      kernel<<<pairs, threads, 0, ex.stream>>>(a, keys, s.bounds, maxp, cdiv(maxp, threads), s.topk, s.selected);
+    };
+    if (maxp <= FUSE_MAX) {
+      // 16 pages a wave, all at once
+      if (maxp <= 64) select(page_select_kernel<256, 1, T>, 256);
+      else select(page_select_kernel<512, 1, T>, 512);
+      return;
+    }
+    page_score_kernel<T><<<pairs * cdiv(maxp, SCORE_PAGES), 256, 0, ex.stream>>>(a, static_cast<const T*>(s.bounds), maxp, keys);
+    if (maxp <= 1024) select(page_select_kernel<256, 4>, 256);
+    else if (maxp <= 4096) select(page_select_kernel<512, 8>, 512);
+    else if (maxp <= 16384) select(page_select_kernel<1024, 16>, 1024);
+    else select(page_select_kernel<1024, 0>, 1024);
   });
-  auto select = [&](auto kernel, int threads) {
-    kernel<<<pairs, threads, 0, ex.stream>>>(a, keys, maxp, cdiv(maxp, threads), s.topk, s.selected);
-  };
-  if (maxp <= 1024) select(page_select_kernel<256, 4>, 256);
-  else if (maxp <= 4096) select(page_select_kernel<512, 8>, 512);
-  else if (maxp <= 16384) select(page_select_kernel<1024, 16>, 1024);
-  else select(page_select_kernel<1024, 0>, 1024);
   attend(ex, a, s.selected, s.topk, ws);
   SPLAT_HIP(hipGetLastError());
 }

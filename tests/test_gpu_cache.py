@@ -435,6 +435,8 @@ PAGED = [
     ([127, 128, 129], 8, 1, 32), ([255, 256, 257], 16, 1, 64), ([500, 1, 300], 17, 1, 256), ([600, 0, 1037], 40, 2, 64),
     ([973], 6, 6, 128), ([2000, 3, 1111], 20, 4, 16), ([6223], 12, 12, 16), ([4096, 4097], 8, 2, 8), ([10000, 17], 6, 3, 64),
     ([24889], 1, 1, 16), ([5] * 40, 3, 3, 8), ([700] * 9, 33, 1, 32), ([13000, 5000], 24, 8, 256),
+    # parts of a block joined, sequences that end inside one, and more sequences than a block sums up
+    ([9000, 1, 0, 7000, 40], 16, 1, 16), ([3000, 3001, 2999, 64, 0, 1], 2, 1, 8), ([1500] + [3, 0, 40] * 400, 2, 1, 8),
 ]
 
 
@@ -672,6 +674,7 @@ SPARSE = [
     ([1], 1, 1, 8, 1), ([100, 0, 9], 4, 2, 8, 1), ([100, 0, 8], 4, 4, 8, 3), ([300, 31], 12, 12, 16, 7), ([1037, 16], 8, 1, 16, 64),
     ([1037, 500, 700], 17, 1, 16, 20), ([2000], 6, 6, 8, 100), ([5000, 4999], 16, 4, 32, 33), ([9000], 3, 3, 8, 1024), ([640] * 6, 20, 4, 64, 200),
     ([6223], 2, 2, 16, 16), ([20000, 300], 2, 1, 8, 300), ([3000], 33, 3, 256, 2),
+    ([1500] + [3, 0, 40] * 400, 2, 1, 8, 150),   # more sequences than a block sums up
 ]
 
 
@@ -685,16 +688,26 @@ def test_sparse_attention(ctx, dtype, lens, heads, kv, ps, topk):
     check_sparse(c, c.table, b, q, heads, topk, out, sel)
 
 
+@pytest.mark.parametrize("longest", [50, 100, 128, 129, 291, 1025, 4200])   # pages: every way that a page is scored and taken
 @pytest.mark.parametrize("topk", [1, 2, 5, 63, 64, 65, 300])
-def test_sparse_attention_equal_scores_go_to_the_lower_page(ctx, topk):
+def test_sparse_attention_equal_scores_go_to_the_lower_page(ctx, topk, longest):
     """Bounds from three values only, in all pages of two sequences: many pages score alike."""
-    c = Cache("bf16", [16 * 290 + 3, 16 * 40], 2, 16)
+    ps = 8 if longest > 1000 else 16
+    c = Cache("bf16", [ps * (longest - 1) + 3, ps * 40], 2, ps)
     g = torch.Generator().manual_seed(topk)
     kinds = torch.randn(3, 2, 2, 64, generator=g).sort(2).values.to(torch.bfloat16)
     b = kinds[torch.randint(0, 3, (c.pages,), generator=g)]
     q = queries(c, 4)
     out, sel = run_sparse(ctx, c, q, 4, b, topk)
     check_sparse(c, c.table, b, q, 4, topk, out, sel)
+
+
+def test_sparse_attention_over_more_pages_than_registers_hold(ctx):
+    c = Cache("bf16", [8 * 16500 - 5], 1, 8, garbage=False)
+    q, b = queries(c, 2), page_bounds_of(c)
+    for topk in (1, 300, 20000):
+        out, sel = run_sparse(ctx, c, q, 2, b, topk)
+        check_sparse(c, c.table, b, q, 2, topk, out, sel)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
