@@ -392,12 +392,30 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int int32x4_v __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(3))) char* lds_cptr;
 
-// 16 bytes a lane from `base + off` into LDS at lds + 16 * lane; offsets from `bytes` on read as zeros.
-__device__ inline void load_lds(const void* base, uint32_t bytes, uint32_t off, uint32_t lds) {
+// N loads of 16 bytes a lane, 1 KB each, from base + off[k] + 1024 k into LDS at lds + 1024 k + 16 * lane; offsets
+// from `bytes` on read as zeros. The instruction's offset goes into both addresses.
+template <int N> __device__ inline void load_lds(const void* base, uint32_t bytes, const uint32_t (&off)[4], int p, uint32_t lds) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   const int32x4_v r = {uniform(int(uint32_t(a))), uniform(int(uint32_t(a >> 32))), uniform(int(bytes)), 0x00020000};
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(uniform(int(lds))), "v"(off), "s"(r)
-               : "memory");
+  const int m0 = uniform(int(lds));
+  if constexpr (N == 4)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 lds\n\t"
+        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 lds\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 lds" ::"s"(m0),
+        "v"(off[p]), "v"(off[p + 1]), "v"(off[p + 2]), "v"(off[p + 3]), "s"(r)
+        : "memory");
+  else if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+        "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds" ::"s"(m0),
+        "v"(off[p]), "v"(off[p + 1]), "s"(r)
+        : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off[p]), "s"(r) : "memory");
 }
 template <int N> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
@@ -546,32 +564,43 @@ template <typename T, bool SPARSE> struct PagedWave {
     some = 0;
   }
 
-  // Loads tile t into slot b of the ring; the rows of each piece that are there, 8 bits a piece. The table's entries
-  // are read whatever the length is, so that both loads are under way together.
-  __device__ inline uint32_t issue(int t, int b) {
+  // Loads tile t, which lies in E pages, into slot b of the ring; the rows of each piece that are there, 8 bits a piece.
+  // The table's entries are read whatever the length is, so that both loads are under way together.
+  template <int E> __device__ inline uint32_t load_tile(int t, int b) {
+    constexpr int PIECES = 4 / E, ROWS = PIECES * PIECE;  // of one page
     const KvCache& c = p.cache;
-    const int ps = c.page_size;
-    uint32_t there = 0;
-    int place[4], entry[4];
+    uint32_t k_off[4], v_off[4], there = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int e = (t * KEYS + k * PIECE) >> c.shift;
-      place[k] = SPARSE ? e < topk ? uload(chosen + min(e, topk - 1)) : -1 : e;
+      k_off[k] = Ops::k_off(lane, k);
+      v_off[k] = Ops::v_off(lane, k);
+    }
+    int place[E], entry[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int at = (t * KEYS + e * ROWS) >> c.shift;
+      place[e] = SPARSE ? at < topk ? uload(chosen + min(at, topk - 1)) : -1 : at;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) entry[k] = uload(row + (SPARSE ? max(min(place[k], p.width - 1), 0) : min(place[k], p.width - 1)));
+    for (int e = 0; e < E; ++e) entry[e] = uload(row + (SPARSE ? max(min(place[e], p.width - 1), 0) : min(place[e], p.width - 1)));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int in_page = (t * KEYS + k * PIECE) & (ps - 1);
-      const bool ok = place[k] >= 0 && place[k] < held && page_ok(entry[k], c.pages);
-      const int rows = ok ? max(0, min(PIECE, len - (place[k] << c.shift) - in_page)) : 0;
-      there |= uint32_t(rows) << (8 * k);
-      const long at = (ok ? page_at(c, entry[k], kh) : 0) + long(in_page) * 64;
-      const uint32_t bytes = uint32_t(rows) * 64 * sizeof(T), to = lds + b * TILE_BYTES + k * 1024;
-      load_lds(static_cast<const T*>(c.k) + at, bytes, Ops::k_off(lane, k), to);
-      load_lds(static_cast<const T*>(c.v) + at, bytes, Ops::v_off(lane, k), to + TILE_BYTES / 2);
+    for (int e = 0; e < E; ++e) {
+      const int in_page = E > 1 ? 0 : (t * KEYS) & (c.page_size - 1);
+      const bool ok = place[e] >= 0 && place[e] < held && page_ok(entry[e], c.pages);
+      const int rows = ok ? max(0, min(ROWS, len - (place[e] << c.shift) - in_page)) : 0;
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) there |= uint32_t(max(0, min(PIECE, rows - k * PIECE))) << (8 * (e * PIECES + k));
+      const long at = (ok ? page_at(c, entry[e], kh) : 0) + in_page * 64;
+      const uint32_t bytes = uint32_t(rows) * 64 * sizeof(T), to = lds + b * TILE_BYTES + e * PIECES * 1024;
+      load_lds<PIECES>(static_cast<const T*>(c.k) + at, bytes, k_off, e * PIECES, to);
+      load_lds<PIECES>(static_cast<const T*>(c.v) + at, bytes, v_off, e * PIECES, to + TILE_BYTES / 2);
     }
     return uniform(int(there));
+  }
+  __device__ inline uint32_t issue(int t, int b) {
+    if (p.cache.page_size >= KEYS) return load_tile<1>(t, b);
+    if (KEYS == 16 || p.cache.page_size == 16) return load_tile<2>(t, b);
+    return load_tile<4>(t, b);
   }
 
   __device__ inline void tile(int b, uint32_t there, float scale) {
@@ -1200,7 +1229,7 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
   for (int e = total + tid; e < topk; e += THREADS) out[e] = -1;
 }
 
-constexpr long QK_WAVES = 8192, JOIN_BLOCKS = 256;
+constexpr long QK_WAVES = 24576, JOIN_BLOCKS = 256;
 constexpr int FUSE_MAX = 128;
 
 // Runs fn with the storage type dt as a value.
