@@ -120,8 +120,8 @@ int splat_kernel_reconstruct(splat_ctx* ctx, int V, int H, int W, const float* d
  * stream. Calls that may run at the same time need workspaces of their own. */
 
 /* The pools [pages][kv_heads][page_size][64] in `dtype`, 16-byte aligned; page_stride elements from one page to
- * the next in both (at least kv_heads * page_size * 64, a multiple of 8; 0: exactly that). page_size is a power
- * of two from 8 to 256, pages * page_size below 2^31. */
+ * the next in both (at least kv_heads * page_size * 64, a multiple of 8, at most 2^31; 0: exactly that). page_size is
+ * a power of two from 8 to 256, pages * page_size below 2^31. */
 typedef struct splat_kv_cache {
   int32_t dtype;
   int32_t pages;

@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs p) {
       turn[wave][0][lane] = c;
       turn[wave][1][lane] = s;
     }
-    __builtin_amdgcn_wave_barrier();  // the wave's own rows: its LDS operations stay in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own rows: its LDS operations stay in order
+    __builtin_amdgcn_wave_barrier();
     *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(&turn[wave][0][4 * j]);
     *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(&turn[wave][1][4 * j]);
   }
@@ -333,8 +334,8 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs p) {
   const long unit = long(blockIdx.x) * 4 + uniform(threadIdx.x >> 6);
   if (unit >= long(p.n) * p.per_seq * c.kv_heads) return;
   const int lane = threadIdx.x & 63, j = lane & 7, ps = 1 << c.shift;
-  const uint32_t of_seq = uint32_t(p.per_seq) * c.kv_heads;
-  const int i = int(quotient(unit, of_seq)), rest = int(unit - long(i) * of_seq), h = rest % c.kv_heads, first = rest / c.kv_heads;
+  const long of_seq = long(p.per_seq) * c.kv_heads;
+  const int i = int(quotient(unit, of_seq)), first = int(quotient(unit - i * of_seq, c.kv_heads)), h = int(unit - i * of_seq - long(first) * c.kv_heads);
   const int len = length_of(uload(p.lens + i), p.width, c.shift, 0x7fffffff);
   const int fresh = p.add ? min(max(uload(p.add + i), 0), len) : len;
   if (fresh == 0) return;

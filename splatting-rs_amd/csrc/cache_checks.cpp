@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 namespace splat {
@@ -12,6 +13,9 @@ namespace {
 long type_size(int dt) { return dt == 0 ? 4 : 2; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(std::initializer_list<const void*> ps) {
+  return std::all_of(ps.begin(), ps.end(), [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; });
+}
 
 void check_page_size(int page_size) {
   SPLAT_CHECK(page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0, BAD_ARGUMENT,
@@ -19,8 +23,7 @@ void check_page_size(int page_size) {
 }
 
 void check_width(int width, int page_size) {
-  SPLAT_CHECK(width >= 1 && long(width) * page_size <= 0x7fffffffL, BAD_ARGUMENT,
-              "a table's row must hold 1 to 2^31 - 1 positions");
+  SPLAT_CHECK(width >= 1 && long(width) * page_size <= (1L << 30), BAD_ARGUMENT, "a table's row must hold 1 to 2^30 positions");
 }
 
 void check_sizes(const KvCache& c) {
@@ -54,6 +57,9 @@ bool meet(const void* a, long wa, const void* b, long wb) {
   return wa > 0 && wb > 0 && rows_meet(a, 0, wa, b, 0, wb, 1);
 }
 
+struct Range { const void* at; long bytes; };
+bool meet(const Range& a, const Range& b) { return meet(a.at, a.bytes, b.at, b.bytes); }
+
 long pool_bytes(const KvCache& c) {
   return ((c.pages - 1L) * c.page_stride + long(c.kv_heads) * c.page_size * 64) * type_size(c.dt);
 }
@@ -72,19 +78,29 @@ void check_attention(PagedArgs& a) {
   // the kernels divide tile counts times waves (up to 2^13) as 64-bit floats
   SPLAT_CHECK(long(a.n) * std::min<long>(a.max_len, long(a.width) * a.cache.page_size) < (1L << 38), BAD_ARGUMENT,
               "attention: more than 2^38 positions");
-  SPLAT_CHECK(std::isfinite(a.scale), BAD_ARGUMENT, "attention: scale is not finite");
+  SPLAT_CHECK(std::isfinite(a.scale * 1.5f), BAD_ARGUMENT, "attention: scale is not finite, or too large");  // times log2(e)
   if (a.n == 0) return;
   SPLAT_CHECK(a.q && a.table && a.lens && a.out, BAD_ARGUMENT, "attention: a required pointer is NULL");
   const long es = type_size(a.cache.dt), w = a.heads * 64L;
   SPLAT_CHECK(aligned16(a.q) && aligned16(a.out) && a.ldq % 8 == 0 && a.ldo % 8 == 0 && a.ldq >= w && a.ldo >= w, BAD_ARGUMENT,
               "attention: rows of q and out must be 16-byte aligned, heads * 64 wide and a multiple of 8 elements apart");
   SPLAT_CHECK(!rows_meet(a.q, a.ldq * es, w * es, a.out, a.ldo * es, w * es, a.n), BAD_ARGUMENT, "attention: out overlaps q");
-  SPLAT_CHECK(!meets_pools(a.cache, a.out, ((a.n - 1L) * a.ldo + w) * es), BAD_ARGUMENT, "attention: out overlaps the cache");
+  SPLAT_CHECK(aligned4({a.table, a.lens}), BAD_ARGUMENT, "attention: table and lens must be 4-byte aligned");
+  const Range out = {a.out, ((a.n - 1L) * a.ldo + w) * es};
+  SPLAT_CHECK(!meets_pools(a.cache, out.at, out.bytes) && !meet(out, {a.table, 4L * a.n * a.width}) && !meet(out, {a.lens, 4L * a.n}),
+              BAD_ARGUMENT, "attention: out overlaps the cache, the table or lens");
 }
 
-void check_workspace(const void* workspace, size_t bytes, size_t need) {
-  SPLAT_CHECK(need == 0 || (workspace && aligned16(workspace) && bytes >= need), BAD_ARGUMENT,
+void check_workspace(const PagedArgs& a, const void* workspace, size_t bytes, size_t need) {
+  if (need == 0) return;
+  SPLAT_CHECK(workspace && aligned16(workspace) && bytes >= need, BAD_ARGUMENT,
               "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+  const long es = type_size(a.cache.dt), w = a.heads * 64L;
+  const Range ws = {workspace, long(need)};
+  SPLAT_CHECK(!meets_pools(a.cache, ws.at, ws.bytes) && !meet(ws, {a.q, ((a.n - 1L) * a.ldq + w) * es}) &&
+                  !meet(ws, {a.out, ((a.n - 1L) * a.ldo + w) * es}) && !meet(ws, {a.table, 4L * a.n * a.width}) &&
+                  !meet(ws, {a.lens, 4L * a.n}),
+              BAD_ARGUMENT, "attention: the workspace overlaps another argument");
 }
 
 }  // namespace
@@ -97,17 +113,18 @@ void check_block_tables(BlockTableArgs& a) {
   SPLAT_CHECK(a.used && a.starts && a.used_out && a.status && (a.n == 0 || (a.past && a.add && a.table && a.lens)) &&
                   (a.pool_size == 0 || a.pool) && (a.cap == 0 || a.slots),
               BAD_ARGUMENT, "block tables: a required pointer is NULL");
-  struct Range { const void* at; long bytes; };
+  SPLAT_CHECK(aligned4({a.past, a.add, a.pool, a.used, a.table, a.lens, a.starts, a.slots, a.positions, a.used_out, a.status}),
+              BAD_ARGUMENT, "block tables: every array must be 4-byte aligned");
   const Range in[] = {{a.past, a.n * 4L}, {a.add, a.n * 4L}, {a.pool, a.pool_size * 4L}, {a.used, 4}};
   const Range out[] = {{a.lens, a.n * 4L}, {a.used_out, 4}, {a.table, 4L * a.n * a.width}, {a.starts, 4L * (a.n + 1L)},
                        {a.slots, a.cap * 4L}, {a.positions, a.cap * 4L}, {a.status, 4}};
   for (int o = 0; o < 7; ++o) {
     for (int i = 0; i < 4; ++i) {
       if ((o == 0 && i == 0 && a.lens == a.past) || (o == 1 && i == 3 && a.used_out == a.used)) continue;
-      SPLAT_CHECK(!meet(out[o].at, out[o].bytes, in[i].at, in[i].bytes), BAD_ARGUMENT, "block tables: an output overlaps an input");
+      SPLAT_CHECK(!meet(out[o], in[i]), BAD_ARGUMENT, "block tables: an output overlaps an input");
     }
     for (int i = 0; i < o; ++i)
-      SPLAT_CHECK(!meet(out[o].at, out[o].bytes, out[i].at, out[i].bytes), BAD_ARGUMENT, "block tables: two outputs overlap");
+      SPLAT_CHECK(!meet(out[o], out[i]), BAD_ARGUMENT, "block tables: two outputs overlap");
   }
   a.shift = __builtin_ctz(a.page_size);
 }
@@ -128,6 +145,7 @@ void check_qk_norm_rope(QkArgs& a, double base) {
   }
   SPLAT_CHECK(aligned16(a.qw) && aligned16(a.qb) && aligned16(a.kw) && aligned16(a.kb), BAD_ARGUMENT,
               "qk norm: qw, qb, kw and kb must be 16-byte aligned");
+  SPLAT_CHECK(aligned4({a.positions, a.slots}), BAD_ARGUMENT, "qk norm: positions and slots must be 4-byte aligned");
   if (a.tokens == 0) return;
   SPLAT_CHECK(a.qkv && a.q_out && (a.rope == ROPE_NONE || a.positions), BAD_ARGUMENT, "qk norm: a required pointer is NULL");
   const long es = type_size(a.dt), cols = (a.heads + 2L * a.kv_heads) * 64, wq = a.heads * 64L, wk = a.kv_heads * 64L;
@@ -158,6 +176,7 @@ void check_page_bounds(BoundsArgs& a) {
   if (a.n == 0) return;
   SPLAT_CHECK(a.table && a.lens && a.bounds && aligned16(a.bounds), BAD_ARGUMENT,
               "page bounds: a required pointer is NULL, or bounds not 16-byte aligned");
+  SPLAT_CHECK(aligned4({a.table, a.lens, a.add}), BAD_ARGUMENT, "page bounds: table, lens and add must be 4-byte aligned");
   SPLAT_CHECK(!meets_pools(a.cache, a.bounds, long(a.cache.pages) * a.cache.kv_heads * 128 * type_size(a.cache.dt)), BAD_ARGUMENT,
               "page bounds: bounds overlap the cache");
   // add positions that end anywhere lie in one page more than they fill
@@ -167,7 +186,7 @@ void check_page_bounds(BoundsArgs& a) {
 
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes) {
   check_attention(a);
-  if (a.n > 0) check_workspace(workspace, bytes, paged_attention_bytes(a.cache, a.n, a.heads, a.max_len));
+  if (a.n > 0) check_workspace(a, workspace, bytes, paged_attention_bytes(a.cache, a.n, a.heads, a.max_len));
 }
 
 void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) {
@@ -177,11 +196,20 @@ void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) 
   if (a.at.n == 0) return;
   SPLAT_CHECK(a.bounds && aligned16(a.bounds) && a.selected, BAD_ARGUMENT,
               "sparse attention: a required pointer is NULL, or bounds not 16-byte aligned");
-  SPLAT_CHECK(!meets_pools(a.at.cache, a.selected, 4L * a.at.n * a.at.cache.kv_heads * a.topk), BAD_ARGUMENT,
-              "sparse attention: selected overlaps the cache");
+  const PagedArgs& p = a.at;
+  const long es = type_size(p.cache.dt), w = p.heads * 64L;
+  const Range sel = {a.selected, 4L * p.n * p.cache.kv_heads * a.topk}, low = {a.bounds, long(p.cache.pages) * p.cache.kv_heads * 128 * es};
+  const Range out = {p.out, ((p.n - 1L) * p.ldo + w) * es};
+  SPLAT_CHECK(aligned4({a.selected}), BAD_ARGUMENT, "sparse attention: selected must be 4-byte aligned");
+  SPLAT_CHECK(!meets_pools(p.cache, sel.at, sel.bytes) && !meet(sel, {p.q, ((p.n - 1L) * p.ldq + w) * es}) && !meet(sel, out) &&
+                  !meet(sel, {p.table, 4L * p.n * p.width}) && !meet(sel, {p.lens, 4L * p.n}) && !meet(sel, low) && !meet(out, low),
+              BAD_ARGUMENT, "sparse attention: selected or out overlaps another argument");
   SPLAT_CHECK(long(a.at.n) * a.at.cache.kv_heads * ((long(a.at.max_len) + a.at.cache.page_size - 1) / a.at.cache.page_size + 63) < (1L << 37),
               BAD_ARGUMENT, "sparse attention: more than 2^37 pages and heads");
-  check_workspace(workspace, bytes, sparse_attention_bytes(a.at.cache, a.at.n, a.at.heads, a.at.max_len, a.topk));
+  const size_t need = sparse_attention_bytes(p.cache, p.n, p.heads, p.max_len, a.topk);
+  check_workspace(p, workspace, bytes, need);
+  SPLAT_CHECK(!meet({workspace, long(need)}, sel) && !meet({workspace, long(need)}, low), BAD_ARGUMENT,
+              "sparse attention: the workspace overlaps another argument");
 }
 
 namespace {

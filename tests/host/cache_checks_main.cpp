@@ -126,8 +126,8 @@ template <typename A> void on(const char* name, A a, void (*check)(A&), const st
 }
 
 void check_qk(QkArgs& a) { check_qk_norm_rope(a, 100.0); }
-void check_paged(PagedArgs& a) { check_paged_attention(a, at(64 * MB), size_t(1) << 40); }
-void check_sparse(SparseArgs& a) { check_sparse_attention(a, at(64 * MB), size_t(1) << 40); }
+void check_paged(PagedArgs& a) { check_paged_attention(a, at(4096 * MB), size_t(1) << 40); }
+void check_sparse(SparseArgs& a) { check_sparse_attention(a, at(4096 * MB), size_t(1) << 40); }
 
 }  // namespace
 
@@ -159,6 +159,7 @@ int main() {
   T("tables lens into past", [](auto& a) { a.lens = const_cast<int*>(a.past) + 1; });
   T("tables slots over table", [](auto& a) { a.slots = a.table + 79; });
   T("tables used_out over pool", [](auto& a) { a.used_out = const_cast<int*>(a.pool) + 99; });
+  T("tables odd lens", [](auto& a) { a.lens = reinterpret_cast<int*>(at(4 * 4096 + 2)); });
   T("tables status over used_out", [](auto& a) { a.status = a.used_out; });
 
   auto Q = [&](const char* n, const std::function<void(QkArgs&)>& f) { on<QkArgs>(n, qk(), check_qk, f); };
@@ -184,6 +185,7 @@ int main() {
   Q("qk qkv NULL", [](auto& a) { a.qkv = nullptr; });
   Q("qk positions NULL", [](auto& a) { a.positions = nullptr; });
   Q("qk odd qkv", [](auto& a) { a.qkv = at(8 * MB + 2); });
+  Q("qk odd slots", [](auto& a) { a.slots = reinterpret_cast<int*>(at(17 * 4 * MB + 1)); });
   Q("qk odd qw", [](auto& a) { a.qw = reinterpret_cast<float*>(at(20 * MB + 4)); });
   Q("qk odd kb", [](auto& a) { a.kb = reinterpret_cast<float*>(at(20 * MB + 8)); });
   Q("qk ld 1028", [](auto& a) { a.ld = 1028; });
@@ -205,6 +207,7 @@ int main() {
   B("bounds n -1", [](auto& a) { a.n = -1; });
   B("bounds max_add -1", [](auto& a) { a.max_add = -1; });
   B("bounds lens NULL", [](auto& a) { a.lens = nullptr; });
+  B("bounds odd lens", [](auto& a) { a.lens = reinterpret_cast<int*>(at(36 * MB + 2)); });
   B("bounds odd", [](auto& a) { a.bounds = at(10 * MB + 4); });
   B("bounds over cache", [](auto& a) { a.bounds = a.cache.v; });
   B("bounds too many", [](auto& a) { a.n = 0x7fffffff; a.add = nullptr; });
@@ -235,6 +238,10 @@ int main() {
   P("paged q NULL", [](auto& a) { a.q = nullptr; });
   P("paged ldo 500", [](auto& a) { a.ldo = 500; });
   P("paged ldq 516", [](auto& a) { a.ldq = 516; });
+  P("paged scale 3e38", [](auto& a) { a.scale = 3e38f; });
+  P("paged width 2^27", [](auto& a) { a.width = 1 << 27; });
+  P("paged odd table", [](auto& a) { a.table = reinterpret_cast<int*>(at(36 * MB + 2)); });
+  P("paged out over table", [](auto& a) { a.out = const_cast<int*>(a.table); });
   P("paged out over q", [](auto& a) { a.out = const_cast<void*>(a.q); });
   P("paged out over cache", [](auto& a) { a.out = a.cache.k; });
 
@@ -244,11 +251,17 @@ int main() {
     a.width = 1 << 16;
     check_paged_attention(a, at(4), size_t(1) << 40);
   });
+  say("paged workspace over q", [] {
+    PagedArgs a = paged();
+    a.max_len = 1 << 20;
+    a.width = 1 << 16;
+    check_paged_attention(a, a.q, size_t(1) << 40);
+  });
   say("paged workspace small", [] {
     PagedArgs a = paged();
     a.max_len = 1 << 20;
     a.width = 1 << 16;
-    check_paged_attention(a, at(64 * MB), paged_attention_bytes(a.cache, a.n, a.heads, a.max_len) - 1);
+    check_paged_attention(a, at(4096 * MB), paged_attention_bytes(a.cache, a.n, a.heads, a.max_len) - 1);
   });
 
   auto S = [&](const char* n, const std::function<void(SparseArgs&)>& f) { on<SparseArgs>(n, sparse(), check_sparse, f); };
@@ -260,10 +273,18 @@ int main() {
   S("sparse bounds NULL", [](auto& a) { a.bounds = nullptr; });
   S("sparse selected NULL", [](auto& a) { a.selected = nullptr; });
   S("sparse selected over cache", [](auto& a) { a.selected = static_cast<int*>(a.at.cache.k); });
+  S("sparse selected over lens", [](auto& a) { a.selected = const_cast<int*>(a.at.lens); });
+  S("sparse selected over bounds", [](auto& a) { a.selected = const_cast<int*>(static_cast<const int*>(a.bounds)); });
+  S("sparse out over bounds", [](auto& a) { a.bounds = a.at.out; });
+  S("sparse odd selected", [](auto& a) { a.selected = reinterpret_cast<int*>(at(13 * 4 * MB + 2)); });
   S("sparse heads 3", [](auto& a) { a.at.heads = 3; });
   say("sparse workspace small", [] {
     SparseArgs a = sparse();
-    check_sparse_attention(a, at(64 * MB), sparse_attention_bytes(a.at.cache, 3, 8, 300, 5) - 1);
+    check_sparse_attention(a, at(4096 * MB), sparse_attention_bytes(a.at.cache, 3, 8, 300, 5) - 1);
+  });
+  say("sparse workspace over selected", [] {
+    SparseArgs a = sparse();
+    check_sparse_attention(a, a.selected, size_t(1) << 40);
   });
   say("workspace ok", [] {
     paged_attention_bytes(cache(), 0, 8, 0);
