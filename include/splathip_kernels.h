@@ -114,7 +114,8 @@ int splat_kernel_reconstruct(splat_ctx* ctx, int V, int H, int W, const float* d
  * Position p of sequence i lies in row p % page_size of page table[i * width + p / page_size]; a slot is
  * page * page_size + row. Lengths, tables and slots are device arrays: nothing here waits for the host. Table entries
  * outside [0, pages) hold no keys (their positions are left out), slots outside [0, pages * page_size) are not
- * written, lengths are clamped to what the table's row and max_len hold, negative ones to 0.
+ * written, lengths are clamped to what the table's row (1 to 2^30 positions) and max_len hold, negative ones to 0.
+ * Outputs and workspaces overlap no other argument but where a call says so.
  *
  * These calls allocate nothing and wait for nothing, so they may be captured into a HIP graph on the context's
  * stream. Calls that may run at the same time need workspaces of their own. */

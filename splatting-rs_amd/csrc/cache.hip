@@ -100,6 +100,9 @@ template <> __device__ inline void store8<float>(float* p, const float (&x)[8]) 
 // over the threads' sums for four tokens at a time, then a walk over at most k requests. A new page begins with
 // a new token, whose thread writes the table's entry.
 // The call takes effect whole or not at all: the status is known before anything is written.
+// Bound by its chain of loads (requests; past and add again; the pool), not by its bytes: 32 requests of one token 4.6 us,
+// 64 of up to 24 views (813008 tokens, 6.6 MB) 6.1 us, where an empty kernel takes 2.2. A thread that searched for each
+// of its tokens took 14.7 us for the same tokens, and the commit as a second launch 3.8 more.
 // FILL writes the table, slots and positions, COMMIT (block 0) lens, starts, used and status; where those lie over
 // past and used and there are several blocks, it runs as a second launch.
 template <int THREADS, bool FILL, bool COMMIT>
@@ -221,6 +224,9 @@ template <> struct Quad<float> {
 // or values. A lane holds the two quads of channels that turn together, (c, c + 32) on a line and (c, c + 16)
 // in each half on a grid, so that no value crosses lanes but in the sums. Lane l < 32 takes frequency l's angle
 // once for all heads, in 64 bits up to the fraction of a turn; all loads are under way before it.
+// Bound by HBM where there are many tokens: 24889 of 24 + 8 + 8 heads (f16) 54 us, 4.7 TB/s, a large copy's rate (one head
+// row over 8 lanes of 8 channels, whose partners and sums crossed lanes through LDS, took 100). 32 tokens of 36 heads
+// (bf16) 3.6 us, 973 of 18 (fp32) 4.4: the launch and two dependent loads (10.1 and 9.1 before the steps were dealt to waves).
 template <typename T, int IT, int ROPE>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs p) {
   using Raw = typename Quad<T>::Raw;
@@ -327,7 +333,10 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs p) {
 __device__ inline float low(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 __device__ inline float high(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// One wave a (sequence, page, head), 8 lanes a row, 8 rows a load, 8 loads under way.
+// One wave a (sequence, page, head), 8 lanes a row, 8 rows a load, 8 loads under way. 1556 pages of 64 rows and 8 heads
+// (f16, 28 MB) 8.2 us, 3.4 TB/s: short waves, whose comparisons and the joining of their 16 values over the lanes take
+// half of that (10.4 with the joining through LDS; two heads a wave 12.4, four 18.2: fewer waves hide less). The pages of
+// 32 new tokens (bf16, 12 heads) 3.5 us: the launch and three dependent loads.
 template <typename T>
 __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs p) {
   const KvCache& c = p.cache;
@@ -381,6 +390,9 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs p) {
 // 16 columns (fewer: columns of zeros, which cost nothing, since the bytes of K and V bound the kernel).
 // The scores come out with a lane holding one head (lane % 16) and keys 4 (lane / 16) + r, which is the
 // operand layout of the second product as it stands; V is read transposed from LDS.
+//
+// Bound by the bytes of K and V: 48 sequences (f16, 8 key heads, 295 MB) in 57 us, 5.1 TB/s, where a kernel that only reads
+// reaches 5.7 and a large copy 4.7. A kernel of the vector unit, one wave a query head, took 1.8 ms.
 //
 // A wave works alone: tiles of 32 keys (16 in fp32: 4 KB of K and 4 KB of V in every type) stream into its own
 // ring in LDS, four loads of 1 KB for each, that many bytes ahead, and no barrier holds it up. A load covers 8
@@ -459,11 +471,11 @@ template <typename T> struct TileOps {  // bf16, f16: rows of 128 bytes
       x[t] = a;
     }
   }
-  __device__ static inline void weigh(const char* vt, int lane, const f32x4 (&w)[T16], f32x4 (&o)[4]) {
-    const int g = lane >> 4, j = (lane >> 2) & 3, cc = lane & 3;
-    const uint4 p = make_uint4(pack2<T>(w[0][0], w[0][1]), pack2<T>(w[0][2], w[0][3]), pack2<T>(w[1][0], w[1][1]),
-                               pack2<T>(w[1][2], w[1][3]));
-    const int row = 4 * g + j;  // and 16 + row, whose chunks lie alike
+  // V^T of the tile as the second product's operand: 16 channels each, keys 4 g + (0..3) and 16 + 4 g + (0..3).
+  struct Values { uint4 f[4]; };
+  __device__ static inline Values values(const char* vt, int lane) {
+    const int g = lane >> 4, j = (lane >> 2) & 3, cc = lane & 3, row = 4 * g + j;  // and 16 + row, whose chunks lie alike
+    Values v;
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
       typedef short v4s __attribute__((ext_vector_type(4)));
@@ -476,8 +488,15 @@ template <typename T> struct TileOps {  // bf16, f16: rows of 128 bytes
         f[2 * t] = u.x;
         f[2 * t + 1] = u.y;
       }
-      o[d] = mma(make_uint4(f[0], f[1], f[2], f[3]), p, o[d]);
+      v.f[d] = make_uint4(f[0], f[1], f[2], f[3]);
     }
+    return v;
+  }
+  __device__ static inline void weigh(const Values& v, const f32x4 (&w)[T16], f32x4 (&o)[4]) {
+    const uint4 p = make_uint4(pack2<T>(w[0][0], w[0][1]), pack2<T>(w[0][2], w[0][3]), pack2<T>(w[1][0], w[1][1]),
+                               pack2<T>(w[1][2], w[1][3]));
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = mma(v.f[d], p, o[d]);
   }
 };
 template <> struct TileOps<float> {  // rows of 256 bytes
@@ -512,18 +531,22 @@ template <> struct TileOps<float> {  // rows of 256 bytes
     }
     x[0] = a;
   }
-  __device__ static inline void weigh(const char* vt, int lane, const f32x4 (&w)[T16], f32x4 (&o)[4]) {
+  struct Values { float f[4][4]; };  // [key 4 g + r][channel 16 d + lane % 16]
+  __device__ static inline Values values(const char* vt, int lane) {
     const int g = lane >> 4, c = lane & 15;
-    float v[4][4];
+    Values v;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int d = 0; d < 4; ++d)
-        v[r][d] = *reinterpret_cast<const float*>(vt + (4 * g + r) * 256 + (((4 * d + (c >> 2)) ^ (4 * g)) * 16) + (c & 3) * 4);
+        v.f[r][d] = *reinterpret_cast<const float*>(vt + (4 * g + r) * 256 + (((4 * d + (c >> 2)) ^ (4 * g)) * 16) + (c & 3) * 4);
+    return v;
+  }
+  __device__ static inline void weigh(const Values& v, const f32x4 (&w)[T16], f32x4 (&o)[4]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][d], w[0][r], o[d], 0, 0, 0);
+      for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.f[r][d], w[0][r], o[d], 0, 0, 0);
   }
 };
 
@@ -609,6 +632,7 @@ template <typename T, bool SPARSE> struct PagedWave {
     const char* kt = ring + b * TILE_BYTES;
     f32x4 x[Ops::T16];
     ops.scores(kt, lane, x);
+    const typename Ops::Values v = Ops::values(kt + TILE_BYTES / 2, lane);  // under way during the softmax
     const int g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < Ops::T16; ++t)
@@ -643,7 +667,7 @@ template <typename T, bool SPARSE> struct PagedWave {
         x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - ref);
         l += x[t][r];
       }
-    Ops::weigh(kt + TILE_BYTES / 2, lane, x, o);
+    Ops::weigh(v, x, o);
   }
 
   // Tiles t, t + step, ... below end: tile k is asked for while tile k - 2 is used, in one copy of either's code (a
@@ -755,7 +779,9 @@ __device__ inline void join_block(const PagedArgs& p, const Wave& w, char* smem,
 }
 
 // One block a (sequence, group of up to 16 heads of one key head): its waves take equal parts of the tiles
-// and join their sums in LDS.
+// and join their sums in LDS. For short sequences (paged_plan has the rule and both sides' times): three of up to 188
+// positions (fp32, 6 heads) 7.4 us, of which the launch and the length take 2.6, the first tiles 2.0, the products of
+// three tiles in fp32 (matrix instructions of 4 keys) 2.0 and the join 0.8.
 template <typename T, bool SPARSE>
 __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const PagedArgs p, const int* sel, int topk, float scale) {
   using Wave = PagedWave<T, SPARSE>;
@@ -783,7 +809,9 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const 
 // lies within one part or one block's is written at once; of the others the parts' sums, unnormalised, are left
 // for paged_join_kernel: slot 0 for the sequence that a wave's part begins in, slot 1 for one that it ends in. With
 // span = PAGED_WAVES the parts that a block's waves end with are joined where they are of one sequence, so that a
-// long sequence leaves one part a block instead of one a wave (span = 1).
+// long sequence leaves one part a block instead of one a wave (span = 1). That costs this kernel 1.5 us and spares the join its
+// batches: one sequence, 12 heads (168 waves each) 25.6 -> 24.7 us, 2 groups of 16 heads (388 waves) 21.6 -> 15.5; 48 sequences
+// (5 waves each) 66 -> 67.5, so it is done from 128 waves a sequence on.
 constexpr int SCAN_MAX = 1024;
 
 
@@ -894,7 +922,9 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
 
 // One block a (sequence, `per` heads of a group): the parts of a sequence that several waves had. SPLIT waves share a
 // head (all eight where the block has one), each with every SPLIT-th part, a channel a lane, JOIN_PARTS parts under way.
-// Bound by its chain of loads (counts, then parts), not by their bytes.
+// Bound by its chain of loads (counts, then parts), not by their bytes: 42 parts of 12 heads 5.0 us, parts of 48 sequences of
+// 32 heads 8.5. Blocks of 4 or 16 waves, 4 to 24 parts under way and other numbers of heads a block were no faster; 64-bit
+// integer divisions for the parts' places made it 18.6.
 constexpr int JOIN_WAVES = 8, JOIN_PARTS = 8;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const PagedArgs p, int workers, int span, int per, const long* before, const float* parts) {
@@ -1046,7 +1076,8 @@ template <typename T> struct PageScore {
 };
 
 // A wave takes 16 pages of one (sequence, key head); bound by its two dependent loads (the table's entry with the
-// length, the bounds) and, in 64 bits, its products.
+// length, the bounds) and, in 64 bits, its products: 3241 pages of 12 heads (bf16) 6.2 us, 1 us of it for the 64 bits; 16
+// lanes a page took 6.4, 64 pages a wave 6.6.
 constexpr int SCORE_PAGES = 64;  // a block
 template <typename T>
 __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, const T* bounds, int maxp, uint64_t* keys) {
@@ -1074,9 +1105,11 @@ __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, cons
 // are counted into up to 512 equal bins of that range, the bins above the border's are taken, and its bin is the
 // next range: two rounds for most scores, seven at most. Counts do not hang on the order of the atomic adds, and
 // every wave reads all bins for itself, so that a round has one barrier: of three sets of bins one is counted
-// into, one cleared, and one may still be read. What bounds the kernel is the chain of these steps.
+// into, one cleared, and one may still be read. What bounds the kernel is the chain of these steps: 405 of 3241 pages, 12
+// heads, 6.0 us on 512 threads (256: 8.9, 1024: 6.5; with block-wide sums between the steps 11.3).
 // Thread t holds keys [t K, (t + 1) K) in registers (K > 0), or reads them every round (K = 0, `k` each). FUSED (K = 1, a
-// wave for every 16 pages): the block scores the pages itself, a launch less for sequences of few pages.
+// wave for every 16 pages): the block scores the pages itself, a launch less for sequences of few pages (3 pages 4.9 us
+// against 3.5 + 4.0, 125 pages 6.6 against 4.3 + 4.7; 256 pages 9.2 against 4.0 + 4.4).
 constexpr int SELECT_BINS = 512;
 template <int THREADS, int K, typename T = void>
 __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, const void* bounds, int maxp, int k, int topk, int* sel) {
@@ -1230,8 +1263,11 @@ __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p,
   for (int e = total + tid; e < topk; e += THREADS) out[e] = -1;
 }
 
-constexpr long QK_WAVES = 24576, JOIN_BLOCKS = 256;
-constexpr int FUSE_MAX = 128;
+// Waves up to which a wave of qk_norm_rope_kernel takes one step (five beyond): 2800 tokens of 6 steps 8.7 us against 9.9,
+// 5600 tokens 14.1 against 13.9.
+constexpr long QK_WAVES = 24576;
+constexpr long JOIN_BLOCKS = 256;  // of paged_join_kernel, beyond which a block takes several heads
+constexpr int FUSE_MAX = 128;      // pages up to which page_select_kernel scores them itself
 
 // Runs fn with the storage type dt as a value.
 template <typename F> void by_type(int dt, F&& fn) {
