@@ -194,7 +194,7 @@ int splat_kernel_paged_attention(splat_ctx* ctx, const splat_kv_cache* cache, co
  * page always among them. A page's score is the most that the dot products of the group's queries with a key between
  * the page's bounds (splat_kernel_page_bounds) can sum to, in 64 bits; the lower page first where scores are equal, NaN
  * above all. selected [n, kv_heads, topk]: the pages' places in the table's row, ascending, -1 behind the last.
- * scale must be positive. */
+ * topk is at most 2^27; scale must be positive. */
 int splat_sparse_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, int topk,
                                      size_t* bytes);
 int splat_kernel_sparse_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* bounds, const void* q,

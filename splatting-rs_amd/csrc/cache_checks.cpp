@@ -67,6 +67,11 @@ bool meets_pools(const KvCache& c, const void* p, long bytes) {
   return meet(c.k, pool_bytes(c), p, bytes) || meet(c.v, pool_bytes(c), p, bytes);
 }
 
+// A table's row holds up to 2^27 pages; the kernels count places past topk in 32 bits.
+void check_topk(int topk) {
+  SPLAT_CHECK(topk >= 1 && topk <= (1 << 27), BAD_ARGUMENT, "sparse attention: topk must be 1 to 2^27");
+}
+
 // What attention over the cache needs, whichever pages it takes.
 void check_attention(PagedArgs& a) {
   check_cache(a.cache);
@@ -191,7 +196,7 @@ void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes) {
 
 void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) {
   check_attention(a.at);
-  SPLAT_CHECK(a.topk >= 1, BAD_ARGUMENT, "sparse attention: topk must be at least 1");
+  check_topk(a.topk);
   SPLAT_CHECK(a.at.scale > 0.f, BAD_ARGUMENT, "sparse attention: scale must be positive");
   if (a.at.n == 0) return;
   SPLAT_CHECK(a.bounds && aligned16(a.bounds) && a.selected, BAD_ARGUMENT,
@@ -246,7 +251,7 @@ size_t paged_attention_bytes(const KvCache& c, int n, int heads, int max_len) {
 
 size_t sparse_attention_bytes(const KvCache& c, int n, int heads, int max_len, int topk) {
   check_workspace_sizes(c, n, heads, max_len);
-  SPLAT_CHECK(topk >= 1, BAD_ARGUMENT, "sparse attention: topk must be at least 1");
+  check_topk(topk);
   return paged_plan(c, n, heads, max_len, topk).bytes + size_t(n) * c.kv_heads * ((long(max_len) + c.page_size - 1) / c.page_size) * 8;
 }
 

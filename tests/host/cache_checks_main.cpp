@@ -266,7 +266,10 @@ int main() {
 
   auto S = [&](const char* n, const std::function<void(SparseArgs&)>& f) { on<SparseArgs>(n, sparse(), check_sparse, f); };
   S("sparse ok", [](auto&) {});
-  S("sparse ok topk 2^30", [](auto& a) { a.topk = 1 << 20; });
+  S("sparse ok topk 2^20", [](auto& a) { a.topk = 1 << 20; });
+  S("sparse ok topk 2^27", [](auto& a) { a.topk = 1 << 27; a.selected = ints(1L << 36); });
+  S("sparse topk past 2^27", [](auto& a) { a.topk = (1 << 27) + 1; a.selected = ints(1L << 36); });
+  S("sparse topk 2^31 - 1", [](auto& a) { a.topk = 0x7fffffff; a.selected = ints(1L << 36); });
   S("sparse topk 0", [](auto& a) { a.topk = 0; });
   S("sparse scale 0", [](auto& a) { a.at.scale = 0.f; });
   S("sparse scale nan", [&](auto& a) { a.at.scale = nan; });
@@ -291,6 +294,7 @@ int main() {
     sparse_attention_bytes(cache(), 0, 8, 0, 1);
   });
   say("workspace heads 5", [] { paged_attention_bytes(cache(), 1, 5, 10); });
+  say("workspace topk 2^31 - 1", [] { sparse_attention_bytes(cache(), 1, 8, 10, 0x7fffffff); });
   say("workspace topk 0", [] { sparse_attention_bytes(cache(), 1, 8, 10, 0); });
   say("workspace page 0", [] {
     KvCache c = cache();
