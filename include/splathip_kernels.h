@@ -115,7 +115,8 @@ int splat_kernel_reconstruct(splat_ctx* ctx, int V, int H, int W, const float* d
  * page * page_size + row. Lengths, tables and slots are device arrays: nothing here waits for the host. Table entries
  * outside [0, pages) hold no keys (their positions are left out), slots outside [0, pages * page_size) are not
  * written, lengths are clamped to what the table's row (1 to 2^30 positions) and max_len hold, negative ones to 0.
- * Outputs and workspaces overlap no other argument but where a call says so.
+ * Outputs and workspaces overlap no other argument but where a call says so. Limits of one call: 2^25 tokens,
+ * 2^21 query rows (n * heads), 2^25 sequences times kv_heads, 2^30 scored pages; beyond them it is refused.
  *
  * These calls allocate nothing and wait for nothing, so they may be captured into a HIP graph on the context's
  * stream. Calls that may run at the same time need workspaces of their own. */

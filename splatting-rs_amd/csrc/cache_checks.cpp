@@ -10,6 +10,9 @@ namespace splat {
 
 namespace {
 
+// A launch has below 2^32 threads in x: up to 1024 for a query row, 64 for a token or for the page of a head.
+constexpr long MOST_ROWS = 1 << 21, MOST_TOKENS = 1 << 25, MOST_UNITS = 1 << 25;
+
 long type_size(int dt) { return dt == 0 ? 4 : 2; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -77,7 +80,7 @@ void check_attention(PagedArgs& a) {
   check_cache(a.cache);
   SPLAT_CHECK(a.n >= 0 && a.heads >= 1 && a.heads <= 32768 && a.heads % a.cache.kv_heads == 0, BAD_ARGUMENT,
               "attention: heads must be a multiple of the cache's kv_heads");
-  SPLAT_CHECK(long(a.n) * a.heads <= (1 << 24), BAD_ARGUMENT, "attention: more than 2^24 query rows");
+  SPLAT_CHECK(long(a.n) * a.heads <= MOST_ROWS, BAD_ARGUMENT, "attention: more than 2^21 query rows");
   check_width(a.width, a.cache.page_size);
   SPLAT_CHECK(a.max_len >= 0, BAD_ARGUMENT, "attention: max_len is negative");
   // the kernels divide tile counts times waves (up to 2^13) as 64-bit floats
@@ -108,6 +111,9 @@ void check_workspace(const PagedArgs& a, const void* workspace, size_t bytes, si
               BAD_ARGUMENT, "attention: the workspace overlaps another argument");
 }
 
+// A generous max_len sizes the workspace, which no shorter one needs more of, but not the launch.
+void cut_to_row(PagedArgs& a) { a.max_len = int(std::min<long>(a.max_len, long(a.width) * a.cache.page_size)); }
+
 }  // namespace
 
 void check_block_tables(BlockTableArgs& a) {
@@ -136,7 +142,7 @@ void check_block_tables(BlockTableArgs& a) {
 
 void check_qk_norm_rope(QkArgs& a, double base) {
   SPLAT_CHECK(a.dt >= 0 && a.dt <= 2, BAD_ARGUMENT, "unknown dtype");
-  SPLAT_CHECK(a.tokens >= 0 && a.heads >= 1 && a.kv_heads >= 1 && a.heads <= 65536 && a.kv_heads <= 4096, BAD_ARGUMENT,
+  SPLAT_CHECK(a.tokens >= 0 && a.tokens <= MOST_TOKENS && a.heads >= 1 && a.kv_heads >= 1 && a.heads <= 65536 && a.kv_heads <= 4096, BAD_ARGUMENT,
               "qk norm: tokens, heads or kv_heads");
   SPLAT_CHECK(a.norm >= NORM_NONE && a.norm <= NORM_RMS, BAD_ARGUMENT, "qk norm: unknown norm");
   SPLAT_CHECK(a.rope >= ROPE_NONE && a.rope <= ROPE_GRID, BAD_ARGUMENT, "qk norm: unknown rotation");
@@ -186,12 +192,15 @@ void check_page_bounds(BoundsArgs& a) {
               "page bounds: bounds overlap the cache");
   // add positions that end anywhere lie in one page more than they fill
   a.per_seq = int(std::min<long>(a.width, a.add ? (long(a.max_add) + a.cache.page_size - 1) / a.cache.page_size + 1 : a.width));
-  SPLAT_CHECK(long(a.n) * a.per_seq * a.cache.kv_heads <= (1L << 32), BAD_ARGUMENT, "page bounds: more than 2^32 pages and heads");
+  SPLAT_CHECK(long(a.n) * a.cache.kv_heads <= MOST_UNITS, BAD_ARGUMENT, "page bounds: more than 2^25 sequences and heads");
+  a.per_seq = int(std::min<long>(a.per_seq, MOST_UNITS / (long(a.n) * a.cache.kv_heads)));  // a wave goes on to the next ones
 }
 
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes) {
   check_attention(a);
-  if (a.n > 0) check_workspace(a, workspace, bytes, paged_attention_bytes(a.cache, a.n, a.heads, a.max_len));
+  if (a.n == 0) return;
+  check_workspace(a, workspace, bytes, paged_attention_bytes(a.cache, a.n, a.heads, a.max_len));
+  cut_to_row(a);
 }
 
 void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) {
@@ -209,18 +218,20 @@ void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) 
   SPLAT_CHECK(!meets_pools(p.cache, sel.at, sel.bytes) && !meet(sel, {p.q, ((p.n - 1L) * p.ldq + w) * es}) && !meet(sel, out) &&
                   !meet(sel, {p.table, 4L * p.n * p.width}) && !meet(sel, {p.lens, 4L * p.n}) && !meet(sel, low) && !meet(out, low),
               BAD_ARGUMENT, "sparse attention: selected or out overlaps another argument");
-  SPLAT_CHECK(long(a.at.n) * a.at.cache.kv_heads * ((long(a.at.max_len) + a.at.cache.page_size - 1) / a.at.cache.page_size + 63) < (1L << 37),
-              BAD_ARGUMENT, "sparse attention: more than 2^37 pages and heads");
   const size_t need = sparse_attention_bytes(p.cache, p.n, p.heads, p.max_len, a.topk);
   check_workspace(p, workspace, bytes, need);
   SPLAT_CHECK(!meet({workspace, long(need)}, sel) && !meet({workspace, long(need)}, low), BAD_ARGUMENT,
               "sparse attention: the workspace overlaps another argument");
+  cut_to_row(a.at);
+  // four threads a page in whole blocks of 64 pages
+  SPLAT_CHECK(long(p.n) * p.cache.kv_heads * ((long(p.max_len) + p.cache.page_size - 1) / p.cache.page_size + 63) < (1L << 30),
+              BAD_ARGUMENT, "sparse attention: more than 2^30 pages and heads");
 }
 
 namespace {
 void check_workspace_sizes(const KvCache& c, int n, int heads, int max_len) {
   check_sizes(c);
-  SPLAT_CHECK(n >= 0 && max_len >= 0 && heads >= 1 && heads <= 32768 && heads % c.kv_heads == 0 && long(n) * heads <= (1 << 24), BAD_ARGUMENT,
+  SPLAT_CHECK(n >= 0 && max_len >= 0 && heads >= 1 && heads <= 32768 && heads % c.kv_heads == 0 && long(n) * heads <= MOST_ROWS, BAD_ARGUMENT,
               "workspace: n, heads or max_len");
 }
 }  // namespace

@@ -4,6 +4,7 @@
 #include <cstdio>
 #include <functional>
 #include <limits>
+#include <string>
 
 #include "../../splatting-rs_amd/csrc/cache.h"
 
@@ -173,6 +174,7 @@ int main() {
   Q("qk dtype 3", [](auto& a) { a.dt = 3; });
   Q("qk heads 0", [](auto& a) { a.heads = 0; });
   Q("qk kv_heads 0", [](auto& a) { a.kv_heads = 0; });
+  Q("qk tokens 2^25 + 1", [](auto& a) { a.tokens = (1 << 25) + 1; a.qkv = at(1L << 42); a.q_out = at(1L << 43); a.k_out = at(1L << 44); });
   Q("qk tokens -1", [](auto& a) { a.tokens = -1; });
   Q("qk norm 3", [](auto& a) { a.norm = 3; });
   Q("qk rope -1", [](auto& a) { a.rope = -1; });
@@ -210,6 +212,14 @@ int main() {
   B("bounds odd lens", [](auto& a) { a.lens = reinterpret_cast<int*>(at(36 * MB + 2)); });
   B("bounds odd", [](auto& a) { a.bounds = at(10 * MB + 4); });
   B("bounds over cache", [](auto& a) { a.bounds = a.cache.v; });
+  say("bounds ok launch", [] {  // the pages of a sequence are dealt out in turns where all at once are too many
+    BoundsArgs a = bounds();
+    a.n = 1 << 20;
+    a.width = 1 << 20;
+    a.add = nullptr;
+    check_page_bounds(a);
+    if (a.per_seq != 8) throw Error(BAD_ARGUMENT, "per_seq " + std::to_string(a.per_seq));
+  });
   B("bounds too many", [](auto& a) { a.n = 0x7fffffff; a.add = nullptr; });
   B("cache dtype -1", [](auto& a) { a.cache.dt = -1; });
   B("cache pages 0", [](auto& a) { a.cache.pages = 0; });
@@ -232,6 +242,8 @@ int main() {
   P("paged heads 0", [](auto& a) { a.heads = 0; });
   P("paged n -1", [](auto& a) { a.n = -1; });
   P("paged n 2^22", [](auto& a) { a.n = 1 << 22; });
+  P("paged ok n 2^18", [](auto& a) { a.n = 1 << 18; a.q = at(1L << 36); a.out = at(1L << 37); a.table = ints(1L << 38); a.lens = ints(1L << 39); });
+  P("paged n 2^18 + 1", [](auto& a) { a.n = (1 << 18) + 1; a.q = at(1L << 36); a.out = at(1L << 37); a.table = ints(1L << 38); a.lens = ints(1L << 39); });
   P("paged width 0", [](auto& a) { a.width = 0; });
   P("paged max_len -1", [](auto& a) { a.max_len = -1; });
   P("paged scale inf", [&](auto& a) { a.scale = inf; });
@@ -270,6 +282,8 @@ int main() {
   S("sparse ok topk 2^27", [](auto& a) { a.topk = 1 << 27; a.selected = ints(1L << 36); });
   S("sparse topk past 2^27", [](auto& a) { a.topk = (1 << 27) + 1; a.selected = ints(1L << 36); });
   S("sparse topk 2^31 - 1", [](auto& a) { a.topk = 0x7fffffff; a.selected = ints(1L << 36); });
+  S("sparse ok max_len 2^31 - 1", [](auto& a) { a.at.max_len = 0x7fffffff; });
+  S("sparse 2^30 pages", [](auto& a) { a.at.max_len = 0x7fffffff; a.at.width = 1 << 26; a.at.n = 4; a.at.table = ints(1L << 38); });
   S("sparse topk 0", [](auto& a) { a.topk = 0; });
   S("sparse scale 0", [](auto& a) { a.at.scale = 0.f; });
   S("sparse scale nan", [&](auto& a) { a.at.scale = nan; });
@@ -288,6 +302,25 @@ int main() {
   say("sparse workspace over selected", [] {
     SparseArgs a = sparse();
     check_sparse_attention(a, a.selected, size_t(1) << 40);
+  });
+  say("paged ok max_len sizes no launch past the row", [] {
+    for (int dt = 0; dt < 3; ++dt)
+      for (int topk : {0, 1, 40, 5000}) {
+        KvCache c = cache();
+        c.dt = dt;
+        for (int n : {1, 7, 300}) {
+          size_t most = 0;
+          for (int len = 1; len > 0 && len < 0x7fffffff / 3; len = len * 3 / 2 + 1) {  // workspaces grow with max_len
+            const size_t bytes = paged_plan(c, n, 8, len, topk).bytes;
+            if (bytes < most) throw Error(BAD_ARGUMENT, "a longer max_len takes a smaller workspace");
+            most = bytes;
+          }
+        }
+      }
+    PagedArgs a = paged();
+    a.max_len = 0x7fffffff;
+    check_paged(a);
+    if (a.max_len != 320) throw Error(BAD_ARGUMENT, "max_len " + std::to_string(a.max_len));
   });
   say("workspace ok", [] {
     paged_attention_bytes(cache(), 0, 8, 0);
