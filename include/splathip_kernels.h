@@ -164,7 +164,7 @@ int splat_kernel_block_tables(splat_ctx* ctx, int n, const int32_t* past, const 
  * [tokens, kv_heads * 64] (NULL: not wanted) have row strides ldq and ldk; they may be qkv's own q and k blocks, and
  * overlap it nowhere else. With cache and slots [tokens] (both or neither) keys and values also go to the cache;
  * a slot outside the pool (-1: padding) stores nothing. The slots of one call are distinct. Row strides are multiples
- * of 8 elements, rows 16-byte aligned. */
+ * of 8 elements and at most 2^31, rows 16-byte aligned. */
 typedef enum splat_norm { SPLAT_NORM_NONE = 0, SPLAT_NORM_LAYER = 1, SPLAT_NORM_RMS = 2 } splat_norm;
 typedef enum splat_rope { SPLAT_ROPE_NONE = 0, SPLAT_ROPE_LINE = 1, SPLAT_ROPE_GRID = 2 } splat_rope;
 int splat_kernel_qk_norm_rope(splat_ctx* ctx, int dtype, const void* qkv, int64_t ld, int tokens, int heads,
@@ -182,7 +182,7 @@ int splat_kernel_page_bounds(splat_ctx* ctx, const splat_kv_cache* cache, int n,
 
 /* Attention of one token a sequence over its lens[i] cached positions: out[i, h] = softmax(scale q[i, h] K^T) V with
  * the keys and values of head h / (heads / kv_heads); zeros for a sequence without keys. q and out [n, heads * 64] in the
- * cache's dtype, row strides ldq and ldo (multiples of 8 elements, rows 16-byte aligned, not overlapping). max_len: an
+ * cache's dtype, row strides ldq and ldo (multiples of 8 elements up to 2^31, rows 16-byte aligned, not overlapping). max_len: an
  * upper bound of the lengths that the host knows, for the launch (longer ones are cut there). In bf16 and f16 the
  * weights go to the matrix cores rounded to that type, as in splat_kernel_attention.
  * workspace: device memory of at least splat_paged_attention_workspace's bytes, 16-byte aligned. */

@@ -11,6 +11,7 @@ namespace splat {
 namespace {
 
 // A launch has below 2^32 threads in x: up to 1024 for a query row, 64 for a token or for the page of a head.
+constexpr long MOST_STRIDE = 1L << 31;  // elements from row to row: sizes in bytes stay within 64 bits
 constexpr long MOST_ROWS = 1 << 21, MOST_TOKENS = 1 << 25, MOST_UNITS = 1 << 25;
 
 long type_size(int dt) { return dt == 0 ? 4 : 2; }
@@ -90,8 +91,9 @@ void check_attention(PagedArgs& a) {
   if (a.n == 0) return;
   SPLAT_CHECK(a.q && a.table && a.lens && a.out, BAD_ARGUMENT, "attention: a required pointer is NULL");
   const long es = type_size(a.cache.dt), w = a.heads * 64L;
-  SPLAT_CHECK(aligned16(a.q) && aligned16(a.out) && a.ldq % 8 == 0 && a.ldo % 8 == 0 && a.ldq >= w && a.ldo >= w, BAD_ARGUMENT,
-              "attention: rows of q and out must be 16-byte aligned, heads * 64 wide and a multiple of 8 elements apart");
+  SPLAT_CHECK(aligned16(a.q) && aligned16(a.out) && a.ldq % 8 == 0 && a.ldo % 8 == 0 && a.ldq >= w && a.ldo >= w &&
+                  a.ldq <= MOST_STRIDE && a.ldo <= MOST_STRIDE,
+              BAD_ARGUMENT, "attention: rows of q and out must be 16-byte aligned, heads * 64 wide and a multiple of 8 elements (at most 2^31) apart");
   SPLAT_CHECK(!rows_meet(a.q, a.ldq * es, w * es, a.out, a.ldo * es, w * es, a.n), BAD_ARGUMENT, "attention: out overlaps q");
   SPLAT_CHECK(aligned4({a.table, a.lens}), BAD_ARGUMENT, "attention: table and lens must be 4-byte aligned");
   const Range out = {a.out, ((a.n - 1L) * a.ldo + w) * es};
@@ -161,8 +163,9 @@ void check_qk_norm_rope(QkArgs& a, double base) {
   SPLAT_CHECK(a.qkv && a.q_out && (a.rope == ROPE_NONE || a.positions), BAD_ARGUMENT, "qk norm: a required pointer is NULL");
   const long es = type_size(a.dt), cols = (a.heads + 2L * a.kv_heads) * 64, wq = a.heads * 64L, wk = a.kv_heads * 64L;
   SPLAT_CHECK(aligned16(a.qkv) && aligned16(a.q_out) && aligned16(a.k_out) && a.ld % 8 == 0 && a.ldq % 8 == 0 && a.ld >= cols &&
-                  a.ldq >= wq && (!a.k_out || (a.ldk % 8 == 0 && a.ldk >= wk)),
-              BAD_ARGUMENT, "qk norm: rows must be 16-byte aligned, as wide as their heads and a multiple of 8 elements apart");
+                  a.ldq >= wq && a.ld <= MOST_STRIDE && a.ldq <= MOST_STRIDE &&
+                  (!a.k_out || (a.ldk % 8 == 0 && a.ldk >= wk && a.ldk <= MOST_STRIDE)),
+              BAD_ARGUMENT, "qk norm: rows must be 16-byte aligned, as wide as their heads and a multiple of 8 elements (at most 2^31) apart");
   const char* in = static_cast<const char*>(a.qkv);
   SPLAT_CHECK((a.q_out == in && a.ldq == a.ld) || !rows_meet(in, a.ld * es, cols * es, a.q_out, a.ldq * es, wq * es, a.tokens),
               BAD_ARGUMENT, "qk norm: q_out overlaps qkv and is not its query block");

@@ -193,6 +193,9 @@ int main() {
   Q("qk ld 1028", [](auto& a) { a.ld = 1028; });
   Q("qk ld short", [](auto& a) { a.ld = 15 * 64; });
   Q("qk ldq short", [](auto& a) { a.ldq = 7 * 64; });
+  Q("qk ld 2^61", [](auto& a) { a.ld = 1L << 61; });
+  Q("qk ldq 2^62", [](auto& a) { a.ldq = 1L << 62; });
+  Q("qk ldk 2^62", [](auto& a) { a.ldk = 1L << 62; });
   Q("qk ldk short", [](auto& a) { a.ldk = 3 * 64; });
   Q("qk q_out over keys", [](auto& a) { a.q_out = at(8 * MB + 1024); a.ldq = a.ld; });
   Q("qk q_out another stride", [](auto& a) { a.q_out = const_cast<void*>(a.qkv); });
@@ -249,6 +252,8 @@ int main() {
   P("paged scale inf", [&](auto& a) { a.scale = inf; });
   P("paged q NULL", [](auto& a) { a.q = nullptr; });
   P("paged ldo 500", [](auto& a) { a.ldo = 500; });
+  P("paged ldq 2^61", [](auto& a) { a.ldq = 1L << 61; });
+  P("paged ldo 2^62", [](auto& a) { a.ldo = 1L << 62; });
   P("paged ldq 516", [](auto& a) { a.ldq = 516; });
   P("paged scale 3e38", [](auto& a) { a.scale = 3e38f; });
   P("paged width 2^27", [](auto& a) { a.width = 1 << 27; });
