@@ -415,10 +415,10 @@ template <int N> __device__ inline void load_lds(const void* base, uint32_t byte
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
         "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
-        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 lds\n\t"
-        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 lds\n\t"
-        "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 lds" ::"s"(m0),
-        "v"(off[p]), "v"(off[p + 1]), "v"(off[p + 2]), "v"(off[p + 3]), "s"(r)
+        "buffer_load_dwordx4 %2, %5, 0 offen offset:%6 lds\n\t"
+        "buffer_load_dwordx4 %3, %5, 0 offen offset:%7 lds\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen offset:%8 lds" ::"s"(m0),
+        "v"(off[p]), "v"(off[p + 1]), "v"(off[p + 2]), "v"(off[p + 3]), "s"(r), "n"(1024), "n"(2 * 1024), "n"(3 * 1024)
         : "memory");
   else if constexpr (N == 2)
     asm volatile(
