@@ -437,6 +437,7 @@ PAGED = [
     ([24889], 1, 1, 16), ([5] * 40, 3, 3, 8), ([700] * 9, 33, 1, 32), ([13000, 5000], 24, 8, 256),
     # parts of a block joined, sequences that end inside one, and more sequences than a block sums up
     ([9000, 1, 0, 7000, 40], 16, 1, 16), ([3000, 3001, 2999, 64, 0, 1], 2, 1, 8), ([1500] + [3, 0, 40] * 400, 2, 1, 8),
+    ([3, 0, 40] * 400 + [9000, 0], 2, 1, 8), ([5, 0, 4500] + [0, 1] * 520, 18, 1, 32),   # the same, cut into parts
 ]
 
 
@@ -675,6 +676,7 @@ SPARSE = [
     ([1037, 500, 700], 17, 1, 16, 20), ([2000], 6, 6, 8, 100), ([5000, 4999], 16, 4, 32, 33), ([9000], 3, 3, 8, 1024), ([640] * 6, 20, 4, 64, 200),
     ([6223], 2, 2, 16, 16), ([20000, 300], 2, 1, 8, 300), ([3000], 33, 3, 256, 2),
     ([1500] + [3, 0, 40] * 400, 2, 1, 8, 150),   # more sequences than a block sums up
+    ([3, 0, 40] * 400 + [9000, 0], 2, 1, 8, 700),   # the same, cut into parts
 ]
 
 
@@ -881,6 +883,55 @@ def test_scenes_that_grow_in_a_captured_graph(ctx):
         other.calls(ctx)
         ctx.synchronize()
         other.check([1, 2])
+
+
+@pytest.mark.parametrize("n,most,ps,topk", [(2, 6000, 16, 130), (1030, 4400, 8, 530)])
+def test_long_scenes_in_a_captured_graph(ctx, n, most, ps, topk):
+    """Attention cut into parts and joined, scores and selection in launches of their own, captured once and replayed
+    over other lengths, queries and bounds in the same memory."""
+    L = lib()
+    full = Cache("bf16", [most] + [9] * (n - 1), 1, ps)
+    heads, cache = 2, full.device()
+    q, b = torch.zeros(n, heads * 64, dtype=torch.bfloat16, device="cuda"), page_bounds_of(full).cuda()
+    lens = full.dlens
+    dense, sparse = torch.zeros_like(q), torch.zeros_like(q)
+    sel = torch.zeros(n, 1, topk, dtype=torch.int32, device="cuda")
+    sizes = L.paged_attention_workspace(cache, n, heads, most), L.sparse_attention_workspace(cache, n, heads, most, topk)
+    assert min(sizes) > 0
+    ws = [torch.full((s,), 255, dtype=torch.uint8, device="cuda") for s in sizes]
+
+    def calls():
+        at = (ptr(q), heads * 64, n, heads, ptr(full.dtable), full.width, ptr(lens), most)
+        ctx.kernel_paged_attention(cache, *at, 0.125, ptr(dense), heads * 64, ptr(ws[0]), sizes[0])
+        ctx.kernel_sparse_attention(cache, ptr(b), *at, topk, 0.125, ptr(sparse), heads * 64, ptr(sel), ptr(ws[1]), sizes[1])
+
+    torch.cuda.synchronize()
+    calls()   # the code objects are loaded
+    ctx.synchronize()
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        calls()
+    for step, first in enumerate((most, 0, 77, most - 1, most // 2)):
+        report("long.graph", n=n, step=step, first=first)
+        now = [first] + [(5 * i + step) % 10 for i in range(n - 1)]
+        q.copy_(queries(full, heads, seed=step).cuda())
+        lens.copy_(ints(now).cuda())
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.synchronize()
+        got = dense.clone(), sparse.clone(), sel.clone()
+        for w in ws:
+            w.fill_(255)   # eager work between the replays; nothing of a call stays in its workspace
+        torch.cuda.synchronize()
+        calls()
+        ctx.synchronize()
+        assert torch.equal(got[0], dense) and torch.equal(got[1], sparse) and torch.equal(got[2], sel)
+        check_sparse(full, full.table, b.cpu(), q.cpu(), heads, topk, sparse.cpu(), sel.cpu().long(), lens=now)
+        real, full.lens = full.lens, now
+        check_paged(None, full, heads, q.cpu(), dense.cpu())
+        full.lens = real
 
 
 def test_scenes_of_two_contexts_at_once(ctx):
