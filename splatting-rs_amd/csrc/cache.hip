@@ -922,7 +922,7 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
 
 // One block a (sequence, `per` heads of a group): the parts of a sequence that several waves had. SPLIT waves share a
 // head (all eight where the block has one), each with every SPLIT-th part, a channel a lane, JOIN_PARTS parts under way.
-// Bound by its chain of loads (counts, then parts), not by their bytes: 42 parts of 12 heads 5.0 us, parts of 48 sequences of
+// Bound by its chain of loads (counts, then parts), not by their bytes: 39 parts of 12 heads 5.0 us, parts of 48 sequences of
 // 32 heads 8.5. Blocks of 4 or 16 waves, 4 to 24 parts under way and other numbers of heads a block were no faster; 64-bit
 // integer divisions for the parts' places made it 18.6.
 constexpr int JOIN_WAVES = 8, JOIN_PARTS = 8;
