@@ -407,13 +407,15 @@ typedef const __attribute__((address_space(3))) char* lds_cptr;
 
 // N loads of 16 bytes a lane, 1 KB each, from base + off[k] + 1024 k into LDS at lds + 1024 k + 16 * lane; offsets
 // from `bytes` on read as zeros. The instruction's offset goes into both addresses.
+// A load wants one wait state after the write of m0, and five after a vector instruction wrote its descriptor, which the compiler
+// does not insert before inline assembly: the write and s_nop 3 are five.
 template <int N> __device__ inline void load_lds(const void* base, uint32_t bytes, const uint32_t (&off)[4], int p, uint32_t lds) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   const int32x4_v r = {uniform(int(uint32_t(a))), uniform(int(uint32_t(a >> 32))), uniform(int(bytes)), 0x00020000};
   const int m0 = uniform(int(lds));
   if constexpr (N == 4)
     asm volatile(
-        "s_mov_b32 m0, %0\n\t"
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\t"
         "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
         "buffer_load_dwordx4 %2, %5, 0 offen offset:%6 lds\n\t"
         "buffer_load_dwordx4 %3, %5, 0 offen offset:%7 lds\n\t"
@@ -422,13 +424,13 @@ template <int N> __device__ inline void load_lds(const void* base, uint32_t byte
         : "memory");
   else if constexpr (N == 2)
     asm volatile(
-        "s_mov_b32 m0, %0\n\t"
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\t"
         "buffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
         "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 lds" ::"s"(m0),
         "v"(off[p]), "v"(off[p + 1]), "s"(r)
         : "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off[p]), "s"(r) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off[p]), "s"(r) : "memory");
 }
 template <int N> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
