@@ -183,8 +183,9 @@ int splat_kernel_page_bounds(splat_ctx* ctx, const splat_kv_cache* cache, int n,
 /* Attention of one token a sequence over its lens[i] cached positions: out[i, h] = softmax(scale q[i, h] K^T) V with
  * the keys and values of head h / (heads / kv_heads); zeros for a sequence without keys. q and out [n, heads * 64] in the
  * cache's dtype, row strides ldq and ldo (multiples of 8 elements up to 2^31, rows 16-byte aligned, not overlapping). max_len: an
- * upper bound of the lengths that the host knows, for the launch (longer ones are cut there). In bf16 and f16 the
- * weights go to the matrix cores rounded to that type, as in splat_kernel_attention.
+ * upper bound of the lengths that the host knows, for the launch (longer ones are cut there). In bf16 and f16 a
+ * weight goes to the matrix cores as two numbers of that type, the second what the first leaves: 16 bits of it in bf16, 22 in
+ * f16 (the first alone for a sequence whose sums hold a NaN, as beside an infinite value).
  * workspace: device memory of at least splat_paged_attention_workspace's bytes, 16-byte aligned. */
 int splat_paged_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, size_t* bytes);
 int splat_kernel_paged_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* q, int64_t ldq, int n,

@@ -1,0 +1,100 @@
+"""What the paged cache's operators keep of their operands, against restatements in 64 bits on the CPU that share no
+formula with the kernels. u = 2^-24, h = half a rounding step of the storage type relative to the value: bf16 2^-8, f16
+2^-11, fp32 2^-24."""
+import math
+
+import pytest
+
+from conftest import report
+from test_gpu_cache import DTYPES, TDT, U, Cache, attention_ref, half, page_bounds_of, queries, run_paged, run_sparse
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+# --- weights of 16-bit types ----------------------------------------------------------------------
+
+def weights_tol(ref, A, e, keys, top, dtype):
+    """|out - ref| <= h |ref| + (h_w + 2 e + (L + 8) u) A as for any softmax over L keys. A weight of a 16-bit type is the sum of
+    two of its numbers: the rest that the first leaves is at most h of the weight, and h of that is lost: h_w = h^2. Terms of
+    f16 below its smallest normal value are off by 2^-25, which is 2^-37 of the largest weight, 2^12."""
+    h = half(dtype)
+    tol = h * ref.abs() + ((0 if dtype == "f32" else h * h) + 2 * e + (keys + 8) * U) * A
+    return tol + (keys * 2.0 ** -37 * top + 2.0 ** -25 if dtype == "f16" else 0.0)
+
+
+def even_cache(dtype, lens, kv, ps):
+    """Keys whose scores differ little, and values of 1 and -1 in equal numbers: the sums nearly cancel, so that the result's own
+    rounding hides nothing of the weights'."""
+    c = Cache(dtype, lens, kv, ps, scale=0.1)
+    g = torch.Generator().manual_seed(len(lens))
+    v = c.v[:, :kv * ps * 64].view(c.pages, kv, ps, 64)
+    for i, n in enumerate(lens):
+        signs = torch.stack([torch.randperm(n, generator=g) % 2 for _ in range(kv * 64)]).T.reshape(n, kv, 64) * 2.0 - 1
+        for j in range(-(-n // ps)):
+            x = signs[j * ps:(j + 1) * ps].transpose(0, 1)
+            v[int(c.table[i, j]), :, :x.shape[1]] = x.to(TDT[dtype])
+    return c
+
+
+def check_weights(c, q, heads, out, places=None):
+    G, worst = heads // c.kv, 0.0
+    for i, n in enumerate(c.lens):
+        for h in range(c.kv):
+            at = range(n) if places is None else [p for j in places[i, h].tolist() if j >= 0 for p in range(j * c.ps, min(n, (j + 1) * c.ps))]
+            k, v = c.head(c.k, i, h, at), c.head(c.v, i, h, at)
+            ref, A, e = attention_ref(q[i].view(c.kv, G, 64)[h].double(), k, v, 0.125)
+            d = (out[i].view(c.kv, G, 64)[h].double() - ref).abs() / weights_tol(ref, A, e, len(k), 1.0, c.dtype)
+            worst = max(worst, float(d.max()))
+    report("weights.err", of_tolerance=f"{worst:.3f}")
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,heads,kv,ps", [([2, 16, 17, 40], 4, 2, 8), ([64, 200, 31], 12, 12, 16), ([2500, 90], 16, 1, 32),
+                                              ([4001], 6, 6, 16)])
+def test_weights_keep_more_than_their_type_holds(ctx, dtype, lens, heads, kv, ps):
+    report("weights", dtype=dtype, lens=lens, heads=heads, kv=kv, ps=ps)
+    c = even_cache(dtype, lens, kv, ps)
+    q = queries(c, heads)
+    check_weights(c, q, heads, run_paged(ctx, c, q, heads))
+    out, sel = run_sparse(ctx, c, q, heads, page_bounds_of(c), 3)
+    check_weights(c, q, heads, out, sel)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,heads,kv", [([1, 2, 33, 300], 6, 2), ([3000], 6, 2), ([2000, 5, 1999], 32, 2)])
+def test_infinite_values(ctx, dtype, lens, heads, kv):
+    """An infinite value has a weight above 0: the channel is infinite, of no number where both signs meet or a value is
+    NaN, and the other channels are what they are without it."""
+    report("infinite", dtype=dtype, lens=lens, heads=heads, kv=kv)
+    c = Cache(dtype, lens, kv, 16, scale=0.3)   # scores of a few units: no weight is too small for f16
+    q = queries(c, heads)
+    v = c.v[:, :kv * 16 * 64].view(c.pages, kv, 16, 64)
+    clean = c.v.clone()
+    inf, want = float("inf"), {}
+    for i, n in enumerate(lens):
+        for at, channel, value in ((0, 3, inf), (n - 1, 17, -inf), (n // 2, 40, inf), (n // 3, 40, -inf), (n // 2, 63, float("nan"))):
+            if n == 1 and channel == 40 and value < 0:
+                continue   # one key holds one value
+            v[int(c.table[i, at // 16]), kv - 1, at % 16, channel] = value
+        want[i] = {3: inf, 17: -inf, 40: inf if n == 1 else math.nan, 63: math.nan}
+    out = run_paged(ctx, c, q, heads).float()
+    c.v = clean
+    G = heads // kv
+    for i, n in enumerate(lens):
+        x = out[i].view(kv, G, 64)[kv - 1]
+        for channel, value in want[i].items():
+            y = x[:, channel]
+            assert torch.isnan(y).all() if value != value else (y == value).all(), (i, channel, y)
+        rest = [ch for ch in range(64) if ch not in want[i]]
+        k, vals = c.head(c.k, i, kv - 1, range(n)), c.head(c.v, i, kv - 1, range(n))
+        ref, A, e = attention_ref(q[i].view(kv, G, 64)[kv - 1].double(), k, vals, 0.125)
+        # beside such a channel a weight is one number of its type: h_w = h
+        h = half(dtype)
+        tol = h * ref.abs() + ((0 if dtype == "f32" else h) + 2 * e + (n + 8) * U) * A
+        if dtype == "f16":
+            tol = tol + n * 2.0 ** -37 * vals.abs().max() + 2.0 ** -25
+        assert ((x.double() - ref).abs() <= tol)[:, rest].all()
+        assert torch.isfinite(out[i].view(kv, G, 64)[:kv - 1]).all()
