@@ -1054,13 +1054,17 @@ __device__ inline uint64_t order_of(double s) {
 // The most that q k can be for a key between the page's bounds, summed over the group's heads, is
 // sum_c hi_c A_c + lo_c B_c, with A and B the sums of the positive and the negative parts of the heads' queries:
 // 128 products a page, however many heads share it. In 64 bits: which of two pages next to the border is
-// taken can hang on less than 32 bits hold. 8 lanes a page, 16 products each.
+// taken can hang on less than 32 bits hold. 8 lanes a page, 16 products each. An infinite bound of the other side, whose
+// factor is 0 because no head has that sign, takes no part: 0 inf would be NaN and place the page first. Such sums are taken again, so
+// that finite ones cost a comparison.
 template <typename T> struct PageScore {
   const PagedArgs& p;
   const T* bounds;
   const int kh, lane;
+  const T* q;  // the sequence's
   double A[8], B[8];
   __device__ inline void load_q(int i) {
+    q = static_cast<const T*>(p.q) + i * p.ldq;
     const int G = p.heads / p.cache.kv_heads, j = lane & 7;
 #pragma unroll
     for (int e = 0; e < 8; ++e) A[e] = B[e] = 0.0;
@@ -1068,7 +1072,7 @@ template <typename T> struct PageScore {
       float x[4][8] = {};
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        if (g0 + g < G) load8(static_cast<const T*>(p.q) + i * p.ldq + (long(kh) * G + g0 + g) * 64 + j * 8, x[g]);
+        if (g0 + g < G) load8(q + (long(kh) * G + g0 + g) * 64 + j * 8, x[g]);
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -1077,6 +1081,32 @@ template <typename T> struct PageScore {
           B[e] += x[g][e] > 0.f ? 0.0 : double(x[g][e]);
         }
     }
+  }
+  // The lane's products as the definition has them, where the plain sum is NaN: a query of 0 beside an infinite bound gives NaN
+  // (as q k does with such a key), one of the other sign leaves it out. All of it read again, one channel at a time: the
+  // registers of the way without it are kept.
+  __device__ inline double careful(int page) const {
+    if (!page_ok(page, p.cache.pages)) return 0.0;  // no place's score
+    const int G = p.heads / p.cache.kv_heads, j = lane & 7;
+    double s = 0;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const T* at = bounds + (long(page) * p.cache.kv_heads + kh) * 128 + j * 8 + e;
+      double l = to_f(at[0]), h = to_f(at[64]), a = 0, b = 0;
+      bool zero = false;
+#pragma unroll 1
+      for (int g = 0; g < G; ++g) {
+        const float x = to_f(q[(long(kh) * G + g) * 64 + j * 8 + e]);
+        a += x > 0.f ? double(x) : 0.0;
+        b += x > 0.f ? 0.0 : double(x);
+        zero |= x == 0.f;
+      }
+      if (!zero && b == 0.0 && fabs(l) == double(INFINITY)) l = 0.0;
+      if (!zero && a == 0.0 && fabs(h) == double(INFINITY)) h = 0.0;
+      s += l * b + h * a;
+      if (zero) s += 0.0 * l + 0.0 * h;
+    }
+    return s;
   }
   // 16 pages, two for each 8 lanes: page[k] is place + 8 k's (below 0: none); put(place, key) once for each place.
   template <typename Put> __device__ inline void score(const int (&page)[2], int place, Put&& put) const {
@@ -1094,6 +1124,7 @@ template <typename T> struct PageScore {
       double s = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += double(lo[k][e]) * B[e] + double(hi[k][e]) * A[e];
+      if (s != s) s = careful(page[k]);
       s = sum8(s);
       if (j == 0) put(place + 8 * k, page_ok(page[k], p.cache.pages) ? order_of(s) : 0);
     }

@@ -98,3 +98,86 @@ def test_infinite_values(ctx, dtype, lens, heads, kv):
             tol = tol + n * 2.0 ** -37 * vals.abs().max() + 2.0 ** -25
         assert ((x.double() - ref).abs() <= tol)[:, rest].all()
         assert torch.isfinite(out[i].view(kv, G, 64)[:kv - 1]).all()
+
+
+# --- the choice of pages --------------------------------------------------------------------------
+
+def most_between(lo, hi, q):
+    """The most that q k can be for k between lo and hi, head by head and summed over them: q [G, 64], lo and hi [64]. A maximum
+    over both ends of every channel, as IEEE products have it (0 inf and NaN give NaN)."""
+    at_lo, at_hi = q * lo, q * hi
+    return float(torch.where(torch.isnan(at_lo) | torch.isnan(at_hi), math.nan, torch.maximum(at_lo, at_hi)).sum())
+
+
+def pages_from_the_maximum(c, bounds, q, heads, topk):
+    G = heads // c.kv
+    out = torch.full((c.n, c.kv, topk), -1, dtype=torch.int64)
+    b = bounds.double()
+    for i, n in enumerate(c.lens):
+        held = -(-n // c.ps)
+        for h in range(c.kv):
+            x = q[i].view(c.kv, G, 64)[h].double()
+            s = [most_between(*b[int(c.table[i, j]), h], x) for j in range(held)]
+            # the newest, then NaN, then the largest; the lower page where they are equal
+            order = sorted(range(held), key=lambda j: (j != held - 1, s[j] == s[j], -s[j] if s[j] == s[j] else 0.0, j))
+            take = sorted(order[:topk])
+            out[i, h, :len(take)] = torch.tensor(take, dtype=torch.int64)
+    return out
+
+
+def check_choice(ctx, c, bounds, q, heads, topks, scale=0.125):
+    for topk in topks:
+        want = pages_from_the_maximum(c, bounds, q, heads, topk)
+        _, got = run_sparse(ctx, c, q, heads, bounds, topk, scale=scale)
+        assert torch.equal(got, want), (topk, (got != want).nonzero()[:4])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pages", [40, 400])   # scored by the selection, and before it
+@pytest.mark.parametrize("heads,kv", [(2, 2), (6, 2), (17, 1)])
+def test_infinite_bounds_take_part_where_the_query_does(ctx, dtype, pages, heads, kv):
+    """Bounds of one infinite side in random channels, beside queries of one sign, of both and of 0 in the group."""
+    report("infinite.bounds", dtype=dtype, pages=pages, heads=heads, kv=kv)
+    c = Cache(dtype, [16 * pages, 16 * 7 + 3], kv, 16, garbage=False)
+    b = page_bounds_of(c)
+    g = torch.Generator().manual_seed(pages + heads)
+    inf = float("inf")
+    for p in range(0, c.pages, 2):
+        for h in range(kv):
+            low, high = torch.randint(0, 16, (2,), generator=g).tolist()   # lowest bounds in channels 0-15, highest in 16-31
+            b[p, h, 0, low] = -inf
+            if p % 4:
+                b[p, h, 1, 16 + high] = inf
+            if p % 16 == 6:   # both sides of one channel
+                b[p, h, 0, 32 + high], b[p, h, 1, 32 + high] = -inf, inf
+            if p % 32 == 12:   # every key of the page
+                b[p, h, :, 48] = -inf if h else inf
+    q = queries(c, heads)
+    x = q.view(c.n, kv, heads // kv, 64)
+    x[:, :, :, :14] = x[:, :, :, :14].abs() + 0.01    # -inf is the least there, whatever the head
+    x[:, :, :, 16:30] = -x[:, :, :, 16:30].abs() - 0.01
+    x[1, :, 0, 5], x[1, :, -1, 20], x[1, :, 0, 33] = 0.0, 0.0, 0.0   # no number in the second sequence
+    check_choice(ctx, c, b, q, heads, (1, 2, 5, 17, pages // 2, pages + 3))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_harmless_infinity_displaces_no_page(ctx, dtype):
+    """Queries above 0 and a key of -inf, or below 0 and +inf: the page's score is that of its other end."""
+    for sign, side in ((1.0, 0), (-1.0, 1)):
+        c = Cache(dtype, [16 * 4], 1, 16, garbage=False)
+        b = page_bounds_of(c)
+        q = queries(c, 1)
+        q[0, 2] = sign
+        scores = [most_between(*b[int(c.table[0, j]), 0].double(), q[0].view(1, 64).double()) for j in range(3)]
+        least = scores.index(min(scores))
+        b[int(c.table[0, least]), 0, side, 2] = -sign * float("inf")
+        _, got = run_sparse(ctx, c, q, 1, b, 3)
+        assert got.flatten().tolist() == [j for j in range(4) if j != least]
+        check_choice(ctx, c, b, q, 1, (1, 2, 3, 4))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pages,heads,kv", [(30, 12, 4), (300, 16, 2), (1500, 3, 3)])
+def test_the_choice_is_the_definitions(ctx, dtype, pages, heads, kv):
+    c = Cache(dtype, [16 * pages - 5, 16 * 9], kv, 16, garbage=False)
+    check_choice(ctx, c, page_bounds_of(c), queries(c, heads), heads, (2, 9, pages // 3, pages))
