@@ -193,11 +193,12 @@ int splat_kernel_paged_attention(splat_ctx* ctx, const splat_kv_cache* cache, co
                                  float scale, void* out, int64_t ldo, void* workspace, size_t workspace_bytes);
 
 /* splat_kernel_paged_attention over the topk pages of each (sequence, key head) with the largest scores, the newest
- * page always among them. A page's score is the most that the dot products of the group's queries with a key between
- * the page's bounds (splat_kernel_page_bounds) can sum to, in 64 bits; the lower page first where scores are equal, NaN
- * above all (a NaN bound or query, or a query of 0 beside an infinite bound; of an infinite bound that a query's sign does not
- * choose nothing is taken). selected [n, kv_heads, topk]: the pages' places in the table's row, ascending, -1 behind the last.
- * topk is at most 2^27; scale must be positive. */
+ * page always among them. A page's score is a sum over the heads of the group, in 64 bits: of each head the most that its
+ * query's product with a key between the page's bounds (splat_kernel_page_bounds) can be, each head with a key of its own, so that
+ * no key of the page gives the heads more. The lower page comes first where scores are equal, NaN above all (a NaN bound or
+ * query, or a query of 0 beside an infinite bound; an infinite bound that a query's sign does not choose takes no part).
+ * selected [n, kv_heads, topk]: the pages' places in the table's row, ascending, -1 behind the last. topk is at most 2^27;
+ * scale must be positive. */
 int splat_sparse_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, int topk,
                                      size_t* bytes);
 int splat_kernel_sparse_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* bounds, const void* q,

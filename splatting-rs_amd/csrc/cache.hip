@@ -1051,7 +1051,8 @@ __device__ inline uint64_t order_of(double s) {
   return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
 
-// The most that q k can be for a key between the page's bounds, summed over the group's heads, is
+// The most that each head's q k can be for a key between the page's bounds, summed over the group's heads (bounding a page's
+// scores by its keys' lowest and highest channels: Tang et al., query-aware sparsity for long contexts, 2024), is
 // sum_c hi_c A_c + lo_c B_c, with A and B the sums of the positive and the negative parts of the heads' queries:
 // 128 products a page, however many heads share it. In 64 bits: which of two pages next to the border is
 // taken can hang on less than 32 bits hold. 8 lanes a page, 16 products each. An infinite bound of the other side, whose

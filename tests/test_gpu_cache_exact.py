@@ -177,6 +177,21 @@ def test_one_harmless_infinity_displaces_no_page(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_a_score_is_the_sum_of_each_heads_most(ctx, dtype):
+    """Two heads of opposite signs: the page with the wide channel comes first, though one key there gives their sum nothing."""
+    c = Cache(dtype, [16 * 5], 1, 16, garbage=False)
+    b = torch.zeros(c.pages, 1, 2, 64, dtype=TDT[dtype])
+    at = c.table[0].long()
+    b[at[1], 0, 0, 7], b[at[1], 0, 1, 7] = -4.0, 4.0   # 8 by two heads of 1 and -1
+    b[at[2], 0, :, 9] = 3.0                            # 6 by two heads of 1
+    q = torch.zeros(1, 128, dtype=TDT[dtype])
+    q[0, 7], q[0, 64 + 7], q[0, 9], q[0, 64 + 9] = 1.0, -1.0, 1.0, 1.0
+    _, got = run_sparse(ctx, c, q, 2, b, 2)
+    assert got.flatten().tolist() == [1, 4]
+    check_choice(ctx, c, b, q, 2, (1, 2, 3, 4, 5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("pages,heads,kv", [(30, 12, 4), (300, 16, 2), (1500, 3, 3)])
 def test_the_choice_is_the_definitions(ctx, dtype, pages, heads, kv):
     c = Cache(dtype, [16 * pages - 5, 16 * 9], kv, 16, garbage=False)
