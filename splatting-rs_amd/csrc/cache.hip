@@ -434,13 +434,17 @@ template <int N> __device__ inline void load_lds(const void* base, uint32_t byte
 }
 template <int N> __device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
+// 2^TOP e^d. Scores are subtracted from the largest one before the turn to powers of two: log2(e) times a large score would round
+// off what the difference holds.
+template <int TOP = 0> __device__ inline float exp_of(float d) { return __builtin_amdgcn_exp2f(fmaf(d, 1.44269504088896341f, float(TOP))); }
+
 __device__ inline float max_groups(float v) { return over_rows(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ inline float sum_groups(float v) { return over_rows(v, [](float a, float b) { return a + b; }); }
 // The two products on a tile in LDS. KEYS keys in T16 groups of 16; PIECE rows to a load.
 template <typename T> struct TileOps {  // bf16, f16: rows of 128 bytes
   static constexpr int KEYS = 32, T16 = 2, PIECE = 8;
   // f16 weights below 2^-14 lose bits: the largest one is 2^12, so that they do so from 2^-26 of it on.
-  static constexpr float TOP = std::is_same<T, f16>::value ? 12.f : 0.f;
+  static constexpr int TOP = std::is_same<T, f16>::value ? 12 : 0;
   uint4 q[2];
   __device__ inline void load_q(const T* row, int g, bool in) {
 #pragma unroll
@@ -513,7 +517,7 @@ template <typename T> struct TileOps {  // bf16, f16: rows of 128 bytes
 };
 template <> struct TileOps<float> {  // rows of 256 bytes
   static constexpr int KEYS = 16, T16 = 1, PIECE = 4;
-  static constexpr float TOP = 0.f;
+  static constexpr int TOP = 0;
   float4 q[4];
   __device__ inline void load_q(const float* row, int g, bool in) {
 #pragma unroll
@@ -658,9 +662,9 @@ template <typename T, bool SPARSE> struct PagedWave {
     float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
     if constexpr (Ops::T16 == 2) mx = fmaxf(mx, fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
     const float mn = fmaxf(m, max_groups(mx));
-    const float ref = mn == -INFINITY ? 0.f : mn - Ops::TOP;
-    // the weights are 2^(x - ref); what was summed against another reference moves along
-    const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    // the weights are 2^TOP e^(x - ref); what was summed against another reference moves along
+    const float keep = m == -INFINITY ? 0.f : exp_of(m - mn);
     m = mn;
     l *= keep;
 #pragma unroll
@@ -671,7 +675,7 @@ template <typename T, bool SPARSE> struct PagedWave {
     for (int t = 0; t < Ops::T16; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[t][r] = __builtin_amdgcn_exp2f(x[t][r] - ref);
+        x[t][r] = exp_of<Ops::TOP>(x[t][r] - ref);
         l += x[t][r];
       }
     Ops::weigh(v, x, o, rest);
@@ -778,7 +782,7 @@ __device__ inline void join_block(const PagedArgs& p, const Wave& w, char* smem,
         if (k < r || k >= e) continue;
         const float* ml = state(k) + 1024 + col * 4;
         const int had = __float_as_int(ml[2]);
-        f[k] = !had || ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mn);
+        f[k] = !had || ml[0] == -INFINITY ? 0.f : exp_of(ml[0] - mn);
         if (!had) continue;  // no key: its sums are zeros, whatever the others hold
         some = 1;
         sum += ml[1] * f[k];
@@ -1005,14 +1009,14 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const Paged
             mx = fmaxf(mx, ml[u].x);
             some = 1;
           }
-        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+        const float keep = m == -INFINITY ? 0.f : exp_of(m - mx);
         acc *= keep;
         sum *= keep;
         m = mx;
 #pragma unroll
         for (int u = 0; u < JOIN_PARTS; ++u)
           if (k0 + u * split < count && !(ml[u].y < 0.f)) {
-            const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mx);
+            const float f = ml[u].x == -INFINITY ? 0.f : exp_of(ml[u].x - mx);
             acc += o[u] * f;
             sum += ml[u].y * f;
           }
@@ -1032,7 +1036,7 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) paged_join_kernel(const Paged
         for (int k = 0; k < split; ++k) {
           if (!somes[wave + k]) continue;
           some = 1;
-          const float f = refs[wave + k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(refs[wave + k] - mx);
+          const float f = refs[wave + k] == -INFINITY ? 0.f : exp_of(refs[wave + k] - mx);
           acc += accs[wave + k][lane] * f;
           sum += sums[wave + k] * f;
         }
@@ -1394,23 +1398,22 @@ void page_bounds(const Exec& ex, const BoundsArgs& args) {
 // The launches of attention over the cache. topk: 0, or the pages that sel lists.
 void attend(const Exec& ex, const PagedArgs& a, const int* sel, int topk, char* workspace) {
   const PagedPlan plan = paged_plan(a.cache, a.n, a.heads, a.max_len, topk);
-  const float scale = a.scale * 1.44269504088896341f;  // scores as exponents of 2
   long* before = reinterpret_cast<long*>(workspace);
   float* parts = reinterpret_cast<float*>(workspace + plan.before_bytes);
   auto launch = [&](auto t, auto sparse) {
     using T = decltype(t);
     constexpr bool S = decltype(sparse)::value;
     if (!plan.workers) {
-      paged_whole_kernel<T, S><<<dim3(a.n, plan.cols), PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale);
+      paged_whole_kernel<T, S><<<dim3(a.n, plan.cols), PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, a.scale);
       return;
     }
     const dim3 grid(plan.workers / PAGED_WAVES, plan.cols);
     const int span = plan.workers >= 128L * a.n ? PAGED_WAVES : 1;
     if (a.n <= SCAN_MAX) {
-      paged_parts_kernel<T, S, true><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, span, before, parts);
+      paged_parts_kernel<T, S, true><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, a.scale, plan.workers, span, before, parts);
     } else {
       paged_scan_kernel<TileOps<T>::KEYS><<<1, 1024, 0, ex.stream>>>(a, topk, before);
-      paged_parts_kernel<T, S, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, scale, plan.workers, span, before, parts);
+      paged_parts_kernel<T, S, false><<<grid, PAGED_WAVES * 64, 0, ex.stream>>>(a, sel, topk, a.scale, plan.workers, span, before, parts);
     }
     // a head a block, with eight waves on its parts, until there are blocks enough
     const int most = std::min(a.heads / a.cache.kv_heads, 16), per = int(std::min<long>(most, std::max<long>(1, long(a.n) * a.heads / JOIN_BLOCKS)));

@@ -87,7 +87,7 @@ void check_attention(PagedArgs& a) {
   // the kernels divide tile counts times waves (up to 2^13) as 64-bit floats
   SPLAT_CHECK(long(a.n) * std::min<long>(a.max_len, long(a.width) * a.cache.page_size) < (1L << 38), BAD_ARGUMENT,
               "attention: more than 2^38 positions");
-  SPLAT_CHECK(std::isfinite(a.scale * 1.5f), BAD_ARGUMENT, "attention: scale is not finite, or too large");  // times log2(e)
+  SPLAT_CHECK(std::isfinite(a.scale * 1.5f), BAD_ARGUMENT, "attention: scale is not finite, or too large");  // 1.5: a score of 1 stays finite in powers of two
   if (a.n == 0) return;
   SPLAT_CHECK(a.q && a.table && a.lens && a.out, BAD_ARGUMENT, "attention: a required pointer is NULL");
   const long es = type_size(a.cache.dt), w = a.heads * 64L;

@@ -100,6 +100,49 @@ def test_infinite_values(ctx, dtype, lens, heads, kv):
         assert torch.isfinite(out[i].view(kv, G, 64)[:kv - 1]).all()
 
 
+# --- large scores ---------------------------------------------------------------------------------
+
+def exact_scores(dtype, lens, heads, kv, ps):
+    """Whole numbers whose products and sums hold no rounding: scores of 8192 and some units more or less, in eighths."""
+    c = Cache(dtype, lens, kv, ps, garbage=False)
+    g = torch.Generator().manual_seed(len(lens) + heads)
+    k = torch.randint(-2, 3, (c.pages, kv, ps, 64), generator=g).float()
+    v = torch.randint(0, 2, (c.pages, kv, ps, 64), generator=g) * 2.0 - 1
+    q = torch.randint(-2, 3, (c.n, heads, 64), generator=g).float()
+    k[..., 0] = q[..., 0] = 256.0
+    c.k[:, :kv * ps * 64], c.v[:, :kv * ps * 64] = k.view(c.pages, -1).to(TDT[dtype]), v.view(c.pages, -1).to(TDT[dtype])
+    return c, q.view(c.n, -1).to(TDT[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,heads,kv,ps", [([2, 9, 40], 4, 2, 8), ([33, 100], 16, 1, 16), ([3000, 7], 6, 6, 16)])
+def test_large_scores_lose_nothing(ctx, dtype, lens, heads, kv, ps):
+    """A score s that holds no rounding gives the weight e^d, d = s - max, which is off by 2 u |d| (log2(e) and its product) and 3 u
+    (exp2 and a product); each later tile or part that moves the largest score adds 3 u, L u in all; and the sums L u, the
+    weights of 16-bit types h^2: |out - ref| <= h |ref| + sum w (|v| + |ref|) (2 |d| + 3 + 2 L + 8) u / sum w + h_w A."""
+    report("large", dtype=dtype, lens=lens, heads=heads, kv=kv)
+    c, q = exact_scores(dtype, lens, heads, kv, ps)
+    out = run_paged(ctx, c, q, heads)
+    G, worst, h = heads // kv, 0.0, half(dtype)
+    for i, n in enumerate(lens):
+        for hk in range(kv):
+            k, v = c.head(c.k, i, hk, range(n)), c.head(c.v, i, hk, range(n))
+            s = q[i].view(kv, G, 64)[hk].double() @ k.T * 0.125
+            assert s.min() > 8000
+            d = s - s.amax(-1, keepdim=True)
+            w = torch.softmax(s, -1)
+            ref = w @ v
+            of = 2 * d.abs() + 3 + 2 * n + 8
+            tol = h * ref.abs() + U * ((w * of) @ v.abs() + (w * of).sum(-1, keepdim=True) * ref.abs())
+            if dtype != "f32":
+                tol = tol + h * h * (w @ v.abs())
+            if dtype == "f16":
+                tol = tol + n * 2.0 ** -37 + 2.0 ** -25
+            worst = max(worst, float(((out[i].view(kv, G, 64)[hk].double() - ref).abs() / tol).max()))
+    report("large.err", of_tolerance=f"{worst:.3f}")
+    assert worst <= 1, worst
+
+
 # --- the choice of pages --------------------------------------------------------------------------
 
 def most_between(lo, hi, q):
