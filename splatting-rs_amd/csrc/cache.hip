@@ -223,7 +223,7 @@ template <> struct Quad<float> {
 // A wave takes one token and up to IT steps of 8 head rows, 8 lanes a row; a step's rows are all queries, keys
 // or values. A lane holds the two quads of channels that turn together, (c, c + 32) on a line and (c, c + 16)
 // in each half on a grid, so that no value crosses lanes but in the sums. Lane l < 32 takes frequency l's angle
-// once for all heads, in 64 bits up to the fraction of a turn; all loads are under way before it.
+// once for all heads, in 64 bits up to the fraction of a quarter turn; all loads are under way before it.
 // Bound by HBM where there are many tokens: 24889 of 24 + 8 + 8 heads (f16) 54 us, 4.7 TB/s, a large copy's rate (one head
 // row over 8 lanes of 8 channels, whose partners and sums crossed lanes through LDS, took 100). 32 tokens of 36 heads
 // (bf16) 3.6 us, 973 of 18 (fp32) 4.4: the launch and two dependent loads (10.1 and 9.1 before the steps were dealt to waves).
@@ -258,11 +258,18 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs p) {
   if constexpr (ROPE != ROPE_NONE) {
     if (lane < 32) {
       const int pos = ROPE == ROPE_LINE ? p.positions[t] : p.positions[2L * t + (lane >> 4)];
-      const double x = double(pos) * p.freq[ROPE == ROPE_LINE ? lane : lane & 15];
+      // less whole quarters of a turn (below 2^31), so that 32 bits hold what is left to 2^-27 of a half turn
+      const double x = double(pos) * p.freq[ROPE == ROPE_LINE ? lane : lane & 15], quarters = rint(4.0 * x);
+      const int quarter = int(quarters);
       float s, c;
-      sincospif(float(2.0 * (x - rint(x))), &s, &c);
-      turn[wave][0][lane] = c;
-      turn[wave][1][lane] = s;
+      sincospif(float(2.0 * (x - 0.25 * quarters)), &s, &c);
+      if (quarter & 1) {
+        const float t = c;
+        c = -s;
+        s = t;
+      }
+      turn[wave][0][lane] = quarter & 2 ? -c : c;
+      turn[wave][1][lane] = quarter & 2 ? -s : s;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own rows: its LDS operations stay in order
     __builtin_amdgcn_wave_barrier();

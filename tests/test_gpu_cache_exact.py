@@ -6,7 +6,7 @@ import math
 import pytest
 
 from conftest import report
-from test_gpu_cache import DTYPES, TDT, U, Cache, attention_ref, half, page_bounds_of, queries, run_paged, run_sparse
+from test_gpu_cache import DTYPES, TDT, U, Cache, attention_ref, half, lib, page_bounds_of, ptr, queries, run_paged, run_sparse
 
 pytestmark = pytest.mark.gpu
 
@@ -141,6 +141,48 @@ def test_large_scores_lose_nothing(ctx, dtype, lens, heads, kv, ps):
             worst = max(worst, float(((out[i].view(kv, G, 64)[hk].double() - ref).abs() / tol).max()))
     report("large.err", of_tolerance=f"{worst:.3f}")
     assert worst <= 1, worst
+
+
+# --- angles ---------------------------------------------------------------------------------------
+
+def run_turns(ctx, rope, pos, base):
+    """Cosines and sines as the rotation has them: [tokens, 32] each, the pairs (1, 0) turned."""
+    L = lib()
+    T = len(pos)
+    x = torch.zeros(T, 3, 2, 2, 16)   # q, k, v of one head; halves of two spans of 16 (grid), or of one of 32 (line)
+    x[:, 0, :, 0] = 1.0 if rope == "grid" else 0.0
+    if rope == "line":
+        x[:, 0, 0] = 1.0
+    qkv, d_pos = x.reshape(T, 192).cuda(), pos.to(torch.int32).cuda()
+    out = torch.full((T, 64), float("nan"), device="cuda")
+    torch.cuda.synchronize()
+    ctx.kernel_qk_norm_rope(L.F32, ptr(qkv), 192, T, 1, 1, L.NORM_NONE, 0, 0, 0, 0, 0.0,
+                            L.ROPE_GRID if rope == "grid" else L.ROPE_LINE, base, ptr(d_pos), ptr(out), 64)
+    ctx.synchronize()
+    out = out.cpu().double()
+    if rope == "line":
+        return out[:, :32], out[:, 32:]
+    out = out.view(T, 2, 2, 16)
+    return out[:, :, 0].reshape(T, 32), out[:, :, 1].reshape(T, 32)
+
+
+@pytest.mark.parametrize("rope", ["line", "grid"])
+@pytest.mark.parametrize("base", [100.0, 10000.0, 1.0])
+def test_angles(ctx, rope, base):
+    """At positions up to 4096 the turns in 64 bits are off by less than 2^-40. What 32 bits take of them is below an eighth of a
+    turn, 2^-27 of a half turn off at most (pi 2^-27 in the angle), and cosine and sine of it by one ulp of numbers below
+    1, 2^-24."""
+    n = 4097
+    if rope == "line":
+        pos = torch.arange(n)
+        turns = pos.double()[:, None] * base ** (-torch.arange(32, dtype=torch.float64) / 32)
+    else:
+        pos = torch.stack([torch.arange(n), torch.arange(n).flip(0)], 1)
+        turns = (pos.double()[:, :, None] * base ** (-torch.arange(16, dtype=torch.float64) / 16)).reshape(n, 32)
+    cs, sn = run_turns(ctx, rope, pos, base)
+    worst = max(float((cs - torch.cos(turns)).abs().max()), float((sn - torch.sin(turns)).abs().max()))
+    report("angles.err", rope=rope, base=base, units=f"{worst / 2.0 ** -24:.3f}")
+    assert worst <= 2.0 ** -24 + math.pi * 2.0 ** -27
 
 
 # --- the choice of pages --------------------------------------------------------------------------
