@@ -191,8 +191,10 @@ void check_page_bounds(BoundsArgs& a) {
   SPLAT_CHECK(a.table && a.lens && a.bounds && aligned16(a.bounds), BAD_ARGUMENT,
               "page bounds: a required pointer is NULL, or bounds not 16-byte aligned");
   SPLAT_CHECK(aligned4({a.table, a.lens, a.add}), BAD_ARGUMENT, "page bounds: table, lens and add must be 4-byte aligned");
-  SPLAT_CHECK(!meets_pools(a.cache, a.bounds, long(a.cache.pages) * a.cache.kv_heads * 128 * type_size(a.cache.dt)), BAD_ARGUMENT,
-              "page bounds: bounds overlap the cache");
+  const Range out = {a.bounds, long(a.cache.pages) * a.cache.kv_heads * 128 * type_size(a.cache.dt)};
+  SPLAT_CHECK(!meets_pools(a.cache, out.at, out.bytes), BAD_ARGUMENT, "page bounds: bounds overlap the cache");
+  SPLAT_CHECK(!meet(out, {a.table, 4L * a.n * a.width}) && !meet(out, {a.lens, 4L * a.n}) && !meet(out, {a.add, 4L * a.n}), BAD_ARGUMENT,
+              "page bounds: bounds overlap the table, lens or add");
   // add positions that end anywhere lie in one page more than they fill
   a.per_seq = int(std::min<long>(a.width, a.add ? (long(a.max_add) + a.cache.page_size - 1) / a.cache.page_size + 1 : a.width));
   SPLAT_CHECK(long(a.n) * a.cache.kv_heads <= MOST_UNITS, BAD_ARGUMENT, "page bounds: more than 2^25 sequences and heads");
