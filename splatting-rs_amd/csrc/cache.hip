@@ -1394,6 +1394,7 @@ void qk_norm_rope(const Exec& ex, const QkArgs& args, double base) {
 void page_bounds(const Exec& ex, const BoundsArgs& args) {
   BoundsArgs a = args;
   check_page_bounds(a);
+  check_overlaps(a);
   if (a.n == 0 || ex.dry) return;
   const long units = long(a.n) * a.per_seq * a.cache.kv_heads;
   ProfScope prof(ex, "page_bounds", 128.0 * units * a.cache.page_size,

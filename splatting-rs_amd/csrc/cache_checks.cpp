@@ -67,6 +67,7 @@ bool meet(const Range& a, const Range& b) { return meet(a.at, a.bytes, b.at, b.b
 long pool_bytes(const KvCache& c) {
   return ((c.pages - 1L) * c.page_stride + long(c.kv_heads) * c.page_size * 64) * type_size(c.dt);
 }
+long bounds_bytes(const KvCache& c) { return long(c.pages) * c.kv_heads * 128 * type_size(c.dt); }
 bool meets_pools(const KvCache& c, const void* p, long bytes) {
   return meet(c.k, pool_bytes(c), p, bytes) || meet(c.v, pool_bytes(c), p, bytes);
 }
@@ -191,14 +192,18 @@ void check_page_bounds(BoundsArgs& a) {
   SPLAT_CHECK(a.table && a.lens && a.bounds && aligned16(a.bounds), BAD_ARGUMENT,
               "page bounds: a required pointer is NULL, or bounds not 16-byte aligned");
   SPLAT_CHECK(aligned4({a.table, a.lens, a.add}), BAD_ARGUMENT, "page bounds: table, lens and add must be 4-byte aligned");
-  const Range out = {a.bounds, long(a.cache.pages) * a.cache.kv_heads * 128 * type_size(a.cache.dt)};
-  SPLAT_CHECK(!meets_pools(a.cache, out.at, out.bytes), BAD_ARGUMENT, "page bounds: bounds overlap the cache");
-  SPLAT_CHECK(!meet(out, {a.table, 4L * a.n * a.width}) && !meet(out, {a.lens, 4L * a.n}) && !meet(out, {a.add, 4L * a.n}), BAD_ARGUMENT,
-              "page bounds: bounds overlap the table, lens or add");
+  SPLAT_CHECK(!meets_pools(a.cache, a.bounds, bounds_bytes(a.cache)), BAD_ARGUMENT, "page bounds: bounds overlap the cache");
   // add positions that end anywhere lie in one page more than they fill
   a.per_seq = int(std::min<long>(a.width, a.add ? (long(a.max_add) + a.cache.page_size - 1) / a.cache.page_size + 1 : a.width));
   SPLAT_CHECK(long(a.n) * a.cache.kv_heads <= MOST_UNITS, BAD_ARGUMENT, "page bounds: more than 2^25 sequences and heads");
   a.per_seq = int(std::min<long>(a.per_seq, MOST_UNITS / (long(a.n) * a.cache.kv_heads)));  // a wave goes on to the next ones
+}
+
+void check_overlaps(const BoundsArgs& a) {
+  if (a.n == 0) return;
+  const Range out = {a.bounds, bounds_bytes(a.cache)};
+  SPLAT_CHECK(!meet(out, {a.table, 4L * a.n * a.width}) && !meet(out, {a.lens, 4L * a.n}) && !meet(out, {a.add, 4L * a.n}), BAD_ARGUMENT,
+              "page bounds: bounds overlap the table, lens or add");
 }
 
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes) {
@@ -217,7 +222,7 @@ void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) 
               "sparse attention: a required pointer is NULL, or bounds not 16-byte aligned");
   const PagedArgs& p = a.at;
   const long es = type_size(p.cache.dt), w = p.heads * 64L;
-  const Range sel = {a.selected, 4L * p.n * p.cache.kv_heads * a.topk}, low = {a.bounds, long(p.cache.pages) * p.cache.kv_heads * 128 * es};
+  const Range sel = {a.selected, 4L * p.n * p.cache.kv_heads * a.topk}, low = {a.bounds, bounds_bytes(p.cache)};
   const Range out = {p.out, ((p.n - 1L) * p.ldo + w) * es};
   SPLAT_CHECK(aligned4({a.selected}), BAD_ARGUMENT, "sparse attention: selected must be 4-byte aligned");
   SPLAT_CHECK(!meets_pools(p.cache, sel.at, sel.bytes) && !meet(sel, {p.q, ((p.n - 1L) * p.ldq + w) * es}) && !meet(sel, out) &&

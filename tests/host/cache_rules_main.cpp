@@ -60,6 +60,7 @@ void bounds_overlaps() {
       BoundsArgs a = bounds();
       f(a);
       check_page_bounds(a);
+      check_overlaps(a);
     });
   };
   B("ok", [](auto&) {});
