@@ -72,7 +72,8 @@ struct SparseArgs {
 void check_block_tables(BlockTableArgs& a);
 void check_qk_norm_rope(QkArgs& a, double base);
 void check_page_bounds(BoundsArgs& a);
-void check_overlaps(const BoundsArgs& a);  // of outputs with index arrays, after the check above
+void check_overlaps(const BoundsArgs& a);  // of outputs with index arrays and weights, after the checks above
+void check_overlaps(const QkArgs& a);
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes);
 void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes);
 

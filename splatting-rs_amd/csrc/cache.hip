@@ -1371,6 +1371,7 @@ void block_tables(const Exec& ex, const BlockTableArgs& args) {
 void qk_norm_rope(const Exec& ex, const QkArgs& args, double base) {
   QkArgs a = args;
   check_qk_norm_rope(a, base);
+  check_overlaps(a);
   if (a.tokens == 0 || ex.dry) return;
   if (a.rope != ROPE_NONE) rope_turns(a.rope, base, a.freq);
   const double values = double(a.tokens) * (a.heads + (a.has_cache ? 2 : 1) * a.kv_heads) * 64;

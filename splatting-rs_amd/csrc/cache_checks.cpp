@@ -72,6 +72,15 @@ bool meets_pools(const KvCache& c, const void* p, long bytes) {
   return meet(c.k, pool_bytes(c), p, bytes) || meet(c.v, pool_bytes(c), p, bytes);
 }
 
+// `count` rows of `width` bytes, `stride` apart.
+struct Rows { const void* at; long stride, width, count; };
+bool row_meets(const Rows& a, const Range& b) {
+  if (!a.at || !b.at || a.count <= 0 || b.bytes <= 0) return false;
+  const intptr_t pa = reinterpret_cast<intptr_t>(a.at), pb = reinterpret_cast<intptr_t>(b.at);
+  const long row = std::max<long>(0, (pb - pa - a.width) / a.stride + (pb - pa >= a.width));  // the first that ends behind b's beginning
+  return row < a.count && pa + row * a.stride < pb + b.bytes;
+}
+
 // A table's row holds up to 2^27 pages; the kernels count places past topk in 32 bits.
 void check_topk(int topk) {
   SPLAT_CHECK(topk >= 1 && topk <= (1 << 27), BAD_ARGUMENT, "sparse attention: topk must be 1 to 2^27");
@@ -204,6 +213,18 @@ void check_overlaps(const BoundsArgs& a) {
   const Range out = {a.bounds, bounds_bytes(a.cache)};
   SPLAT_CHECK(!meet(out, {a.table, 4L * a.n * a.width}) && !meet(out, {a.lens, 4L * a.n}) && !meet(out, {a.add, 4L * a.n}), BAD_ARGUMENT,
               "page bounds: bounds overlap the table, lens or add");
+}
+
+void check_overlaps(const QkArgs& a) {
+  if (a.tokens == 0) return;
+  const long es = type_size(a.dt), page = a.kv_heads * 64L * a.cache.page_size * es, stride = a.cache.page_stride * es;
+  const Rows out[] = {{a.q_out, a.ldq * es, a.heads * 64 * es, a.tokens}, {a.k_out, a.ldk * es, a.kv_heads * 64 * es, a.tokens},
+                      {a.has_cache ? a.cache.k : nullptr, stride, page, a.cache.pages}, {a.has_cache ? a.cache.v : nullptr, stride, page, a.cache.pages}};
+  const long position = a.rope == ROPE_GRID ? 8 : a.rope == ROPE_LINE ? 4 : 0, weight = a.norm == NORM_NONE ? 0 : 256;
+  const Range in[] = {{a.positions, position * a.tokens}, {a.slots, 4L * a.tokens}, {a.qw, weight}, {a.qb, weight}, {a.kw, weight}, {a.kb, weight}};
+  for (const Rows& o : out)
+    for (const Range& i : in)
+      SPLAT_CHECK(!row_meets(o, i), BAD_ARGUMENT, "qk norm: an output or the cache overlaps the positions, the slots or a weight");
 }
 
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes) {

@@ -73,9 +73,72 @@ void bounds_overlaps() {
   B("over add", [](auto& a) { a.add = ints(300 * MB - 8); });
 }
 
+// 10 rows of 8 + 4 heads of 64 bf16: q_out 10 rows of 1024 bytes, 1536 apart; pools of 100 pages of 8192 bytes.
+QkArgs qk() {
+  QkArgs a;
+  a.dt = 1;
+  a.tokens = 10;
+  a.heads = 8;
+  a.kv_heads = 4;
+  a.qkv = at(200 * MB);
+  a.ld = 16 * 64;
+  a.norm = NORM_LAYER;
+  a.eps = 1e-5f;
+  a.rope = ROPE_GRID;
+  a.positions = ints(300 * MB);
+  a.q_out = at(400 * MB);
+  a.ldq = 12 * 64;
+  a.k_out = at(500 * MB);
+  a.ldk = 4 * 64;
+  a.has_cache = true;
+  a.cache = cache();
+  a.slots = ints(600 * MB);
+  a.qw = floats(700 * MB);
+  a.qb = floats(701 * MB);
+  a.kw = floats(702 * MB);
+  a.kb = floats(703 * MB);
+  return a;
+}
+
+void qk_overlaps() {
+  const auto Q = [](const std::string& n, const std::function<void(QkArgs&)>& f) {
+    say("qk " + n, [&] {
+      QkArgs a = qk();
+      f(a);
+      check_qk_norm_rope(a, 100.0);
+      check_overlaps(a);
+    });
+  };
+  Q("ok", [](auto&) {});
+  Q("ok no weights", [](auto& a) { a.qw = a.qb = a.kw = a.kb = nullptr; });
+  Q("ok one weight for both", [](auto& a) { a.kw = a.qw; a.kb = a.qb; });
+  Q("ok nothing", [](auto& a) { a.tokens = 0; a.positions = static_cast<const int*>(a.q_out); });
+  Q("ok weights between rows", [](auto& a) { a.qw = floats(400 * MB + 1024); a.kw = floats(400 * MB + 1536 + 1280); });
+  Q("ok slots behind the last row", [](auto& a) { a.slots = ints(400 * MB + 9 * 1536 + 1024); });
+  Q("ok slots before k_out", [](auto& a) { a.slots = ints(500 * MB - 40); });
+  Q("ok weights in a page's gap", [](auto& a) { a.cache.page_stride += 128; a.kb = floats(7 * (8192 + 256) + 8192); });
+  Q("ok positions unread", [](auto& a) { a.rope = ROPE_NONE; a.positions = static_cast<const int*>(a.q_out); });
+  Q("ok weights unread", [](auto& a) { a.norm = NORM_NONE; a.qw = static_cast<const float*>(a.q_out); });
+  Q("q_out over positions", [](auto& a) { a.positions = ints(400 * MB - 76); });
+  Q("q_out over the grid's second positions", [](auto& a) { a.positions = ints(400 * MB - 44); });
+  Q("q_out over slots", [](auto& a) { a.slots = ints(400 * MB + 9 * 1536 + 1020); });
+  Q("q_out over qw", [](auto& a) { a.qw = floats(400 * MB + 1024 - 16); });
+  Q("q_out over qb", [](auto& a) { a.qb = floats(400 * MB + 3 * 1536 - 128); });
+  Q("q_out over kw", [](auto& a) { a.kw = floats(400 * MB + 9 * 1536); });
+  Q("q_out over kb", [](auto& a) { a.kb = floats(400 * MB - 240); });
+  Q("k_out over positions", [](auto& a) { a.positions = ints(500 * MB + 100); });
+  Q("k_out over slots", [](auto& a) { a.slots = ints(500 * MB + 5116); });
+  Q("k_out over kw", [](auto& a) { a.kw = floats(500 * MB + 512); });
+  Q("keys over positions", [](auto& a) { a.positions = ints(50 * 8192); });
+  Q("keys over slots", [](auto& a) { a.slots = ints(100 * 8192 - 4); });
+  Q("values over slots", [](auto& a) { a.slots = ints(64 * MB - 36); });
+  Q("values over kb", [](auto& a) { a.kb = floats(64 * MB + 99 * 8192); });
+}
+
 }  // namespace
 
 int main() {
   bounds_overlaps();
+  qk_overlaps();
   return 0;
 }

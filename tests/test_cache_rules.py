@@ -34,3 +34,7 @@ def check(lines, first, least):
 
 def test_bounds_lie_over_no_other_argument(lines):
     check(lines, "bounds", 8)
+
+
+def test_rows_and_pools_lie_over_no_other_argument(lines):
+    check(lines, "qk", 24)
