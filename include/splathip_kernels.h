@@ -186,7 +186,8 @@ int splat_kernel_page_bounds(splat_ctx* ctx, const splat_kv_cache* cache, int n,
  * upper bound of the lengths that the host knows, for the launch (longer ones are cut there). In bf16 and f16 a
  * weight goes to the matrix cores as two numbers of that type, the second what the first leaves: 16 bits of it in bf16, 22 in
  * f16 (the first alone for a sequence whose sums hold a NaN, as beside an infinite value).
- * workspace: device memory of at least splat_paged_attention_workspace's bytes, 16-byte aligned. */
+ * workspace: device memory of at least splat_paged_attention_workspace's bytes, 16-byte aligned. One for the largest n, max_len (and
+ * topk) serves every smaller call. */
 int splat_paged_attention_workspace(const splat_kv_cache* cache, int n, int heads, int max_len, size_t* bytes);
 int splat_kernel_paged_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* q, int64_t ldq, int n,
                                  int heads, const int32_t* table, int width, const int32_t* lens, int max_len,

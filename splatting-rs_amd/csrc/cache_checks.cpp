@@ -12,6 +12,7 @@ namespace {
 
 // A launch has below 2^32 threads in x: up to 1024 for a query row, 64 for a token or for the page of a head.
 constexpr long MOST_STRIDE = 1L << 31;  // elements from row to row: sizes in bytes stay within 64 bits
+constexpr int FULL_BLOCKS = 1024;  // of attention in one launch, from which on they fill the chip several times
 constexpr long MOST_ROWS = 1 << 21, MOST_TOKENS = 1 << 25, MOST_UNITS = 1 << 25;
 
 long type_size(int dt) { return dt == 0 ? 4 : 2; }
@@ -123,6 +124,9 @@ void check_workspace(const PagedArgs& a, const void* workspace, size_t bytes, si
               BAD_ARGUMENT, "attention: the workspace overlaps another argument");
 }
 
+// The scores of every page that max_len allows.
+size_t key_bytes(const KvCache& c, int n, int max_len) { return size_t(n) * c.kv_heads * ((long(max_len) + c.page_size - 1) / c.page_size) * 8; }
+
 // A generous max_len sizes the workspace, which no shorter one needs more of, but not the launch.
 void cut_to_row(PagedArgs& a) { a.max_len = int(std::min<long>(a.max_len, long(a.width) * a.cache.page_size)); }
 
@@ -230,7 +234,7 @@ void check_overlaps(const QkArgs& a) {
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes) {
   check_attention(a);
   if (a.n == 0) return;
-  check_workspace(a, workspace, bytes, paged_attention_bytes(a.cache, a.n, a.heads, a.max_len));
+  check_workspace(a, workspace, bytes, paged_plan(a.cache, a.n, a.heads, a.max_len, 0).bytes);
   cut_to_row(a);
 }
 
@@ -249,7 +253,7 @@ void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes) 
   SPLAT_CHECK(!meets_pools(p.cache, sel.at, sel.bytes) && !meet(sel, {p.q, ((p.n - 1L) * p.ldq + w) * es}) && !meet(sel, out) &&
                   !meet(sel, {p.table, 4L * p.n * p.width}) && !meet(sel, {p.lens, 4L * p.n}) && !meet(sel, low) && !meet(out, low),
               BAD_ARGUMENT, "sparse attention: selected or out overlaps another argument");
-  const size_t need = sparse_attention_bytes(p.cache, p.n, p.heads, p.max_len, a.topk);
+  const size_t need = paged_plan(p.cache, p.n, p.heads, p.max_len, a.topk).bytes + key_bytes(p.cache, p.n, p.max_len);
   check_workspace(p, workspace, bytes, need);
   SPLAT_CHECK(!meet({workspace, long(need)}, sel) && !meet({workspace, long(need)}, low), BAD_ARGUMENT,
               "sparse attention: the workspace overlaps another argument");
@@ -276,7 +280,7 @@ PagedPlan paged_plan(const KvCache& c, int n, int heads, int max_len, int topk) 
   // 12 heads (bf16) 9.3 : 11.2 us at 1000 positions, 11.8 : 11.2 at 1500; 32 heads on 4 (fp32, tiles of 16) 8.8 : 9.9 at 300,
   // 13.4 : 11.1 at 600; and where the blocks fill the chip several times (200 sequences of up to 2000) 44.8 : 52.8, up to 4000
   // 74.5 : 78.0.
-  if (longest <= (long(n) * plan.cols >= 1024 ? 128 : c.dt == 0 ? 28 : 44)) return plan;
+  if (longest <= (long(n) * plan.cols >= FULL_BLOCKS ? 128 : c.dt == 0 ? 28 : 44)) return plan;
   // eight waves on each of 256 CUs, but two tiles at least for each where all sequences are as long as may be
   const long tiles = n * longest;
   const long workers = std::min<long>(2048 / plan.cols, (tiles + 1) / 2);
@@ -290,15 +294,24 @@ PagedPlan paged_plan(const KvCache& c, int n, int heads, int max_len, int topk) 
   return plan;
 }
 
+namespace {
+// What the plan takes for n sequences or fewer: few sequences may leave parts where many leave none.
+size_t plan_bytes(const KvCache& c, int n, int heads, int max_len, int topk) {
+  const PagedPlan all = paged_plan(c, n, heads, max_len, topk);
+  const int few = std::min(n, (FULL_BLOCKS - 1) / all.cols);
+  return few ? std::max(all.bytes, paged_plan(c, few, heads, max_len, topk).bytes) : all.bytes;
+}
+}  // namespace
+
 size_t paged_attention_bytes(const KvCache& c, int n, int heads, int max_len) {
   check_workspace_sizes(c, n, heads, max_len);
-  return paged_plan(c, n, heads, max_len, 0).bytes;
+  return plan_bytes(c, n, heads, max_len, 0);
 }
 
 size_t sparse_attention_bytes(const KvCache& c, int n, int heads, int max_len, int topk) {
   check_workspace_sizes(c, n, heads, max_len);
   check_topk(topk);
-  return paged_plan(c, n, heads, max_len, topk).bytes + size_t(n) * c.kv_heads * ((long(max_len) + c.page_size - 1) / c.page_size) * 8;
+  return plan_bytes(c, n, heads, max_len, topk) + key_bytes(c, n, max_len);
 }
 
 void rope_turns(int rope, double base, double (&freq)[32]) {

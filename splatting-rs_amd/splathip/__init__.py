@@ -521,14 +521,14 @@ def _check_free(rc: int):
 
 
 def paged_attention_workspace(cache: KvCache, n: int, heads: int, max_len: int) -> int:
-    """Bytes of device memory that kernel_paged_attention needs for these sizes."""
+    """Bytes of device memory that kernel_paged_attention needs for these sizes or smaller ones."""
     b = C.c_size_t()
     _check_free(lib().splat_paged_attention_workspace(cache, n, heads, max_len, C.byref(b)))
     return b.value
 
 
 def sparse_attention_workspace(cache: KvCache, n: int, heads: int, max_len: int, topk: int) -> int:
-    """Bytes of device memory that kernel_sparse_attention needs for these sizes."""
+    """Bytes of device memory that kernel_sparse_attention needs for these sizes or smaller ones."""
     b = C.c_size_t()
     _check_free(lib().splat_sparse_attention_workspace(cache, n, heads, max_len, topk, C.byref(b)))
     return b.value

@@ -135,9 +135,70 @@ void qk_overlaps() {
   Q("values over kb", [](auto& a) { a.kb = floats(64 * MB + 99 * 8192); });
 }
 
+// A workspace that is sized for the largest batch, length and selection serves every smaller call.
+void workspaces() {
+  for (int dt = 0; dt < 3; ++dt)
+    for (int kv : {1, 2, 12, 300})
+      for (int group : {1, 8, 20})
+        for (int topk : {0, 1, 60, 100, 3000})
+          say("workspace ok " + std::to_string(dt) + " " + std::to_string(kv) + " " + std::to_string(group) + " " + std::to_string(topk), [&] {
+            const KvCache c = cache(dt, kv);
+            const auto bytes = [&](int n, int len, int k) {
+              return topk ? sparse_attention_bytes(c, n, kv * group, len, k) : paged_attention_bytes(c, n, kv * group, len);
+            };
+            for (int len : {1, 440, 500, 900, 1500, 2000, 4000, 4200, 30000}) {
+              size_t most = 0;
+              for (int n = 1; n <= 1500 && long(n) * kv * group < 1 << 21; n += 1 + n / 60) {
+                const size_t b = bytes(n, len, topk);
+                expect(b >= most, "less for " + std::to_string(n) + " sequences of " + std::to_string(len));
+                expect(bytes(n, len + 1, topk) >= b, "less for a longer max_len");
+                expect(!topk || bytes(n, len, topk + 1) >= b, "less for more pages");
+                most = b;
+              }
+            }
+          });
+  for (int topk : {0, 100})
+    for (int n : {1, 3, 85, 86, 87, 200})
+      say("workspace ok of a larger batch " + std::to_string(topk) + " " + std::to_string(n), [&] {
+        SparseArgs s;
+        PagedArgs& a = s.at;
+        a.cache = cache(1, 12);
+        a.n = n;
+        a.heads = 12;
+        a.q = at(200 * MB);
+        a.ldq = a.ldo = 12 * 64;
+        a.table = ints(300 * MB);
+        a.width = 300;
+        a.lens = ints(400 * MB);
+        a.max_len = topk ? 4000 : 2000;
+        a.scale = 0.125f;
+        a.out = at(500 * MB);
+        s.bounds = at(600 * MB);
+        s.topk = topk;
+        s.selected = ints(700 * MB);
+        if (topk) check_sparse_attention(s, at(800 * MB), sparse_attention_bytes(a.cache, 200, 12, a.max_len, topk));
+        else check_paged_attention(a, at(800 * MB), paged_attention_bytes(a.cache, 200, 12, a.max_len));
+      });
+  say("workspace ok none where no parts are left", [] {
+    PagedArgs a;
+    a.cache = cache(1, 12);
+    a.n = 200;
+    a.heads = 12;
+    a.q = at(200 * MB);
+    a.ldq = a.ldo = 12 * 64;
+    a.table = ints(300 * MB);
+    a.width = 300;
+    a.lens = ints(400 * MB);
+    a.max_len = 2000;
+    a.out = at(500 * MB);
+    check_paged_attention(a, nullptr, 0);
+  });
+}
+
 }  // namespace
 
 int main() {
+  workspaces();
   bounds_overlaps();
   qk_overlaps();
   return 0;

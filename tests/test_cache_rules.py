@@ -38,3 +38,7 @@ def test_bounds_lie_over_no_other_argument(lines):
 
 def test_rows_and_pools_lie_over_no_other_argument(lines):
     check(lines, "qk", 24)
+
+
+def test_a_workspace_for_the_largest_call_serves_every_smaller_one(lines):
+    check(lines, "workspace", 3 * 4 * 3 * 5 + 13)

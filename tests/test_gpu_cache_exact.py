@@ -281,3 +281,35 @@ def test_a_score_is_the_sum_of_each_heads_most(ctx, dtype):
 def test_the_choice_is_the_definitions(ctx, dtype, pages, heads, kv):
     c = Cache(dtype, [16 * pages - 5, 16 * 9], kv, 16, garbage=False)
     check_choice(ctx, c, page_bounds_of(c), queries(c, heads), heads, (2, 9, pages // 3, pages))
+
+
+# --- workspaces -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_a_workspace_for_the_largest_batch_serves_smaller_ones(ctx, sparse):
+    """A serving loop: one workspace, sized for 100 sequences (one launch, no parts), and batches that shrink (parts)."""
+    L = lib()
+    heads, ps, topk, most = 12, 16, 100, 2000
+    full = Cache("bf16", [most] + [(37 * i) % 60 for i in range(99)], heads, ps, garbage=False)
+    cache, bounds = full.device(), page_bounds_of(full).cuda()
+    size = L.sparse_attention_workspace(cache, 100, heads, most, topk) if sparse else L.paged_attention_workspace(cache, 100, heads, most)
+    ws = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+    q = queries(full, heads)
+    dq, sel = q.cuda(), torch.empty(100, heads, topk, dtype=torch.int32, device="cuda")
+    outs = []
+    for n in (100, 86, 85, 3, 1):
+        out = torch.full((100, heads * 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+        at = (ptr(dq), heads * 64, n, heads, ptr(full.dtable), full.width, ptr(full.dlens), most)
+        ws.fill_(255)
+        torch.cuda.synchronize()
+        if sparse:
+            ctx.kernel_sparse_attention(cache, ptr(bounds), *at, topk, 0.125, ptr(out), heads * 64, ptr(sel), ptr(ws), size)
+        else:
+            ctx.kernel_paged_attention(cache, *at, 0.125, ptr(out), heads * 64, ptr(ws), size)
+        ctx.synchronize()
+        outs.append(out.cpu().float())
+        assert torch.isnan(outs[-1][n:]).all() and torch.isfinite(outs[-1][:n]).all()
+        # other cuts of the same sums: each result is off by one rounding to the type, h |ref|, and before it by (L + 8) u + h_w of
+        # the largest value (e is the same for both), so two of them differ by twice that
+        d, h = (outs[-1][:n] - outs[0][:n]).abs(), half("bf16")
+        assert (d <= 2 * (1 + h) * h * outs[0][:n].abs() + 2 * ((most + 8) * U + h * h) * float(full.v.float().abs().max())).all()
