@@ -6,7 +6,7 @@ import math
 import pytest
 
 from conftest import report
-from test_gpu_cache import DTYPES, TDT, U, Cache, attention_ref, half, lib, page_bounds_of, ptr, queries, run_paged, run_sparse
+from test_gpu_cache import DTYPES, TDT, U, Cache, Rope, attention_ref, half, lib, page_bounds_of, ptr, queries, run_paged, run_sparse
 
 pytestmark = pytest.mark.gpu
 
@@ -183,6 +183,58 @@ def test_angles(ctx, rope, base):
     worst = max(float((cs - torch.cos(turns)).abs().max()), float((sn - torch.sin(turns)).abs().max()))
     report("angles.err", rope=rope, base=base, units=f"{worst / 2.0 ** -24:.3f}")
     assert worst <= 2.0 ** -24 + math.pi * 2.0 ** -27
+
+
+# --- norms, each within its own bound -------------------------------------------------------------
+
+def norm_tol(x, w, b, norm, rope, eps, ref, dtype):
+    """Rows x [.., 64] in 64 bits. In units of u, before the rounding to the type (h |ref|):
+      sums of 64 terms of one sign: 8 additions in a lane, 3 across, a rounding of each term: 12.
+      rms: the root halves those, and it, eps, the division, x r, w and b add one each: 12 S at most, S = |x| r |w| + |b|.
+      layer: the mean is off by 12 M (M = max |x|), so a difference by that and 1 of itself, and the variance, relative to itself, by
+        2 * 12 M / sd + 12 + 2: y = d r by 12 M / sd (1 + |y|) + 12 |y|, and w and b add one each of S.
+      rotation: cosines and sines are off by 1.4 and two products and their sum round: the parts' errors add up, and
+        2 * 2.4 + 1 of the largest S.
+    """
+    top = lambda t: t.abs().amax(-1, keepdim=True)  # noqa: E731
+    W = top(w) if w is not None else 1.0
+    B = top(b) if b is not None else 0.0
+    if norm == "none":
+        S, E = top(x), 0.0
+    elif norm == "rms":
+        S = top(x) / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * W + B
+        E = 12 * S
+    else:
+        sd = torch.sqrt(x.var(-1, unbiased=False, keepdim=True) + eps)
+        Y = top(x - x.mean(-1, keepdim=True)) / sd
+        S = Y * W + B
+        E = W * (12 * top(x) / sd * (1 + Y) + 12 * Y) + 2 * S
+    tol = half(dtype) * ref.abs() + U * (E if rope == "none" else 2 * E + 6 * S)
+    return tol + (2.0 ** -25 if dtype == "f16" else 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm", ["none", "layer", "rms"])
+@pytest.mark.parametrize("rope", ["none", "line", "grid"])
+def test_norms_within_their_own_bound(ctx, dtype, norm, rope):
+    for T, heads, kv, kw in ((33, 6, 6, {}), (70, 8, 2, {"bias": False}), (5, 3, 1, {"weights": False, "bias": False})):
+        report("norms", dtype=dtype, norm=norm, rope=rope, T=T, heads=heads, kv=kv, **kw)
+        r = Rope(dtype, T, heads, kv, norm, rope, cache=False, **kw)
+        x = r.qkv.float()
+        x[::3] = x[::3] * 0.05 + 4.0      # a mean far from 0
+        x[1::3] *= 30.0
+        r.qkv = x.to(TDT[dtype])
+        q = torch.empty(T, heads * 64, dtype=TDT[dtype], device="cuda")
+        k = torch.empty(T, kv * 64, dtype=TDT[dtype], device="cuda")
+        r.call(ctx, q, heads * 64, k, kv * 64, None, None)
+        (xq, rq), (xk, rk), _ = r.refs()
+        worst = 0.0
+        for got, xs, ref, w, b in ((q, xq, rq, r.w[0], r.b[0]), (k, xk, rk, r.w[1], r.b[1])):
+            w, b = (None if t is None else t.double() for t in (w, b))
+            d = (got.cpu().double().reshape(ref.shape) - ref).abs()
+            worst = max(worst, float((d / norm_tol(xs, w, b, norm, rope, r.eps, ref, dtype).clamp(min=1e-300)).max()))
+        report("norms.err", of_tolerance=f"{worst:.3f}")
+        assert worst <= 1, worst
 
 
 # --- the choice of pages --------------------------------------------------------------------------
