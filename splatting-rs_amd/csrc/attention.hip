@@ -380,8 +380,9 @@ __device__ inline int32x4_t make_rsrc_a(const void* p, uint32_t bytes) {
 // 16 bytes per lane from rsrc at voffset + soffset into LDS at lds + 16 * lane. A voffset of
 // 0x80000000 reads zeros whatever soffset holds: every valid voffset + soffset lies inside the
 // buffer (below 2^31), so the range check, with or without soffset, rejects only that one.
+// The wait state is what a load into LDS wants after a write of m0, which the compiler does not insert before inline assembly.
 __device__ inline void load_lds_a(const int32x4_t& rsrc, uint32_t voffset, uint32_t soffset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))),
                "v"(voffset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(int(soffset)))
                : "memory");
 }

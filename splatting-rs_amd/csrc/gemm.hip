@@ -818,9 +818,9 @@ __device__ inline uint32_t lds_addr(const void* p) {
 // voffset + soffset stays inside the buffer, so the range check of either form (with or
 // without soffset) gives the same result.
 __device__ inline void load_to_lds(const int32x4_t& rsrc, uint32_t voffset, uint32_t soffset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))),
                "v"(voffset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(int(soffset)))
-               : "memory");  // m0 is set here and used by nothing else in these kernels
+               : "memory");  // m0 is set here and used by nothing else in these kernels; a load into LDS wants a wait state after it
 }
 
 template <int N> __device__ inline void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }

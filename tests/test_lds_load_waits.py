@@ -79,7 +79,8 @@ def functions(tmp_path_factory):
     return {k: v for k, v in out.items() if any("lds" in i and i.startswith("buffer_load") for i in v)}
 
 
-@pytest.mark.parametrize("kernel", ["paged_whole_kernel", "paged_parts_kernel"])
+@pytest.mark.parametrize("kernel", ["paged_whole_kernel", "paged_parts_kernel", "gemm_mfma_kernel", "conv3x3_halo_kernel", "attn_bf16_kernel",
+                                    "attn_f32_kernel"])
 def test_loads_into_lds_wait_for_their_registers(functions, kernel):
     found = {k: v for k, v in functions.items() if kernel in k}
     assert found
