@@ -143,6 +143,25 @@ def test_large_scores_lose_nothing(ctx, dtype, lens, heads, kv, ps):
     assert worst <= 1, worst
 
 
+def test_fp32_scores_are_summed_in_quarters(ctx):
+    """Products of 2^16 and -2^16 in the first and last channel, and 32 small ones between, whose sum is 3.6 steps of fp32 at 2^16.
+    A chain through all channels rounds each of them off there; sums of a quarter's 16 channels hold them, and their three
+    additions round by half a step, 2^-8, each: the score is off by 3 2^-8, tanh(score / 2) by half of that."""
+    c = Cache("f32", [2], 1, 16, garbage=False)
+    t = 0.1125 * 2.0 ** -7   # four of them, a step's products, are less than half of the step at 2^16, 2^-7
+    k, q = torch.zeros(64), torch.ones(64)
+    k[0], q[0], k[63], q[63] = 256.0, 256.0, 256.0, -256.0
+    k[16:48] = t
+    page = c.k[int(c.table[0, 0])].view(16, 64)
+    page[0], page[1] = 0.0, k
+    c.v[int(c.table[0, 0])].view(16, 64)[0], c.v[int(c.table[0, 0])].view(16, 64)[1] = -1.0, 1.0
+    out = run_paged(ctx, c, q[None], 1, scale=1.0).double()
+    ref = math.tanh(float((q.double() * k.double()).sum()) / 2)
+    worst = float((out - ref).abs().max())
+    report("quarters", ref=f"{ref:.5f}", off=f"{worst:.5f}")
+    assert worst <= 1.5 * 2.0 ** -8 + 8 * U
+
+
 # --- angles ---------------------------------------------------------------------------------------
 
 def run_turns(ctx, rope, pos, base):
