@@ -276,11 +276,11 @@ PagedPlan paged_plan(const KvCache& c, int n, int heads, int max_len, int topk) 
   PagedPlan plan;
   plan.cols = c.kv_heads * ((G + 15) / 16);
   const long most = topk ? std::min<long>(max_len, long(topk) * c.page_size) : max_len, longest = (most + keys - 1) / keys;
-  // One block a sequence, without a join, for few tiles a sequence. Measured, one launch against two: one sequence of
-  // 12 heads (bf16) 9.3 : 11.2 us at 1000 positions, 11.8 : 11.2 at 1500; 32 heads on 4 (fp32, tiles of 16) 8.8 : 9.9 at 300,
-  // 13.4 : 11.1 at 600; and where the blocks fill the chip several times (200 sequences of up to 2000) 44.8 : 52.8, up to 4000
-  // 74.5 : 78.0.
-  if (longest <= (long(n) * plan.cols >= FULL_BLOCKS ? 128 : c.dt == 0 ? 28 : 44)) return plan;
+  // One block a sequence, without a join, for few tiles a sequence. Measured, one launch against two, a call among others: one
+  // sequence of 12 heads (bf16) 10.2 : 11.4 us at 1024 positions, 11.7 : 11.3 at 1280, 12.4 : 11.3 at 1300; 32 heads on 4 11.4 : 11.5 at
+  // 1280; in fp32 (tiles of 16) 10.9 : 12.3 at 448 and 11.9 : 11.9 at 512; and where the blocks fill the chip several times
+  // (200 sequences of up to 2000, 12 heads) 39.0 : 47.5, up to 4000 70.5 : 69.
+  if (longest <= (long(n) * plan.cols >= FULL_BLOCKS ? 128 : c.dt == 0 ? 28 : 40)) return plan;
   // eight waves on each of 256 CUs, but two tiles at least for each where all sequences are as long as may be
   const long tiles = n * longest;
   const long workers = std::min<long>(2048 / plan.cols, (tiles + 1) / 2);
