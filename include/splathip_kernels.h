@@ -78,7 +78,8 @@ int splat_kernel_conv_transpose2d(splat_ctx* ctx, int dtype, const void* in, int
                                   const void* w, int Cout, int ldw, int s, const float* bias, void* out);
 
 /* Per-kernel-class timing of the following forwards: HIP events around every launch on the
- * context's stream, with each launch's algorithmic work. Graph replay is bypassed while on. */
+ * context's stream, with each launch's algorithmic work. Graph replay is bypassed while on. The lengths in a paged
+ * cache are not known to the host: its calls count every sequence as long as the call allows, an upper bound. */
 typedef struct splat_kernel_stat {
   char name[32];
   int launches;
@@ -107,9 +108,12 @@ int splat_kernel_reconstruct(splat_ctx* ctx, int V, int H, int W, const float* d
                              float* points, float* conf_out);
 
 /* --- a paged cache of keys and values ------------------------------------------------------------
- * For scenes that grow: the keys and values of the tokens that are there stay in pages, and what is new
- * attends to them. No counterpart in the reference, whose models see every view in every call. Heads of 64
- * channels, as in splat_kernel_attention.
+ * For networks of the caller's in which a token's keys and values stay as they are when others come: they are kept in pages,
+ * and in each call one token of each sequence attends to those of its sequence. The two networks of this library are none: in
+ * their global blocks every token sees every other, so that a new view changes the keys of all of them behind the first such
+ * block, and no forward here uses the cache. Many tokens of one view are many sequences to these calls, each of which reads the whole
+ * cache; splat_kernel_attention is for whole views. No counterpart in the reference. Heads of 64 channels, as in
+ * splat_kernel_attention.
  *
  * Position p of sequence i lies in row p % page_size of page table[i * width + p / page_size]; a slot is
  * page * page_size + row. Lengths, tables and slots are device arrays: nothing here waits for the host. Table entries
