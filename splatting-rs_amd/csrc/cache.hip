@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs p) {
 // The scores come out with a lane holding one head (lane % 16) and keys 4 (lane / 16) + r, which is the
 // operand layout of the second product as it stands; V is read transposed from LDS.
 //
-// Bound by the bytes of K and V: 48 sequences (f16, 8 key heads, 295 MB) in 57 us, 5.1 TB/s, where a kernel that only reads
+// Bound by the bytes of K and V: 48 sequences (f16, 8 key heads, 295 MB) in 59 us, 5.0 TB/s, where a kernel that only reads
 // reaches 5.7 and a large copy 4.7. A kernel of the vector unit, one wave a query head, took 1.8 ms.
 //
 // A wave works alone: tiles of 32 keys (16 in fp32: 4 KB of K and 4 KB of V in every type) stream into its own
@@ -817,8 +817,8 @@ __device__ inline void join_block(const PagedArgs& p, const Wave& w, char* smem,
 
 // One block a (sequence, group of up to 16 heads of one key head): its waves take equal parts of the tiles
 // and join their sums in LDS. For short sequences (paged_plan has the rule and both sides' times): three of up to 188
-// positions (fp32, 6 heads) 7.4 us, of which the launch and the length take 2.6, the first tiles 2.0, the products of
-// three tiles in fp32 (matrix instructions of 4 keys) 2.0 and the join 0.8.
+// positions (fp32, 6 heads) 7.8 us, of which the launch and the length take 2.6, the first tiles 2.0, the products of
+// three tiles in fp32 (matrix instructions of 4 keys) 2.2 and the join 0.8.
 template <typename T, bool SPARSE>
 __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const PagedArgs p, const int* sel, int topk, float scale) {
   using Wave = PagedWave<T, SPARSE>;
@@ -847,8 +847,9 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const 
 // for paged_join_kernel: slot 0 for the sequence that a wave's part begins in, slot 1 for one that it ends in. With
 // span = PAGED_WAVES the parts that a block's waves end with are joined where they are of one sequence, so that a
 // long sequence leaves one part a block instead of one a wave (span = 1). That costs this kernel 1.5 us and spares the join its
-// batches: one sequence, 12 heads (168 waves each) 25.6 -> 24.7 us, 2 groups of 16 heads (388 waves) 21.6 -> 15.5; 48 sequences
-// (5 waves each) 66 -> 67.5, so it is done from 128 waves a sequence on.
+// batches: one sequence, 12 heads (156 waves each) 22.9 -> 22.4 us, 2 groups of 16 heads (260 waves) 16.4 -> 13.3; with fewer waves a
+// sequence it gives or costs a microsecond (8 sequences of 8000, 12 heads on 12 38.5 -> 39.6; 48 sequences, 32 heads on 8 57.6 ->
+// 56.8), so it is done from 128 waves a sequence on.
 constexpr int SCAN_MAX = 1024;
 
 
@@ -960,7 +961,7 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
 // One block a (sequence, `per` heads of a group): the parts of a sequence that several waves had. SPLIT waves share a
 // head (all eight where the block has one), each with every SPLIT-th part, a channel a lane, JOIN_PARTS parts under way.
 // Bound by its chain of loads (counts, then parts), not by their bytes: 39 parts of 12 heads 5.0 us, parts of 48 sequences of
-// 32 heads 8.5. Blocks of 4 or 16 waves, 4 to 24 parts under way and other numbers of heads a block were no faster; 64-bit
+// 32 heads 8.8. Blocks of 4 or 16 waves, 4 to 24 parts under way and other numbers of heads a block were no faster; 64-bit
 // integer divisions for the parts' places made it 18.6.
 constexpr int JOIN_WAVES = 8, JOIN_PARTS = 8;
 template <typename T>
@@ -1178,7 +1179,7 @@ __global__ void __launch_bounds__(256) page_score_kernel(const PagedArgs p, cons
 // heads, 6.0 us on 512 threads (256: 8.9, 1024: 6.5; with block-wide sums between the steps 11.3).
 // Thread t holds keys [t K, (t + 1) K) in registers (K > 0), or reads them every round (K = 0, `k` each). FUSED (K = 1, a
 // wave for every 16 pages): the block scores the pages itself, a launch less for sequences of few pages (3 pages 4.9 us
-// against 3.5 + 4.0, 125 pages 6.6 against 4.3 + 4.7; 256 pages 9.2 against 4.0 + 4.4).
+// against 3.5 + 4.0, 125 pages 6.9 against 4.3 + 4.7; 256 pages 9.2 against 4.0 + 4.4).
 constexpr int SELECT_BINS = 512;
 template <int THREADS, int K, typename T = void>
 __global__ void __launch_bounds__(THREADS) page_select_kernel(const PagedArgs p, const uint64_t* keys, const void* bounds, int maxp, int k, int topk, int* sel) {
