@@ -591,6 +591,7 @@ template <typename T, bool SPARSE> struct PagedWave {
   const PagedArgs& p;
   const int* sel;  // [n, kv_heads, topk] (SPARSE)
   const int topk, kh, lane;
+  const bool in;  // the lane's column has a head
   const uint32_t lds;   // of the wave's ring
   const char* ring;
   Ops ops;
@@ -691,7 +692,7 @@ template <typename T, bool SPARSE> struct PagedWave {
 
   // Tiles t, t + step, ... below end: tile k is asked for while tile k - 2 is used, in one copy of either's code (a
   // launch begins with a cold instruction cache). Where a sum is NaN they are taken again without the weights' second terms:
-  // beside an infinite value these make inf - inf or 0 inf.
+  // beside an infinite value these make inf - inf or 0 inf. Columns of zeros do not count, which an infinite key makes NaN.
   __device__ inline void run(int t, int step, int end, float scale) {
     const int count = t < end ? (end - t + step - 1) / step : 0;
     bool rest = sizeof(T) == 2;
@@ -720,7 +721,7 @@ template <typename T, bool SPARSE> struct PagedWave {
       for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) nan |= o[d][r] != o[d][r];
-      if (!__any(nan)) return;
+      if (!__any(nan && in)) return;
       rest = false;
     }
   }
@@ -829,7 +830,7 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_whole_kernel(const 
   const int i = blockIdx.x, kh = int(blockIdx.y) / groups, g0 = int(blockIdx.y) % groups * 16;
   const int col = lane & 15, head = kh * G + g0 + col;
   char* ring = smem + wave * STAGES * TILE_BYTES;
-  Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
+  Wave w{p, sel, topk, kh, lane, g0 + col < G, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
   w.ops.load_q(static_cast<const T*>(p.q) + i * p.ldq + long(head) * 64, lane >> 4, g0 + col < G);
   w.begin(i);
   if (threadIdx.x < PAGED_WAVES) {
@@ -906,7 +907,7 @@ __global__ void __launch_bounds__(PAGED_WAVES * 64, 2) paged_parts_kernel(const 
   const Part part(G);
   auto place = [&](long worker, bool only) { return parts + ((worker * cols + blockIdx.y) * 2 + (only ? 0 : 1)) * part.size(); };
   char* ring = smem + wave * STAGES * TILE_BYTES;
-  Wave w{p, sel, topk, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
+  Wave w{p, sel, topk, kh, lane, g0 + col < G, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring};
   w.m = w.l = 0.f;
   w.some = 0;
 #pragma unroll

@@ -64,6 +64,33 @@ def test_weights_keep_more_than_their_type_holds(ctx, dtype, lens, heads, kv, ps
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,heads,kv,ps", [([17, 40], 2, 2, 8), ([300, 31], 6, 2, 16), ([2500, 90], 16, 1, 32)])
+def test_a_key_of_infinity_costs_the_others_no_bits(ctx, dtype, lens, heads, kv, ps):
+    """Keys whose score is -inf have weight 0; the other keys' weights keep all their bits."""
+    report("infinite.key", dtype=dtype, lens=lens, heads=heads, kv=kv)
+    c = even_cache(dtype, lens, kv, ps)
+    q = queries(c, heads)
+    x = q.view(c.n, heads, 64)
+    x[:, :, 5] = x[:, :, 5].abs() + 0.25
+    gone = {}
+    for i, n in enumerate(lens):
+        gone[i] = [n // 2, n - 1]
+        for at in gone[i]:
+            c.k[int(c.table[i, at // ps]), :kv * ps * 64].view(kv, ps, 64)[:, at % ps, 5] = -float("inf")
+    out = run_paged(ctx, c, q, heads)
+    G, worst = heads // kv, 0.0
+    for i, n in enumerate(lens):
+        at = [p for p in range(n) if p not in gone[i]]
+        for h in range(kv):
+            k, v = c.head(c.k, i, h, at), c.head(c.v, i, h, at)
+            ref, A, e = attention_ref(q[i].view(kv, G, 64)[h].double(), k, v, 0.125)
+            d = (out[i].view(kv, G, 64)[h].double() - ref).abs() / weights_tol(ref, A, e, n, 1.0, dtype)
+            worst = max(worst, float(d.max()))
+    report("infinite.key.err", of_tolerance=f"{worst:.3f}")
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lens,heads,kv", [([1, 2, 33, 300], 6, 2), ([3000], 6, 2), ([2000, 5, 1999], 32, 2)])
 def test_infinite_values(ctx, dtype, lens, heads, kv):
     """An infinite value has a weight above 0: the channel is infinite, of no number where both signs meet or a value is
