@@ -329,8 +329,8 @@ def _run_own(s):
         return {name: s[name] for name in ("table", "lens_out", "src", "dst", "rows", "used_out", "status")}
     if kind == "free":
         ctx.kernel_free_pages(c["n"], p["keep"], p["lens"], c["ps"], s["pages"], p["pool"], s["pool"].numel(), p["used"], p["table"],
-                              s["width"], p["lens_out"], p["pool_out"], p["used_out"], p["status"], p["workspace"], size)
-        return {name: s[name] for name in ("lens_out", "pool_out", "used_out", "status")}
+                              s["width"], p["lens_out"], p["used_out"], p["status"], p["workspace"], size)
+        return {name: s[name] for name in ("lens_out", "pool", "used_out", "status")}
     if kind == "compact":
         ctx.kernel_compact_pages(c["n"], p["lens"], c["ps"], s["pages"], p["pool"], s["pool"].numel(), p["used"], p["table"], s["width"],
                                  p["table_out"], p["pool_out"], p["src"], p["dst"], s["cap"], p["count"], p["status"], p["workspace"], size)
@@ -387,7 +387,7 @@ def _free_plain(s):
     rank, count = torch.cumsum(gone, 0) - 1, gone.sum()
     pool = torch.cat([s["pool"], s["pool"][:1]])
     pool[torch.where(gone, used - count + rank, size)] = torch.arange(pages, device=DEV, dtype=torch.int32)
-    return {"lens_out": s["keep"].clone(), "pool_out": pool[:size], "used_out": _i32(used - count),
+    return {"lens_out": s["keep"].clone(), "pool": pool[:size], "used_out": _i32(used - count),
             "status": torch.zeros(1, dtype=torch.int32, device=DEV)}
 
 
@@ -533,7 +533,7 @@ def _exact_pages(c, s):
         for row, v, w in zip(table, keep, lens):
             gone.update(x for x in row[-(-v // ps):-(-w // ps)] if 0 <= x < pages and x not in held)
         pool[used - len(gone):used] = sorted(gone)
-        return {"lens_out": _int(keep), "pool_out": _int(pool), "used_out": _int([used - len(gone)]), "status": _int([0])}
+        return {"lens_out": _int(keep), "pool": _int(pool), "used_out": _int([used - len(gone)]), "status": _int([0])}
     live = {x for row, v in zip(table, lens) for x in row[:-(-v // ps)] if 0 <= x < pages}
     both = sorted(live | set(pool[used:]))
     low, high = both[:len(live)], both[len(live):]
