@@ -138,12 +138,14 @@ typedef struct splat_kv_cache {
   void* v;
 } splat_kv_cache;
 
-/* Status that splat_kernel_block_tables leaves on the device. */
+/* Status that the calls on tables leave on the device. */
 typedef enum splat_table_status {
   SPLAT_TABLE_OK = 0,
-  SPLAT_TABLE_BAD_LENGTH = 1, /* a negative length, one past the table's width, or `used` outside the pool */
+  SPLAT_TABLE_BAD_LENGTH = 1, /* a negative length, one past the table's width or its row, or `used` outside the pool */
   SPLAT_TABLE_POOL_EMPTY = 2, /* the pool holds fewer pages than are needed */
-  SPLAT_TABLE_SLOTS_FULL = 3  /* more than `cap` new tokens */
+  SPLAT_TABLE_SLOTS_FULL = 3, /* more than `cap` new tokens, or moves */
+  SPLAT_TABLE_BAD_ROW = 4,    /* a fork's row that is not empty, or a parent that is no row or a fork itself */
+  SPLAT_TABLE_BAD_PAGE = 5    /* a free page that is in use, twice free or none, or more pages given back than taken */
 } splat_table_status;
 
 /* Block tables and slot maps of n requests that hold past[i] positions and get add[i] new ones. The pages that
@@ -210,6 +212,72 @@ int splat_kernel_sparse_attention(splat_ctx* ctx, const splat_kv_cache* cache, c
                                   int64_t ldq, int n, int heads, const int32_t* table, int width,
                                   const int32_t* lens, int max_len, int topk, float scale, void* out, int64_t ldo,
                                   int32_t* selected, void* workspace, size_t workspace_bytes);
+
+/* --- pages that rows share, give back, and that move ------------------------------------------------
+ * On the tables of splat_kernel_block_tables: rows of `width` entries, of which row i holds ceil(lens[i] / page_size); the
+ * free pages are pool[*used .. pool_size). One page may be in several rows. A page is in use as long as a row
+ * holds it; there are no counts to keep. The tables serve all layers of a network, whose pools splat_kernel_copy_pages
+ * takes together. n up to 65536; entries outside [0, pages) are no pages. If *status is not SPLAT_TABLE_OK nothing was done:
+ * table and pool stay, lens_out and used_out are lens and *used, src, dst -1 and *count 0. lens_out may be lens and used_out
+ * used; other outputs and workspaces overlap nothing but where a call says so. */
+
+/* Rows with a parent become forks: with parents[i] = p, the empty row i (lens[i] 0) gets the first keep[i] positions of row p
+ * (keep NULL: all lens[p]), which is no fork in the same call; parents[i] -1: row i stays. Full pages are shared; a begun one is
+ * the next of the pool instead, requests in order, for new tokens to go into, and its keys and values are to be copied: rows[i]
+ * rows of page src[i] to page dst[i] (-1, -1 and 0: none). An entry that is no page stays one. keep is not
+ * looked at where there is no parent. */
+int splat_kernel_fork_pages(splat_ctx* ctx, int n, const int32_t* parents, const int32_t* keep, const int32_t* lens,
+                            int page_size, int pages, const int32_t* pool, int pool_size, const int32_t* used,
+                            int32_t* table, int width, int32_t* lens_out, int32_t* src, int32_t* dst, int32_t* rows,
+                            int32_t* used_out, int32_t* status);
+
+/* Rows are cut to their first keep[i] of lens[i] positions (0: the row ends). Pages behind those that no row keeps and that are
+ * not free already go back into the pool, ascending, in front of the free ones: into pool[*used_out .. *used). The table stays: what
+ * it holds behind a row's pages means nothing. Every row that may hold a page has to be in the call. lens_out may also be
+ * keep. workspace: splat_pages_workspace's bytes, 16-byte aligned; one for the most pages serves every smaller call. */
+int splat_pages_workspace(int pages, size_t* bytes);
+int splat_kernel_free_pages(splat_ctx* ctx, int n, const int32_t* keep, const int32_t* lens, int page_size, int pages,
+                            int32_t* pool, int pool_size, const int32_t* used, const int32_t* table, int width,
+                            int32_t* lens_out, int32_t* used_out, int32_t* status, void* workspace,
+                            size_t workspace_bytes);
+
+/* Of the pages in rows and the free ones together, the lowest come to be in use: the k-th page in use that lies behind as many
+ * pages as are in use moves to the k-th free page before there, src[k] to dst[k], -1 behind the *count moves (`cap` places; half of
+ * `pages` is always enough). table_out (may be table) has the pages' new places, behind a row's pages what the
+ * table has; pool_out (may be pool) from *used on the pages that are free now, ascending. *used stays as it is. Every row that
+ * holds a page has to be in the call. The keys and values are to be moved by splat_kernel_copy_pages. */
+int splat_kernel_compact_pages(splat_ctx* ctx, int n, const int32_t* lens, int page_size, int pages, const int32_t* pool,
+                               int pool_size, const int32_t* used, const int32_t* table, int width, int32_t* table_out,
+                               int32_t* pool_out, int32_t* src, int32_t* dst, int cap, int32_t* count, int32_t* status,
+                               void* workspace, size_t workspace_bytes);
+
+/* In every layer's pools, the first rows[i] rows (NULL: all) of each head of page src[i] are copied to page dst[i], for i below n
+ * and *count (NULL: n). A pair with a page outside the pool (-1) is left out. No page is twice in dst, or in src and dst of different
+ * pairs. caches [layers] (up to 64) are alike but for k and v; no pool overlaps another. bounds (NULL: none): of each layer the
+ * pages' bounds (splat_kernel_page_bounds), which go along whole: wider than need be for a page that got some of the
+ * rows, until splat_kernel_page_bounds takes that page again. */
+int splat_kernel_copy_pages(splat_ctx* ctx, const splat_kv_cache* caches, int layers, void* const* bounds, int n,
+                            const int32_t* src, const int32_t* dst, const int32_t* rows, const int32_t* count);
+
+/* Attention of n tokens over positions that many of them have in common, read once for all of them. The tokens of group g are those
+ * from starts[g] up to starts[g + 1] (ascending; with those of block_tables' `starts`, the new tokens of a request);
+ * rows of out that belong to no group stay. Token i sees the positions below lens[i] (lens NULL: below shared[g]): those below
+ * shared[g] lie in row g of prefix [groups, prefix_width], the others in row i of table [n, width], at their places from 0 on
+ * (NULL: there are none), as after splat_kernel_fork_pages. So the forks of a scene attend to it with prefix its row and
+ * table theirs, and the tokens of a view to a cache, or in causal order with lens = position + 1, with prefix the request's row.
+ * out[i, h] = softmax(scale q[i, h] K^T) V over what it sees, with the keys and values of head h / (heads / kv_heads); zeros where
+ * that is nothing. max_shared and max_own: upper bounds of shared[g] and of lens[i] - shared[g] that the host knows; what is
+ * behind them is cut off. q, out, strides, and weights as in splat_kernel_paged_attention, infinities and NaN in
+ * values that a token does not see leave its row alone. workspace: splat_prefix_attention_workspace's bytes, 16-byte aligned; one for the
+ * largest n, groups, max_shared and max_own serves every smaller call. starts that descend: nothing is written. groups times
+ * kv_heads up to 2^21. */
+int splat_prefix_attention_workspace(const splat_kv_cache* cache, int n, int heads, int groups, int max_shared,
+                                     int max_own, size_t* bytes);
+int splat_kernel_prefix_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* q, int64_t ldq, int n,
+                                  int heads, const int32_t* starts, int groups, const int32_t* prefix,
+                                  int prefix_width, const int32_t* shared, int max_shared, const int32_t* table,
+                                  int width, const int32_t* lens, int max_own, float scale, void* out, int64_t ldo,
+                                  void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

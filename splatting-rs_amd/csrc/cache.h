@@ -24,7 +24,7 @@ struct KvCache {
   void* k = nullptr; void* v = nullptr;
 };
 
-enum TableStatus { TABLE_OK = 0, TABLE_BAD_LENGTH = 1, TABLE_POOL_EMPTY = 2, TABLE_SLOTS_FULL = 3 };
+enum TableStatus { TABLE_OK = 0, TABLE_BAD_LENGTH = 1, TABLE_POOL_EMPTY = 2, TABLE_SLOTS_FULL = 3, TABLE_BAD_ROW = 4, TABLE_BAD_PAGE = 5 };
 struct BlockTableArgs {
   int n = 0; const int* past = nullptr; const int* add = nullptr;
   int page_size = 0, shift = 0;
@@ -32,6 +32,39 @@ struct BlockTableArgs {
   int* table = nullptr; int width = 0;
   int* lens = nullptr; int* starts = nullptr; int* slots = nullptr; int* positions = nullptr; int cap = 0;
   int* used_out = nullptr; int* status = nullptr;
+};
+
+// Rows that become forks of others, rows that give pages back, and pages that move: tables of page_size positions an
+// entry over pages [0, pages), pool[used..pool_size) the free ones.
+struct PagesArgs {
+  int n = 0; int page_size = 0, shift = 0, pages = 0;
+  int* pool = nullptr; int pool_size = 0; const int* used = nullptr;
+  int* table = nullptr; int width = 0;
+  const int* lens = nullptr;
+  int* status = nullptr;
+};
+struct ForkArgs {
+  PagesArgs at;
+  const int* parents = nullptr; const int* keep = nullptr;
+  int* lens_out = nullptr; int* src = nullptr; int* dst = nullptr; int* rows = nullptr; int* used_out = nullptr;
+};
+struct FreeArgs {
+  PagesArgs at;
+  const int* keep = nullptr; int* lens_out = nullptr; int* used_out = nullptr;
+};
+struct CompactArgs {
+  PagesArgs at;
+  int* table_out = nullptr; int* pool_out = nullptr;
+  int* src = nullptr; int* dst = nullptr; int cap = 0; int* count = nullptr;
+};
+// Rows [0, rows[i]) of page src[i] to page dst[i] in the pools of several layers, which are alike but for k and v.
+constexpr int MOST_LAYERS = 64;
+struct CopyArgs {
+  KvCache cache;  // of every layer, without k and v
+  int layers = 0;
+  void* k[MOST_LAYERS]; void* v[MOST_LAYERS]; void* bounds[MOST_LAYERS];
+  bool has_bounds = false;
+  int n = 0; const int* src = nullptr; const int* dst = nullptr; const int* rows = nullptr; const int* count = nullptr;
 };
 
 enum Norm { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
@@ -67,6 +100,18 @@ struct SparseArgs {
   const void* bounds = nullptr; int topk = 0; int* selected = nullptr;
 };
 
+// One token each of n sequences, the tokens of group g from starts[g] to starts[g + 1]: positions below shared[g] lie in row g
+// of `prefix`, the others in row i of `table` (NULL: none).
+struct PrefixArgs {
+  KvCache cache;
+  const void* q = nullptr; long ldq = 0; int n = 0, heads = 0;
+  const int* starts = nullptr; int groups = 0;
+  const int* prefix = nullptr; int prefix_width = 0; const int* shared = nullptr; int max_shared = 0;
+  const int* table = nullptr; int width = 0; const int* lens = nullptr; int max_own = 0;
+  float scale = 1.f;
+  void* out = nullptr; long ldo = 0;
+};
+
 // Each throws Error(BAD_ARGUMENT, ...) for a call that is refused and sets what the launch derives. A call
 // without rows (n or tokens 0) passes with its row pointers NULL.
 void check_block_tables(BlockTableArgs& a);
@@ -76,6 +121,31 @@ void check_overlaps(const BoundsArgs& a);  // of outputs with index arrays and w
 void check_overlaps(const QkArgs& a);
 void check_paged_attention(PagedArgs& a, const void* workspace, size_t bytes);
 void check_sparse_attention(SparseArgs& a, const void* workspace, size_t bytes);
+void check_fork_pages(ForkArgs& a);
+void check_free_pages(FreeArgs& a, const void* workspace, size_t bytes);
+void check_compact_pages(CompactArgs& a, const void* workspace, size_t bytes);
+void check_copy_pages(CopyArgs& a);
+void check_prefix_attention(PrefixArgs& a, const void* workspace, size_t bytes);
+
+// The workspace of free_pages and compact_pages: bits of the pages in two maps, what lies before every word of 32 of them, and
+// the counts of every CHUNK words.
+constexpr int PAGE_CHUNK = 1024;
+struct PagesPlan {
+  long words = 0, chunks = 0;
+  size_t second = 0, before = 0, counts = 0, head = 0, bytes = 0;  // offsets; the first map is at 0
+};
+PagesPlan pages_plan(int pages);
+size_t pages_bytes(int pages);
+
+// How prefix attention is launched: items of `rows` (token, head) pairs of one group and key head, `blocks` blocks that take equal
+// parts of their tiles (as many as items can be: no item is cut), `own` parts of each token's own positions.
+struct PrefixPlan {
+  int rows = 0, blocks = 0, own = 0;
+  bool join = false;  // parts are left for a joining launch
+  size_t parts = 0, own_parts = 0, bytes = 0;  // offsets in the workspace, and all of it
+};
+PrefixPlan prefix_plan(const PrefixArgs& a);
+size_t prefix_attention_bytes(const KvCache& c, int n, int heads, int groups, int max_shared, int max_own);
 
 // How attention over the cache is launched: `cols` groups of up to 16 query heads of one key head, and for long
 // sequences `workers` waves for each, which leave parts to join; 0: one block a sequence and group. topk 0: all

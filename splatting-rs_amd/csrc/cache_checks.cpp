@@ -314,6 +314,225 @@ size_t sparse_attention_bytes(const KvCache& c, int n, int heads, int max_len, i
   return plan_bytes(c, n, heads, max_len, topk) + key_bytes(c, n, max_len);
 }
 
+namespace {
+
+void check_pages(int pages, int page_size) {
+  check_page_size(page_size);
+  SPLAT_CHECK(pages >= 1 && long(pages) * page_size <= 0x7fffffffL, BAD_ARGUMENT, "pages times page_size must be 1 to 2^31 - 1");
+}
+
+// What the calls on a table's pages have in common. A call without rows passes with its row pointers NULL.
+void check_table(PagesArgs& a, const char* what) {
+  const std::string name = what;
+  check_pages(a.pages, a.page_size);
+  check_width(a.width, a.page_size);
+  SPLAT_CHECK(a.n >= 0 && a.n <= 65536, BAD_ARGUMENT, name + ": n must be 0 to 65536");
+  SPLAT_CHECK(a.pool_size >= 0, BAD_ARGUMENT, name + ": pool_size is negative");
+  SPLAT_CHECK(a.used && a.status && (a.n == 0 || (a.lens && a.table)) && (a.pool_size == 0 || a.pool), BAD_ARGUMENT,
+              name + ": a required pointer is NULL");
+  SPLAT_CHECK(aligned4({a.pool, a.used, a.table, a.lens, a.status}), BAD_ARGUMENT, name + ": every array must be 4-byte aligned");
+  a.shift = __builtin_ctz(a.page_size);
+}
+
+// Outputs that lie over no input and no other output; `same` names the pairs that may be one array.
+struct Output { Range at; const void* same; const void* too; };
+void check_apart(const char* what, std::initializer_list<Range> in, std::initializer_list<Output> out) {
+  const std::string name = what;
+  for (auto o = out.begin(); o != out.end(); ++o) {
+    for (const Range& i : in)
+      SPLAT_CHECK((i.at == o->at.at && (i.at == o->same || i.at == o->too)) || !meet(o->at, i), BAD_ARGUMENT, name + ": an output overlaps an input");
+    for (auto other = out.begin(); other != o; ++other)
+      SPLAT_CHECK(!meet(o->at, other->at), BAD_ARGUMENT, name + ": two outputs overlap");
+  }
+}
+
+void check_map(const PagesArgs& a, const void* workspace, size_t bytes, const char* what) {
+  const size_t need = pages_plan(a.pages).bytes;
+  SPLAT_CHECK(workspace && aligned16(workspace) && bytes >= need, BAD_ARGUMENT,
+              std::string(what) + ": the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+}
+
+}  // namespace
+
+void check_fork_pages(ForkArgs& a) {
+  PagesArgs& p = a.at;
+  check_table(p, "fork pages");
+  SPLAT_CHECK(a.used_out && (p.n == 0 || (a.parents && a.lens_out && a.src && a.dst && a.rows)), BAD_ARGUMENT,
+              "fork pages: a required pointer is NULL");
+  SPLAT_CHECK(aligned4({a.parents, a.keep, a.lens_out, a.src, a.dst, a.rows, a.used_out}), BAD_ARGUMENT,
+              "fork pages: every array must be 4-byte aligned");
+  const long n = 4L * p.n;
+  check_apart("fork pages", {{a.parents, n}, {a.keep, a.keep ? n : 0}, {p.lens, n}, {p.pool, 4L * p.pool_size}, {p.used, 4}},
+              {{{a.lens_out, n}, p.lens, nullptr}, {{a.used_out, 4}, p.used, nullptr}, {{p.table, n * p.width}, nullptr, nullptr}, {{a.src, n}, nullptr, nullptr},
+               {{a.dst, n}, nullptr, nullptr}, {{a.rows, n}, nullptr, nullptr}, {{p.status, 4}, nullptr, nullptr}});
+}
+
+void check_free_pages(FreeArgs& a, const void* workspace, size_t bytes) {
+  PagesArgs& p = a.at;
+  check_table(p, "free pages");
+  SPLAT_CHECK(a.used_out && (p.n == 0 || (a.keep && a.lens_out)), BAD_ARGUMENT, "free pages: a required pointer is NULL");
+  SPLAT_CHECK(aligned4({a.keep, a.lens_out, a.used_out}), BAD_ARGUMENT, "free pages: every array must be 4-byte aligned");
+  check_map(p, workspace, bytes, "free pages");
+  const long n = 4L * p.n;
+  check_apart("free pages", {{a.keep, n}, {p.lens, n}, {p.table, n * p.width}, {p.used, 4}},
+              {{{a.lens_out, n}, p.lens, a.keep}, {{a.used_out, 4}, p.used, nullptr}, {{p.pool, 4L * p.pool_size}, nullptr, nullptr},
+               {{p.status, 4}, nullptr, nullptr}, {{workspace, long(pages_plan(p.pages).bytes)}, nullptr, nullptr}});
+}
+
+void check_compact_pages(CompactArgs& a, const void* workspace, size_t bytes) {
+  PagesArgs& p = a.at;
+  check_table(p, "compact pages");
+  SPLAT_CHECK(a.cap >= 0, BAD_ARGUMENT, "compact pages: cap is negative");
+  SPLAT_CHECK(a.count && (p.n == 0 || a.table_out) && (p.pool_size == 0 || a.pool_out) && (a.cap == 0 || (a.src && a.dst)), BAD_ARGUMENT,
+              "compact pages: a required pointer is NULL");
+  SPLAT_CHECK(aligned4({a.table_out, a.pool_out, a.src, a.dst, a.count}), BAD_ARGUMENT, "compact pages: every array must be 4-byte aligned");
+  check_map(p, workspace, bytes, "compact pages");
+  const long n = 4L * p.n, cap = 4L * a.cap, pool = 4L * p.pool_size;
+  check_apart("compact pages", {{p.lens, n}, {p.table, n * p.width}, {p.pool, pool}, {p.used, 4}},
+              {{{a.table_out, n * p.width}, p.table, nullptr}, {{a.pool_out, pool}, p.pool, nullptr}, {{a.src, cap}, nullptr, nullptr},
+               {{a.dst, cap}, nullptr, nullptr}, {{a.count, 4}, nullptr, nullptr}, {{p.status, 4}, nullptr, nullptr},
+               {{workspace, long(pages_plan(p.pages).bytes)}, nullptr, nullptr}});
+}
+
+void check_copy_pages(CopyArgs& a) {
+  SPLAT_CHECK(a.layers >= 0 && a.layers <= MOST_LAYERS && a.n >= 0, BAD_ARGUMENT, "copy pages: layers must be 0 to 64, n not negative");
+  if (a.layers == 0) return;
+  for (int i = 0; i < a.layers; ++i) {
+    a.cache.k = a.k[i];
+    a.cache.v = a.v[i];
+    check_cache(a.cache);
+    SPLAT_CHECK(!a.has_bounds || (a.bounds[i] && aligned16(a.bounds[i])), BAD_ARGUMENT, "copy pages: bounds are NULL or not 16-byte aligned");
+  }
+  if (a.n == 0) return;
+  SPLAT_CHECK(a.src && a.dst, BAD_ARGUMENT, "copy pages: a required pointer is NULL");
+  SPLAT_CHECK(aligned4({a.src, a.dst, a.rows, a.count}), BAD_ARGUMENT, "copy pages: every array must be 4-byte aligned");
+  // the kernel divides numbers of pieces of 16 KB as 64-bit floats
+  const long es = type_size(a.cache.dt), page = long(a.cache.kv_heads) * a.cache.page_size * 64 * es, arrays = a.layers * (a.has_bounds ? 3L : 2L);
+  SPLAT_CHECK(long(a.n) * arrays * ((page + 16383) / 16384) < (1L << 50), BAD_ARGUMENT, "copy pages: more than 2^50 pieces");
+  const long stride = a.cache.page_stride * es;
+  const Range in[] = {{a.src, 4L * a.n}, {a.dst, 4L * a.n}, {a.rows, a.rows ? 4L * a.n : 0}, {a.count, a.count ? 4 : 0}};
+  auto rows = [&](int k) {  // of array k: the layers' keys, values and bounds
+    const int i = k % a.layers;
+    if (k >= 2 * a.layers) return Rows{a.bounds[i], bounds_bytes(a.cache), bounds_bytes(a.cache), 1};
+    return Rows{k < a.layers ? a.k[i] : a.v[i], stride, page, a.cache.pages};
+  };
+  for (int k = 0; k < arrays; ++k) {
+    const Rows x = rows(k);
+    for (const Range& i : in) SPLAT_CHECK(!row_meets(x, i), BAD_ARGUMENT, "copy pages: a pool overlaps the lists of pages");
+    for (int other = 0; other < k; ++other) {
+      const Rows y = rows(other);
+      const bool same = x.count == y.count && x.stride == y.stride;
+      SPLAT_CHECK(!(same ? rows_meet(x.at, x.stride, x.width, y.at, y.stride, y.width, x.count)
+                         : x.count == 1 ? row_meets(y, {x.at, x.width}) : row_meets(x, {y.at, y.width})),
+                  BAD_ARGUMENT, "copy pages: two pools overlap");
+    }
+  }
+}
+
+PagesPlan pages_plan(int pages) {
+  PagesPlan plan;
+  plan.words = (long(pages) + 31) / 32;
+  plan.chunks = (plan.words + PAGE_CHUNK - 1) / PAGE_CHUNK;
+  const size_t map = size_t(plan.words + 3) / 4 * 16;
+  plan.second = map;
+  plan.before = 2 * map;
+  plan.counts = 3 * map;
+  plan.head = plan.counts + size_t(plan.chunks + 1) / 2 * 16;
+  plan.bytes = plan.head + 32;
+  return plan;
+}
+
+size_t pages_bytes(int pages) {
+  SPLAT_CHECK(pages >= 1 && pages <= (1 << 28), BAD_ARGUMENT, "workspace: pages must be 1 to 2^28");
+  return pages_plan(pages).bytes;
+}
+
+void check_prefix_attention(PrefixArgs& a, const void* workspace, size_t bytes) {
+  check_cache(a.cache);
+  SPLAT_CHECK(a.n >= 0 && a.heads >= 1 && a.heads <= 32768 && a.heads % a.cache.kv_heads == 0, BAD_ARGUMENT,
+              "prefix attention: heads must be a multiple of the cache's kv_heads");
+  SPLAT_CHECK(long(a.n) * a.heads <= MOST_ROWS, BAD_ARGUMENT, "prefix attention: more than 2^21 query rows");
+  SPLAT_CHECK(a.groups >= 0 && a.groups <= 65536 && long(a.groups) * a.cache.kv_heads <= MOST_ROWS, BAD_ARGUMENT,
+              "prefix attention: groups must be 0 to 65536, and at most 2^21 with the key heads");
+  check_width(a.prefix_width, a.cache.page_size);
+  SPLAT_CHECK(a.max_shared >= 0 && a.max_own >= 0, BAD_ARGUMENT, "prefix attention: max_shared or max_own is negative");
+  SPLAT_CHECK(std::isfinite(a.scale * 1.5f), BAD_ARGUMENT, "prefix attention: scale is not finite, or too large");
+  if (a.table) check_width(a.width, a.cache.page_size);
+  SPLAT_CHECK(!a.table || a.lens, BAD_ARGUMENT, "prefix attention: a table needs lens");
+  if (a.n == 0 || a.groups == 0) return;
+  SPLAT_CHECK(a.q && a.out && a.starts && a.prefix && a.shared, BAD_ARGUMENT, "prefix attention: a required pointer is NULL");
+  const long es = type_size(a.cache.dt), w = a.heads * 64L;
+  SPLAT_CHECK(aligned16(a.q) && aligned16(a.out) && a.ldq % 8 == 0 && a.ldo % 8 == 0 && a.ldq >= w && a.ldo >= w && a.ldq <= MOST_STRIDE &&
+                  a.ldo <= MOST_STRIDE,
+              BAD_ARGUMENT, "prefix attention: rows of q and out must be 16-byte aligned, heads * 64 wide and a multiple of 8 elements (at most 2^31) apart");
+  SPLAT_CHECK(!rows_meet(a.q, a.ldq * es, w * es, a.out, a.ldo * es, w * es, a.n), BAD_ARGUMENT, "prefix attention: out overlaps q");
+  SPLAT_CHECK(aligned4({a.starts, a.prefix, a.shared, a.table, a.lens}), BAD_ARGUMENT, "prefix attention: index arrays must be 4-byte aligned");
+  const Range in[] = {{a.starts, 4L * (a.groups + 1L)}, {a.prefix, 4L * a.groups * a.prefix_width}, {a.shared, 4L * a.groups},
+                      {a.table, a.table ? 4L * a.n * a.width : 0}, {a.lens, a.lens ? 4L * a.n : 0}};
+  const Rows out = {a.out, a.ldo * es, w * es, a.n};
+  const Range all = {a.out, ((a.n - 1L) * a.ldo + w) * es};
+  SPLAT_CHECK(!meets_pools(a.cache, all.at, all.bytes), BAD_ARGUMENT, "prefix attention: out overlaps the cache");
+  for (const Range& i : in) SPLAT_CHECK(!row_meets(out, i), BAD_ARGUMENT, "prefix attention: out overlaps an index array");
+  const size_t need = prefix_attention_bytes(a.cache, a.n, a.heads, a.groups, a.max_shared, a.table ? a.max_own : 0);
+  SPLAT_CHECK(need == 0 || (workspace && aligned16(workspace) && bytes >= need), BAD_ARGUMENT,
+              "prefix attention: the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+  const Range ws = {workspace, long(need)};
+  SPLAT_CHECK(need == 0 || (!meets_pools(a.cache, ws.at, ws.bytes) && !meet(ws, {a.q, ((a.n - 1L) * a.ldq + w) * es}) && !meet(ws, all)), BAD_ARGUMENT,
+              "prefix attention: the workspace overlaps another argument");
+  for (const Range& i : in) SPLAT_CHECK(!meet(ws, i), BAD_ARGUMENT, "prefix attention: the workspace overlaps another argument");
+  a.max_shared = int(std::min<long>(a.max_shared, long(a.prefix_width) * a.cache.page_size));
+  if (a.table) a.max_own = int(std::min<long>(a.max_own, long(a.width) * a.cache.page_size));
+  else a.max_own = a.width = 0;
+}
+
+namespace {
+constexpr int WIDE_ROWS = 256;    // the most of an item
+constexpr int MORE_BLOCKS = 512;  // that cut items' tiles: two on each of 256 CUs
+constexpr long OWN_BLOCKS = 1024; // of the tokens' own positions, up to which these are cut
+
+// Items of one key head, at most: every group's rows are cut into items of their own.
+long most_items(long n, int G, int groups, int rows) { return n * G / rows + std::min<long>(groups, n); }
+// Parts that a token's own positions are cut into: of 16 tiles at least.
+int own_parts(long n, long cols, int max_own, int keys) {
+  const long tiles = (max_own + keys - 1) / keys + 1;
+  return max_own == 0 ? 0 : int(std::max<long>(1, std::min<long>(tiles / 16, OWN_BLOCKS / std::max<long>(1, n * cols))));
+}
+}  // namespace
+
+PrefixPlan prefix_plan(const PrefixArgs& a) {
+  PrefixPlan plan;
+  const KvCache& c = a.cache;
+  const int G = a.heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;
+  plan.rows = 16;
+  const long items = most_items(a.n, G, a.groups, plan.rows) * c.kv_heads, tiles = (a.max_shared + keys - 1) / keys;
+  // no more blocks than give each 8 tiles, two a wave
+  const long more = items >= MORE_BLOCKS ? 0 : std::min<long>(MORE_BLOCKS, items * (tiles / 8));
+  plan.blocks = int(items + more);
+  plan.own = own_parts(a.n, long(c.kv_heads) * ((G + 15) / 16), a.max_own, keys);
+  plan.join = more > 0 || plan.own > 0;
+  if (!plan.join) return plan;
+  plan.parts = (16 + a.groups * 16L);
+  plan.own_parts = plan.parts + size_t(plan.blocks) * plan.rows * PART_HEAD * 4;
+  plan.bytes = plan.own_parts + size_t(a.n) * a.heads * plan.own * PART_HEAD * 4;
+  return plan;
+}
+
+// An upper bound for every plan of these sizes or smaller ones, whichever rows an item has.
+size_t prefix_attention_bytes(const KvCache& c, int n, int heads, int groups, int max_shared, int max_own) {
+  check_sizes(c);
+  SPLAT_CHECK(n >= 0 && groups >= 0 && groups <= 65536 && max_shared >= 0 && max_own >= 0 && heads >= 1 && heads <= 32768 && heads % c.kv_heads == 0 &&
+                  long(n) * heads <= MOST_ROWS && long(groups) * c.kv_heads <= MOST_ROWS,
+              BAD_ARGUMENT, "workspace: n, heads, groups, max_shared or max_own");
+  if (n == 0 || groups == 0) return 0;
+  const int G = heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;
+  const size_t item = long(n) * heads + std::min<long>(groups, n) * c.kv_heads * WIDE_ROWS;
+  const size_t cut = std::min<size_t>(size_t(MORE_BLOCKS) * WIDE_ROWS, item * ((max_shared + keys - 1L) / keys));
+  // own parts: one a token and column group, or as many as there are blocks for
+  const size_t cols = size_t(c.kv_heads) * ((G + 15) / 16);
+  const size_t own = max_own == 0 ? 0 : std::max<size_t>(size_t(n) * heads, size_t(OWN_BLOCKS) / cols * heads);
+  return 16 + groups * 16L + (item + cut + own) * PART_HEAD * 4;
+}
+
 void rope_turns(int rope, double base, double (&freq)[32]) {
   // products of powers of two of the step: at most five roundings each
   const int h = rope == ROPE_LINE ? 32 : 16;

@@ -181,6 +181,21 @@ PagedArgs paged_args(const splat_kv_cache* cache, const void* q, int64_t ldq, in
   a.ldo = ldo;
   return a;
 }
+PagesArgs pages_args(int n, const int32_t* lens, int page_size, int pages, const int32_t* pool, int pool_size, const int32_t* used,
+                     const int32_t* table, int width, int32_t* status) {
+  PagesArgs a;
+  a.n = n;
+  a.lens = lens;
+  a.page_size = page_size;
+  a.pages = pages;
+  a.pool = const_cast<int32_t*>(pool);
+  a.pool_size = pool_size;
+  a.used = used;
+  a.table = const_cast<int32_t*>(table);
+  a.width = width;
+  a.status = status;
+  return a;
+}
 template <typename T>
 void d2h(Context* ctx, T* host, const void* dev, size_t count) {
   if (host) SPLAT_HIP(hipMemcpyAsync(host, dev, count * sizeof(T), hipMemcpyDeviceToHost, ctx->stream));
@@ -609,6 +624,126 @@ int splat_kernel_sparse_attention(splat_ctx* ctx, const splat_kv_cache* cache, c
     a.topk = topk;
     a.selected = selected;
     sparse_attention(C(ctx)->ex, a, workspace, workspace_bytes);
+  });
+}
+
+int splat_pages_workspace(int pages, size_t* bytes) {
+  return guard_free([&] {
+    SPLAT_CHECK(bytes != nullptr, BAD_ARGUMENT, "bytes is NULL");
+    *bytes = pages_bytes(pages);
+  });
+}
+
+int splat_kernel_fork_pages(splat_ctx* ctx, int n, const int32_t* parents, const int32_t* keep, const int32_t* lens,
+                            int page_size, int pages, const int32_t* pool, int pool_size, const int32_t* used,
+                            int32_t* table, int width, int32_t* lens_out, int32_t* src, int32_t* dst, int32_t* rows,
+                            int32_t* used_out, int32_t* status) {
+  return guard(C(ctx), [&] {
+    ForkArgs a;
+    a.at = pages_args(n, lens, page_size, pages, pool, pool_size, used, table, width, status);
+    a.parents = parents;
+    a.keep = keep;
+    a.lens_out = lens_out;
+    a.src = src;
+    a.dst = dst;
+    a.rows = rows;
+    a.used_out = used_out;
+    fork_pages(C(ctx)->ex, a);
+  });
+}
+
+int splat_kernel_free_pages(splat_ctx* ctx, int n, const int32_t* keep, const int32_t* lens, int page_size, int pages,
+                            int32_t* pool, int pool_size, const int32_t* used, const int32_t* table, int width,
+                            int32_t* lens_out, int32_t* used_out, int32_t* status, void* workspace,
+                            size_t workspace_bytes) {
+  return guard(C(ctx), [&] {
+    FreeArgs a;
+    a.at = pages_args(n, lens, page_size, pages, pool, pool_size, used, table, width, status);
+    a.keep = keep;
+    a.lens_out = lens_out;
+    a.used_out = used_out;
+    free_pages(C(ctx)->ex, a, workspace, workspace_bytes);
+  });
+}
+
+int splat_kernel_compact_pages(splat_ctx* ctx, int n, const int32_t* lens, int page_size, int pages, const int32_t* pool,
+                               int pool_size, const int32_t* used, const int32_t* table, int width, int32_t* table_out,
+                               int32_t* pool_out, int32_t* src, int32_t* dst, int cap, int32_t* count, int32_t* status,
+                               void* workspace, size_t workspace_bytes) {
+  return guard(C(ctx), [&] {
+    CompactArgs a;
+    a.at = pages_args(n, lens, page_size, pages, pool, pool_size, used, table, width, status);
+    a.table_out = table_out;
+    a.pool_out = pool_out;
+    a.src = src;
+    a.dst = dst;
+    a.cap = cap;
+    a.count = count;
+    compact_pages(C(ctx)->ex, a, workspace, workspace_bytes);
+  });
+}
+
+int splat_kernel_copy_pages(splat_ctx* ctx, const splat_kv_cache* caches, int layers, void* const* bounds, int n,
+                            const int32_t* src, const int32_t* dst, const int32_t* rows, const int32_t* count) {
+  return guard(C(ctx), [&] {
+    SPLAT_CHECK(layers >= 0 && layers <= MOST_LAYERS, BAD_ARGUMENT, "copy pages: layers must be 0 to 64");
+    SPLAT_CHECK(layers == 0 || caches, BAD_ARGUMENT, "cache is NULL");
+    CopyArgs a;
+    a.layers = layers;
+    a.has_bounds = bounds != nullptr;
+    for (int i = 0; i < layers; ++i) {
+      const KvCache c = kv_cache(caches + i);
+      if (i == 0) a.cache = c;
+      SPLAT_CHECK(c.dt == a.cache.dt && c.pages == a.cache.pages && c.page_size == a.cache.page_size &&
+                      c.kv_heads == a.cache.kv_heads && c.page_stride == a.cache.page_stride,
+                  BAD_ARGUMENT, "copy pages: the layers' caches differ in more than k and v");
+      a.k[i] = c.k;
+      a.v[i] = c.v;
+      a.bounds[i] = bounds ? bounds[i] : nullptr;
+    }
+    a.n = n;
+    a.src = src;
+    a.dst = dst;
+    a.rows = rows;
+    a.count = count;
+    copy_pages(C(ctx)->ex, a);
+  });
+}
+
+int splat_prefix_attention_workspace(const splat_kv_cache* cache, int n, int heads, int groups, int max_shared,
+                                     int max_own, size_t* bytes) {
+  return guard_free([&] {
+    SPLAT_CHECK(bytes != nullptr, BAD_ARGUMENT, "bytes is NULL");
+    *bytes = prefix_attention_bytes(kv_cache(cache), n, heads, groups, max_shared, max_own);
+  });
+}
+
+int splat_kernel_prefix_attention(splat_ctx* ctx, const splat_kv_cache* cache, const void* q, int64_t ldq, int n,
+                                  int heads, const int32_t* starts, int groups, const int32_t* prefix,
+                                  int prefix_width, const int32_t* shared, int max_shared, const int32_t* table,
+                                  int width, const int32_t* lens, int max_own, float scale, void* out, int64_t ldo,
+                                  void* workspace, size_t workspace_bytes) {
+  return guard(C(ctx), [&] {
+    PrefixArgs a;
+    a.cache = kv_cache(cache);
+    a.q = q;
+    a.ldq = ldq;
+    a.n = n;
+    a.heads = heads;
+    a.starts = starts;
+    a.groups = groups;
+    a.prefix = prefix;
+    a.prefix_width = prefix_width;
+    a.shared = shared;
+    a.max_shared = max_shared;
+    a.table = table;
+    a.width = width;
+    a.lens = lens;
+    a.max_own = max_own;
+    a.scale = scale;
+    a.out = out;
+    a.ldo = ldo;
+    prefix_attention(C(ctx)->ex, a, workspace, workspace_bytes);
   });
 }
 

@@ -237,5 +237,12 @@ void qk_norm_rope(const Exec& ex, const QkArgs& a, double base);
 void page_bounds(const Exec& ex, const BoundsArgs& a);
 void paged_attention(const Exec& ex, const PagedArgs& a, void* workspace, size_t bytes);
 void sparse_attention(const Exec& ex, const SparseArgs& a, void* workspace, size_t bytes);
+// pages.hip
+void fork_pages(const Exec& ex, const ForkArgs& a);
+void free_pages(const Exec& ex, const FreeArgs& a, void* workspace, size_t bytes);
+void compact_pages(const Exec& ex, const CompactArgs& a, void* workspace, size_t bytes);
+void copy_pages(const Exec& ex, const CopyArgs& a);
+// prefix.hip
+void prefix_attention(const Exec& ex, const PrefixArgs& a, void* workspace, size_t bytes);
 
 }  // namespace splat

@@ -1,0 +1,554 @@
+// What happens to the pages of a cache: rows that become forks of others and share their pages, pages given back that no row
+// holds any more, pages moved so that those in use come first, and the copies that forks and moves ask for.
+//
+// Which pages are in use follows from the tables alone: no counts of holders are kept that a call could miss. Maps of one
+// bit a page are filled from the rows and read in the order of the pages, so that what is given back, and what moves where,
+// does not hang on the order in which threads come. Entries outside [0, pages) are no pages.
+#include "paged.h"
+
+namespace splat {
+
+namespace {
+
+// The sums before thread tid and over all of the block's; `sums` has room for a value a wave.
+template <int THREADS> __device__ inline uint64_t scan_block(uint64_t v, uint64_t* sums, uint64_t& total) {
+  const auto plus = [](uint64_t a, uint64_t b) { return a + b; };
+  const uint64_t s = scan_wave(v, uint64_t(0), plus);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();  // the sums of the call before are read
+  if (lane == 63) sums[wave] = s;
+  __syncthreads();
+  uint64_t before = s - v;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  return before;
+}
+
+__device__ inline int places_of(int len, int shift) { return int((long(len) + (1 << shift) - 1) >> shift); }
+
+// --- forks --------------------------------------------------------------------------------------
+
+// Every block looks the rows over and sums up the pages that begun pages need (a thread its k rows), so that the call takes
+// effect whole or not at all without a launch before; then row blockIdx.x, ... takes its parent's full pages, and block 0
+// writes what there is one of for a row. FILL and COMMIT as in block_tables_kernel: two launches where lens_out lies over lens
+// or used_out over used and there are several blocks.
+// Bound by its chain of loads (parents, lengths, entries, the pool).
+template <int THREADS, bool FILL, bool COMMIT>
+__global__ void __launch_bounds__(THREADS) fork_pages_kernel(const ForkArgs a) {
+  __shared__ uint64_t sums[THREADS / 64];
+  const PagesArgs& p = a.at;
+  const int tid = threadIdx.x, k = (p.n + THREADS - 1) / THREADS, ps = 1 << p.shift;
+  const int i0 = int(min(long(tid) * k, long(p.n))), i1 = int(min(long(i0) + k, long(p.n)));
+  const long most = long(p.width) << p.shift;
+  const int used = *p.used;
+  bool bad = used < 0 || used > p.pool_size, no_row = false;
+  int need = 0;
+  // the entry of the page that the fork begins with a copy, -1: none
+  auto begun = [&](int from, int len) { return len & (ps - 1) ? p.table[long(from) * p.width + (len >> p.shift)] : -1; };
+  for (int i = i0; i < i1; ++i) {
+    const int from = a.parents[i];
+    if (from == -1) continue;
+    if (from < 0 || from >= p.n || a.parents[from] != -1 || p.lens[i] != 0) {
+      no_row = true;
+      continue;
+    }
+    const int have = p.lens[from], len = a.keep ? a.keep[i] : have;
+    if (have < 0 || have > most || len < 0 || len > have) bad = true;
+    else need += page_ok(begun(from, len), p.pages);
+  }
+  uint64_t total;
+  long rank = long(scan_block<THREADS>(uint64_t(need), sums, total));
+  const bool broken = __syncthreads_or(bad), stray = __syncthreads_or(no_row);
+  const int status = broken ? TABLE_BAD_LENGTH : stray ? TABLE_BAD_ROW : long(total) > long(p.pool_size) - used ? TABLE_POOL_EMPTY : TABLE_OK;
+  if constexpr (FILL) {
+    if (status == TABLE_OK)
+      for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
+        const int from = a.parents[i];
+        if (from == -1) continue;
+        const int full = (a.keep ? a.keep[i] : p.lens[from]) >> p.shift, step = int(gridDim.y) * THREADS;
+        const int* old = p.table + long(from) * p.width;
+        int* row = p.table + long(i) * p.width;
+        for (long j0 = long(blockIdx.y) * THREADS + tid; j0 < full; j0 += 4L * step) {
+          int page[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (j0 + long(u) * step < full) page[u] = old[j0 + long(u) * step];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (j0 + long(u) * step < full) row[j0 + long(u) * step] = page[u];
+        }
+      }
+  }
+  if constexpr (COMMIT) {
+    if (blockIdx.x || blockIdx.y) return;
+    for (int i = i0; i < i1; ++i) {
+      const int from = status == TABLE_OK ? a.parents[i] : -1;
+      int len = p.lens[i], src = -1, dst = -1, rows = 0;
+      if (from != -1) {
+        len = a.keep ? a.keep[i] : p.lens[from];
+        const int page = begun(from, len);
+        if (page_ok(page, p.pages)) {
+          src = page;
+          dst = p.pool[used + rank++];
+          rows = len & (ps - 1);
+        }
+        if (len & (ps - 1)) p.table[long(i) * p.width + (len >> p.shift)] = rows ? dst : page;
+      }
+      a.lens_out[i] = len;
+      a.src[i] = src;
+      a.dst[i] = dst;
+      a.rows[i] = rows;
+    }
+    if (tid == 0) {
+      *a.used_out = status == TABLE_OK ? used + int(total) : used;
+      *p.status = status;
+    }
+  }
+}
+
+// --- maps of pages ------------------------------------------------------------------------------
+
+constexpr int MAP_THREADS = PAGE_CHUNK;  // a word of a map a thread
+constexpr int UNIT = 256;                // places of a row that a wave takes at once
+struct MapHead {  // in the workspace, one for the launches of a call
+  int used, bad;  // bad: bit 0 a length, bit 1 a page
+  int kept, moved, status;  // of compact_pages: live pages that stay, and those that move
+};
+
+// Most pages are in many rows: the bit is looked at before it is set, which two waves in three find done.
+__device__ inline uint32_t set_bit(uint32_t* map, int page) {
+  const uint32_t bit = 1u << (page & 31);
+  uint32_t* at = map + (page >> 5);
+  if (__hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit) return bit;
+  return __hip_atomic_fetch_or(at, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit;
+}
+
+// Bits of the pages in the rows, by waves wave, wave + waves, ...: those of the first keep[i] positions in `held`, the others
+// up to lens[i] in `gone` (keep NULL: all of them are held). True where a length is none.
+__device__ inline bool mark_rows(const PagesArgs& p, const int* keep, uint32_t* held, uint32_t* gone, long wave, long waves) {
+  const int lane = threadIdx.x & 63, segs = (p.width + UNIT - 1) / UNIT;
+  bool bad = false;
+  for (long u = wave; u < long(p.n) * segs; u += waves) {
+    const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * UNIT;
+    const int len = p.lens[i], stays = keep ? keep[i] : len;
+    if (len < 0 || len > (long(p.width) << p.shift) || stays < 0 || stays > len) {
+      bad = true;
+      continue;
+    }
+    const int all = places_of(len, p.shift), kept = places_of(stays, p.shift);
+    if (j0 >= all) continue;
+    const int* row = p.table + long(i) * p.width;
+    int page[UNIT / 64];
+#pragma unroll
+    for (int k = 0; k < UNIT / 64; ++k) page[k] = row[min(j0 + 64 * k + lane, all - 1)];
+#pragma unroll
+    for (int k = 0; k < UNIT / 64; ++k) {
+      const int j = j0 + 64 * k + lane;
+      if (j < all && page_ok(page[k], p.pages)) set_bit(j < kept ? held : gone, page[k]);
+    }
+  }
+  return bad;
+}
+
+// Bits of the free pages; true where one is there twice, or is none.
+__device__ inline bool mark_pool(const PagesArgs& p, int used, uint32_t* map, long thread, long threads) {
+  bool bad = false;
+  for (long k = used + thread; k < p.pool_size; k += threads) {
+    const int page = p.pool[k];
+    bad |= !page_ok(page, p.pages) || set_bit(map, page);
+  }
+  return bad;
+}
+
+__global__ void __launch_bounds__(256) pages_clear_kernel(uint32_t* maps, long words, MapHead* head, const int* used) {
+  const long t = long(blockIdx.x) * 256 + threadIdx.x;
+  for (long w = t; w < words; w += long(gridDim.x) * 256) maps[w] = 0;
+  if (t == 0) *head = {*used, 0, 0, 0, 0};
+}
+
+// The first map from kept places (and free pages), the second from those given back; compact: live pages, then free ones.
+template <bool COMPACT>
+__global__ void __launch_bounds__(256) pages_mark_kernel(const PagesArgs p, const int* keep, uint32_t* first, uint32_t* second, MapHead* head) {
+  const long t = long(blockIdx.x) * 256 + threadIdx.x, all = long(gridDim.x) * 256;
+  const int used = head->used;
+  int bad = 0;
+  if (used < 0 || used > p.pool_size) bad = 1;
+  else if (mark_pool(p, used, COMPACT ? second : first, t, all) && COMPACT) bad |= 2;
+  if (mark_rows(p, keep, first, second, t >> 6, all >> 6)) bad |= 1;
+  if (bad) atomicOr(&head->bad, bad);
+}
+
+// Pages of a word that are given back; live and free pages (low and high half). A page that is both is bad.
+template <bool COMPACT> __device__ inline uint64_t count_word(uint32_t first, uint32_t second, bool& bad) {
+  if (!COMPACT) return __popc(second & ~first);
+  bad |= (first & second) != 0;
+  return uint64_t(__popc(second)) << 32 | uint64_t(__popc(first));
+}
+
+template <bool COMPACT>
+__global__ void __launch_bounds__(MAP_THREADS) pages_count_kernel(const uint32_t* first, const uint32_t* second, long words, uint64_t* counts, MapHead* head) {
+  __shared__ uint64_t sums[MAP_THREADS / 64];
+  const long w = long(blockIdx.x) * PAGE_CHUNK + threadIdx.x;
+  bool bad = false;
+  const uint64_t v = w < words ? count_word<COMPACT>(first[w], second[w], bad) : 0;
+  uint64_t total;
+  scan_block<MAP_THREADS>(v, sums, total);
+  if (threadIdx.x == 0) counts[blockIdx.x] = total;
+  if (bad) atomicOr(&head->bad, 2);
+}
+
+// The sums of counts before chunk `chunk` and of all of them.
+__device__ inline uint64_t sum_counts(const uint64_t* counts, long chunks, long chunk, uint64_t* sums, uint64_t& total) {
+  uint64_t before = 0, all = 0, b, t;
+  for (long c = threadIdx.x; c < chunks; c += MAP_THREADS) {
+    all += counts[c];
+    if (c < chunk) before += counts[c];
+  }
+  scan_block<MAP_THREADS>(before, sums, b);
+  scan_block<MAP_THREADS>(all, sums, t);
+  total = t;
+  return b;
+}
+
+// A chunk's pages that are given back, in their order, into the pool in front of the free ones.
+__device__ inline void write_freed(const FreeArgs& a, uint32_t bits, long word, uint64_t rank, uint64_t total, int used, int bad, long thread, long threads) {
+  const PagesArgs& p = a.at;
+  const int status = bad & 1 ? TABLE_BAD_LENGTH : long(total) > used ? TABLE_BAD_PAGE : TABLE_OK;
+  if (status == TABLE_OK)
+    for (long at = used - long(total) + long(rank); bits; bits &= bits - 1, ++at) p.pool[at] = int(word * 32) + __builtin_ctz(bits);
+  for (long i = thread; i < p.n; i += threads) a.lens_out[i] = status == TABLE_OK ? a.keep[i] : p.lens[i];
+  if (thread == 0) {
+    *a.used_out = status == TABLE_OK ? used - int(total) : used;
+    *p.status = status;
+  }
+}
+
+__global__ void __launch_bounds__(MAP_THREADS) pages_free_kernel(const FreeArgs a, const uint32_t* held, const uint32_t* gone, long words, const uint64_t* counts,
+                                                                 const MapHead* head) {
+  __shared__ uint64_t sums[MAP_THREADS / 64];
+  const long w = long(blockIdx.x) * PAGE_CHUNK + threadIdx.x;
+  const uint32_t bits = w < words ? gone[w] & ~held[w] : 0;
+  uint64_t total;
+  uint64_t rank = scan_block<MAP_THREADS>(__popc(bits), sums, total);
+  if (gridDim.x > 1) rank += sum_counts(counts, gridDim.x, blockIdx.x, sums, total);
+  write_freed(a, bits, w, rank, total, head->used, head->bad, w, long(gridDim.x) * MAP_THREADS);
+}
+
+// Few rows and pages: the maps in LDS and all of it in one launch.
+__global__ void __launch_bounds__(MAP_THREADS) pages_free_small_kernel(const FreeArgs a) {
+  __shared__ uint64_t sums[MAP_THREADS / 64];
+  __shared__ uint32_t held[PAGE_CHUNK], gone[PAGE_CHUNK];
+  const int tid = threadIdx.x, used = *a.at.used;
+  held[tid] = gone[tid] = 0;
+  __syncthreads();
+  bool bad = used < 0 || used > a.at.pool_size;
+  if (!bad) mark_pool(a.at, used, held, tid, MAP_THREADS);
+  bad |= mark_rows(a.at, a.keep, held, gone, tid >> 6, MAP_THREADS / 64);
+  bad = __syncthreads_or(bad);
+  const uint32_t bits = gone[tid] & ~held[tid];
+  uint64_t total;
+  const uint64_t rank = scan_block<MAP_THREADS>(__popc(bits), sums, total);
+  write_freed(a, bits, tid, rank, total, used, bad, tid, MAP_THREADS);
+}
+
+// --- compaction ---------------------------------------------------------------------------------
+
+// Of the pages in use (L) and the free ones, in their order, the first L are to be in use. The free ones among those are the holes,
+// M of them, and the live ones behind them move there, both in their order: the first L - M live pages stay.
+
+// Free pages among the first `need` (at least one) of a word's pages.
+__device__ inline int holes_in(uint32_t live, uint32_t free, int need) {
+  uint32_t both = live | free;
+  int holes = 0;
+  for (; need > 0; --need, both &= both - 1) holes += (free & (both & -both)) != 0;
+  return holes;
+}
+
+// A word's part of the result. before: live (low half) and free pages before it.
+__device__ inline void write_moves(const CompactArgs& a, uint32_t live, uint32_t free, long word, uint64_t before, int used, long in_use, long moved) {
+  uint32_t both = live | free;
+  long l = long(before & 0xffffffffu), f = long(before >> 32);
+  for (; both; both &= both - 1) {
+    const int page = int(word * 32) + __builtin_ctz(both);
+    const bool is_live = live & (both & -both);
+    const long rank = l + f - in_use;  // among the pages that are to be free
+    if (rank >= 0) a.pool_out[used + rank] = page;
+    if (is_live && rank >= 0) a.src[l - (in_use - moved)] = page;
+    if (!is_live && rank < 0) a.dst[f] = page;
+    if (is_live) ++l;
+    else ++f;
+  }
+}
+
+// What there is besides the moves: places of src and dst behind them, and the pool as it was where nothing is done.
+__device__ inline void write_rest(const CompactArgs& a, int status, int used, long moved, long thread, long threads) {
+  for (long k = (status == TABLE_OK ? moved : 0) + thread; k < a.cap; k += threads) a.src[k] = a.dst[k] = -1;
+  if (status != TABLE_OK && a.pool_out != a.at.pool && used >= 0)
+    for (long k = used + thread; k < a.at.pool_size; k += threads) a.pool_out[k] = a.at.pool[k];
+  if (thread == 0) {
+    *a.count = status == TABLE_OK ? int(moved) : 0;
+    *a.at.status = status;
+  }
+}
+
+// The rows' entries where their pages are now. before[w]: live pages before word w.
+__device__ inline void rewrite_rows(const CompactArgs& a, const uint32_t* live, const int* before, int status, int kept, long wave, long waves) {
+  const PagesArgs& p = a.at;
+  const bool in_place = a.table_out == p.table;
+  const int lane = threadIdx.x & 63, segs = (p.width + UNIT - 1) / UNIT;
+  if (status != TABLE_OK && in_place) return;
+  for (long u = wave; u < long(p.n) * segs; u += waves) {
+    const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * UNIT;
+    const int all = status == TABLE_OK ? places_of(p.lens[i], p.shift) : 0, end = in_place ? all : p.width;
+    const int* row = p.table + long(i) * p.width;
+    int* out = a.table_out + long(i) * p.width;
+    int page[UNIT / 64];
+#pragma unroll
+    for (int k = 0; k < UNIT / 64; ++k) {
+      const int j = j0 + 64 * k + lane;
+      page[k] = j < end ? row[j] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < UNIT / 64; ++k) {
+      const int j = j0 + 64 * k + lane;
+      if (j >= end) continue;
+      int now = page[k];
+      if (j < all && page_ok(now, p.pages)) {
+        const int w = now >> 5, rank = before[w] + __popc(live[w] & ((1u << (now & 31)) - 1));
+        if (rank >= kept) now = a.dst[rank - kept];
+      }
+      out[j] = now;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(MAP_THREADS) pages_move_kernel(const CompactArgs a, const uint32_t* live, const uint32_t* free, long words, int* before,
+                                                                 const uint64_t* counts, MapHead* head) {
+  __shared__ uint64_t sums[MAP_THREADS / 64];
+  __shared__ long at_chunk, at_count;
+  __shared__ uint64_t at_before;
+  const int tid = threadIdx.x;
+  const long w = long(blockIdx.x) * PAGE_CHUNK + tid, chunks = gridDim.x;
+  const uint32_t l = w < words ? live[w] : 0, f = w < words ? free[w] : 0;
+  bool both = false;
+  uint64_t total, ahead = scan_block<MAP_THREADS>(count_word<true>(l, f, both), sums, total);
+  if (chunks > 1) ahead += sum_counts(counts, chunks, blockIdx.x, sums, total);
+  const bool twice = __syncthreads_or(both);  // with several chunks the count has looked at all of them
+  const long in_use = long(total & 0xffffffffu);
+  // the chunk that holds the last of the first `in_use` pages, then the word in it: the holes are the free pages before there
+  auto pages_in = [](uint64_t v) { return long(v & 0xffffffffu) + long(v >> 32); };
+  if (tid == 0) {
+    at_chunk = at_count = 0;
+    at_before = 0;
+  }
+  __syncthreads();
+  if (chunks > 1) {
+    uint64_t base = 0;
+    for (long c0 = 0; c0 < chunks; c0 += MAP_THREADS) {
+      const uint64_t v = c0 + tid < chunks ? counts[c0 + tid] : 0;
+      uint64_t sum;
+      const uint64_t b = base + scan_block<MAP_THREADS>(v, sums, sum);
+      if (pages_in(b) < in_use && in_use <= pages_in(b) + pages_in(v)) {
+        at_chunk = c0 + tid;
+        at_before = b;
+      }
+      base += sum;
+    }
+    __syncthreads();
+  }
+  const long w2 = at_chunk * PAGE_CHUNK + tid;
+  const uint32_t l2 = w2 < words ? live[w2] : 0, f2 = w2 < words ? free[w2] : 0;
+  uint64_t sum2;
+  const uint64_t v2 = count_word<true>(l2, f2, both), b2 = at_before + scan_block<MAP_THREADS>(v2, sums, sum2);
+  if (pages_in(b2) < in_use && in_use <= pages_in(b2) + pages_in(v2)) at_count = long(b2 >> 32) + holes_in(l2, f2, int(in_use - pages_in(b2)));
+  __syncthreads();
+  const long moved = at_count;
+  const int used = head->used, bad = head->bad | (twice ? 2 : 0);
+  const int status = bad & 1 ? TABLE_BAD_LENGTH : bad ? TABLE_BAD_PAGE : moved > a.cap ? TABLE_SLOTS_FULL : TABLE_OK;
+  if (w < words) before[w] = int(ahead & 0xffffffffu);
+  if (status == TABLE_OK && w < words) write_moves(a, l, f, w, ahead, used, in_use, moved);
+  write_rest(a, status, used, moved, w, chunks * MAP_THREADS);
+  if (w == 0) {
+    head->kept = int(in_use - moved);
+    head->status = status;
+  }
+}
+
+__global__ void __launch_bounds__(256) pages_rewrite_kernel(const CompactArgs a, const uint32_t* live, const int* before, const MapHead* head) {
+  const long t = long(blockIdx.x) * 256 + threadIdx.x;
+  rewrite_rows(a, live, before, head->status, head->kept, t >> 6, long(gridDim.x) * 4);
+}
+
+// Few rows and pages: the maps in LDS and all of it in one launch.
+__global__ void __launch_bounds__(MAP_THREADS) pages_compact_small_kernel(const CompactArgs a) {
+  __shared__ uint64_t sums[MAP_THREADS / 64];
+  __shared__ uint32_t live[PAGE_CHUNK], free[PAGE_CHUNK];
+  __shared__ int before[PAGE_CHUNK];
+  __shared__ long holes;
+  const int tid = threadIdx.x, used = *a.at.used;
+  live[tid] = free[tid] = 0;
+  if (tid == 0) holes = 0;
+  __syncthreads();
+  bool bad = used < 0 || used > a.at.pool_size, none = false;
+  if (!bad) none = mark_pool(a.at, used, free, tid, MAP_THREADS);
+  bad |= mark_rows(a.at, nullptr, live, nullptr, tid >> 6, MAP_THREADS / 64);
+  bad = __syncthreads_or(bad);
+  const uint32_t l = live[tid], f = free[tid];
+  uint64_t total;
+  const uint64_t v = count_word<true>(l, f, none), ahead = scan_block<MAP_THREADS>(v, sums, total);
+  none = __syncthreads_or(none);
+  const long in_use = long(total & 0xffffffffu), first = long(ahead & 0xffffffffu) + long(ahead >> 32), here = long(v & 0xffffffffu) + long(v >> 32);
+  if (first < in_use && in_use <= first + here) holes = long(ahead >> 32) + holes_in(l, f, int(in_use - first));
+  before[tid] = int(ahead & 0xffffffffu);
+  __syncthreads();
+  const long moved = holes;
+  const int status = bad ? TABLE_BAD_LENGTH : none ? TABLE_BAD_PAGE : moved > a.cap ? TABLE_SLOTS_FULL : TABLE_OK;
+  if (status == TABLE_OK) write_moves(a, l, f, tid, ahead, used, in_use, moved);
+  write_rest(a, status, used, moved, tid, MAP_THREADS);
+  __syncthreads();  // dst is there
+  rewrite_rows(a, live, before, status, int(in_use - moved), tid >> 6, MAP_THREADS / 64);
+}
+
+// --- copies -------------------------------------------------------------------------------------
+
+constexpr int COPY_THREADS = 256, COPY_AT_ONCE = 4;
+constexpr int COPY_PIECE = COPY_THREADS * COPY_AT_ONCE;  // pieces of 16 bytes a block has under way
+
+// 16 bytes a thread, four of them under way. A block takes (pair, array, part of a page) units in turn; arrays are the layers' keys,
+// values and bounds. Bound by HBM.
+__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyArgs a, int es, int parts, long units) {
+  const KvCache& c = a.cache;
+  const int arrays = a.layers * (a.has_bounds ? 3 : 2), row_shift = es == 4 ? 4 : 3;  // 16-byte pieces of a row
+  const int page16 = c.kv_heads << (c.shift + row_shift), bounds16 = c.kv_heads << (row_shift + 1);
+  if (a.count) units = min(units, long(min(max(*a.count, 0), a.n)) * arrays * parts);
+  for (long u = blockIdx.x; u < units; u += gridDim.x) {
+    const int i = int(quotient(u, long(arrays) * parts)), r = int(u - long(i) * arrays * parts), array = r / parts, part = r - array * parts;
+    const int src = a.src[i], dst = a.dst[i];
+    if (!page_ok(src, c.pages) || !page_ok(dst, c.pages) || src == dst) continue;
+    const int layer = array < a.layers ? array : array < 2 * a.layers ? array - a.layers : array - 2 * a.layers;
+    const bool bounds = array >= 2 * a.layers;
+    char* base = static_cast<char*>(bounds ? a.bounds[layer] : array < a.layers ? a.k[layer] : a.v[layer]);
+    const long stride = bounds ? bounds16 * 16L : c.page_stride * es;
+    const int end = bounds ? bounds16 : page16, rows = bounds || !a.rows ? 1 << c.shift : a.rows[i];
+    const uint4* from = reinterpret_cast<const uint4*>(base + src * stride);
+    uint4* to = reinterpret_cast<uint4*>(base + dst * stride);
+    uint4 v[COPY_AT_ONCE];
+    auto there = [&](int q) { return q < end && (bounds || ((q >> row_shift) & ((1 << c.shift) - 1)) < rows); };
+#pragma unroll
+    for (int k = 0; k < COPY_AT_ONCE; ++k) {
+      const int q = part * COPY_PIECE + k * COPY_THREADS + int(threadIdx.x);
+      if (there(q)) v[k] = from[q];
+    }
+#pragma unroll
+    for (int k = 0; k < COPY_AT_ONCE; ++k) {
+      const int q = part * COPY_PIECE + k * COPY_THREADS + int(threadIdx.x);
+      if (there(q)) to[q] = v[k];
+    }
+  }
+}
+
+// Places of all rows up to which one block marks them in LDS.
+constexpr long SMALL_PLACES = 65536;
+
+bool small(const PagesArgs& p) { return pages_plan(p.pages).chunks == 1 && long(p.n) * p.width <= SMALL_PLACES; }
+
+// Waves that the rows' units fill, four a block, no more than the chip holds several times.
+int mark_blocks(const PagesArgs& p) { return int(std::max<long>(1, std::min<long>(2048, (long(p.n) * cdiv(p.width, UNIT) + 3) / 4))); }
+
+struct Maps {
+  uint32_t* first; uint32_t* second; int* before; uint64_t* counts; MapHead* head;
+  Maps(const PagesPlan& plan, void* workspace) {
+    char* ws = static_cast<char*>(workspace);
+    first = reinterpret_cast<uint32_t*>(ws);
+    second = reinterpret_cast<uint32_t*>(ws + plan.second);
+    before = reinterpret_cast<int*>(ws + plan.before);
+    counts = reinterpret_cast<uint64_t*>(ws + plan.counts);
+    head = reinterpret_cast<MapHead*>(ws + plan.head);
+  }
+};
+
+// The maps of a call's pages, and the counts of their chunks where there are several.
+template <bool COMPACT> void fill_maps(const Exec& ex, const PagesArgs& p, const int* keep, const PagesPlan& plan, const Maps& m) {
+  const long words = (plan.second + plan.words * 4) / 4;
+  pages_clear_kernel<<<std::max(1, std::min(cdiv(words, 256), 2048)), 256, 0, ex.stream>>>(m.first, words, m.head, p.used);
+  pages_mark_kernel<COMPACT><<<mark_blocks(p), 256, 0, ex.stream>>>(p, keep, m.first, m.second, m.head);
+  if (plan.chunks > 1) pages_count_kernel<COMPACT><<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(m.first, m.second, plan.words, m.counts, m.head);
+}
+
+}  // namespace
+
+void fork_pages(const Exec& ex, const ForkArgs& args) {
+  ForkArgs a = args;
+  check_fork_pages(a);
+  if (ex.dry) return;
+  const PagesArgs& p = a.at;
+  ProfScope prof(ex, "fork_pages", 0, 8.0 * p.n * p.width + 32.0 * p.n);
+  auto launch = [&](auto threads) {
+    constexpr int N = decltype(threads)::value;
+    const dim3 grid(std::max(1, std::min(p.n, 1024)), std::max(1, std::min(cdiv(p.width, 4 * N), cdiv(1024, std::max(p.n, 1)))));
+    if ((grid.x == 1 && grid.y == 1) || (a.lens_out != p.lens && a.used_out != p.used)) {
+      fork_pages_kernel<N, true, true><<<grid, N, 0, ex.stream>>>(a);
+    } else {
+      fork_pages_kernel<N, true, false><<<grid, N, 0, ex.stream>>>(a);
+      fork_pages_kernel<N, false, true><<<1, N, 0, ex.stream>>>(a);
+    }
+  };
+  if (p.n <= 256) launch(std::integral_constant<int, 256>());
+  else launch(std::integral_constant<int, 1024>());
+  SPLAT_HIP(hipGetLastError());
+}
+
+void free_pages(const Exec& ex, const FreeArgs& args, void* workspace, size_t bytes) {
+  FreeArgs a = args;
+  check_free_pages(a, workspace, bytes);
+  if (ex.dry) return;
+  const PagesArgs& p = a.at;
+  ProfScope prof(ex, "free_pages", 0, 4.0 * p.n * p.width + 12.0 * p.n);
+  if (small(p)) {
+    pages_free_small_kernel<<<1, MAP_THREADS, 0, ex.stream>>>(a);
+  } else {
+    const PagesPlan plan = pages_plan(p.pages);
+    const Maps m(plan, workspace);
+    fill_maps<false>(ex, p, a.keep, plan, m);
+    pages_free_kernel<<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(a, m.first, m.second, plan.words, m.counts, m.head);
+  }
+  SPLAT_HIP(hipGetLastError());
+}
+
+void compact_pages(const Exec& ex, const CompactArgs& args, void* workspace, size_t bytes) {
+  CompactArgs a = args;
+  check_compact_pages(a, workspace, bytes);
+  if (ex.dry) return;
+  const PagesArgs& p = a.at;
+  ProfScope prof(ex, "compact_pages", 0, 8.0 * p.n * p.width + 8.0 * p.pages);
+  if (small(p)) {
+    pages_compact_small_kernel<<<1, MAP_THREADS, 0, ex.stream>>>(a);
+  } else {
+    const PagesPlan plan = pages_plan(p.pages);
+    const Maps m(plan, workspace);
+    fill_maps<true>(ex, p, nullptr, plan, m);
+    pages_move_kernel<<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(a, m.first, m.second, plan.words, m.before, m.counts, m.head);
+    pages_rewrite_kernel<<<mark_blocks(p), 256, 0, ex.stream>>>(a, m.first, m.before, m.head);
+  }
+  SPLAT_HIP(hipGetLastError());
+}
+
+void copy_pages(const Exec& ex, const CopyArgs& args) {
+  CopyArgs a = args;
+  check_copy_pages(a);
+  if (a.n == 0 || a.layers == 0 || ex.dry) return;
+  const KvCache& c = a.cache;
+  const int es = int(dtype_size(c.dt));
+  const long page16 = long(c.kv_heads) * c.page_size * 4 * es;  // 16-byte pieces
+  const int parts = cdiv(page16, COPY_PIECE), arrays = a.layers * (a.has_bounds ? 3 : 2);
+  ProfScope prof(ex, "copy_pages", 0, 2.0 * a.n * a.layers * (2.0 * page16 + (a.has_bounds ? c.kv_heads * 8.0 * es : 0.0)) * 16);
+  const long units = long(a.n) * arrays * parts;
+  copy_pages_kernel<<<int(std::min<long>(units, 16384)), COPY_THREADS, 0, ex.stream>>>(a, es, parts, units);
+  SPLAT_HIP(hipGetLastError());
+}
+
+}  // namespace splat

@@ -27,7 +27,7 @@ F32, BF16, F16 = 0, 1, 2
 DTYPES = {"f32": F32, "fp32": F32, "bf16": BF16, "f16": F16}
 NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 ROPE_NONE, ROPE_LINE, ROPE_GRID = 0, 1, 2
-TABLE_OK, TABLE_BAD_LENGTH, TABLE_POOL_EMPTY, TABLE_SLOTS_FULL = 0, 1, 2, 3
+TABLE_OK, TABLE_BAD_LENGTH, TABLE_POOL_EMPTY, TABLE_SLOTS_FULL, TABLE_BAD_ROW, TABLE_BAD_PAGE = range(6)
 STAGE_BLOCK, STAGE_DENSE_HEAD, STAGE_CAMERA_HEAD = 0, 1, 2
 FILTER_TRIANGLE, FILTER_CATMULLROM, FILTER_LANCZOS3 = 1, 2, 3   # image 0.25.10 imageops::FilterType
 
@@ -144,6 +144,24 @@ SIGNATURES = {
                                                 C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int,
                                                 C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
                                                 C.c_size_t]),
+    "splat_pages_workspace": (C.c_int, [C.c_int, C.POINTER(C.c_size_t)]),
+    "splat_kernel_fork_pages": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                          C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
+                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "splat_kernel_free_pages": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
+                                          C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                          C.c_void_p, C.c_size_t]),
+    "splat_kernel_compact_pages": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int,
+                                             C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
+    "splat_kernel_copy_pages": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.c_int, C.POINTER(C.c_void_p), C.c_int,
+                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "splat_prefix_attention_workspace": (C.c_int, [C.POINTER(KvCache), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                                   C.POINTER(C.c_size_t)]),
+    "splat_kernel_prefix_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCache), C.c_void_p, C.c_int64, C.c_int, C.c_int,
+                                                C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                                C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_float, C.c_void_p,
+                                                C.c_int64, C.c_void_p, C.c_size_t]),
     "splat_profile_begin": (C.c_int, [C.c_void_p]),
     "splat_profile_end": (C.c_int, [C.c_void_p, C.POINTER(KernelStatC), C.c_int, C.POINTER(C.c_int)]),
     "splat_kernel_conv2d": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
@@ -487,6 +505,42 @@ class Context:
                                                            lens, max_len, topk, scale, out, ldo, selected, workspace,
                                                            workspace_bytes))
 
+    def kernel_fork_pages(self, n: int, parents: int, keep: int, lens: int, page_size: int, pages: int, pool: int,
+                          pool_size: int, used: int, table: int, width: int, lens_out: int, src: int, dst: int,
+                          rows: int, used_out: int, status: int):
+        self.check(self._lib.splat_kernel_fork_pages(self.handle, n, parents, keep, lens, page_size, pages, pool,
+                                                     pool_size, used, table, width, lens_out, src, dst, rows, used_out,
+                                                     status))
+
+    def kernel_free_pages(self, n: int, keep: int, lens: int, page_size: int, pages: int, pool: int, pool_size: int,
+                          used: int, table: int, width: int, lens_out: int, used_out: int, status: int, workspace: int,
+                          workspace_bytes: int):
+        self.check(self._lib.splat_kernel_free_pages(self.handle, n, keep, lens, page_size, pages, pool, pool_size,
+                                                     used, table, width, lens_out, used_out, status, workspace,
+                                                     workspace_bytes))
+
+    def kernel_compact_pages(self, n: int, lens: int, page_size: int, pages: int, pool: int, pool_size: int, used: int,
+                             table: int, width: int, table_out: int, pool_out: int, src: int, dst: int, cap: int,
+                             count: int, status: int, workspace: int, workspace_bytes: int):
+        self.check(self._lib.splat_kernel_compact_pages(self.handle, n, lens, page_size, pages, pool, pool_size, used,
+                                                        table, width, table_out, pool_out, src, dst, cap, count, status,
+                                                        workspace, workspace_bytes))
+
+    def kernel_copy_pages(self, caches, bounds, n: int, src: int, dst: int, rows: int = 0, count: int = 0):
+        """caches: layers(...) of the network's KvCaches, or one of them; bounds: pointers(...) of theirs, or None."""
+        count_layers = 1 if isinstance(caches, KvCache) else len(caches)
+        if bounds is not None and len(bounds) != count_layers:
+            raise SplatError(BAD_ARGUMENT, "copy pages: as many bounds as layers")
+        self.check(self._lib.splat_kernel_copy_pages(self.handle, caches, count_layers, bounds, n, src, dst, rows, count))
+
+    def kernel_prefix_attention(self, cache: KvCache, q: int, ldq: int, n: int, heads: int, starts: int, groups: int,
+                                prefix: int, prefix_width: int, shared: int, max_shared: int, table: int, width: int,
+                                lens: int, max_own: int, scale: float, out: int, ldo: int, workspace: int,
+                                workspace_bytes: int):
+        self.check(self._lib.splat_kernel_prefix_attention(self.handle, cache, q, ldq, n, heads, starts, groups, prefix,
+                                                           prefix_width, shared, max_shared, table, width, lens,
+                                                           max_own, scale, out, ldo, workspace, workspace_bytes))
+
     def kernel_conv2d(self, dtype, inp, V, H, W, Cin, w, Cout, ldw, ks, stride, bias, relu_in, act, res, out):
         self.check(self._lib.splat_kernel_conv2d(self.handle, dtype, C.c_void_p(inp), V, H, W, Cin, C.c_void_p(w), Cout,
                                                  ldw, ks, stride, C.c_void_p(bias), relu_in, act, C.c_void_p(res),
@@ -532,6 +586,32 @@ def sparse_attention_workspace(cache: KvCache, n: int, heads: int, max_len: int,
     b = C.c_size_t()
     _check_free(lib().splat_sparse_attention_workspace(cache, n, heads, max_len, topk, C.byref(b)))
     return b.value
+
+
+def pages_workspace(pages: int) -> int:
+    """Bytes of device memory that kernel_free_pages and kernel_compact_pages need for so many pages or fewer."""
+    b = C.c_size_t()
+    _check_free(lib().splat_pages_workspace(pages, C.byref(b)))
+    return b.value
+
+
+def prefix_attention_workspace(cache: KvCache, n: int, heads: int, groups: int, max_shared: int, max_own: int) -> int:
+    """Bytes of device memory that kernel_prefix_attention needs for these sizes or smaller ones."""
+    b = C.c_size_t()
+    _check_free(lib().splat_prefix_attention_workspace(cache, n, heads, groups, max_shared, max_own, C.byref(b)))
+    return b.value
+
+
+def layers(caches):
+    """The caches of a network's layers as kernel_copy_pages takes them."""
+    caches = list(caches)
+    return (KvCache * len(caches))(*caches)
+
+
+def pointers(values):
+    """Device pointers (ints) as kernel_copy_pages takes them."""
+    values = list(values)
+    return (C.c_void_p * len(values))(*values)
 
 
 def da3_model_input_size(width: int, height: int):
