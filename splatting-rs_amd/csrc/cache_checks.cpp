@@ -502,14 +502,29 @@ int own_parts(long n, long cols, int max_own, int keys) {
 PrefixPlan prefix_plan(const PrefixArgs& a) {
   PrefixPlan plan;
   const KvCache& c = a.cache;
-  const int G = a.heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;
-  plan.rows = 16;
+  const int G = a.heads / c.kv_heads, small = c.dt == 0 ? 16 : 32;
+  const long each = (long(a.n) * G + a.groups - 1) / a.groups;  // rows of a group and key head, if all are alike
+  plan.rows = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 || c.dt == 0 ? 64 : each <= 128 ? 128 : 256;
+  const int keys = plan.rows >= 128 ? 64 : small, waves = plan.rows >= 128 ? 1 : 4;  // that take tiles of their own
   const long items = most_items(a.n, G, a.groups, plan.rows) * c.kv_heads, tiles = (a.max_shared + keys - 1) / keys;
-  // no more blocks than give each 8 tiles, two a wave
-  const long more = items >= MORE_BLOCKS ? 0 : std::min<long>(MORE_BLOCKS, items * (tiles / 8));
-  plan.blocks = int(items + more);
-  plan.own = own_parts(a.n, long(c.kv_heads) * ((G + 15) / 16), a.max_own, keys);
-  plan.join = more > 0 || plan.own > 0;
+  // blocks for so many parts of an item that the chip's rounds of blocks end full, or as many as there are, of two tiles a wave at least
+  const long most = std::max<long>(1, tiles / (2 * waves));
+  long blocks = items;
+  if (items < MORE_BLOCKS) {
+    blocks = std::max(items, std::min<long>(MORE_BLOCKS, items * most));
+  } else {
+    double best = 1e30;
+    for (long p = 1; p <= std::min<long>(4, most); ++p) {
+      const double cost = double((items * p + MORE_BLOCKS - 1) / MORE_BLOCKS) / p * (1 + 0.03 * (p - 1));
+      if (items * p <= items + MORE_BLOCKS * 4 && cost < best) {
+        best = cost;
+        blocks = items * p;
+      }
+    }
+  }
+  plan.blocks = int(blocks);
+  plan.own = own_parts(a.n, long(c.kv_heads) * ((G + 15) / 16), a.max_own, small);
+  plan.join = blocks > items || plan.own > 0;
   if (!plan.join) return plan;
   plan.parts = (16 + a.groups * 16L);
   plan.own_parts = plan.parts + size_t(plan.blocks) * plan.rows * PART_HEAD * 4;
@@ -526,7 +541,7 @@ size_t prefix_attention_bytes(const KvCache& c, int n, int heads, int groups, in
   if (n == 0 || groups == 0) return 0;
   const int G = heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;
   const size_t item = long(n) * heads + std::min<long>(groups, n) * c.kv_heads * WIDE_ROWS;
-  const size_t cut = std::min<size_t>(size_t(MORE_BLOCKS) * WIDE_ROWS, item * ((max_shared + keys - 1L) / keys));
+  const size_t cut = std::min<size_t>(size_t(MORE_BLOCKS) * 4 * WIDE_ROWS, item * ((max_shared + keys - 1L) / keys));
   // own parts: one a token and column group, or as many as there are blocks for
   const size_t cols = size_t(c.kv_heads) * ((G + 15) / 16);
   const size_t own = max_own == 0 ? 0 : std::max<size_t>(size_t(n) * heads, size_t(OWN_BLOCKS) / cols * heads);

@@ -418,6 +418,8 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_compact_small_kernel(const 
 constexpr int COPY_THREADS = 256, COPY_AT_ONCE = 4;
 constexpr int COPY_PIECE = COPY_THREADS * COPY_AT_ONCE;  // pieces of 16 bytes a block has under way
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // 16 bytes a thread, four of them under way. A block takes (pair, array, part of a page) units in turn; arrays are the layers' keys,
 // values and bounds. Bound by HBM.
 __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyArgs a, int es, int parts, long units) {
@@ -434,9 +436,9 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyArgs
     char* base = static_cast<char*>(bounds ? a.bounds[layer] : array < a.layers ? a.k[layer] : a.v[layer]);
     const long stride = bounds ? bounds16 * 16L : c.page_stride * es;
     const int end = bounds ? bounds16 : page16, rows = bounds || !a.rows ? 1 << c.shift : a.rows[i];
-    const uint4* from = reinterpret_cast<const uint4*>(base + src * stride);
-    uint4* to = reinterpret_cast<uint4*>(base + dst * stride);
-    uint4 v[COPY_AT_ONCE];
+    const u32x4* from = reinterpret_cast<const u32x4*>(base + src * stride);
+    u32x4* to = reinterpret_cast<u32x4*>(base + dst * stride);
+    u32x4 v[COPY_AT_ONCE];
     auto there = [&](int q) { return q < end && (bounds || ((q >> row_shift) & ((1 << c.shift) - 1)) < rows); };
 #pragma unroll
     for (int k = 0; k < COPY_AT_ONCE; ++k) {

@@ -190,8 +190,8 @@ template <typename T, int NT> struct PrefixWave {
     }
   }
 
-  // Tiles t, t + step, ... below stop: tile k is asked for while tile k - 2 is used. Where a sum is NaN they are taken again with
-  // care: a weight of 0 times an infinity, or one beside the second term of a weight, is no answer.
+  // Tiles t, t + step, ...: tile k is asked for while tile k - 2 is used. Where a sum is NaN they are to be taken again with care: a
+  // weight of 0 times an infinity, or an infinity beside the second term of a weight, is no answer.
   template <bool CAREFUL> __device__ inline bool pass(int t, int step, int count, float scale) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -221,30 +221,31 @@ template <typename T, int NT> struct PrefixWave {
         for (int r = 0; r < 4; ++r) nan |= o[n][d][r] != o[n][d][r];
     return __any(nan);
   }
-  __device__ inline void run(int t, int step, int stop, float scale) {
-    const int count = t < stop ? (stop - t + step - 1) / step : 0;
+  // True where a sum is NaN: then again, with care.
+  template <bool CAREFUL> __device__ inline bool run(int t, int step, int stop, float scale) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) ops[n].pin_q();
-    if (pass<false>(t, step, count, scale)) pass<true>(t, step, count, scale);
+    const bool nan = pass<CAREFUL>(t, step, t < stop ? (stop - t + step - 1) / step : 0, scale);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       l[n] = sum_groups(l[n]);
       some[n] = over_rows(float(some[n]), [](float a, float b) { return fmaxf(a, b); }) > 0.f;
     }
+    return nan;
   }
 };
 
 // --- a block ------------------------------------------------------------------------------------
 
-// A part: `columns` times 64 sums, then (m, l) of each; l is -1 where no key was there.
+// A part: `columns` times 64 sums, then (m, l) of each, the sums being of weights e^(x - m); l is -1 where no key was there.
 __device__ inline float* part_at(char* workspace, size_t offset, long index, int columns) {
   return reinterpret_cast<float*>(workspace + offset) + index * columns * long(PART_HEAD);
 }
 
-// The waves' sums join in LDS: wave d adds up channels 16 d + (0..15) of every column. place(column) gives the output's row
-// (normalised, where `whole`) or nullptr for columns without one; the others go to `part`.
+// The waves' sums join in LDS: wave d adds up channels 16 d + (0..15) of columns first, first + 1, ... place(n) gives the output's row
+// for the lane's column of NT (normalised, where `whole`) or nullptr if there is none; else they go to `part`.
 template <typename T, int NT, typename Place>
-__device__ inline void join_waves(const PrefixWave<T, NT>& w, char* smem, float (*stats)[NT * 16][4], int wave, bool whole, float* part, int columns, Place&& place) {
+__device__ inline void join_waves(const PrefixWave<T, NT>& w, char* smem, float (*stats)[4], int wave, bool whole, float* part, int first, int columns, Place&& place) {
   const int lane = w.lane, col = lane & 15, g = lane >> 4;
   float* mine = reinterpret_cast<float*>(smem + wave * RING * TILE_BYTES);  // its tiles are used up
 #pragma unroll
@@ -254,7 +255,7 @@ __device__ inline void join_waves(const PrefixWave<T, NT>& w, char* smem, float 
 #pragma unroll
       for (int r = 0; r < 4; ++r) mine[((n * 4 + d) * 4 + r) * 64 + lane] = w.o[n][d][r];
     if (g == 0) {
-      float* s = stats[wave][n * 16 + col];
+      float* s = stats[(wave * NT + n) * 16 + col];
       s[0] = w.m[n];
       s[1] = w.l[n];
       s[2] = float(w.some[n]);
@@ -263,14 +264,14 @@ __device__ inline void join_waves(const PrefixWave<T, NT>& w, char* smem, float 
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int column = n * 16 + col;
+    const int column = first + n * 16 + col;
     float mn = -INFINITY, sum = 0.f, v[4] = {};
     bool some = false;
 #pragma unroll
-    for (int k = 0; k < WAVES; ++k) mn = fmaxf(mn, stats[k][column][0]);
+    for (int k = 0; k < WAVES; ++k) mn = fmaxf(mn, stats[(k * NT + n) * 16 + col][0]);
 #pragma unroll
     for (int k = 0; k < WAVES; ++k) {
-      const float* s = stats[k][column];
+      const float* s = stats[(k * NT + n) * 16 + col];
       if (s[2] == 0.f) continue;  // no key: its sums are zeros, whatever the others hold
       some = true;
       const float f = s[0] == -INFINITY ? 0.f : exp_of(s[0] - mn);
@@ -281,7 +282,7 @@ __device__ inline void join_waves(const PrefixWave<T, NT>& w, char* smem, float 
     }
     if (column >= columns) continue;
     if (whole) {
-      T* out = place(column);
+      T* out = place(n);
       if (!out) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = some ? v[r] / sum : 0.f;
@@ -290,19 +291,21 @@ __device__ inline void join_waves(const PrefixWave<T, NT>& w, char* smem, float 
       else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     } else {
       *reinterpret_cast<float4*>(part + column * 64 + 16 * wave + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
-      if (wave == 0 && g == 0) *reinterpret_cast<float2*>(part + columns * 64 + column * 2) = make_float2(mn, some ? sum : -1.f);
+      if (wave == 0 && g == 0) *reinterpret_cast<float2*>(part + columns * 64 + column * 2) = make_float2(mn - TileOps<T>::TOP * 0.693147180559945309f, some ? sum : -1.f);
     }
   }
 }
 
 // A block's part of the groups' items.
 struct Mine {
-  int group, item, kh, part, parts;  // group -1: nothing
+  int id;  // of the block among those with work, -1: nothing to do
+  int group, item, kh, part, parts;
   int start, tokens, shared;
 };
 
-// Thread t sums up its k groups; block 0 leaves the plan for the join. The tiles of a part: as many as leave no more parts
-// than blocks (an item of T tiles has at most T / each + 1).
+// Thread t sums up its k groups; block 0 leaves the plan for the join. The tiles of a part: as few as leave no more parts than
+// blocks. all tiles / blocks is tried first, which fits where the groups are alike; an item of T tiles has at most T / each + 1 parts,
+// so that all tiles / (blocks - items) always fits.
 template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a, int blocks, char* workspace, bool join) {
   __shared__ long sums[WAVES];
   __shared__ Mine found;
@@ -322,36 +325,41 @@ template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a,
     }
     return total;
   };
-  if (tid == 0) found.group = -1;
+  auto items_of = [&](int m) { return (m * G + R - 1) / R; };  // of a key head; m G is below 2^21
+  auto tokens_of = [&](int g) { return max(0, start_of(a, g + 1) - start_of(a, g)); };
+  auto tiles_of = [&](int shared) { return (shared + KEYS - 1) / KEYS; };
+  if (tid == 0) found.id = -1;
   long items = 0, tiles = 0, tokens = 0, before;
   for (int g = g0; g < g1; ++g) {
-    const int m = max(0, start_of(a, g + 1) - start_of(a, g));
-    const long its = (long(m) * G + R - 1) / R;
-    items += its * kv;
-    tiles += its * kv * ((shared_of(a, g) + KEYS - 1) / KEYS);
+    const int m = tokens_of(g), its = items_of(m) * kv;
+    items += its;
+    tiles += long(its) * tiles_of(shared_of(a, g));
     tokens += m;
   }
   const bool valid = total_of(tokens, before) <= a.n;  // more only where starts descend: nothing is done
-  const long all_items = total_of(items, before), all_tiles = total_of(tiles, before);
-  const long spare = blocks - all_items, each = join && spare > 0 ? max(1L, quotient(all_tiles + spare - 1, spare)) : 1L << 40;
-  long count = 0;
-  auto parts_of = [&](int shared) { return int(max(1L, quotient((shared + KEYS - 1) / KEYS + each - 1, each))); };
-  for (int g = g0; g < g1; ++g) {
-    const int m = max(0, start_of(a, g + 1) - start_of(a, g));
-    count += (long(m) * G + R - 1) / R * kv * parts_of(shared_of(a, g));
+  long all_items = total_of(items, before), all_tiles = 0, count = 0, total = 0, each = 1L << 40;
+  auto parts_of = [&](int shared) { return int(max(1L, quotient(tiles_of(shared) + each - 1, each))); };
+  if (join) all_tiles = total_of(tiles, before);
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    const long share = attempt == 0 ? blocks : blocks - all_items;
+    if (join && share > 0) each = max(1L, quotient(all_tiles + share - 1, share));
+    else each = 1L << 40;
+    count = 0;
+    for (int g = g0; g < g1; ++g) count += long(items_of(tokens_of(g))) * kv * parts_of(shared_of(a, g));
+    total = total_of(count, before);
+    if (total <= blocks) break;
   }
-  total_of(valid ? count : 0, before);
+  // those that read the same keys run at the same time on the same XCD: items fastest, contiguous ids an XCD
   if (valid) {
+    const long id = long(blockIdx.x) < total ? xcd_contiguous(int(blockIdx.x), int(total)) : -1;
     long at = before;
     for (int g = g0; g < g1; ++g) {
-      const int start = start_of(a, g), m = max(0, start_of(a, g + 1) - start), shared = shared_of(a, g), parts = parts_of(shared);
-      const int its = int((long(m) * G + R - 1) / R);
+      const int start = start_of(a, g), m = tokens_of(g), shared = shared_of(a, g), parts = parts_of(shared), its = items_of(m);
       const long here = long(its) * kv * parts;
       if (join && blockIdx.x == 0) reinterpret_cast<GroupPlan*>(workspace + sizeof(PlanHead))[g] = {int(at), parts, its, start};
-      if (long(blockIdx.x) >= at && long(blockIdx.x) < at + here) {
-        // items fastest: those that read the same keys run at the same time
-        const int r = int(blockIdx.x - at), item = r % its, rest = r / its;
-        found = {g, item, rest / parts, rest % parts, parts, start, m, shared};
+      if (id >= at && id < at + here) {
+        const int r = int(id - at), item = r % its, rest = r / its;
+        found = {int(id), g, item, rest / parts, rest % parts, parts, start, m, shared};
       }
       at += here;
     }
@@ -361,33 +369,62 @@ template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a,
   return found;
 }
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const PrefixArgs a, int blocks, int own, bool join, size_t parts, size_t own_parts, char* workspace) {
+// A token's own positions: the part of block `u` of them.
+template <typename T>
+__device__ inline void own_part(const PrefixArgs& a, int u, int own, size_t own_parts, char* workspace, char* smem, float (*stats)[4]) {
   using Ops = TileOps<T>;
-  constexpr int KEYS = Ops::KEYS, R = NT * 16;
-  __shared__ __attribute__((aligned(1024))) char smem[WAVES * RING * TILE_BYTES];
-  __shared__ float stats[WAVES][R][4];
+  constexpr int KEYS = Ops::KEYS;
   const KvCache& c = a.cache;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int G = a.heads / c.kv_heads;
+  const int G = a.heads / c.kv_heads, groups = (G + 15) / 16, cols = c.kv_heads * groups, columns = min(G, 16);
+  const int part = u % own, i = u / own / cols, group = u / own % cols, kh = group / groups, h0 = group % groups * 16;
+  const int grp = group_of(a, i);
+  char* ring = smem + wave * RING * TILE_BYTES;
+  PrefixWave<T, 1> w{c, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring, a.table + long(i) * a.width, a.width};
+  const bool in = h0 + col < G;
+  w.ops[0].load_q(static_cast<const T*>(a.q) + long(i) * a.ldq + long(kh * G + h0 + (in ? col : 0)) * 64, g, in);
+  w.lo = grp < 0 ? 0 : uniform(shared_of(a, grp));
+  w.end = grp < 0 ? 0 : uniform(int(min(long(length_of(a.lens[i], a.width, c.shift, 0x7fffffff)), long(w.lo) + a.max_own)));
+  w.least = w.hi[0] = w.end;
+  const int first = w.lo / KEYS, tiles = w.end > w.lo ? (w.end + KEYS - 1) / KEYS - first : 0;
+  const int t0 = first + int(long(tiles) * part / own) + wave, t1 = first + int(long(tiles) * (part + 1) / own);
+  if (w.template run<false>(t0, WAVES, t1, a.scale)) w.template run<true>(t0, WAVES, t1, a.scale);
+  join_waves<T, 1>(w, smem, stats, wave, false, part_at(workspace, own_parts, u, columns), 0, columns, [](int) { return static_cast<T*>(nullptr); });
+}
+
+// Few rows an item: each wave streams its own tiles through a ring of its own, and the block's waves join in LDS.
+template <typename T, int NT>
+__global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const PrefixArgs a, int blocks, int own, bool join, size_t parts, size_t own_parts, char* workspace) {
+  constexpr int KEYS = TileOps<T>::KEYS, R = NT * 16;
+  __shared__ __attribute__((aligned(1024))) char smem[WAVES * RING * TILE_BYTES];
+  __shared__ float stats[WAVES * R][4];
+  if (int(blockIdx.x) >= blocks) {
+    own_part<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
+    return;
+  }
+  const Mine mine = find_item<KEYS, R>(a, blocks, workspace, join);
+  if (uniform(mine.id) < 0) return;
+  const KvCache& c = a.cache;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, G = a.heads / c.kv_heads;
+  const int kh = uniform(mine.kh), shared = uniform(mine.shared), rows = uniform(mine.tokens) * G, item = uniform(mine.item), start = uniform(mine.start);
   char* ring = smem + wave * RING * TILE_BYTES;
   const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring));
-  if (int(blockIdx.x) < blocks) {
-    const Mine mine = find_item<KEYS, R>(a, blocks, workspace, join);
-    if (uniform(mine.group) < 0) return;
-    const int kh = uniform(mine.kh), shared = uniform(mine.shared);
-    PrefixWave<T, NT> w{c, kh, lane, lds, ring, a.prefix + long(uniform(mine.group)) * a.prefix_width, a.prefix_width};
-    const int rows = uniform(mine.tokens) * G;
-    int most = 0, least = 0x7fffffff;
-    int token[NT], head[NT];
+  const int* row = a.prefix + long(uniform(mine.group)) * a.prefix_width;
+  float* part = part_at(workspace, parts, uniform(mine.id), R);
+  // The item's columns from `first` on: M times 16. True where a sum is NaN, and nothing is written then.
+  auto columns = [&](auto count, auto careful, int first) {
+    constexpr int M = decltype(count)::value;
+    constexpr bool CAREFUL = decltype(careful)::value;
+    PrefixWave<T, M> w{c, kh, lane, lds, ring, row, a.prefix_width};
+    int most = 0, least = 0x7fffffff, token[M], head[M];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = uniform(mine.item) * R + n * 16 + col;  // below 2^21
+    for (int n = 0; n < M; ++n) {
+      const int r = item * R + first + n * 16 + col;  // below 2^21
       const bool in = r < rows;
-      token[n] = uniform(mine.start) + (in ? r / G : 0);
+      token[n] = start + (in ? r / G : 0);
       head[n] = in ? kh * G + r % G : -1;
       w.hi[n] = in ? max(0, min(a.lens ? a.lens[token[n]] : shared, shared)) : 0;
-      w.ops[n].load_q(static_cast<const T*>(a.q) + long(token[n]) * a.ldq + long(max(head[n], 0)) * 64, g, in);
+      w.ops[n].load_q(static_cast<const T*>(a.q) + long(token[n]) * a.ldq + long(max(head[n], 0)) * 64, lane >> 4, in);
       most = max(most, w.hi[n]);
       if (in) least = min(least, w.hi[n]);
     }
@@ -400,42 +437,398 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
     w.lo = 0;
     w.end = uniform(most);
     w.least = uniform(least);
-    const int tiles = (shared + KEYS - 1) / KEYS, seen = (w.end + KEYS - 1) / KEYS, part = uniform(mine.part), of = uniform(mine.parts);
-    const int t0 = int(long(tiles) * part / of), t1 = min(seen, int(long(tiles) * (part + 1) / of));
-    w.run(t0 + wave, WAVES, t1, a.scale);
-    join_waves<T, NT>(w, smem, stats, wave, !join, part_at(workspace, parts, blockIdx.x, R), R, [&](int column) {
-      const int n = column >> 4;
+    const int tiles = (shared + KEYS - 1) / KEYS, seen = (w.end + KEYS - 1) / KEYS, k = uniform(mine.part), of = uniform(mine.parts);
+    const int t0 = int(long(tiles) * k / of), t1 = min(seen, int(long(tiles) * (k + 1) / of));
+    const bool nan = w.template run<CAREFUL>(t0 + wave, WAVES, t1, a.scale);
+    if (!CAREFUL && __syncthreads_or(nan)) return true;
+    join_waves<T, M>(w, smem, stats, wave, !join, part, first, R, [&](int n) {
       T* out = nullptr;
 #pragma unroll
-      for (int k = 0; k < NT; ++k)
+      for (int k = 0; k < M; ++k)
         if (k == n && head[k] >= 0) out = static_cast<T*>(a.out) + long(token[k]) * a.ldo + long(head[k]) * 64;
       return out;
     });
+    return false;
+  };
+  if (!columns(std::integral_constant<int, NT>(), std::false_type(), 0)) return;
+#pragma unroll 1
+  for (int n = 0; n < NT; ++n) {  // a few columns at a time: what the careful form keeps leaves no registers for more
+    __syncthreads();              // the ring and the statistics are read
+    columns(std::integral_constant<int, 1>(), std::true_type(), n * 16);
+  }
+}
+
+// --- many rows an item --------------------------------------------------------------------------
+//
+// Four waves of 64 columns share tiles of 64 keys, on the 32x32 matrix instructions: S^T = K Q^T leaves a lane one
+// column (lane % 32) and 16 keys of each 32, which is the second operand of O^T = V^T P^T as it stands. Bound by the matrix
+// instructions and the exponentials that run beside them.
+//
+// The weights are 2^(c s - r), c = |scale| log2(e), in one fused multiply-add: its one rounding is of the difference, and what r was
+// rounded by is the same for all weights of a column. r follows the largest score, but only when that has grown by 2^SLACK, so that
+// the sums are seldom multiplied. The weights are rounded once to the values' type, where the two terms of the other form would
+// cost half the matrix instructions again; their sum is of the rounded ones, so that what a column's weights have in common cancels.
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
+
+template <typename T> __device__ inline f32x16 mma32(const uint4& a, const uint4& b, const f32x16& c) {
+  if constexpr (std::is_same<T, bf16>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_v, a), __builtin_bit_cast(f16x8_v, b), c, 0, 0, 0);
+}
+// acc + both values of a packed pair
+template <typename T> __device__ inline float add_pair(uint32_t pair, float acc) {
+  if constexpr (std::is_same<T, bf16>::value)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pair), __builtin_bit_cast(bf16x2_v, 0x3f803f80u), acc, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_v, pair), __builtin_bit_cast(f16x2_v, 0x3c003c00u), acc, false);
+}
+__device__ inline float most_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN stays
+// fn over lanes l and l ^ 32
+template <typename F> __device__ inline float over_two(float v, F&& fn) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fn(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+constexpr int WIDE_KEYS = 64, WIDE_BYTES = WIDE_KEYS * 256;  // a tile: K, then V
+constexpr int WIDE_RING = 4;
+
+template <typename T, int QT> struct WideWave {
+  static constexpr float SLACK = 8.f;
+  static constexpr float TOP = std::is_same<T, f16>::value ? 7.f : 0.f;  // f16 weights below 2^-14 lose bits: the largest is 2^15
+  const KvCache& c;
+  const int kh, lane, wave;
+  char* smem;
+  const int* row;  // of pages
+  int width, end;  // positions from `end` on are seen by no column of the block
+  // 64 entries of the row, one a lane: those of the tiles that are loaded now, and the next ones; ok: which are pages
+  int chunk, entries, ahead;
+  uint64_t ok;
+  int hi[QT], most, least;  // of the wave's columns
+  uint4 q[QT][4];
+  f32x16 o[QT][2];
+  float r[QT], l[QT];
+  bool some[QT];  // keys were there
+
+  __device__ inline int load_entries(int k) const { return row[min(long(k) * 64 + lane, long(width) - 1)]; }
+  __device__ inline void begin_entries(int t) {
+    chunk = ((t * WIDE_KEYS) >> c.shift) >> 6;
+    entries = load_entries(chunk);
+    ahead = load_entries(chunk + 1);
+    ok = __ballot(page_ok(entries, c.pages));
+  }
+  // The tile's pages that are there, a bit each.
+  __device__ inline uint32_t pages_of(int t) const {
+    const int per = max(1, WIDE_KEYS >> c.shift);
+    return uint32_t(ok >> (((t * WIDE_KEYS) >> c.shift) & 63)) & ((1u << per) - 1);
+  }
+  // Asks for this wave's rows of tile t (8 w and 32 + 8 w on) into slot t of the ring; which of the tile's pages are there.
+  __device__ inline uint32_t issue(int t) {
+    const int place0 = (t * WIDE_KEYS) >> c.shift;
+    if ((place0 >> 6) != chunk) {
+      chunk = place0 >> 6;
+      entries = ahead;
+      ahead = load_entries(chunk + 1);
+      ok = __ballot(page_ok(entries, c.pages));
+    }
+    const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)smem)) + (t % WIDE_RING) * WIDE_BYTES;
+    const int lrow = lane >> 3;
+    const uint32_t k_off[4] = {uint32_t(lrow * 128 + (((lane & 7) ^ ((4 * (wave & 1) + (lrow >> 1)) & 7)) * 16))};
+    const uint32_t v_off[4] = {uint32_t(lrow * 128 + (((lane & 7) ^ ((lrow & 3) << 1)) * 16))};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int piece = i * WAVES + wave, first = t * WIDE_KEYS + piece * 8;
+      const int page = __builtin_amdgcn_readlane(entries, (first >> c.shift) & 63);
+      const int rows = page_ok(page, c.pages) ? max(0, min(8, end - first)) : 0;
+      const long at = (rows ? page_at(c, page, kh) : 0) + (first & (c.page_size - 1)) * 64;
+      load_lds<1>(static_cast<const T*>(c.k) + at, rows * 128, k_off, 0, lds + piece * 1024);
+      load_lds<1>(static_cast<const T*>(c.v) + at, rows * 128, v_off, 0, lds + WIDE_BYTES / 2 + piece * 1024);
+    }
+    return pages_of(t);
+  }
+
+  // V^T of 16 keys from 32 kt + 16 hh on and channels 32 dt on, in the order of the weights (as in TileOps, for 32 rows of output).
+  __device__ inline uint4 values(const char* vt, int kt, int hh, int dt) const {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    const int G = lane >> 4, j = (lane >> 2) & 3, cc = lane & 3;
+    const int at = (4 * (G >> 1) + j) * 128 + (((4 * dt + 2 * (G & 1) + (cc >> 1)) ^ (j << 1)) * 16) + (cc & 1) * 8;
+    uint32_t w[4];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)((lds_cptr)(vt + (kt * 32 + 16 * hh + 8 * half) * 128 + at)));
+      const uint2 u = __builtin_bit_cast(uint2, x);
+      w[2 * half] = u.x;
+      w[2 * half + 1] = u.y;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  template <typename F> __device__ static inline uint4 map_pairs(const uint4& v, F&& fn) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = pack2<T>(fn(u16f<T>(u[k])), fn(u16f<T>(u[k] >> 16)));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+
+  template <bool CAREFUL> __device__ inline void tile(int t, uint32_t pages, float scale) {
+    const char* kt = smem + (t % WIDE_RING) * WIDE_BYTES;
+    const char* vt = kt + WIDE_BYTES / 2;
+    const int g = lane >> 5, l32 = lane & 31, first = t * WIDE_KEYS, sw = (l32 >> 1) & 7;
+    f32x16 s[QT][2];
+    const f32x16 zero = {};
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const uint4 kf = *reinterpret_cast<const uint4*>(kt + (k2 * 32 + l32) * 128 + ((2 * st + g) ^ sw) * 16);
+#pragma unroll
+        for (int n = 0; n < QT; ++n) s[n][k2] = mma32<T>(kf, q[n][st], st == 0 ? zero : s[n][k2]);
+      }
+    __builtin_amdgcn_s_setprio(0);
+    const uint32_t all = (1u << max(1, WIDE_KEYS >> c.shift)) - 1;
+    const bool edge = pages != all || first + WIDE_KEYS > least;
+    auto seen = [&](int n, int k2, int x) {
+      const int key = k2 * 32 + 8 * (x >> 2) + 4 * g + (x & 3), place = ((first & (c.page_size - 1)) + k2 * 32 + 8 * (x >> 2)) >> c.shift;
+      return first + key < hi[n] && (pages >> place & 1);
+    };
+    if (edge) {
+      asm volatile("");  // a branch: as selections these would be a hundred instructions in every tile
+#pragma unroll
+      for (int n = 0; n < QT; ++n)
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const bool sees = seen(n, k2, x);
+            some[n] |= sees;
+            if (!sees) s[n][k2][x] = -INFINITY;
+          }
+    } else {
+#pragma unroll
+      for (int n = 0; n < QT; ++n) some[n] = true;
+    }
+    bool grow = false;
+    float top[QT];
+#pragma unroll
+    for (int n = 0; n < QT; ++n) {
+      float m[11];
+#pragma unroll
+      for (int k = 0; k < 10; ++k) {
+        const int e = 3 * k;
+        m[k] = most_of(most_of(s[n][e >> 4][e & 15], s[n][(e + 1) >> 4][(e + 1) & 15]), s[n][(e + 2) >> 4][(e + 2) & 15]);
+      }
+      m[10] = most_of(s[n][1][14], s[n][1][15]);
+      const float a = most_of(most_of(m[0], m[1]), m[2]), b = most_of(most_of(m[3], m[4]), m[5]), d = most_of(most_of(m[6], m[7]), m[8]);
+      const float mx = over_two(most_of(most_of(most_of(a, b), d), most_of(m[9], m[10])), most_of) * scale;
+      top[n] = mx > r[n] + SLACK ? mx : r[n];
+      grow |= top[n] != r[n];
+    }
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+      for (int n = 0; n < QT; ++n) {
+        const float keep = r[n] == top[n] ? 1.f : __builtin_amdgcn_exp2f(r[n] - top[n]);
+        l[n] *= keep;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          o[n][0][x] *= keep;
+          o[n][1][x] *= keep;
+        }
+        r[n] = top[n];
+      }
+    }
+    uint32_t p[QT][2][8];
+#pragma unroll
+    for (int n = 0; n < QT; ++n) {
+      const float ref = TOP - (r[n] == -INFINITY ? 0.f : r[n]);
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float a = __builtin_amdgcn_exp2f(fmaf(s[n][k2][2 * x], scale, ref)), b = __builtin_amdgcn_exp2f(fmaf(s[n][k2][2 * x + 1], scale, ref));
+          p[n][k2][x] = pack2<T>(a, b);
+          l[n] = add_pair<T>(p[n][k2][x], l[n]);
+        }
+    }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          uint4 vf = values(vt, k2, hh, dt);
+          if constexpr (CAREFUL) {
+            // infinities and NaN count where they are seen and nowhere else: how many of each kind a column sees
+            const uint4 raw = vf;
+            vf = map_pairs(raw, [](float y) { return fabsf(y) < INFINITY ? y : 0.f; });
+#pragma unroll
+            for (int n = 0; n < QT; ++n) {
+              uint32_t one[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                one[k] = pack2<T>(seen(n, k2, 8 * hh + 2 * k) ? 1.f : 0.f, seen(n, k2, 8 * hh + 2 * k + 1) ? 1.f : 0.f);
+              const uint4 sees = make_uint4(one[0], one[1], one[2], one[3]);
+              const f32x16 none = mma32<T>(map_pairs(raw, [](float y) { return y != y ? 1.f : 0.f; }), sees, zero);
+              const f32x16 up = mma32<T>(map_pairs(raw, [](float y) { return y == INFINITY ? 1.f : 0.f; }), sees, zero);
+              const f32x16 down = mma32<T>(map_pairs(raw, [](float y) { return y == -INFINITY ? 1.f : 0.f; }), sees, zero);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                if (none[x] > 0.f) o[n][dt][x] = NAN;
+                if (up[x] > 0.f) o[n][dt][x] += INFINITY;
+                if (down[x] > 0.f) o[n][dt][x] -= INFINITY;
+              }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < QT; ++n)
+            o[n][dt] = mma32<T>(vf, make_uint4(p[n][k2][4 * hh], p[n][k2][4 * hh + 1], p[n][k2][4 * hh + 2], p[n][k2][4 * hh + 3]), o[n][dt]);
+        }
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  // Tiles t0 up to t1, asked for three ahead. The barrier of a tile says that its loads have come, all waves', and that the
+  // tile before it is used up, into whose slot the next load goes.
+  template <bool CAREFUL> __device__ inline bool pass(int t0, int t1, float scale) {
+#pragma unroll
+    for (int n = 0; n < QT; ++n) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) o[n][0][x] = o[n][1][x] = 0.f;
+      r[n] = -INFINITY;
+      l[n] = 0.f;
+      some[n] = false;
+    }
+    uint32_t pages[WIDE_RING - 1] = {};  // of the tiles under way
+    if (t0 < t1) begin_entries(t0);
+#pragma unroll
+    for (int k = 0; k < WIDE_RING - 1; ++k)
+      if (t0 + k < t1) pages[k] = issue(t0 + k);
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      // four loads a tile of this wave
+      if (t + 2 < t1) wait_loads<8>();
+      else if (t + 1 < t1) wait_loads<4>();
+      else wait_loads<0>();
+      asm volatile("s_barrier" ::: "memory");
+      const uint32_t now = pages[0];
+#pragma unroll
+      for (int k = 0; k + 1 < WIDE_RING - 1; ++k) pages[k] = pages[k + 1];
+      if (t + WIDE_RING - 1 < t1) pages[WIDE_RING - 2] = issue(t + WIDE_RING - 1);
+      if (t * WIDE_KEYS < most) tile<CAREFUL>(t, now, scale);
+    }
+    bool nan = false;
+#pragma unroll
+    for (int n = 0; n < QT; ++n)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) nan |= o[n][0][x] != o[n][0][x] || o[n][1][x] != o[n][1][x];
+    return __syncthreads_or(nan && most > 0);
+  }
+};
+
+template <typename T, int QT>
+__global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const PrefixArgs a, int blocks, int own, bool join, size_t parts, size_t own_parts, char* workspace) {
+  constexpr int R = WAVES * QT * 32;
+  __shared__ __attribute__((aligned(1024))) char smem[WAVES * RING * TILE_BYTES];
+  static_assert(sizeof(smem) >= WIDE_RING * WIDE_BYTES, "the ring");
+  __shared__ float stats[WAVES * 16][4];
+  __shared__ int ends[WAVES];
+  if (int(blockIdx.x) >= blocks) {
+    own_part<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
     return;
   }
-  // a token's own positions
-  const int cols = c.kv_heads * ((G + 15) / 16), columns = min(G, 16);
-  const int u = int(blockIdx.x) - blocks, part = u % own, i = u / own / cols, group = u / own % cols, kh = group / ((G + 15) / 16), h0 = group % ((G + 15) / 16) * 16;
-  const int grp = group_of(a, i);
-  PrefixWave<T, 1> w{c, kh, lane, lds, ring, a.table + long(i) * a.width, a.width};
-  const bool in = h0 + col < G;
-  w.ops[0].load_q(static_cast<const T*>(a.q) + long(i) * a.ldq + long(kh * G + h0 + (in ? col : 0)) * 64, g, in);
-  w.lo = grp < 0 ? 0 : uniform(shared_of(a, grp));
-  w.end = grp < 0 ? 0 : uniform(int(min(long(length_of(a.lens[i], a.width, c.shift, 0x7fffffff)), long(w.lo) + a.max_own)));
-  w.least = w.hi[0] = w.end;
-  const int first = w.lo / KEYS, tiles = w.end > w.lo ? (w.end + KEYS - 1) / KEYS - first : 0;
-  w.run(first + int(long(tiles) * part / own) + wave, WAVES, first + int(long(tiles) * (part + 1) / own), a.scale);
-  float* to = part_at(workspace, own_parts, u, columns);
-  __shared__ float own_stats[WAVES][16][4];
-  join_waves<T, 1>(w, smem, own_stats, wave, false, to, columns, [](int) { return static_cast<T*>(nullptr); });
+  const Mine mine = find_item<WIDE_KEYS, R>(a, blocks, workspace, join);
+  if (uniform(mine.id) < 0) return;
+  const KvCache& c = a.cache;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 5, G = a.heads / c.kv_heads;
+  const int kh = uniform(mine.kh), shared = uniform(mine.shared), rows = uniform(mine.tokens) * G, item = uniform(mine.item), start = uniform(mine.start);
+  const int* row = a.prefix + long(uniform(mine.group)) * a.prefix_width;
+  // a scale's sign goes into the queries, exactly, and a scale of 0: the largest score is then the largest product
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, hold = a.scale == 0.f ? 0u : ~0u;
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
+  // M of each wave's QT times 32 columns, from `first` on. True where a sum is NaN, and nothing is written then.
+  auto columns = [&](auto count, auto careful, int first) {
+    constexpr int M = decltype(count)::value;
+    constexpr bool CAREFUL = decltype(careful)::value;
+    WideWave<T, M> w{c, kh, lane, wave, smem, row, a.prefix_width};
+    int most = 0, least = 0x7fffffff, token[M], head[M];
+#pragma unroll
+    for (int n = 0; n < M; ++n) {
+      const int r = item * R + (wave * QT + first + n) * 32 + (lane & 31);
+      const bool in = r < rows;
+      token[n] = start + (in ? r / G : 0);
+      head[n] = in ? kh * G + r % G : -1;
+      w.hi[n] = in ? max(0, min(a.lens ? a.lens[token[n]] : shared, shared)) : 0;
+      const T* q = static_cast<const T*>(a.q) + long(token[n]) * a.ldq + long(max(head[n], 0)) * 64;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const uint4 x = in ? *reinterpret_cast<const uint4*>(q + st * 16 + g * 8) : make_uint4(0, 0, 0, 0);
+        w.q[n][st] = make_uint4((x.x ^ flip) & hold, (x.y ^ flip) & hold, (x.z ^ flip) & hold, (x.w ^ flip) & hold);
+      }
+      most = max(most, w.hi[n]);
+      if (in) least = min(least, w.hi[n]);
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      most = max(most, __shfl_xor(most, x));
+      least = min(least, __shfl_xor(least, x));
+    }
+    w.most = uniform(most);
+    w.least = uniform(least);
+    if (lane == 0) ends[wave] = most;
+    __syncthreads();
+    w.end = 0;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) w.end = max(w.end, uniform(ends[k]));
+    const int tiles = (shared + WIDE_KEYS - 1) / WIDE_KEYS, seen = (w.end + WIDE_KEYS - 1) / WIDE_KEYS, k = uniform(mine.part), of = uniform(mine.parts);
+    const bool nan = w.template pass<CAREFUL>(int(long(tiles) * k / of), min(seen, int(long(tiles) * (k + 1) / of)), scale);
+    if (!CAREFUL && nan) return true;
+    float* part = part_at(workspace, parts, uniform(mine.id), R);
+#pragma unroll
+    for (int n = 0; n < M; ++n) {
+      const float sum = over_two(w.l[n], [](float x, float y) { return x + y; });
+      const bool some = over_two(w.some[n] ? 1.f : 0.f, most_of) > 0.f;
+      if (join) {
+        const int column = (wave * QT + first + n) * 32 + (lane & 31);
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(part + column * 64 + dt * 32 + 8 * k + 4 * g) =
+                make_float4(w.o[n][dt][4 * k], w.o[n][dt][4 * k + 1], w.o[n][dt][4 * k + 2], w.o[n][dt][4 * k + 3]);
+        if (g == 0) *reinterpret_cast<float2*>(part + R * 64 + column * 2) = make_float2((w.r[n] - w.TOP) * 0.693147180559945309f, some ? sum : -1.f);
+      } else if (head[n] >= 0) {
+        const float inv = 1.f / sum;
+        T* out = static_cast<T*>(a.out) + long(token[n]) * a.ldo + long(head[n]) * 64 + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = some ? w.o[n][dt][4 * k + e] * inv : 0.f;
+            *reinterpret_cast<uint2*>(out + dt * 32 + 8 * k) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+          }
+      }
+    }
+    return false;
+  };
+  if (!columns(std::integral_constant<int, QT>(), std::false_type(), 0)) return;
+#pragma unroll 1
+  for (int n = 0; n < QT; ++n) {
+    __syncthreads();  // `ends` is read
+    columns(std::integral_constant<int, 1>(), std::true_type(), n);
+  }
 }
 
 // --- the join -----------------------------------------------------------------------------------
 
 // One wave a (token, head): a channel a lane, AT_ONCE parts under way.
 constexpr int JOIN_WAVES = 4, AT_ONCE = 8;
-template <typename T, int R>
-__global__ void __launch_bounds__(JOIN_WAVES * 64) prefix_join_kernel(const PrefixArgs a, int own, size_t parts, size_t own_parts, char* workspace) {
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WAVES * 64) prefix_join_kernel(const PrefixArgs a, int R, int own, size_t parts, size_t own_parts, char* workspace) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int u = int(blockIdx.x) * JOIN_WAVES + wave;  // below 2^21
   if (u >= a.n * a.heads || !reinterpret_cast<const PlanHead*>(workspace)->valid) return;
@@ -499,9 +892,18 @@ void prefix_attention(const Exec& ex, const PrefixArgs& args, void* workspace, s
   char* ws = static_cast<char*>(workspace);
   by_type(c.dt, [&](auto t) {
     using T = decltype(t);
-    prefix_parts_kernel<T, 1><<<int(plan.blocks + own), WAVES * 64, 0, ex.stream>>>(a, plan.blocks, plan.own, plan.join, plan.parts, plan.own_parts, ws);
+    auto launch = [&](auto kernel) {
+      kernel<<<int(plan.blocks + own), WAVES * 64, 0, ex.stream>>>(a, plan.blocks, plan.own, plan.join, plan.parts, plan.own_parts, ws);
+    };
+    if constexpr (sizeof(T) == 2) {
+      if (plan.rows == 256) launch(prefix_wide_kernel<T, 2>);
+      if (plan.rows == 128) launch(prefix_wide_kernel<T, 1>);
+    }
+    if (plan.rows == 64) launch(prefix_parts_kernel<T, 4>);
+    if (plan.rows == 32) launch(prefix_parts_kernel<T, 2>);
+    if (plan.rows == 16) launch(prefix_parts_kernel<T, 1>);
     if (plan.join)
-      prefix_join_kernel<T, 16><<<cdiv(long(a.n) * a.heads, JOIN_WAVES), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.own, plan.parts, plan.own_parts, ws);
+      prefix_join_kernel<T><<<cdiv(long(a.n) * a.heads, JOIN_WAVES), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.rows, plan.own, plan.parts, plan.own_parts, ws);
   });
   SPLAT_HIP(hipGetLastError());
 }
