@@ -505,17 +505,17 @@ PrefixPlan prefix_plan(const PrefixArgs& a) {
   const int G = a.heads / c.kv_heads, small = c.dt == 0 ? 16 : 32;
   const long each = (long(a.n) * G + a.groups - 1) / a.groups;  // rows of a group and key head, if all are alike
   plan.rows = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 || c.dt == 0 ? 64 : each <= 128 ? 128 : 256;
-  const int keys = plan.rows >= 128 ? 64 : small, waves = plan.rows >= 128 ? 1 : 4;  // that take tiles of their own
+  const int keys = plan.rows >= 128 ? 64 : small, waves = plan.rows >= 128 ? 2 : 4;  // that take tiles of their own (two tiles deep in the wide form)
   const long items = most_items(a.n, G, a.groups, plan.rows) * c.kv_heads, tiles = (a.max_shared + keys - 1) / keys;
   // blocks for so many parts of an item that the chip's rounds of blocks end full, or as many as there are, of two tiles a wave at least
-  const long most = std::max<long>(1, tiles / (2 * waves));
+  const long most = std::max<long>(1, tiles / (2 * waves)), round = MORE_BLOCKS;
   long blocks = items;
-  if (items < MORE_BLOCKS) {
-    blocks = std::max(items, std::min<long>(MORE_BLOCKS, items * most));
+  if (items < round) {
+    blocks = std::max(items, std::min<long>(round, items * most));
   } else {
     double best = 1e30;
     for (long p = 1; p <= std::min<long>(4, most); ++p) {
-      const double cost = double((items * p + MORE_BLOCKS - 1) / MORE_BLOCKS) / p * (1 + 0.03 * (p - 1));
+      const double cost = double((items * p + round - 1) / round) / p * (1 + 0.03 * (p - 1));
       if (items * p <= items + MORE_BLOCKS * 4 && cost < best) {
         best = cost;
         blocks = items * p;

@@ -306,11 +306,11 @@ struct Mine {
 // Thread t sums up its k groups; block 0 leaves the plan for the join. The tiles of a part: as few as leave no more parts than
 // blocks. all tiles / blocks is tried first, which fits where the groups are alike; an item of T tiles has at most T / each + 1 parts,
 // so that all tiles / (blocks - items) always fits.
-template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a, int blocks, char* workspace, bool join) {
-  __shared__ long sums[WAVES];
+template <int KEYS, int R, int NW> __device__ inline Mine find_item(const PrefixArgs& a, int blocks, char* workspace, bool join) {
+  __shared__ long sums[NW];
   __shared__ Mine found;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.heads / a.cache.kv_heads, kv = a.cache.kv_heads;
-  const int k = (a.groups + WAVES * 64 - 1) / (WAVES * 64), g0 = min(tid * k, a.groups), g1 = min(g0 + k, a.groups);
+  const int k = (a.groups + NW * 64 - 1) / (NW * 64), g0 = min(tid * k, a.groups), g1 = min(g0 + k, a.groups);
   auto total_of = [&](long v, long& before) {
     const long s = long(scan_wave(uint64_t(v), uint64_t(0), [](uint64_t x, uint64_t y) { return x + y; }));
     __syncthreads();
@@ -319,7 +319,7 @@ template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a,
     before = s - v;
     long total = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = 0; w < NW; ++w) {
       if (w < wave) before += sums[w];
       total += sums[w];
     }
@@ -369,13 +369,13 @@ template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a,
   return found;
 }
 
-// A token's own positions: the part of block `u` of them.
+// A token's own positions: part `u` of them, by four waves of a block, which all come here.
 template <typename T>
 __device__ inline void own_part(const PrefixArgs& a, int u, int own, size_t own_parts, char* workspace, char* smem, float (*stats)[4]) {
   using Ops = TileOps<T>;
   constexpr int KEYS = Ops::KEYS;
   const KvCache& c = a.cache;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) % WAVES, col = lane & 15, g = lane >> 4;
   const int G = a.heads / c.kv_heads, groups = (G + 15) / 16, cols = c.kv_heads * groups, columns = min(G, 16);
   const int part = u % own, i = u / own / cols, group = u / own % cols, kh = group / groups, h0 = group % groups * 16;
   const int grp = group_of(a, i);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
     own_part<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
     return;
   }
-  const Mine mine = find_item<KEYS, R>(a, blocks, workspace, join);
+  const Mine mine = find_item<KEYS, R, WAVES>(a, blocks, workspace, join);
   if (uniform(mine.id) < 0) return;
   const KvCache& c = a.cache;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, G = a.heads / c.kv_heads;
@@ -460,18 +460,20 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
 
 // --- many rows an item --------------------------------------------------------------------------
 //
-// Four waves of 64 columns share tiles of 64 keys, on the 32x32 matrix instructions: S^T = K Q^T leaves a lane one
-// column (lane % 32) and 16 keys of each 32, which is the second operand of O^T = V^T P^T as it stands. Bound by the matrix
-// instructions and the exponentials that run beside them.
+// Four waves of QT times 32 columns share tiles of 64 keys, on the 32x32 matrix instructions: S^T = K Q^T leaves a lane one
+// column (lane % 32) and 16 keys of each 32, which is the second operand of O^T = V^T P^T as it stands.
+//
+// Bound by the matrix instructions and by the vector unit's work on the scores, about as much of either: so half a tile's products
+// with K and the half before the last one's with V are under way while the half between becomes weights, all in one wave's stream,
+// and two waves share a SIMD.
 //
 // The weights are 2^(c s - r), c = |scale| log2(e), in one fused multiply-add: its one rounding is of the difference, and what r was
-// rounded by is the same for all weights of a column. r follows the largest score, but only when that has grown by 2^SLACK, so that
-// the sums are seldom multiplied. The weights are rounded once to the values' type, where the two terms of the other form would
-// cost half the matrix instructions again; their sum is of the rounded ones, so that what a column's weights have in common cancels.
+// rounded by is the same for all weights of a column. r is the largest score of the first half tile with a key; sums that overflow
+// with it (2^64, in f16 weights of 2^16) are taken again with care. The weights are rounded once to the values' type, where the two
+// terms of the other form would cost half the matrix instructions again; their sum is of the rounded ones, so that what a column's
+// weights have in common cancels.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
 
 template <typename T> __device__ inline f32x16 mma32(const uint4& a, const uint4& b, const f32x16& c) {
   if constexpr (std::is_same<T, bf16>::value)
@@ -480,6 +482,8 @@ template <typename T> __device__ inline f32x16 mma32(const uint4& a, const uint4
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_v, a), __builtin_bit_cast(f16x8_v, b), c, 0, 0, 0);
 }
 // acc + both values of a packed pair
+typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
 template <typename T> __device__ inline float add_pair(uint32_t pair, float acc) {
   if constexpr (std::is_same<T, bf16>::value)
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pair), __builtin_bit_cast(bf16x2_v, 0x3f803f80u), acc, false);
@@ -497,73 +501,90 @@ constexpr int WIDE_KEYS = 64, WIDE_BYTES = WIDE_KEYS * 256;  // a tile: K, then 
 constexpr int WIDE_RING = 4;
 
 template <typename T, int QT> struct WideWave {
-  static constexpr float SLACK = 8.f;
-  static constexpr float TOP = std::is_same<T, f16>::value ? 7.f : 0.f;  // f16 weights below 2^-14 lose bits: the largest is 2^15
+  // f16 weights below 2^-14 lose bits and 2^16 is beyond them: the first tile's largest weight is 2^4
+  static constexpr float TOP = std::is_same<T, f16>::value ? 4.f : 0.f;
   const KvCache& c;
   const int kh, lane, wave;
-  char* smem;
+  char* ring;
   const int* row;  // of pages
   int width, end;  // positions from `end` on are seen by no column of the block
-  // 64 entries of the row, one a lane: those of the tiles that are loaded now, and the next ones; ok: which are pages
-  int chunk, entries, ahead;
+  // 64 entries of the row, one a lane: where the keys of the pages lie that tiles are loaded from now (ok: which are pages), and the
+  // next entries
+  int chunk, ahead;
+  uint32_t at_lo, at_hi;
   uint64_t ok;
+  uint32_t full;            // bits of a tile's pages
   int hi[QT], most, least;  // of the wave's columns
   uint4 q[QT][4];
   f32x16 o[QT][2];
   float r[QT], l[QT];
-  bool some[QT];  // keys were there
+  int key0;  // the first position of the tiles with a page: a column that sees it has met a key
 
   __device__ inline int load_entries(int k) const { return row[min(long(k) * 64 + lane, long(width) - 1)]; }
-  __device__ inline void begin_entries(int t) {
-    chunk = ((t * WIDE_KEYS) >> c.shift) >> 6;
-    entries = load_entries(chunk);
-    ahead = load_entries(chunk + 1);
-    ok = __ballot(page_ok(entries, c.pages));
+  __device__ inline void take_entries(int k, int these) {
+    chunk = k;
+    asm volatile("" : "+v"(these));  // these are here: the wait for them is not to be one for the next
+    const bool page = page_ok(these, c.pages);
+    const uint64_t at = reinterpret_cast<uint64_t>(static_cast<const T*>(c.k) + (page ? page_at(c, these, kh) : 0));
+    at_lo = uint32_t(at);
+    at_hi = uint32_t(at >> 32);
+    ok = __ballot(page);
+    ahead = load_entries(k + 1);
   }
-  // The tile's pages that are there, a bit each.
-  __device__ inline uint32_t pages_of(int t) const {
-    const int per = max(1, WIDE_KEYS >> c.shift);
-    return uint32_t(ok >> (((t * WIDE_KEYS) >> c.shift) & 63)) & ((1u << per) - 1);
-  }
-  // Asks for this wave's rows of tile t (8 w and 32 + 8 w on) into slot t of the ring; which of the tile's pages are there.
-  __device__ inline uint32_t issue(int t) {
+  // Before tile t is asked for: which of its pages are there, a bit each.
+  __device__ inline uint32_t pages_of(int t) {
     const int place0 = (t * WIDE_KEYS) >> c.shift;
-    if ((place0 >> 6) != chunk) {
-      chunk = place0 >> 6;
-      entries = ahead;
-      ahead = load_entries(chunk + 1);
-      ok = __ballot(page_ok(entries, c.pages));
-    }
-    const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)smem)) + (t % WIDE_RING) * WIDE_BYTES;
+    if ((place0 >> 6) != chunk) take_entries(place0 >> 6, (place0 >> 6) == chunk + 1 ? ahead : load_entries(place0 >> 6));
+    return uint32_t(ok >> (place0 & 63)) & full;
+  }
+  // Asks for this wave's 16 rows of tile t (16 w on), which lie in PIECES pages, into slot b of the ring. What is behind `end` reads as zeros.
+  template <int PIECES> __device__ inline void ask(int t, int b, uint32_t pages) const {
     const int lrow = lane >> 3;
-    const uint32_t k_off[4] = {uint32_t(lrow * 128 + (((lane & 7) ^ ((4 * (wave & 1) + (lrow >> 1)) & 7)) * 16))};
-    const uint32_t v_off[4] = {uint32_t(lrow * 128 + (((lane & 7) ^ ((lrow & 3) << 1)) * 16))};
+    const uint32_t k_off[4] = {uint32_t(lrow * 128 + (((lane & 7) ^ (lrow >> 1)) * 16)), uint32_t(lrow * 128 + (((lane & 7) ^ (4 + (lrow >> 1))) * 16))};
+    const uint32_t v_off[4] = {uint32_t(lrow * 128 + (((lane & 7) ^ ((lrow & 3) << 1)) * 16)), uint32_t(lrow * 128 + (((lane & 7) ^ ((lrow & 3) << 1)) * 16))};
+    const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)) + b * WIDE_BYTES + wave * 2048;
+    const uint64_t apart = reinterpret_cast<uint64_t>(c.v) - reinterpret_cast<uint64_t>(c.k);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int piece = i * WAVES + wave, first = t * WIDE_KEYS + piece * 8;
-      const int page = __builtin_amdgcn_readlane(entries, (first >> c.shift) & 63);
-      const int rows = page_ok(page, c.pages) ? max(0, min(8, end - first)) : 0;
-      const long at = (rows ? page_at(c, page, kh) : 0) + (first & (c.page_size - 1)) * 64;
-      load_lds<1>(static_cast<const T*>(c.k) + at, rows * 128, k_off, 0, lds + piece * 1024);
-      load_lds<1>(static_cast<const T*>(c.v) + at, rows * 128, v_off, 0, lds + WIDE_BYTES / 2 + piece * 1024);
+    for (int i = 0; i < PIECES; ++i) {
+      const int first = t * WIDE_KEYS + 16 * wave + 8 * i, from = first >> c.shift;
+      int rows = 16 / PIECES;
+      if (pages != full || first + rows > end) {
+        const int here = c.page_size < WIDE_KEYS ? (16 * wave + 8 * i) >> c.shift : 0;
+        rows = pages >> here & 1 ? uniform(max(0, min(rows, end - first))) : 0;
+      }
+      uint64_t k = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(at_hi), from & 63))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(at_lo), from & 63));
+      k += (first & (c.page_size - 1)) * 128;
+      load_lds<2 / PIECES>(reinterpret_cast<const void*>(k), rows * 128, k_off, i, lds + i * 1024);
+      load_lds<2 / PIECES>(reinterpret_cast<const void*>(k + apart), rows * 128, v_off, i, lds + WIDE_BYTES / 2 + i * 1024);
     }
-    return pages_of(t);
+  }
+  __device__ inline uint32_t issue(int t) {
+    const uint32_t pages = pages_of(t);
+    if (c.page_size >= 16) ask<1>(t, t % WIDE_RING, pages);
+    else ask<2>(t, t % WIDE_RING, pages);
+    return pages;
   }
 
-  // V^T of 16 keys from 32 kt + 16 hh on and channels 32 dt on, in the order of the weights (as in TileOps, for 32 rows of output).
-  __device__ inline uint4 values(const char* vt, int kt, int hh, int dt) const {
+  // V^T of 16 keys from 32 half + 16 hh on and channels 32 dt on, in the order of the weights (as in TileOps, for 32 rows of output).
+  __device__ inline uint4 values(int b, int half, int hh, int dt) const {
     typedef short v4s __attribute__((ext_vector_type(4)));
+    const char* vt = ring + b * WIDE_BYTES + WIDE_BYTES / 2;
     const int G = lane >> 4, j = (lane >> 2) & 3, cc = lane & 3;
     const int at = (4 * (G >> 1) + j) * 128 + (((4 * dt + 2 * (G & 1) + (cc >> 1)) ^ (j << 1)) * 16) + (cc & 1) * 8;
     uint32_t w[4];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)((lds_cptr)(vt + (kt * 32 + 16 * hh + 8 * half) * 128 + at)));
+    for (int e = 0; e < 2; ++e) {
+      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)((lds_cptr)(vt + (half * 32 + 16 * hh + 8 * e) * 128 + at)));
       const uint2 u = __builtin_bit_cast(uint2, x);
-      w[2 * half] = u.x;
-      w[2 * half + 1] = u.y;
+      w[2 * e] = u.x;
+      w[2 * e + 1] = u.y;
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // K of 32 keys from 32 half on and 16 channels from 16 st on.
+  __device__ inline uint4 keys(int b, int half, int st) const {
+    const int g = lane >> 5, l32 = lane & 31, sw = (l32 >> 1) & 7;
+    return *reinterpret_cast<const uint4*>(ring + b * WIDE_BYTES + (half * 32 + l32) * 128 + ((2 * st + g) ^ sw) * 16);
   }
   template <typename F> __device__ static inline uint4 map_pairs(const uint4& v, F&& fn) {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -573,173 +594,248 @@ template <typename T, int QT> struct WideWave {
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 
-  template <bool CAREFUL> __device__ inline void tile(int t, uint32_t pages, float scale) {
-    const char* kt = smem + (t % WIDE_RING) * WIDE_BYTES;
-    const char* vt = kt + WIDE_BYTES / 2;
-    const int g = lane >> 5, l32 = lane & 31, first = t * WIDE_KEYS, sw = (l32 >> 1) & 7;
-    f32x16 s[QT][2];
+  // Half a tile: scores, weights.
+  struct Scores { f32x16 s[QT]; };
+  struct Weights { uint32_t p[QT][8]; };
+  __device__ inline void score(Scores& x, const uint4 (&kf)[4]) const {
     const f32x16 zero = {};
-    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2)
+    for (int st = 0; st < 4; ++st)
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        const uint4 kf = *reinterpret_cast<const uint4*>(kt + (k2 * 32 + l32) * 128 + ((2 * st + g) ^ sw) * 16);
-#pragma unroll
-        for (int n = 0; n < QT; ++n) s[n][k2] = mma32<T>(kf, q[n][st], st == 0 ? zero : s[n][k2]);
-      }
-    __builtin_amdgcn_s_setprio(0);
-    const uint32_t all = (1u << max(1, WIDE_KEYS >> c.shift)) - 1;
-    const bool edge = pages != all || first + WIDE_KEYS > least;
-    auto seen = [&](int n, int k2, int x) {
-      const int key = k2 * 32 + 8 * (x >> 2) + 4 * g + (x & 3), place = ((first & (c.page_size - 1)) + k2 * 32 + 8 * (x >> 2)) >> c.shift;
-      return first + key < hi[n] && (pages >> place & 1);
-    };
-    if (edge) {
-      asm volatile("");  // a branch: as selections these would be a hundred instructions in every tile
-#pragma unroll
-      for (int n = 0; n < QT; ++n)
-#pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const bool sees = seen(n, k2, x);
-            some[n] |= sees;
-            if (!sees) s[n][k2][x] = -INFINITY;
-          }
-    } else {
-#pragma unroll
-      for (int n = 0; n < QT; ++n) some[n] = true;
-    }
-    bool grow = false;
-    float top[QT];
+      for (int n = 0; n < QT; ++n) x.s[n] = mma32<T>(kf[st], q[n][st], st == 0 ? zero : x.s[n]);
+  }
+  __device__ inline void weights(Weights& w, const Scores& x, float scale, const float (&ref)[QT]) {
 #pragma unroll
     for (int n = 0; n < QT; ++n) {
-      float m[11];
+      float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < 10; ++k) {
-        const int e = 3 * k;
-        m[k] = most_of(most_of(s[n][e >> 4][e & 15], s[n][(e + 1) >> 4][(e + 1) & 15]), s[n][(e + 2) >> 4][(e + 2) & 15]);
+      for (int e = 0; e < 8; ++e) {
+        const float a = __builtin_amdgcn_exp2f(fmaf(x.s[n][2 * e], scale, ref[n])), b = __builtin_amdgcn_exp2f(fmaf(x.s[n][2 * e + 1], scale, ref[n]));
+        w.p[n][e] = pack2<T>(a, b);
+        sum = add_pair<T>(w.p[n][e], sum);
       }
-      m[10] = most_of(s[n][1][14], s[n][1][15]);
-      const float a = most_of(most_of(m[0], m[1]), m[2]), b = most_of(most_of(m[3], m[4]), m[5]), d = most_of(most_of(m[6], m[7]), m[8]);
-      const float mx = over_two(most_of(most_of(most_of(a, b), d), most_of(m[9], m[10])), most_of) * scale;
-      top[n] = mx > r[n] + SLACK ? mx : r[n];
-      grow |= top[n] != r[n];
+      l[n] += sum;
     }
-    if (__builtin_amdgcn_ballot_w64(grow)) {
+  }
+  __device__ inline void weigh(const Weights& w, const uint4 (&vf)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int n = 0; n < QT; ++n) {
-        const float keep = r[n] == top[n] ? 1.f : __builtin_amdgcn_exp2f(r[n] - top[n]);
-        l[n] *= keep;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          o[n][0][x] *= keep;
-          o[n][1][x] *= keep;
-        }
-        r[n] = top[n];
+        const uint32_t* p = w.p[n] + 4 * (k >> 1);
+        o[n][k & 1] = mma32<T>(vf[k], make_uint4(p[0], p[1], p[2], p[3]), o[n][k & 1]);
       }
-    }
-    uint32_t p[QT][2][8];
+  }
+  __device__ inline void load_keys(uint4 (&kf)[4], int b, int half) const {
 #pragma unroll
-    for (int n = 0; n < QT; ++n) {
-      const float ref = TOP - (r[n] == -INFINITY ? 0.f : r[n]);
+    for (int st = 0; st < 4; ++st) kf[st] = keys(b, half, st);
+  }
+  __device__ inline void load_values(uint4 (&vf)[4], int b, int half) const {
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float a = __builtin_amdgcn_exp2f(fmaf(s[n][k2][2 * x], scale, ref)), b = __builtin_amdgcn_exp2f(fmaf(s[n][k2][2 * x + 1], scale, ref));
-          p[n][k2][x] = pack2<T>(a, b);
-          l[n] = add_pair<T>(p[n][k2][x], l[n]);
-        }
-    }
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          uint4 vf = values(vt, k2, hh, dt);
-          if constexpr (CAREFUL) {
-            // infinities and NaN count where they are seen and nowhere else: how many of each kind a column sees
-            const uint4 raw = vf;
-            vf = map_pairs(raw, [](float y) { return fabsf(y) < INFINITY ? y : 0.f; });
-#pragma unroll
-            for (int n = 0; n < QT; ++n) {
-              uint32_t one[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                one[k] = pack2<T>(seen(n, k2, 8 * hh + 2 * k) ? 1.f : 0.f, seen(n, k2, 8 * hh + 2 * k + 1) ? 1.f : 0.f);
-              const uint4 sees = make_uint4(one[0], one[1], one[2], one[3]);
-              const f32x16 none = mma32<T>(map_pairs(raw, [](float y) { return y != y ? 1.f : 0.f; }), sees, zero);
-              const f32x16 up = mma32<T>(map_pairs(raw, [](float y) { return y == INFINITY ? 1.f : 0.f; }), sees, zero);
-              const f32x16 down = mma32<T>(map_pairs(raw, [](float y) { return y == -INFINITY ? 1.f : 0.f; }), sees, zero);
-#pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                if (none[x] > 0.f) o[n][dt][x] = NAN;
-                if (up[x] > 0.f) o[n][dt][x] += INFINITY;
-                if (down[x] > 0.f) o[n][dt][x] -= INFINITY;
-              }
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < QT; ++n)
-            o[n][dt] = mma32<T>(vf, make_uint4(p[n][k2][4 * hh], p[n][k2][4 * hh + 1], p[n][k2][4 * hh + 2], p[n][k2][4 * hh + 3]), o[n][dt]);
-        }
-    __builtin_amdgcn_s_setprio(0);
+    for (int k = 0; k < 4; ++k) vf[k] = values(b, half, k >> 1, k & 1);
   }
 
-  // Tiles t0 up to t1, asked for three ahead. The barrier of a tile says that its loads have come, all waves', and that the
-  // tile before it is used up, into whose slot the next load goes.
+  // The largest score of column n, times scale.
+  __device__ inline float largest(const Scores& x, int n, float scale) const {
+    const f32x16& s = x.s[n];
+    float m = most_of(most_of(s[0], s[1]), s[2]);
+#pragma unroll
+    for (int e = 3; e < 15; e += 2) m = most_of(most_of(m, s[e]), s[e + 1]);
+    return over_two(most_of(m, s[15]), most_of) * scale;
+  }
+  // Keys of half a tile from position `first` on (a multiple of 32): those of the four groups of 8 in one page that column n sees, counted
+  // from the lane's own of the group on.
+  __device__ inline int limit(int n, int first, uint32_t pages, int group) const {
+    const int at = (first & (WIDE_KEYS - 1)) + group * 8, bit = c.page_size < WIDE_KEYS ? at >> c.shift : 0;
+    return pages >> bit & 1 ? hi[n] - first - 4 * (lane >> 5) - 8 * group : -WIDE_KEYS;
+  }
+
+  // Half a tile by itself: keys that not all columns see, and columns whose reference is not there yet. CAREFUL: the reference follows
+  // the largest score, and infinities and NaN among the values count where they are seen and nowhere else.
+  template <bool CAREFUL> __device__ inline void half_tile(int t, int half, uint32_t pages, float scale, float (&ref)[QT]) {
+    const int b = t % WIDE_RING, first = t * WIDE_KEYS + half * 32;
+    uint4 kf[4], vf[4];
+    Scores x;
+    Weights w;
+    load_keys(kf, b, half);
+    score(x, kf);
+    load_values(vf, b, half);
+#pragma unroll
+    for (int n = 0; n < QT; ++n) {
+#pragma unroll
+      for (int x4 = 0; x4 < 4; ++x4) {
+        const int below = limit(n, first, pages, x4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.s[n][4 * x4 + e] = e < below ? x.s[n][4 * x4 + e] : -INFINITY;
+      }
+      const float mx = largest(x, n, scale), top = r[n] == -INFINITY || (CAREFUL && mx > r[n]) ? mx : r[n];
+      if (CAREFUL) {  // where there was none, the sums are zeros
+        const float keep = r[n] == top ? 1.f : __builtin_amdgcn_exp2f(r[n] - top);
+        l[n] *= keep;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          o[n][0][e] *= keep;
+          o[n][1][e] *= keep;
+        }
+      }
+      r[n] = top;
+      ref[n] = TOP - (top == -INFINITY ? 0.f : top);
+    }
+    weights(w, x, scale, ref);
+    if constexpr (CAREFUL) {
+      const f32x16 zero = {};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 raw = vf[k];
+        vf[k] = map_pairs(raw, [](float y) { return fabsf(y) < INFINITY ? y : 0.f; });
+#pragma unroll
+        for (int n = 0; n < QT; ++n) {  // how many of each other kind the column sees
+          uint32_t one[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int below = limit(n, first, pages, 2 * (k >> 1) + e / 2) - 2 * (e & 1);
+            one[e] = pack2<T>(below > 0 ? 1.f : 0.f, below > 1 ? 1.f : 0.f);
+          }
+          const uint4 sees = make_uint4(one[0], one[1], one[2], one[3]);
+          const f32x16 none = mma32<T>(map_pairs(raw, [](float y) { return y != y ? 1.f : 0.f; }), sees, zero);
+          const f32x16 up = mma32<T>(map_pairs(raw, [](float y) { return y == INFINITY ? 1.f : 0.f; }), sees, zero);
+          const f32x16 down = mma32<T>(map_pairs(raw, [](float y) { return y == -INFINITY ? 1.f : 0.f; }), sees, zero);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (none[e] > 0.f) o[n][k & 1][e] = NAN;
+            if (up[e] > 0.f) o[n][k & 1][e] += INFINITY;
+            if (down[e] > 0.f) o[n][k & 1][e] -= INFINITY;
+          }
+        }
+      }
+    }
+    weigh(w, vf);
+  }
+
+  // Weights are taken here, not where they are used first: that is behind the next barrier.
+  __device__ inline void pin(Weights& w) {
+#pragma unroll
+    for (int n = 0; n < QT; ++n) asm volatile("" : "+v"(l[n]));
+#pragma unroll
+    for (int n = 0; n < QT; ++n)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) asm volatile("" : "+v"(w.p[n][e]), "+v"(w.p[n][e + 1]), "+v"(w.p[n][e + 2]), "+v"(w.p[n][e + 3]));
+  }
+  // Beside the 8 QT matrix instructions of half a tile: its share of the vector unit's work between each two.
+  __device__ static inline void interleave() {
+#pragma unroll
+    for (int k = 0; k < 8 * QT; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+    }
+  }
+
+  // Tiles t0 up to t1. True where the sums are not to be taken: a NaN, an infinity, or weights beyond 2^64.
   template <bool CAREFUL> __device__ inline bool pass(int t0, int t1, float scale) {
+    float ref[QT];
 #pragma unroll
     for (int n = 0; n < QT; ++n) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) o[n][0][x] = o[n][1][x] = 0.f;
       r[n] = -INFINITY;
       l[n] = 0.f;
-      some[n] = false;
+      ref[n] = 0.f;
     }
-    uint32_t pages[WIDE_RING - 1] = {};  // of the tiles under way
-    if (t0 < t1) begin_entries(t0);
-#pragma unroll
-    for (int k = 0; k < WIDE_RING - 1; ++k)
-      if (t0 + k < t1) pages[k] = issue(t0 + k);
-#pragma unroll 1
-    for (int t = t0; t < t1; ++t) {
-      // four loads a tile of this wave
-      if (t + 2 < t1) wait_loads<8>();
-      else if (t + 1 < t1) wait_loads<4>();
+    key0 = 0x7fffffff;
+    full = (1u << max(1, WIDE_KEYS >> c.shift)) - 1;
+    uint32_t pages = 0, pages1 = 0, pages2 = 0;  // of tiles t, t + 1, t + 2
+    if (t0 < t1) {
+      const int k = ((t0 * WIDE_KEYS) >> c.shift) >> 6;
+      take_entries(k, load_entries(k));
+      pages1 = issue(t0);
+      if (t0 + 1 < t1) pages2 = issue(t0 + 1);
+    }
+    // Tile t is there, all waves' loads, and tile t - 2 used up: its slot is tile t + 2's.
+    auto arrive = [&](int t) {
+      if (t + 1 < t1) wait_loads<4>();  // of this wave for tile t + 1
       else wait_loads<0>();
       asm volatile("s_barrier" ::: "memory");
-      const uint32_t now = pages[0];
+      pages = pages1;
+      pages1 = pages2;
+      if (t + 2 < t1) pages2 = issue(t + 2);
+    };
+    auto plain = [&](int t, uint32_t there) {  // all columns see all of tile t
+      bool none = false;
 #pragma unroll
-      for (int k = 0; k + 1 < WIDE_RING - 1; ++k) pages[k] = pages[k + 1];
-      if (t + WIDE_RING - 1 < t1) pages[WIDE_RING - 2] = issue(t + WIDE_RING - 1);
-      if (t * WIDE_KEYS < most) tile<CAREFUL>(t, now, scale);
+      for (int n = 0; n < QT; ++n) none |= r[n] == -INFINITY && hi[n] > 0;
+      return !CAREFUL && there == full && (t + 1) * WIDE_KEYS <= least && !__builtin_amdgcn_ballot_w64(none);
+    };
+    int t = t0;
+    if (t < t1) arrive(t);
+#pragma unroll 1
+    while (t < t1) {
+      if (!plain(t, pages)) {
+        if (t * WIDE_KEYS < most) {
+          if (pages && key0 == 0x7fffffff) key0 = t * WIDE_KEYS + (__builtin_ctz(pages) << c.shift);
+          half_tile<CAREFUL>(t, 0, pages, scale, ref);
+          half_tile<CAREFUL>(t, 1, pages, scale, ref);
+        }
+        if (++t < t1) arrive(t);
+        continue;
+      }
+      if constexpr (!CAREFUL) {
+        // the first half's scores, and weights of 0 in the place of the half before it
+        Scores sa, sb;
+        Weights pa, pb = {};
+        uint4 kf[4], vf[4];
+        load_keys(kf, t % WIDE_RING, 0);
+        load_values(vf, t % WIDE_RING, 0);
+        score(sa, kf);
+        bool more;
+#pragma unroll 1
+        do {
+          const int b = t % WIDE_RING;
+          load_keys(kf, b, 1);
+          weigh(pb, vf);
+          weights(pa, sa, scale, ref);
+          load_values(vf, b, 0);
+          score(sb, kf);
+          interleave();
+          pin(pa);
+          more = ++t < t1;
+          if (more) {
+            arrive(t);
+            more = plain(t, pages);
+          }
+          load_keys(kf, (b + 1) % WIDE_RING, 0);  // where that is no plain tile, keys long used: its scores are not
+          weigh(pa, vf);
+          weights(pb, sb, scale, ref);
+          load_values(vf, b, 1);
+          score(sa, kf);
+          interleave();
+          pin(pb);
+        } while (more);
+        weigh(pb, vf);
+      }
     }
-    bool nan = false;
+    bool bad = false;
 #pragma unroll
-    for (int n = 0; n < QT; ++n)
+    for (int n = 0; n < QT; ++n) {
+      bad |= !(l[n] <= 18446744073709551616.f);
 #pragma unroll
-      for (int x = 0; x < 16; ++x) nan |= o[n][0][x] != o[n][0][x] || o[n][1][x] != o[n][1][x];
-    return __syncthreads_or(nan && most > 0);
+      for (int x = 0; x < 16; ++x) bad |= !(fabsf(o[n][0][x]) < INFINITY) || !(fabsf(o[n][1][x]) < INFINITY);
+    }
+    return __syncthreads_or(bad && most > 0);
   }
 };
 
 template <typename T, int QT>
 __global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const PrefixArgs a, int blocks, int own, bool join, size_t parts, size_t own_parts, char* workspace) {
   constexpr int R = WAVES * QT * 32;
-  __shared__ __attribute__((aligned(1024))) char smem[WAVES * RING * TILE_BYTES];
-  static_assert(sizeof(smem) >= WIDE_RING * WIDE_BYTES, "the ring");
+  __shared__ __attribute__((aligned(1024))) char smem[WIDE_RING * WIDE_BYTES];
+  static_assert(sizeof(smem) >= WAVES * RING * TILE_BYTES, "the rings of a token's own positions");
   __shared__ float stats[WAVES * 16][4];
   __shared__ int ends[WAVES];
   if (int(blockIdx.x) >= blocks) {
     own_part<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
     return;
   }
-  const Mine mine = find_item<WIDE_KEYS, R>(a, blocks, workspace, join);
+  const Mine mine = find_item<WIDE_KEYS, R, WAVES>(a, blocks, workspace, join);
   if (uniform(mine.id) < 0) return;
   const KvCache& c = a.cache;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 5, G = a.heads / c.kv_heads;
@@ -753,15 +849,16 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const Prefix
     constexpr int M = decltype(count)::value;
     constexpr bool CAREFUL = decltype(careful)::value;
     WideWave<T, M> w{c, kh, lane, wave, smem, row, a.prefix_width};
-    int most = 0, least = 0x7fffffff, token[M], head[M];
+    int most = 0, least = 0x7fffffff;
+    // the row of a column of this lane, which is asked for again when the sums are there: kept, it would cost registers meanwhile
+    auto row_of = [&](int n, int ln) { return item * R + (wave * QT + first + n) * 32 + (ln & 31); };
 #pragma unroll
     for (int n = 0; n < M; ++n) {
-      const int r = item * R + (wave * QT + first + n) * 32 + (lane & 31);
+      const int r = row_of(n, lane);
       const bool in = r < rows;
-      token[n] = start + (in ? r / G : 0);
-      head[n] = in ? kh * G + r % G : -1;
-      w.hi[n] = in ? max(0, min(a.lens ? a.lens[token[n]] : shared, shared)) : 0;
-      const T* q = static_cast<const T*>(a.q) + long(token[n]) * a.ldq + long(max(head[n], 0)) * 64;
+      const int token = start + (in ? r / G : 0);
+      w.hi[n] = in ? max(0, min(a.lens ? a.lens[token] : shared, shared)) : 0;
+      const T* q = static_cast<const T*>(a.q) + long(token) * a.ldq + long(kh * G + (in ? r % G : 0)) * 64;
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         const uint4 x = in ? *reinterpret_cast<const uint4*>(q + st * 16 + g * 8) : make_uint4(0, 0, 0, 0);
@@ -783,13 +880,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const Prefix
 #pragma unroll
     for (int k = 0; k < WAVES; ++k) w.end = max(w.end, uniform(ends[k]));
     const int tiles = (shared + WIDE_KEYS - 1) / WIDE_KEYS, seen = (w.end + WIDE_KEYS - 1) / WIDE_KEYS, k = uniform(mine.part), of = uniform(mine.parts);
-    const bool nan = w.template pass<CAREFUL>(int(long(tiles) * k / of), min(seen, int(long(tiles) * (k + 1) / of)), scale);
-    if (!CAREFUL && nan) return true;
+    const bool bad = w.template pass<CAREFUL>(int(long(tiles) * k / of), min(seen, int(long(tiles) * (k + 1) / of)), scale);
+    if (!CAREFUL && bad) return true;
     float* part = part_at(workspace, parts, uniform(mine.id), R);
 #pragma unroll
     for (int n = 0; n < M; ++n) {
       const float sum = over_two(w.l[n], [](float x, float y) { return x + y; });
-      const bool some = over_two(w.some[n] ? 1.f : 0.f, most_of) > 0.f;
       if (join) {
         const int column = (wave * QT + first + n) * 32 + (lane & 31);
 #pragma unroll
@@ -798,17 +894,21 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const Prefix
           for (int k = 0; k < 4; ++k)
             *reinterpret_cast<float4*>(part + column * 64 + dt * 32 + 8 * k + 4 * g) =
                 make_float4(w.o[n][dt][4 * k], w.o[n][dt][4 * k + 1], w.o[n][dt][4 * k + 2], w.o[n][dt][4 * k + 3]);
-        if (g == 0) *reinterpret_cast<float2*>(part + R * 64 + column * 2) = make_float2((w.r[n] - w.TOP) * 0.693147180559945309f, some ? sum : -1.f);
-      } else if (head[n] >= 0) {
+        if (g == 0) *reinterpret_cast<float2*>(part + R * 64 + column * 2) = make_float2((w.r[n] - w.TOP) * 0.693147180559945309f, w.hi[n] > w.key0 ? sum : -1.f);
+        continue;
+      }
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      if (const int r = row_of(n, ln); r < rows) {
         const float inv = 1.f / sum;
-        T* out = static_cast<T*>(a.out) + long(token[n]) * a.ldo + long(head[n]) * 64 + 4 * g;
+        T* out = static_cast<T*>(a.out) + long(start + r / G) * a.ldo + long(kh * G + r % G) * 64 + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = some ? w.o[n][dt][4 * k + e] * inv : 0.f;
+            for (int e = 0; e < 4; ++e) v[e] = w.hi[n] > w.key0 ? w.o[n][dt][4 * k + e] * inv : 0.f;
             *reinterpret_cast<uint2*>(out + dt * 32 + 8 * k) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
           }
       }
@@ -818,7 +918,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const Prefix
   if (!columns(std::integral_constant<int, QT>(), std::false_type(), 0)) return;
 #pragma unroll 1
   for (int n = 0; n < QT; ++n) {
-    __syncthreads();  // `ends` is read
+    __syncthreads();  // `ends` and the rings are read
     columns(std::integral_constant<int, 1>(), std::true_type(), n);
   }
 }

@@ -245,10 +245,12 @@ def test_large_scores(ctx, dtype, members):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("members", [5, 150])
 def test_infinities_and_nan_count_where_they_are_seen(ctx, dtype, members):
-    """Values of positions that some tokens see and others do not; a NaN query."""
+    """Values of positions that some tokens see and others do not; a NaN query. What they do not reach stays within the bound of
+    the file's head, whose sum A is over values that nearly cancel: two results within it differ by up to twice the bound, which
+    a step of the output's type can be far below."""
     sees = [(53 * i) % 301 for i in range(members)]
     s = Shared(dtype, [members], [300], None, 4, 2, 16, sees=sees)
-    clean = s.run(ctx)
+    clean, refs = s.run(ctx), [s.ref(i) for i in range(members)]
     marks = {17: float("inf"), 100: float("nan"), 160: -float("inf"), 161: float("inf"), 299: float("nan")}
     for p, x in marks.items():
         s.v[int(s.prefix[0, p // 16])].view(s.kv, 16, 64)[1, p % 16, 3 * (p % 5)] = x
@@ -258,16 +260,17 @@ def test_infinities_and_nan_count_where_they_are_seen(ctx, dtype, members):
     for i, v in enumerate(sees):
         for c in range(64):
             x = [m for p, m in marks.items() if p < v and 3 * (p % 5) == c]
-            got, was = out[i, 2:, c].float(), clean[i, 2:, c].float()
+            got = out[i, 2:, c].float()
             if not x:
-                assert (got - was).abs().max() <= 2 * torch.finfo(TDT[dtype]).eps * max(1e-3, float(was.abs().max())), (i, c)
+                ref, tol = (r[1, :, c] for r in refs[i])
+                assert ((got.double() - ref).abs() <= tol).all(), (i, c)
             elif any(m != m for m in x) or (float("inf") in x and -float("inf") in x):
                 assert torch.isnan(got).all(), (i, c)
             else:
                 assert (got == x[0]).all(), (i, c)
     # keys: NaN where a token sees one, nobody else
     t = Shared(dtype, [members], [300], None, 4, 2, 16, sees=sees)
-    clean = t.run(ctx).view(members, 4, 64)
+    refs = [t.ref(i) for i in range(members)]
     t.k[int(t.prefix[0, 200 // 16])].view(t.kv, 16, 64)[0, 200 % 16, 5] = float("nan")
     t.q[2, 2 * 64 + 7] = float("nan")
     out = t.run(ctx).view(members, 4, 64)
@@ -276,7 +279,8 @@ def test_infinities_and_nan_count_where_they_are_seen(ctx, dtype, members):
             if v and (h < 2 and v > 200 or (i, h) == (2, 2)):
                 assert torch.isnan(out[i, h]).all(), (i, h)
             else:
-                assert (out[i, h].float() - clean[i, h].float()).abs().max() <= 2 * torch.finfo(TDT[dtype]).eps * max(1e-3, float(clean[i, h].float().abs().max()))
+                ref, tol = (r.view(4, 64)[h] for r in refs[i])
+                assert ((out[i, h].double() - ref).abs() <= tol).all(), (i, h)
 
 
 def test_offsets_past_32_bits(ctx):
