@@ -486,9 +486,9 @@ void check_prefix_attention(PrefixArgs& a, const void* workspace, size_t bytes) 
 }
 
 namespace {
-constexpr int WIDE_ROWS = 256;    // the most of an item
-constexpr int MORE_BLOCKS = 512;  // that cut items' tiles: two on each of 256 CUs
-constexpr long OWN_BLOCKS = 1024; // of the tokens' own positions, up to which these are cut
+constexpr int WIDE_ROWS = 128;     // the most of an item
+constexpr int WIDE_BLOCKS = 512, NARROW_BLOCKS = 256;  // that cut items' tiles: two of the wide form on each of 256 CUs, one of the others
+constexpr long OWN_BLOCKS = 1024;  // of the tokens' own positions, up to which these are cut
 
 // Items of one key head, at most: every group's rows are cut into items of their own.
 long most_items(long n, int G, int groups, int rows) { return n * G / rows + std::min<long>(groups, n); }
@@ -499,31 +499,38 @@ int own_parts(long n, long cols, int max_own, int keys) {
 }
 }  // namespace
 
+// Measured, a call among others, 12 heads, one group and no own positions unless said so. Rows of an item: 16 / 32 / 128 at 16 tokens on 24889
+// positions (bf16) 24.0 / 26.3 / 32.6 us, at 32 28.9 / 26.5 / 31.8, at 48 34.9 / 35.3 / 31.9, at 64 43.8 / 36.1 / 31.6, at 128 92.6 / 56.4 /
+// 32.5; 48 forks of four scenes (32 heads on 8, own positions) 32 rows 43.6, 128 rows 46.9; in fp32 16 / 32 / 64 on 12000 positions at 16 tokens
+// 24.8 / 31.0 / 43.6, at 32 33.1 / 31.5 / 44.0, at 64 52.8 / 46.6 / 44.7, at 256 208 / 168 / 126. Blocks: 256 / 512 of the narrow forms at 16
+// tokens 24.0 / 26.5, 64 forks with a view of their own 44 / 52 (own positions run beside, on each CU's second block); 512 / 1024 of
+// the wide form at 128 tokens 34.6 / 47.8, at 1037 124.8 / 126.0, at 2074 230 / 213.
 PrefixPlan prefix_plan(const PrefixArgs& a) {
   PrefixPlan plan;
   const KvCache& c = a.cache;
   const int G = a.heads / c.kv_heads, small = c.dt == 0 ? 16 : 32;
   const long each = (long(a.n) * G + a.groups - 1) / a.groups;  // rows of a group and key head, if all are alike
-  plan.rows = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 || c.dt == 0 ? 64 : each <= 128 ? 128 : 256;
-  const int keys = plan.rows >= 128 ? 64 : small, waves = plan.rows >= 128 ? 2 : 4;  // that take tiles of their own (two tiles deep in the wide form)
+  plan.rows = each <= 16 ? 16 : c.dt == 0 ? (each <= 32 ? 32 : 64) : each <= 48 ? 32 : WIDE_ROWS;
+  const bool wide = plan.rows == WIDE_ROWS;
+  const int keys = wide ? 64 : small;
+  plan.own = own_parts(a.n, long(c.kv_heads) * ((G + 15) / 16), a.max_own, small);
+  // of an item that is cut, parts of eight tiles at least (two a wave), in the wide form of four
   const long items = most_items(a.n, G, a.groups, plan.rows) * c.kv_heads, tiles = (a.max_shared + keys - 1) / keys;
-  // blocks for so many parts of an item that the chip's rounds of blocks end full, or as many as there are, of two tiles a wave at least
-  const long most = std::max<long>(1, tiles / (2 * waves)), round = MORE_BLOCKS;
+  const long most = std::max<long>(1, tiles / (wide ? 4 : 8)), round = wide && !plan.own ? WIDE_BLOCKS : NARROW_BLOCKS;
   long blocks = items;
   if (items < round) {
     blocks = std::max(items, std::min<long>(round, items * most));
-  } else {
+  } else {  // so many parts of an item that the chip's rounds of blocks end full
     double best = 1e30;
-    for (long p = 1; p <= std::min<long>(4, most); ++p) {
+    for (long p = 1; p <= std::min<long>(4, most) && items * (p - 1) <= 4 * WIDE_BLOCKS; ++p) {
       const double cost = double((items * p + round - 1) / round) / p * (1 + 0.03 * (p - 1));
-      if (items * p <= items + MORE_BLOCKS * 4 && cost < best) {
+      if (cost < best) {
         best = cost;
         blocks = items * p;
       }
     }
   }
   plan.blocks = int(blocks);
-  plan.own = own_parts(a.n, long(c.kv_heads) * ((G + 15) / 16), a.max_own, small);
   plan.join = blocks > items || plan.own > 0;
   if (!plan.join) return plan;
   plan.parts = (16 + a.groups * 16L);
@@ -541,7 +548,7 @@ size_t prefix_attention_bytes(const KvCache& c, int n, int heads, int groups, in
   if (n == 0 || groups == 0) return 0;
   const int G = heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;
   const size_t item = long(n) * heads + std::min<long>(groups, n) * c.kv_heads * WIDE_ROWS;
-  const size_t cut = std::min<size_t>(size_t(MORE_BLOCKS) * 4 * WIDE_ROWS, item * ((max_shared + keys - 1L) / keys));
+  const size_t cut = std::min<size_t>(size_t(WIDE_BLOCKS) * 4 * WIDE_ROWS, item * ((max_shared + keys - 1L) / keys));
   // own parts: one a token and column group, or as many as there are blocks for
   const size_t cols = size_t(c.kv_heads) * ((G + 15) / 16);
   const size_t own = max_own == 0 ? 0 : std::max<size_t>(size_t(n) * heads, size_t(OWN_BLOCKS) / cols * heads);

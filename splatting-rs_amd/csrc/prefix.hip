@@ -303,92 +303,118 @@ struct Mine {
   int start, tokens, shared;
 };
 
-// Thread t sums up its k groups; block 0 leaves the plan for the join. The tiles of a part: as few as leave no more parts than
-// blocks. all tiles / blocks is tried first, which fits where the groups are alike; an item of T tiles has at most T / each + 1 parts,
-// so that all tiles / (blocks - items) always fits.
-template <int KEYS, int R, int NW> __device__ inline Mine find_item(const PrefixArgs& a, int blocks, char* workspace, bool join) {
-  __shared__ long sums[NW];
-  __shared__ Mine found;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.heads / a.cache.kv_heads, kv = a.cache.kv_heads;
-  const int k = (a.groups + NW * 64 - 1) / (NW * 64), g0 = min(tid * k, a.groups), g1 = min(g0 + k, a.groups);
-  auto total_of = [&](long v, long& before) {
-    const long s = long(scan_wave(uint64_t(v), uint64_t(0), [](uint64_t x, uint64_t y) { return x + y; }));
-    __syncthreads();
-    if (lane == 63) sums[wave] = s;
-    __syncthreads();
-    before = s - v;
-    long total = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (w < wave) before += sums[w];
-      total += sums[w];
-    }
-    return total;
+// Every wave for itself, 64 groups at a time, a group a lane: two loads one after the other and no barrier where there are no more of
+// them. Block 0 leaves the plan for the join. The tiles of a part: as few as leave no more parts than blocks. All tiles / blocks is
+// tried first, which fits where the groups are alike; an item of T tiles has at most T / each + 1 parts, so that all tiles /
+// (blocks - items) always fits.
+template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a, int blocks, char* workspace, bool join) {
+  const int lane = threadIdx.x & 63, G = a.heads / a.cache.kv_heads, kv = a.cache.kv_heads, rounds = (a.groups + 63) / 64;
+  struct Group { int start, tokens, shared, items, tiles; };  // items of a key head
+  auto group_at = [&](int k) {
+    const int g = 64 * k + lane, at = min(g, a.groups - 1);
+    Group x;
+    x.start = start_of(a, at);
+    x.tokens = g < a.groups ? max(0, start_of(a, at + 1) - x.start) : 0;
+    x.shared = shared_of(a, at);
+    x.items = (x.tokens * G + R - 1) / R;  // tokens times G are below 2^21
+    x.tiles = (x.shared + KEYS - 1) / KEYS;
+    return x;
   };
-  auto items_of = [&](int m) { return (m * G + R - 1) / R; };  // of a key head; m G is below 2^21
-  auto tokens_of = [&](int g) { return max(0, start_of(a, g + 1) - start_of(a, g)); };
-  auto tiles_of = [&](int shared) { return (shared + KEYS - 1) / KEYS; };
-  if (tid == 0) found.id = -1;
-  long items = 0, tiles = 0, tokens = 0, before;
-  for (int g = g0; g < g1; ++g) {
-    const int m = tokens_of(g), its = items_of(m) * kv;
-    items += its;
-    tiles += long(its) * tiles_of(shared_of(a, g));
-    tokens += m;
+  const Group first = group_at(0);
+  auto group_of_round = [&](int k) { return k == 0 ? first : group_at(k); };
+  const auto plus = [](uint64_t x, uint64_t y) { return x + y; };
+  auto last = [&](uint64_t v) { return long(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), 63))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(v), 63))); };
+  long tokens = 0, items = 0, tiles = 0, total = 0, each = 1L << 40;
+  for (int k = 0; k < rounds; ++k) {
+    const Group x = group_of_round(k);
+    tokens += last(scan_wave(uint64_t(x.tokens), uint64_t(0), plus));
+    items += last(scan_wave(uint64_t(x.items) * kv, uint64_t(0), plus));
+    tiles += last(scan_wave(uint64_t(x.items) * kv * x.tiles, uint64_t(0), plus));
   }
-  const bool valid = total_of(tokens, before) <= a.n;  // more only where starts descend: nothing is done
-  long all_items = total_of(items, before), all_tiles = 0, count = 0, total = 0, each = 1L << 40;
-  auto parts_of = [&](int shared) { return int(max(1L, quotient(tiles_of(shared) + each - 1, each))); };
-  if (join) all_tiles = total_of(tiles, before);
+  const bool valid = tokens <= a.n;  // more only where starts descend: nothing is done
+  auto parts_of = [&](const Group& x) { return int(max(1L, quotient(x.tiles + each - 1, each))); };
   for (int attempt = 0; attempt < 2; ++attempt) {
-    const long share = attempt == 0 ? blocks : blocks - all_items;
-    if (join && share > 0) each = max(1L, quotient(all_tiles + share - 1, share));
-    else each = 1L << 40;
-    count = 0;
-    for (int g = g0; g < g1; ++g) count += long(items_of(tokens_of(g))) * kv * parts_of(shared_of(a, g));
-    total = total_of(count, before);
+    const long share = attempt == 0 ? blocks : blocks - items;
+    each = join && share > 0 ? max(1L, quotient(tiles + share - 1, share)) : 1L << 40;
+    total = 0;
+    for (int k = 0; k < rounds; ++k) {
+      const Group x = group_of_round(k);
+      total += last(scan_wave(uint64_t(x.items) * kv * parts_of(x), uint64_t(0), plus));
+    }
     if (total <= blocks) break;
   }
+  Mine mine;
+  mine.id = valid && long(blockIdx.x) < total ? xcd_contiguous(int(blockIdx.x), int(total)) : -1;
+  const bool leave = join && blockIdx.x == 0 && threadIdx.x < 64;
+  if (leave && lane == 0) reinterpret_cast<PlanHead*>(workspace)->valid = valid;
+  if (!valid || (mine.id < 0 && !leave)) return mine;
   // those that read the same keys run at the same time on the same XCD: items fastest, contiguous ids an XCD
-  if (valid) {
-    const long id = long(blockIdx.x) < total ? xcd_contiguous(int(blockIdx.x), int(total)) : -1;
-    long at = before;
-    for (int g = g0; g < g1; ++g) {
-      const int start = start_of(a, g), m = tokens_of(g), shared = shared_of(a, g), parts = parts_of(shared), its = items_of(m);
-      const long here = long(its) * kv * parts;
-      if (join && blockIdx.x == 0) reinterpret_cast<GroupPlan*>(workspace + sizeof(PlanHead))[g] = {int(at), parts, its, start};
-      if (id >= at && id < at + here) {
-        const int r = int(id - at), item = r % its, rest = r / its;
-        found = {int(id), g, item, rest / parts, rest % parts, parts, start, m, shared};
-      }
-      at += here;
+  uint64_t before = 0;
+  for (int k = 0; k < rounds; ++k) {
+    const Group x = group_of_round(k);
+    const int parts = parts_of(x), here = x.items * kv * parts;
+    const uint64_t sum = scan_wave(uint64_t(here), uint64_t(0), plus);
+    const int at = int(before + sum) - here;  // below `blocks`
+    if (leave && 64 * k + lane < a.groups)
+      reinterpret_cast<GroupPlan*>(workspace + sizeof(PlanHead))[64 * k + lane] = {at, parts, x.items, x.start};
+    const uint64_t there = __ballot(mine.id >= at && mine.id < at + here);
+    if (there) {
+      const int l = __builtin_ctzll(there);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      const int its = of(x.items), r = mine.id - of(at), rest = r / its;
+      mine.group = 64 * k + l;
+      mine.item = r % its;
+      mine.parts = of(parts);
+      mine.kh = rest / mine.parts;
+      mine.part = rest % mine.parts;
+      mine.start = of(x.start);
+      mine.tokens = of(x.tokens);
+      mine.shared = of(x.shared);
+      if (!leave) break;
     }
+    before += last(sum);
   }
-  if (join && blockIdx.x == 0 && tid == 0) reinterpret_cast<PlanHead*>(workspace)->valid = valid;
-  __syncthreads();
-  return found;
+  return mine;
 }
 
-// A token's own positions: part `u` of them, by four waves of a block, which all come here.
+// A token's own positions: part `part` of `of` of those of token i and up to 16 heads (column group `group` of the key heads'), every
+// step-th tile from the first-th on by this wave. Returns the wave, whose sums are there.
 template <typename T>
-__device__ inline void own_part(const PrefixArgs& a, int u, int own, size_t own_parts, char* workspace, char* smem, float (*stats)[4]) {
-  using Ops = TileOps<T>;
-  constexpr int KEYS = Ops::KEYS;
+__device__ inline PrefixWave<T, 1> own_tiles(const PrefixArgs& a, int i, int group, int part, int of, int first, int step, char* ring) {
+  constexpr int KEYS = TileOps<T>::KEYS;
   const KvCache& c = a.cache;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) % WAVES, col = lane & 15, g = lane >> 4;
-  const int G = a.heads / c.kv_heads, groups = (G + 15) / 16, cols = c.kv_heads * groups, columns = min(G, 16);
-  const int part = u % own, i = u / own / cols, group = u / own % cols, kh = group / groups, h0 = group % groups * 16;
-  const int grp = group_of(a, i);
-  char* ring = smem + wave * RING * TILE_BYTES;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int G = a.heads / c.kv_heads, groups = (G + 15) / 16, kh = group / groups, h0 = group % groups * 16;
   PrefixWave<T, 1> w{c, kh, lane, uint32_t(reinterpret_cast<uintptr_t>((lds_cptr)ring)), ring, a.table + long(i) * a.width, a.width};
   const bool in = h0 + col < G;
   w.ops[0].load_q(static_cast<const T*>(a.q) + long(i) * a.ldq + long(kh * G + h0 + (in ? col : 0)) * 64, g, in);
-  w.lo = grp < 0 ? 0 : uniform(shared_of(a, grp));
-  w.end = grp < 0 ? 0 : uniform(int(min(long(length_of(a.lens[i], a.width, c.shift, 0x7fffffff)), long(w.lo) + a.max_own)));
+  // for up to 64 groups what is asked of them comes in one load, a group a lane
+  const int near = min(lane, a.groups - 1), begin = start_of(a, near), end = start_of(a, near + 1);
+  int shared = shared_of(a, near), len = a.lens[i], at = -1;
+  if (a.groups <= 64) {
+    const uint64_t of_token = __ballot(lane < a.groups && begin <= i && i < end);
+    if (of_token) {
+      at = 63 - __builtin_clzll(of_token);
+      shared = __builtin_amdgcn_readlane(shared, at);
+    }
+  } else if ((at = group_of(a, i)) >= 0) {
+    shared = shared_of(a, at);
+  }
+  w.lo = at < 0 ? 0 : uniform(shared);
+  w.end = at < 0 ? 0 : uniform(int(min(long(length_of(len, a.width, c.shift, 0x7fffffff)), long(w.lo) + a.max_own)));
   w.least = w.hi[0] = w.end;
-  const int first = w.lo / KEYS, tiles = w.end > w.lo ? (w.end + KEYS - 1) / KEYS - first : 0;
-  const int t0 = first + int(long(tiles) * part / own) + wave, t1 = first + int(long(tiles) * (part + 1) / own);
-  if (w.template run<false>(t0, WAVES, t1, a.scale)) w.template run<true>(t0, WAVES, t1, a.scale);
+  const int from = w.lo / KEYS, tiles = w.end > w.lo ? (w.end + KEYS - 1) / KEYS - from : 0;
+  const int t0 = from + int(long(tiles) * part / of) + first, t1 = from + int(long(tiles) * (part + 1) / of);
+  if (w.template run<false>(t0, step, t1, a.scale)) w.template run<true>(t0, step, t1, a.scale);
+  return w;
+}
+
+// Block `u` of those for the tokens' own positions, whose waves share one of `own` parts. (A wave with a token by itself, of which 64 forks
+// of 12 heads have enough: 52 -> 62 us, by the longest of them.)
+template <typename T>
+__device__ inline void own_block(const PrefixArgs& a, int u, int own, size_t own_parts, char* workspace, char* smem, float (*stats)[4]) {
+  const int wave = uniform(threadIdx.x >> 6), G = a.heads / a.cache.kv_heads, cols = a.cache.kv_heads * ((G + 15) / 16), columns = min(G, 16);
+  const PrefixWave<T, 1> w = own_tiles<T>(a, u / own / cols, u / own % cols, u % own, own, wave, WAVES, smem + wave * RING * TILE_BYTES);
   join_waves<T, 1>(w, smem, stats, wave, false, part_at(workspace, own_parts, u, columns), 0, columns, [](int) { return static_cast<T*>(nullptr); });
 }
 
@@ -399,10 +425,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
   __shared__ __attribute__((aligned(1024))) char smem[WAVES * RING * TILE_BYTES];
   __shared__ float stats[WAVES * R][4];
   if (int(blockIdx.x) >= blocks) {
-    own_part<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
+    own_block<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
     return;
   }
-  const Mine mine = find_item<KEYS, R, WAVES>(a, blocks, workspace, join);
+  const Mine mine = find_item<KEYS, R>(a, blocks, workspace, join);
   if (uniform(mine.id) < 0) return;
   const KvCache& c = a.cache;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, G = a.heads / c.kv_heads;
@@ -460,12 +486,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
 
 // --- many rows an item --------------------------------------------------------------------------
 //
-// Four waves of QT times 32 columns share tiles of 64 keys, on the 32x32 matrix instructions: S^T = K Q^T leaves a lane one
+// Four waves of 32 columns each share tiles of 64 keys, on the 32x32 matrix instructions: S^T = K Q^T leaves a lane one
 // column (lane % 32) and 16 keys of each 32, which is the second operand of O^T = V^T P^T as it stands.
 //
 // Bound by the matrix instructions and by the vector unit's work on the scores, about as much of either: so half a tile's products
 // with K and the half before the last one's with V are under way while the half between becomes weights, all in one wave's stream,
-// and two waves share a SIMD.
+// and two waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 109 us and the join's 13; 768 tokens on
+// as many 0.76 PFLOP/s in all. Waves of 64 columns took as long (half the reads of LDS, but twice the registers), three blocks a CU of
+// three tiles of loads 7% less for 1037 tokens and 4% more for 128; two teams of waves that multiply and exponentiate in turn took 140 us.
 //
 // The weights are 2^(c s - r), c = |scale| log2(e), in one fused multiply-add: its one rounding is of the difference, and what r was
 // rounded by is the same for all weights of a column. r is the largest score of the first half tile with a key; sums that overflow
@@ -500,7 +528,7 @@ template <typename F> __device__ inline float over_two(float v, F&& fn) {
 constexpr int WIDE_KEYS = 64, WIDE_BYTES = WIDE_KEYS * 256;  // a tile: K, then V
 constexpr int WIDE_RING = 4;
 
-template <typename T, int QT> struct WideWave {
+template <typename T> struct WideWave {
   // f16 weights below 2^-14 lose bits and 2^16 is beyond them: the first tile's largest weight is 2^4
   static constexpr float TOP = std::is_same<T, f16>::value ? 4.f : 0.f;
   const KvCache& c;
@@ -513,11 +541,11 @@ template <typename T, int QT> struct WideWave {
   int chunk, ahead;
   uint32_t at_lo, at_hi;
   uint64_t ok;
-  uint32_t full;            // bits of a tile's pages
-  int hi[QT], most, least;  // of the wave's columns
-  uint4 q[QT][4];
-  f32x16 o[QT][2];
-  float r[QT], l[QT];
+  uint32_t full;        // bits of a tile's pages
+  int hi, most, least;  // what the lane's column sees; of the wave's columns
+  uint4 q[4];
+  f32x16 o[2];
+  float r, l;
   int key0;  // the first position of the tiles with a page: a column that sees it has met a key
 
   __device__ inline int load_entries(int k) const { return row[min(long(k) * 64 + lane, long(width) - 1)]; }
@@ -538,6 +566,7 @@ template <typename T, int QT> struct WideWave {
     return uint32_t(ok >> (place0 & 63)) & full;
   }
   // Asks for this wave's 16 rows of tile t (16 w on), which lie in PIECES pages, into slot b of the ring. What is behind `end` reads as zeros.
+  // Chunk x of row y lies in slot x ^ (y / 2) of keys and x ^ 2 (y % 4) of values, so that the rows that a read takes lie in different banks.
   template <int PIECES> __device__ inline void ask(int t, int b, uint32_t pages) const {
     const int lrow = lane >> 3;
     const uint32_t k_off[4] = {uint32_t(lrow * 128 + (((lane & 7) ^ (lrow >> 1)) * 16)), uint32_t(lrow * 128 + (((lane & 7) ^ (4 + (lrow >> 1))) * 16))};
@@ -594,38 +623,8 @@ template <typename T, int QT> struct WideWave {
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 
-  // Half a tile: scores, weights.
-  struct Scores { f32x16 s[QT]; };
-  struct Weights { uint32_t p[QT][8]; };
-  __device__ inline void score(Scores& x, const uint4 (&kf)[4]) const {
-    const f32x16 zero = {};
-#pragma unroll
-    for (int st = 0; st < 4; ++st)
-#pragma unroll
-      for (int n = 0; n < QT; ++n) x.s[n] = mma32<T>(kf[st], q[n][st], st == 0 ? zero : x.s[n]);
-  }
-  __device__ inline void weights(Weights& w, const Scores& x, float scale, const float (&ref)[QT]) {
-#pragma unroll
-    for (int n = 0; n < QT; ++n) {
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = __builtin_amdgcn_exp2f(fmaf(x.s[n][2 * e], scale, ref[n])), b = __builtin_amdgcn_exp2f(fmaf(x.s[n][2 * e + 1], scale, ref[n]));
-        w.p[n][e] = pack2<T>(a, b);
-        sum = add_pair<T>(w.p[n][e], sum);
-      }
-      l[n] += sum;
-    }
-  }
-  __device__ inline void weigh(const Weights& w, const uint4 (&vf)[4]) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int n = 0; n < QT; ++n) {
-        const uint32_t* p = w.p[n] + 4 * (k >> 1);
-        o[n][k & 1] = mma32<T>(vf[k], make_uint4(p[0], p[1], p[2], p[3]), o[n][k & 1]);
-      }
-  }
+  // Half a tile: its operands, scores, weights, and what those add to the sums.
+  struct Weights { uint32_t p[8]; };
   __device__ inline void load_keys(uint4 (&kf)[4], int b, int half) const {
 #pragma unroll
     for (int st = 0; st < 4; ++st) kf[st] = keys(b, half, st);
@@ -634,78 +633,91 @@ template <typename T, int QT> struct WideWave {
 #pragma unroll
     for (int k = 0; k < 4; ++k) vf[k] = values(b, half, k >> 1, k & 1);
   }
-
-  // The largest score of column n, times scale.
-  __device__ inline float largest(const Scores& x, int n, float scale) const {
-    const f32x16& s = x.s[n];
+  __device__ inline void score(f32x16& s, const uint4 (&kf)[4]) const {
+    const f32x16 zero = {};
+#pragma unroll
+    for (int st = 0; st < 4; ++st) s = mma32<T>(kf[st], q[st], st == 0 ? zero : s);
+  }
+  __device__ inline void weights(Weights& w, const f32x16& s, float scale, float ref) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w.p[e] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[2 * e], scale, ref)), __builtin_amdgcn_exp2f(fmaf(s[2 * e + 1], scale, ref)));
+      sum = add_pair<T>(w.p[e], sum);
+    }
+    l += sum;
+  }
+  __device__ inline void weigh(const Weights& w, const uint4 (&vf)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t* p = w.p + 4 * (k >> 1);
+      o[k & 1] = mma32<T>(vf[k], make_uint4(p[0], p[1], p[2], p[3]), o[k & 1]);
+    }
+  }
+  // The largest score of the lane's column, times scale.
+  __device__ static inline float largest(const f32x16& s, float scale) {
     float m = most_of(most_of(s[0], s[1]), s[2]);
 #pragma unroll
     for (int e = 3; e < 15; e += 2) m = most_of(most_of(m, s[e]), s[e + 1]);
     return over_two(most_of(m, s[15]), most_of) * scale;
   }
-  // Keys of half a tile from position `first` on (a multiple of 32): those of the four groups of 8 in one page that column n sees, counted
-  // from the lane's own of the group on.
-  __device__ inline int limit(int n, int first, uint32_t pages, int group) const {
+  // Of half a tile from position `first` on (a multiple of 32), in the group of 8 keys in one page: how many from the lane's own first
+  // one on its column sees.
+  __device__ inline int limit(int first, uint32_t pages, int group) const {
     const int at = (first & (WIDE_KEYS - 1)) + group * 8, bit = c.page_size < WIDE_KEYS ? at >> c.shift : 0;
-    return pages >> bit & 1 ? hi[n] - first - 4 * (lane >> 5) - 8 * group : -WIDE_KEYS;
+    return pages >> bit & 1 ? hi - first - 4 * (lane >> 5) - 8 * group : -WIDE_KEYS;
   }
 
   // Half a tile by itself: keys that not all columns see, and columns whose reference is not there yet. CAREFUL: the reference follows
   // the largest score, and infinities and NaN among the values count where they are seen and nowhere else.
-  template <bool CAREFUL> __device__ inline void half_tile(int t, int half, uint32_t pages, float scale, float (&ref)[QT]) {
+  template <bool CAREFUL> __device__ inline void half_tile(int t, int half, uint32_t pages, float scale, float& ref) {
     const int b = t % WIDE_RING, first = t * WIDE_KEYS + half * 32;
     uint4 kf[4], vf[4];
-    Scores x;
+    f32x16 s;
     Weights w;
     load_keys(kf, b, half);
-    score(x, kf);
+    score(s, kf);
     load_values(vf, b, half);
 #pragma unroll
-    for (int n = 0; n < QT; ++n) {
+    for (int x4 = 0; x4 < 4; ++x4) {
+      const int below = limit(first, pages, x4);
 #pragma unroll
-      for (int x4 = 0; x4 < 4; ++x4) {
-        const int below = limit(n, first, pages, x4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x.s[n][4 * x4 + e] = e < below ? x.s[n][4 * x4 + e] : -INFINITY;
-      }
-      const float mx = largest(x, n, scale), top = r[n] == -INFINITY || (CAREFUL && mx > r[n]) ? mx : r[n];
-      if (CAREFUL) {  // where there was none, the sums are zeros
-        const float keep = r[n] == top ? 1.f : __builtin_amdgcn_exp2f(r[n] - top);
-        l[n] *= keep;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          o[n][0][e] *= keep;
-          o[n][1][e] *= keep;
-        }
-      }
-      r[n] = top;
-      ref[n] = TOP - (top == -INFINITY ? 0.f : top);
+      for (int e = 0; e < 4; ++e) s[4 * x4 + e] = e < below ? s[4 * x4 + e] : -INFINITY;
     }
-    weights(w, x, scale, ref);
+    const float mx = largest(s, scale), top = r == -INFINITY || (CAREFUL && mx > r) ? mx : r;
+    if (CAREFUL) {  // where there was none, the sums are zeros
+      const float keep = r == top ? 1.f : __builtin_amdgcn_exp2f(r - top);
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        o[0][e] *= keep;
+        o[1][e] *= keep;
+      }
+    }
+    r = top;
+    ref = TOP - (top == -INFINITY ? 0.f : top);
+    weights(w, s, scale, ref);
     if constexpr (CAREFUL) {
       const f32x16 zero = {};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint4 raw = vf[k];
         vf[k] = map_pairs(raw, [](float y) { return fabsf(y) < INFINITY ? y : 0.f; });
+        uint32_t one[4];  // how many of each other kind the column sees
 #pragma unroll
-        for (int n = 0; n < QT; ++n) {  // how many of each other kind the column sees
-          uint32_t one[4];
+        for (int e = 0; e < 4; ++e) {
+          const int below = limit(first, pages, 2 * (k >> 1) + e / 2) - 2 * (e & 1);
+          one[e] = pack2<T>(below > 0 ? 1.f : 0.f, below > 1 ? 1.f : 0.f);
+        }
+        const uint4 sees = make_uint4(one[0], one[1], one[2], one[3]);
+        const f32x16 none = mma32<T>(map_pairs(raw, [](float y) { return y != y ? 1.f : 0.f; }), sees, zero);
+        const f32x16 up = mma32<T>(map_pairs(raw, [](float y) { return y == INFINITY ? 1.f : 0.f; }), sees, zero);
+        const f32x16 down = mma32<T>(map_pairs(raw, [](float y) { return y == -INFINITY ? 1.f : 0.f; }), sees, zero);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int below = limit(n, first, pages, 2 * (k >> 1) + e / 2) - 2 * (e & 1);
-            one[e] = pack2<T>(below > 0 ? 1.f : 0.f, below > 1 ? 1.f : 0.f);
-          }
-          const uint4 sees = make_uint4(one[0], one[1], one[2], one[3]);
-          const f32x16 none = mma32<T>(map_pairs(raw, [](float y) { return y != y ? 1.f : 0.f; }), sees, zero);
-          const f32x16 up = mma32<T>(map_pairs(raw, [](float y) { return y == INFINITY ? 1.f : 0.f; }), sees, zero);
-          const f32x16 down = mma32<T>(map_pairs(raw, [](float y) { return y == -INFINITY ? 1.f : 0.f; }), sees, zero);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (none[e] > 0.f) o[n][k & 1][e] = NAN;
-            if (up[e] > 0.f) o[n][k & 1][e] += INFINITY;
-            if (down[e] > 0.f) o[n][k & 1][e] -= INFINITY;
-          }
+        for (int e = 0; e < 16; ++e) {
+          if (none[e] > 0.f) o[k & 1][e] = NAN;
+          if (up[e] > 0.f) o[k & 1][e] += INFINITY;
+          if (down[e] > 0.f) o[k & 1][e] -= INFINITY;
         }
       }
     }
@@ -714,17 +726,15 @@ template <typename T, int QT> struct WideWave {
 
   // Weights are taken here, not where they are used first: that is behind the next barrier.
   __device__ inline void pin(Weights& w) {
+    asm volatile("" : "+v"(l));
 #pragma unroll
-    for (int n = 0; n < QT; ++n) asm volatile("" : "+v"(l[n]));
-#pragma unroll
-    for (int n = 0; n < QT; ++n)
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) asm volatile("" : "+v"(w.p[n][e]), "+v"(w.p[n][e + 1]), "+v"(w.p[n][e + 2]), "+v"(w.p[n][e + 3]));
+    for (int e = 0; e < 8; e += 4) asm volatile("" : "+v"(w.p[e]), "+v"(w.p[e + 1]), "+v"(w.p[e + 2]), "+v"(w.p[e + 3]));
   }
-  // Beside the 8 QT matrix instructions of half a tile: its share of the vector unit's work between each two.
+  // Beside the eight matrix instructions of half a tile: the vector unit's work, five of its instructions between each two (6 to 9 were
+  // slower, none, the compiler's own order, 6%).
   __device__ static inline void interleave() {
 #pragma unroll
-    for (int k = 0; k < 8 * QT; ++k) {
+    for (int k = 0; k < 8; ++k) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
     }
@@ -732,15 +742,11 @@ template <typename T, int QT> struct WideWave {
 
   // Tiles t0 up to t1. True where the sums are not to be taken: a NaN, an infinity, or weights beyond 2^64.
   template <bool CAREFUL> __device__ inline bool pass(int t0, int t1, float scale) {
-    float ref[QT];
+    float ref = 0.f;
 #pragma unroll
-    for (int n = 0; n < QT; ++n) {
-#pragma unroll
-      for (int x = 0; x < 16; ++x) o[n][0][x] = o[n][1][x] = 0.f;
-      r[n] = -INFINITY;
-      l[n] = 0.f;
-      ref[n] = 0.f;
-    }
+    for (int x = 0; x < 16; ++x) o[0][x] = o[1][x] = 0.f;
+    r = -INFINITY;
+    l = 0.f;
     key0 = 0x7fffffff;
     full = (1u << max(1, WIDE_KEYS >> c.shift)) - 1;
     uint32_t pages = 0, pages1 = 0, pages2 = 0;  // of tiles t, t + 1, t + 2
@@ -759,17 +765,14 @@ template <typename T, int QT> struct WideWave {
       pages1 = pages2;
       if (t + 2 < t1) pages2 = issue(t + 2);
     };
-    auto plain = [&](int t, uint32_t there) {  // all columns see all of tile t
-      bool none = false;
-#pragma unroll
-      for (int n = 0; n < QT; ++n) none |= r[n] == -INFINITY && hi[n] > 0;
-      return !CAREFUL && there == full && (t + 1) * WIDE_KEYS <= least && !__builtin_amdgcn_ballot_w64(none);
+    auto plain = [&](int t) {  // all columns see all of tile t, and have their reference
+      return !CAREFUL && pages == full && (t + 1) * WIDE_KEYS <= least && !__builtin_amdgcn_ballot_w64(r == -INFINITY && hi > 0);
     };
     int t = t0;
     if (t < t1) arrive(t);
 #pragma unroll 1
     while (t < t1) {
-      if (!plain(t, pages)) {
+      if (!plain(t)) {
         if (t * WIDE_KEYS < most) {
           if (pages && key0 == 0x7fffffff) key0 = t * WIDE_KEYS + (__builtin_ctz(pages) << c.shift);
           half_tile<CAREFUL>(t, 0, pages, scale, ref);
@@ -780,7 +783,7 @@ template <typename T, int QT> struct WideWave {
       }
       if constexpr (!CAREFUL) {
         // the first half's scores, and weights of 0 in the place of the half before it
-        Scores sa, sb;
+        f32x16 sa, sb;
         Weights pa, pb = {};
         uint4 kf[4], vf[4];
         load_keys(kf, t % WIDE_RING, 0);
@@ -800,9 +803,9 @@ template <typename T, int QT> struct WideWave {
           more = ++t < t1;
           if (more) {
             arrive(t);
-            more = plain(t, pages);
+            more = plain(t);
           }
-          load_keys(kf, (b + 1) % WIDE_RING, 0);  // where that is no plain tile, keys long used: its scores are not
+          load_keys(kf, (b + 1) % WIDE_RING, 0);  // where that is no plain tile, of any: its scores are not used
           weigh(pa, vf);
           weights(pb, sb, scale, ref);
           load_values(vf, b, 1);
@@ -813,167 +816,165 @@ template <typename T, int QT> struct WideWave {
         weigh(pb, vf);
       }
     }
-    bool bad = false;
+    bool bad = !(l <= 18446744073709551616.f);
 #pragma unroll
-    for (int n = 0; n < QT; ++n) {
-      bad |= !(l[n] <= 18446744073709551616.f);
-#pragma unroll
-      for (int x = 0; x < 16; ++x) bad |= !(fabsf(o[n][0][x]) < INFINITY) || !(fabsf(o[n][1][x]) < INFINITY);
-    }
+    for (int x = 0; x < 16; ++x) bad |= !(fabsf(o[0][x]) < INFINITY) || !(fabsf(o[1][x]) < INFINITY);
     return __syncthreads_or(bad && most > 0);
   }
 };
 
-template <typename T, int QT>
+template <typename T>
 __global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const PrefixArgs a, int blocks, int own, bool join, size_t parts, size_t own_parts, char* workspace) {
-  constexpr int R = WAVES * QT * 32;
+  constexpr int R = WAVES * 32;
   __shared__ __attribute__((aligned(1024))) char smem[WIDE_RING * WIDE_BYTES];
   static_assert(sizeof(smem) >= WAVES * RING * TILE_BYTES, "the rings of a token's own positions");
   __shared__ float stats[WAVES * 16][4];
   __shared__ int ends[WAVES];
   if (int(blockIdx.x) >= blocks) {
-    own_part<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
+    own_block<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
     return;
   }
-  const Mine mine = find_item<WIDE_KEYS, R, WAVES>(a, blocks, workspace, join);
+  const Mine mine = find_item<WIDE_KEYS, R>(a, blocks, workspace, join);
   if (uniform(mine.id) < 0) return;
   const KvCache& c = a.cache;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 5, G = a.heads / c.kv_heads;
-  const int kh = uniform(mine.kh), shared = uniform(mine.shared), rows = uniform(mine.tokens) * G, item = uniform(mine.item), start = uniform(mine.start);
-  const int* row = a.prefix + long(uniform(mine.group)) * a.prefix_width;
+  const int kh = uniform(mine.kh), shared = uniform(mine.shared), rows = uniform(mine.tokens) * G, start = uniform(mine.start);
+  WideWave<T> w{c, kh, lane, wave, smem, a.prefix + long(uniform(mine.group)) * a.prefix_width, a.prefix_width};
   // a scale's sign goes into the queries, exactly, and a scale of 0: the largest score is then the largest product
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, hold = a.scale == 0.f ? 0u : ~0u;
   const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
-  // M of each wave's QT times 32 columns, from `first` on. True where a sum is NaN, and nothing is written then.
-  auto columns = [&](auto count, auto careful, int first) {
-    constexpr int M = decltype(count)::value;
-    constexpr bool CAREFUL = decltype(careful)::value;
-    WideWave<T, M> w{c, kh, lane, wave, smem, row, a.prefix_width};
-    int most = 0, least = 0x7fffffff;
-    // the row of a column of this lane, which is asked for again when the sums are there: kept, it would cost registers meanwhile
-    auto row_of = [&](int n, int ln) { return item * R + (wave * QT + first + n) * 32 + (ln & 31); };
+  const int column = wave * 32 + (lane & 31), row = uniform(mine.item) * R + column;
+  const bool in = row < rows;
+  const int token = start + (in ? row / G : 0), head = kh * G + (in ? row % G : 0);
+  w.hi = in ? max(0, min(a.lens ? a.lens[token] : shared, shared)) : 0;
 #pragma unroll
-    for (int n = 0; n < M; ++n) {
-      const int r = row_of(n, lane);
-      const bool in = r < rows;
-      const int token = start + (in ? r / G : 0);
-      w.hi[n] = in ? max(0, min(a.lens ? a.lens[token] : shared, shared)) : 0;
-      const T* q = static_cast<const T*>(a.q) + long(token) * a.ldq + long(kh * G + (in ? r % G : 0)) * 64;
+  for (int st = 0; st < 4; ++st) {
+    const uint4 x = in ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + long(token) * a.ldq + long(head) * 64 + st * 16 + g * 8) : make_uint4(0, 0, 0, 0);
+    w.q[st] = make_uint4((x.x ^ flip) & hold, (x.y ^ flip) & hold, (x.z ^ flip) & hold, (x.w ^ flip) & hold);
+  }
+  int most = w.hi, least = in ? w.hi : 0x7fffffff;
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        const uint4 x = in ? *reinterpret_cast<const uint4*>(q + st * 16 + g * 8) : make_uint4(0, 0, 0, 0);
-        w.q[n][st] = make_uint4((x.x ^ flip) & hold, (x.y ^ flip) & hold, (x.z ^ flip) & hold, (x.w ^ flip) & hold);
-      }
-      most = max(most, w.hi[n]);
-      if (in) least = min(least, w.hi[n]);
-    }
+  for (int x = 1; x < 32; x <<= 1) {
+    most = max(most, __shfl_xor(most, x));
+    least = min(least, __shfl_xor(least, x));
+  }
+  w.most = uniform(most);
+  w.least = uniform(least);
+  if (lane == 0) ends[wave] = most;
+  __syncthreads();
+  w.end = 0;
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      most = max(most, __shfl_xor(most, x));
-      least = min(least, __shfl_xor(least, x));
-    }
-    w.most = uniform(most);
-    w.least = uniform(least);
-    if (lane == 0) ends[wave] = most;
-    __syncthreads();
-    w.end = 0;
-#pragma unroll
-    for (int k = 0; k < WAVES; ++k) w.end = max(w.end, uniform(ends[k]));
-    const int tiles = (shared + WIDE_KEYS - 1) / WIDE_KEYS, seen = (w.end + WIDE_KEYS - 1) / WIDE_KEYS, k = uniform(mine.part), of = uniform(mine.parts);
-    const bool bad = w.template pass<CAREFUL>(int(long(tiles) * k / of), min(seen, int(long(tiles) * (k + 1) / of)), scale);
-    if (!CAREFUL && bad) return true;
+  for (int k = 0; k < WAVES; ++k) w.end = max(w.end, uniform(ends[k]));
+  const int tiles = (shared + WIDE_KEYS - 1) / WIDE_KEYS, seen = (w.end + WIDE_KEYS - 1) / WIDE_KEYS, k = uniform(mine.part), of = uniform(mine.parts);
+  const int t0 = int(long(tiles) * k / of), t1 = min(seen, int(long(tiles) * (k + 1) / of));
+  if (w.template pass<false>(t0, t1, scale)) w.template pass<true>(t0, t1, scale);
+  const float sum = over_two(w.l, [](float x, float y) { return x + y; });
+  const bool some = w.hi > w.key0;
+  if (join) {
     float* part = part_at(workspace, parts, uniform(mine.id), R);
 #pragma unroll
-    for (int n = 0; n < M; ++n) {
-      const float sum = over_two(w.l[n], [](float x, float y) { return x + y; });
-      if (join) {
-        const int column = (wave * QT + first + n) * 32 + (lane & 31);
+    for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt)
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<float4*>(part + column * 64 + dt * 32 + 8 * k + 4 * g) =
+            make_float4(w.o[dt][4 * k], w.o[dt][4 * k + 1], w.o[dt][4 * k + 2], w.o[dt][4 * k + 3]);
+    if (g == 0) *reinterpret_cast<float2*>(part + R * 64 + column * 2) = make_float2((w.r - w.TOP) * 0.693147180559945309f, some ? sum : -1.f);
+  } else if (in) {
+    const float inv = 1.f / sum;
+    T* out = static_cast<T*>(a.out) + long(token) * a.ldo + long(head) * 64 + 4 * g;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<float4*>(part + column * 64 + dt * 32 + 8 * k + 4 * g) =
-                make_float4(w.o[n][dt][4 * k], w.o[n][dt][4 * k + 1], w.o[n][dt][4 * k + 2], w.o[n][dt][4 * k + 3]);
-        if (g == 0) *reinterpret_cast<float2*>(part + R * 64 + column * 2) = make_float2((w.r[n] - w.TOP) * 0.693147180559945309f, w.hi[n] > w.key0 ? sum : -1.f);
-        continue;
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = some ? w.o[dt][4 * k + e] * inv : 0.f;
+        *reinterpret_cast<uint2*>(out + dt * 32 + 8 * k) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
       }
-      int ln = lane;
-      asm volatile("" : "+v"(ln));
-      if (const int r = row_of(n, ln); r < rows) {
-        const float inv = 1.f / sum;
-        T* out = static_cast<T*>(a.out) + long(start + r / G) * a.ldo + long(kh * G + r % G) * 64 + 4 * g;
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = w.hi[n] > w.key0 ? w.o[n][dt][4 * k + e] * inv : 0.f;
-            *reinterpret_cast<uint2*>(out + dt * 32 + 8 * k) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-          }
-      }
-    }
-    return false;
-  };
-  if (!columns(std::integral_constant<int, QT>(), std::false_type(), 0)) return;
-#pragma unroll 1
-  for (int n = 0; n < QT; ++n) {
-    __syncthreads();  // `ends` and the rings are read
-    columns(std::integral_constant<int, 1>(), std::true_type(), n);
   }
 }
 
 // --- the join -----------------------------------------------------------------------------------
 
-// One wave a (token, head): a channel a lane, AT_ONCE parts under way.
+// One wave a (token, head): 16 lanes a part, four channels each, so that four parts are one load and 4 AT_ONCE are under way. Bound by its
+// chain of loads (starts, the plan, the parts), and by the parts' bytes where there are many rows.
 constexpr int JOIN_WAVES = 4, AT_ONCE = 8;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WAVES * 64) prefix_join_kernel(const PrefixArgs a, int R, int own, size_t parts, size_t own_parts, char* workspace) {
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), quad = lane & 15, g = lane >> 4;
   const int u = int(blockIdx.x) * JOIN_WAVES + wave;  // below 2^21
-  if (u >= a.n * a.heads || !reinterpret_cast<const PlanHead*>(workspace)->valid) return;
-  const int i = u / a.heads, head = u % a.heads, g = group_of(a, i);
-  if (g < 0) return;
+  if (u >= a.n * a.heads) return;
+  const GroupPlan* plans = reinterpret_cast<const GroupPlan*>(workspace + sizeof(PlanHead));
+  // for up to 64 groups what is asked of them comes in one load, a group a lane
+  const int near = min(lane, a.groups - 1), valid = reinterpret_cast<const PlanHead*>(workspace)->valid, begin = start_of(a, near), end = start_of(a, near + 1);
+  GroupPlan plan = plans[near];
+  if (!valid) return;
+  const int i = u / a.heads, head = u % a.heads;
+  if (a.groups <= 64) {
+    const uint64_t in = __ballot(lane < a.groups && begin <= i && i < end);
+    if (!in) return;
+    const int l = 63 - __builtin_clzll(in);
+    plan = {__builtin_amdgcn_readlane(plan.block0, l), __builtin_amdgcn_readlane(plan.parts, l), __builtin_amdgcn_readlane(plan.items, l),
+            __builtin_amdgcn_readlane(plan.row0, l)};
+  } else {
+    const int group = group_of(a, i);
+    if (group < 0) return;
+    plan = plans[group];
+  }
   const KvCache& c = a.cache;
   const int G = a.heads / c.kv_heads, kh = head / G, e = head % G;
-  const GroupPlan plan = reinterpret_cast<const GroupPlan*>(workspace + sizeof(PlanHead))[g];
   const int r = (i - plan.row0) * G + e, item = r / R, column = r % R, columns = min(G, 16), cols = c.kv_heads * ((G + 15) / 16);
   const long own0 = (long(i) * cols + kh * ((G + 15) / 16) + e / 16) * own;
   const int count = plan.parts + own;
-  float acc = 0.f, sum = 0.f, m = -INFINITY;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f, m = -INFINITY;
   bool some = false;
-  for (int k0 = 0; k0 < count; k0 += AT_ONCE) {
+  for (int k0 = 0; k0 < count; k0 += 4 * AT_ONCE) {
     float2 ml[AT_ONCE];
-    float o[AT_ONCE], mx = m;
+    float4 o[AT_ONCE];
+    float mx = m;
 #pragma unroll
     for (int x = 0; x < AT_ONCE; ++x) {
-      const int k = min(k0 + x, count - 1);
+      const int k = k0 + 4 * x + g;
+      ml[x] = make_float2(0.f, -1.f);
+      if (k0 + 4 * x >= count || k >= count) continue;
       const bool mine = k >= plan.parts;
       const int width = mine ? columns : R, at = mine ? e % 16 : column;
       const float* p = mine ? part_at(workspace, own_parts, own0 + k - plan.parts, columns)
                             : part_at(workspace, parts, plan.block0 + (long(kh) * plan.parts + k) * plan.items + item, R);
       ml[x] = *reinterpret_cast<const float2*>(p + width * 64 + at * 2);
-      o[x] = p[at * 64 + lane];
+      o[x] = *reinterpret_cast<const float4*>(p + at * 64 + quad * 4);
     }
 #pragma unroll
     for (int x = 0; x < AT_ONCE; ++x)
-      if (k0 + x < count && !(ml[x].y < 0.f)) {  // NaN stays
+      if (!(ml[x].y < 0.f)) {  // NaN stays
         mx = fmaxf(mx, ml[x].x);
         some = true;
       }
     const float keep = m == -INFINITY ? 0.f : exp_of(m - mx);
-    acc *= keep;
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
     sum *= keep;
     m = mx;
 #pragma unroll
     for (int x = 0; x < AT_ONCE; ++x)
-      if (k0 + x < count && !(ml[x].y < 0.f)) {
+      if (!(ml[x].y < 0.f)) {
         const float f = ml[x].x == -INFINITY ? 0.f : exp_of(ml[x].x - mx);
-        acc += o[x] * f;
+        acc = make_float4(acc.x + o[x].x * f, acc.y + o[x].y * f, acc.z + o[x].z * f, acc.w + o[x].w * f);
         sum += ml[x].y * f;
       }
   }
-  static_cast<T*>(a.out)[long(i) * a.ldo + long(head) * 64 + lane] = from_f<T>(some ? acc / sum : 0.f);
+  // the four groups of lanes; one without a key has zeros, whatever the others hold
+  const float top = max_groups(m), f = m == -INFINITY ? 0.f : exp_of(m - top);
+  const bool any = max_groups(some ? 1.f : 0.f) > 0.f;
+  auto all = [&](float v) { return sum_groups(some ? v * f : 0.f); };
+  const float inv = all(sum), v[4] = {all(acc.x), all(acc.y), all(acc.z), all(acc.w)};
+  if (g) return;
+  float w[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) w[x] = any ? v[x] / inv : 0.f;
+  T* out = static_cast<T*>(a.out) + long(i) * a.ldo + long(head) * 64 + quad * 4;
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(w[0], w[1], w[2], w[3]);
+  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(w[0], w[1]), pack2<T>(w[2], w[3]));
 }
 
 }  // namespace
@@ -995,13 +996,10 @@ void prefix_attention(const Exec& ex, const PrefixArgs& args, void* workspace, s
     auto launch = [&](auto kernel) {
       kernel<<<int(plan.blocks + own), WAVES * 64, 0, ex.stream>>>(a, plan.blocks, plan.own, plan.join, plan.parts, plan.own_parts, ws);
     };
-    if constexpr (sizeof(T) == 2) {
-      if (plan.rows == 256) launch(prefix_wide_kernel<T, 2>);
-      if (plan.rows == 128) launch(prefix_wide_kernel<T, 1>);
-    }
-    if (plan.rows == 64) launch(prefix_parts_kernel<T, 4>);
-    if (plan.rows == 32) launch(prefix_parts_kernel<T, 2>);
     if (plan.rows == 16) launch(prefix_parts_kernel<T, 1>);
+    else if (plan.rows == 32) launch(prefix_parts_kernel<T, 2>);
+    else if constexpr (sizeof(T) == 4) launch(prefix_parts_kernel<T, 4>);
+    else launch(prefix_wide_kernel<T>);
     if (plan.join)
       prefix_join_kernel<T><<<cdiv(long(a.n) * a.heads, JOIN_WAVES), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.rows, plan.own, plan.parts, plan.own_parts, ws);
   });
