@@ -487,7 +487,8 @@ void check_prefix_attention(PrefixArgs& a, const void* workspace, size_t bytes) 
 
 namespace {
 constexpr int WIDE_ROWS = 128;     // the most of an item
-constexpr int WIDE_BLOCKS = 512, NARROW_BLOCKS = 256;  // that cut items' tiles: two of the wide form on each of 256 CUs, one of the others
+constexpr int WIDE_BLOCKS = 768, NARROW_BLOCKS = 256;  // that cut items' tiles: three of the wide form on each of 256 CUs, one of the others
+constexpr long MOST_PARTS = 40;    // of an item, whose join costs what more blocks would gain
 constexpr long OWN_BLOCKS = 1024;  // of the tokens' own positions, up to which these are cut
 
 // Items of one key head, at most: every group's rows are cut into items of their own.
@@ -501,22 +502,22 @@ int own_parts(long n, long cols, int max_own, int keys) {
 
 // Measured, a call among others, 12 heads, one group and no own positions unless said so. Rows of an item: 16 / 32 / 128 at 16 tokens on 24889
 // positions (bf16) 24.0 / 26.3 / 32.6 us, at 32 28.9 / 26.5 / 31.8, at 48 34.9 / 35.3 / 31.9, at 64 43.8 / 36.1 / 31.6, at 128 92.6 / 56.4 /
-// 32.5; 48 forks of four scenes (32 heads on 8, own positions) 32 rows 43.6, 128 rows 46.9; in fp32 16 / 32 / 64 on 12000 positions at 16 tokens
-// 24.8 / 31.0 / 43.6, at 32 33.1 / 31.5 / 44.0, at 64 52.8 / 46.6 / 44.7, at 256 208 / 168 / 126. Blocks: 256 / 512 of the narrow forms at 16
-// tokens 24.0 / 26.5, 64 forks with a view of their own 44 / 52 (own positions run beside, on each CU's second block); 512 / 1024 of
-// the wide form at 128 tokens 34.6 / 47.8, at 1037 124.8 / 126.0, at 2074 230 / 213.
+// 32.5; with own positions, which the narrow forms take in the same launch, 64 forks 46.7 / 48.1 (32 / 128 rows), 48 forks of four scenes (32
+// heads on 8) 43.6 / 46.9; in fp32 16 / 32 / 64 on 12000 positions at 16 tokens 24.8 / 31.0 / 43.6, at 32 33.1 / 31.5 / 44.0, at 64 52.8 /
+// 46.6 / 44.7, at 256 208 / 168 / 126. Blocks: 256 / 512 of the narrow forms at 16 tokens 24.0 / 26.5, 64 forks 44 / 52 (own positions run beside,
+// on each CU's second block); 512 / 768 / 1024 of the wide form at 128 tokens 36 / 39 / 48 (parts to join), at 1037 127 / 120 / 128.
 PrefixPlan prefix_plan(const PrefixArgs& a) {
   PrefixPlan plan;
   const KvCache& c = a.cache;
   const int G = a.heads / c.kv_heads, small = c.dt == 0 ? 16 : 32;
   const long each = (long(a.n) * G + a.groups - 1) / a.groups;  // rows of a group and key head, if all are alike
-  plan.rows = each <= 16 ? 16 : c.dt == 0 ? (each <= 32 ? 32 : 64) : each <= 48 ? 32 : WIDE_ROWS;
+  plan.rows = each <= 16 ? 16 : c.dt == 0 ? (each <= 32 ? 32 : 64) : each <= (a.max_own ? 64 : 32) ? 32 : WIDE_ROWS;
   const bool wide = plan.rows == WIDE_ROWS;
   const int keys = wide ? 64 : small;
   plan.own = own_parts(a.n, long(c.kv_heads) * ((G + 15) / 16), a.max_own, small);
   // of an item that is cut, parts of eight tiles at least (two a wave), in the wide form of four
   const long items = most_items(a.n, G, a.groups, plan.rows) * c.kv_heads, tiles = (a.max_shared + keys - 1) / keys;
-  const long most = std::max<long>(1, tiles / (wide ? 4 : 8)), round = wide && !plan.own ? WIDE_BLOCKS : NARROW_BLOCKS;
+  const long most = std::max<long>(1, std::min<long>(MOST_PARTS, tiles / (wide ? 4 : 8))), round = wide ? WIDE_BLOCKS : NARROW_BLOCKS;
   long blocks = items;
   if (items < round) {
     blocks = std::max(items, std::min<long>(round, items * most));

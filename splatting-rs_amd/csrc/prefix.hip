@@ -418,6 +418,14 @@ __device__ inline void own_block(const PrefixArgs& a, int u, int own, size_t own
   join_waves<T, 1>(w, smem, stats, wave, false, part_at(workspace, own_parts, u, columns), 0, columns, [](int) { return static_cast<T*>(nullptr); });
 }
 
+// The tokens' own positions by themselves, beside the wide form, whose blocks leave no room for these.
+template <typename T>
+__global__ void __launch_bounds__(WAVES * 64, 2) prefix_own_kernel(const PrefixArgs a, int own, size_t own_parts, char* workspace) {
+  __shared__ __attribute__((aligned(1024))) char smem[WAVES * RING * TILE_BYTES];
+  __shared__ float stats[WAVES * 16][4];
+  own_block<T>(a, int(blockIdx.x), own, own_parts, workspace, smem, stats);
+}
+
 // Few rows an item: each wave streams its own tiles through a ring of its own, and the block's waves join in LDS.
 template <typename T, int NT>
 __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const PrefixArgs a, int blocks, int own, bool join, size_t parts, size_t own_parts, char* workspace) {
@@ -491,9 +499,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
 //
 // Bound by the matrix instructions and by the vector unit's work on the scores, about as much of either: so half a tile's products
 // with K and the half before the last one's with V are under way while the half between becomes weights, all in one wave's stream,
-// and two waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 109 us and the join's 13; 768 tokens on
-// as many 0.76 PFLOP/s in all. Waves of 64 columns took as long (half the reads of LDS, but twice the registers), three blocks a CU of
-// three tiles of loads 7% less for 1037 tokens and 4% more for 128; two teams of waves that multiply and exponentiate in turn took 140 us.
+// and three waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 113 us and the join's 14 (0.70 PFLOP/s).
+// Of a SIMD's cycles 1024 go to the matrix instructions of a tile of 64 columns and 1250 to the vector unit (half of them
+// exponentials), and 60% of the former lie beside the latter. Two blocks a CU with a tile more under way took 130 us, waves of 64 columns 125, two teams
+// of waves that multiply and exponentiate in turn 140, the compiler's own order of the same instructions 6% more than this one.
 //
 // The weights are 2^(c s - r), c = |scale| log2(e), in one fused multiply-add: its one rounding is of the difference, and what r was
 // rounded by is the same for all weights of a column. r is the largest score of the first half tile with a key; sums that overflow
@@ -526,7 +535,7 @@ template <typename F> __device__ inline float over_two(float v, F&& fn) {
 }
 
 constexpr int WIDE_KEYS = 64, WIDE_BYTES = WIDE_KEYS * 256;  // a tile: K, then V
-constexpr int WIDE_RING = 4;
+constexpr int WIDE_RING = 3, WIDE_OCCUPANCY = 3;
 
 template <typename T> struct WideWave {
   // f16 weights below 2^-14 lose bits and 2^16 is beyond them: the first tile's largest weight is 2^4
@@ -731,7 +740,7 @@ template <typename T> struct WideWave {
     for (int e = 0; e < 8; e += 4) asm volatile("" : "+v"(w.p[e]), "+v"(w.p[e + 1]), "+v"(w.p[e + 2]), "+v"(w.p[e + 3]));
   }
   // Beside the eight matrix instructions of half a tile: the vector unit's work, five of its instructions between each two (6 to 9 were
-  // slower, none, the compiler's own order, 6%).
+  // slower).
   __device__ static inline void interleave() {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -749,21 +758,18 @@ template <typename T> struct WideWave {
     l = 0.f;
     key0 = 0x7fffffff;
     full = (1u << max(1, WIDE_KEYS >> c.shift)) - 1;
-    uint32_t pages = 0, pages1 = 0, pages2 = 0;  // of tiles t, t + 1, t + 2
+    uint32_t pages = 0, next = 0;  // of tiles t and t + 1
     if (t0 < t1) {
       const int k = ((t0 * WIDE_KEYS) >> c.shift) >> 6;
       take_entries(k, load_entries(k));
-      pages1 = issue(t0);
-      if (t0 + 1 < t1) pages2 = issue(t0 + 1);
+      next = issue(t0);
     }
-    // Tile t is there, all waves' loads, and tile t - 2 used up: its slot is tile t + 2's.
+    // Tile t is there, all waves' loads, and tile t - 2 used up: its slot is tile t + 1's.
     auto arrive = [&](int t) {
-      if (t + 1 < t1) wait_loads<4>();  // of this wave for tile t + 1
-      else wait_loads<0>();
+      wait_loads<0>();
       asm volatile("s_barrier" ::: "memory");
-      pages = pages1;
-      pages1 = pages2;
-      if (t + 2 < t1) pages2 = issue(t + 2);
+      pages = next;
+      if (t + 1 < t1) next = issue(t + 1);
     };
     auto plain = [&](int t) {  // all columns see all of tile t, and have their reference
       return !CAREFUL && pages == full && (t + 1) * WIDE_KEYS <= least && !__builtin_amdgcn_ballot_w64(r == -INFINITY && hi > 0);
@@ -824,16 +830,10 @@ template <typename T> struct WideWave {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(WAVES * 64, 2) prefix_wide_kernel(const PrefixArgs a, int blocks, int own, bool join, size_t parts, size_t own_parts, char* workspace) {
+__global__ void __launch_bounds__(WAVES * 64, WIDE_OCCUPANCY) prefix_wide_kernel(const PrefixArgs a, int blocks, bool join, size_t parts, char* workspace) {
   constexpr int R = WAVES * 32;
   __shared__ __attribute__((aligned(1024))) char smem[WIDE_RING * WIDE_BYTES];
-  static_assert(sizeof(smem) >= WAVES * RING * TILE_BYTES, "the rings of a token's own positions");
-  __shared__ float stats[WAVES * 16][4];
   __shared__ int ends[WAVES];
-  if (int(blockIdx.x) >= blocks) {
-    own_block<T>(a, int(blockIdx.x) - blocks, own, own_parts, workspace, smem, stats);
-    return;
-  }
   const Mine mine = find_item<WIDE_KEYS, R>(a, blocks, workspace, join);
   if (uniform(mine.id) < 0) return;
   const KvCache& c = a.cache;
@@ -999,7 +999,10 @@ void prefix_attention(const Exec& ex, const PrefixArgs& args, void* workspace, s
     if (plan.rows == 16) launch(prefix_parts_kernel<T, 1>);
     else if (plan.rows == 32) launch(prefix_parts_kernel<T, 2>);
     else if constexpr (sizeof(T) == 4) launch(prefix_parts_kernel<T, 4>);
-    else launch(prefix_wide_kernel<T>);
+    else {
+      if (own) prefix_own_kernel<T><<<int(own), WAVES * 64, 0, ex.stream>>>(a, plan.own, plan.own_parts, ws);
+      prefix_wide_kernel<T><<<plan.blocks, WAVES * 64, 0, ex.stream>>>(a, plan.blocks, plan.join, plan.parts, ws);
+    }
     if (plan.join)
       prefix_join_kernel<T><<<cdiv(long(a.n) * a.heads, JOIN_WAVES), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.rows, plan.own, plan.parts, plan.own_parts, ws);
   });
