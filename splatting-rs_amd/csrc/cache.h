@@ -127,8 +127,8 @@ void check_compact_pages(CompactArgs& a, const void* workspace, size_t bytes);
 void check_copy_pages(CopyArgs& a);
 void check_prefix_attention(PrefixArgs& a, const void* workspace, size_t bytes);
 
-// The workspace of free_pages and compact_pages: bits of the pages in two maps, what lies before every word of 32 of them, and
-// the counts of every CHUNK words.
+// The workspace of free_pages and compact_pages: two maps of a byte a page, what lies before every word of four pages, and the counts of
+// every PAGE_CHUNK words.
 constexpr int PAGE_CHUNK = 1024;
 struct PagesPlan {
   long words = 0, chunks = 0;

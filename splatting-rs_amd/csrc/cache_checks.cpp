@@ -431,7 +431,7 @@ void check_copy_pages(CopyArgs& a) {
 
 PagesPlan pages_plan(int pages) {
   PagesPlan plan;
-  plan.words = (long(pages) + 31) / 32;
+  plan.words = (long(pages) + 3) / 4;
   plan.chunks = (plan.words + PAGE_CHUNK - 1) / PAGE_CHUNK;
   const size_t map = size_t(plan.words + 3) / 4 * 16;
   plan.second = map;

@@ -33,10 +33,11 @@ __device__ inline int places_of(int len, int shift) { return int((long(len) + (1
 // --- forks --------------------------------------------------------------------------------------
 
 // Every block looks the rows over and sums up the pages that begun pages need (a thread its k rows), so that the call takes
-// effect whole or not at all without a launch before; then row blockIdx.x, ... takes its parent's full pages, and block 0
-// writes what there is one of for a row. FILL and COMMIT as in block_tables_kernel: two launches where lens_out lies over lens
-// or used_out over used and there are several blocks.
+// effect whole or not at all without a launch before; then each wave takes its share of a row's full pages from the parent's, and
+// block 0 writes what there is one of for a row. FILL and COMMIT as in block_tables_kernel: two launches where lens_out lies over
+// lens or used_out over used and there are several blocks.
 // Bound by its chain of loads (parents, lengths, entries, the pool).
+constexpr int FORK_UNIT = 512;  // entries of a row that a wave takes at once
 template <int THREADS, bool FILL, bool COMMIT>
 __global__ void __launch_bounds__(THREADS) fork_pages_kernel(const ForkArgs a) {
   __shared__ uint64_t sums[THREADS / 64];
@@ -65,26 +66,27 @@ __global__ void __launch_bounds__(THREADS) fork_pages_kernel(const ForkArgs a) {
   const bool broken = __syncthreads_or(bad), stray = __syncthreads_or(no_row);
   const int status = broken ? TABLE_BAD_LENGTH : stray ? TABLE_BAD_ROW : long(total) > long(p.pool_size) - used ? TABLE_POOL_EMPTY : TABLE_OK;
   if constexpr (FILL) {
-    if (status == TABLE_OK)
-      for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
+    if (status == TABLE_OK) {
+      const int lane = tid & 63, segs = (p.width + FORK_UNIT - 1) / FORK_UNIT;
+      for (long u = long(blockIdx.x) * (THREADS / 64) + (tid >> 6); u < long(p.n) * segs; u += long(gridDim.x) * (THREADS / 64)) {
+        const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * FORK_UNIT + lane;
         const int from = a.parents[i];
         if (from == -1) continue;
-        const int full = (a.keep ? a.keep[i] : p.lens[from]) >> p.shift, step = int(gridDim.y) * THREADS;
+        const int full = (a.keep ? a.keep[i] : p.lens[from]) >> p.shift;
         const int* old = p.table + long(from) * p.width;
         int* row = p.table + long(i) * p.width;
-        for (long j0 = long(blockIdx.y) * THREADS + tid; j0 < full; j0 += 4L * step) {
-          int page[4];
+        int page[FORK_UNIT / 64];
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (j0 + long(u) * step < full) page[u] = old[j0 + long(u) * step];
+        for (int k = 0; k < FORK_UNIT / 64; ++k)
+          if (j0 + 64 * k < full) page[k] = old[j0 + 64 * k];
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (j0 + long(u) * step < full) row[j0 + long(u) * step] = page[u];
-        }
+        for (int k = 0; k < FORK_UNIT / 64; ++k)
+          if (j0 + 64 * k < full) row[j0 + 64 * k] = page[k];
       }
+    }
   }
   if constexpr (COMMIT) {
-    if (blockIdx.x || blockIdx.y) return;
+    if (blockIdx.x) return;
     for (int i = i0; i < i1; ++i) {
       const int from = status == TABLE_OK ? a.parents[i] : -1;
       int len = p.lens[i], src = -1, dst = -1, rows = 0;
@@ -111,76 +113,116 @@ __global__ void __launch_bounds__(THREADS) fork_pages_kernel(const ForkArgs a) {
 }
 
 // --- maps of pages ------------------------------------------------------------------------------
+//
+// Over many pages a map has a byte a page and the XCDs' caches store into it as they like: all of them store 1. (Bits, set with atomic
+// operations of the device, took 95 us for 320 thousand entries of a thousand rows that share their pages, where the bytes take 6.) Few
+// pages are bits in one block's LDS.
 
-constexpr int MAP_THREADS = PAGE_CHUNK;  // a word of a map a thread
-constexpr int UNIT = 256;                // places of a row that a wave takes at once
+constexpr int MAP_THREADS = PAGE_CHUNK;
+constexpr int UNIT = 256;  // places of a row that a wave takes at once
 struct MapHead {  // in the workspace, one for the launches of a call
   int used, bad;  // bad: bit 0 a length, bit 1 a page
-  int kept, moved, status;  // of compact_pages: live pages that stay, and those that move
+  int kept, status;  // of compact_pages: live pages that stay
 };
 
-// Most pages are in many rows: the bit is looked at before it is set, which two waves in three find done.
-__device__ inline uint32_t set_bit(uint32_t* map, int page) {
-  const uint32_t bit = 1u << (page & 31);
-  uint32_t* at = map + (page >> 5);
-  if (__hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit) return bit;
-  return __hip_atomic_fetch_or(at, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & bit;
-}
+struct ByteMap {
+  uint8_t* at;
+  __device__ inline void set(int page) const { at[page] = 1; }
+};
+struct BitMap {
+  uint32_t* at;
+  __device__ inline void set(int page) const { atomicOr(at + (page >> 5), 1u << (page & 31)); }
+};
 
-// Bits of the pages in the rows, by waves wave, wave + waves, ...: those of the first keep[i] positions in `held`, the others
-// up to lens[i] in `gone` (keep NULL: all of them are held). True where a length is none.
-__device__ inline bool mark_rows(const PagesArgs& p, const int* keep, uint32_t* held, uint32_t* gone, long wave, long waves) {
-  const int lane = threadIdx.x & 63, segs = (p.width + UNIT - 1) / UNIT;
-  bool bad = false;
-  for (long u = wave; u < long(p.n) * segs; u += waves) {
-    const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * UNIT;
-    const int len = p.lens[i], stays = keep ? keep[i] : len;
-    if (len < 0 || len > (long(p.width) << p.shift) || stays < 0 || stays > len) {
-      bad = true;
-      continue;
-    }
-    const int all = places_of(len, p.shift), kept = places_of(stays, p.shift);
-    if (j0 >= all) continue;
+// Places of row i that its keep[i] first positions fill (keep NULL: all), and its lens[i]; false where a length is none.
+__device__ inline bool places_of_row(const PagesArgs& p, const int* keep, int i, int& kept, int& all) {
+  const int len = p.lens[i], stays = keep ? keep[i] : len;
+  const bool ok = len >= 0 && len <= (long(p.width) << p.shift) && stays >= 0 && stays <= len;
+  kept = ok ? places_of(stays, p.shift) : 0;
+  all = ok ? places_of(len, p.shift) : 0;
+  return ok;
+}
+// The pages at places j0 on of row i: kept ones in `held`, the others below `all` in `gone`.
+template <typename Map> struct RowUnit {
+  int page[UNIT / 64], j, kept, all;
+  __device__ inline void load(const PagesArgs& p, int i, int j0, int kept_, int all_) {
+    j = j0 + int(threadIdx.x & 63);
+    kept = kept_;
+    all = all_;
     const int* row = p.table + long(i) * p.width;
-    int page[UNIT / 64];
 #pragma unroll
-    for (int k = 0; k < UNIT / 64; ++k) page[k] = row[min(j0 + 64 * k + lane, all - 1)];
-#pragma unroll
-    for (int k = 0; k < UNIT / 64; ++k) {
-      const int j = j0 + 64 * k + lane;
-      if (j < all && page_ok(page[k], p.pages)) set_bit(j < kept ? held : gone, page[k]);
-    }
+    for (int k = 0; k < UNIT / 64; ++k)
+      if (j + 64 * k < all) page[k] = row[j + 64 * k];
   }
-  return bad;
-}
+  __device__ inline void mark(const PagesArgs& p, const Map& held, const Map& gone) const {
+#pragma unroll
+    for (int k = 0; k < UNIT / 64; ++k)
+      if (j + 64 * k < all && page_ok(page[k], p.pages)) (j + 64 * k < kept ? held : gone).set(page[k]);
+  }
+};
 
-// Bits of the free pages; true where one is there twice, or is none.
-__device__ inline bool mark_pool(const PagesArgs& p, int used, uint32_t* map, long thread, long threads) {
+// The free pages; true where one is none.
+template <typename Map> __device__ inline bool mark_pool(const PagesArgs& p, int used, const Map& map, long thread, long threads) {
   bool bad = false;
   for (long k = used + thread; k < p.pool_size; k += threads) {
     const int page = p.pool[k];
-    bad |= !page_ok(page, p.pages) || set_bit(map, page);
+    if (page_ok(page, p.pages)) map.set(page);
+    else bad = true;
   }
   return bad;
 }
 
-__global__ void __launch_bounds__(256) pages_clear_kernel(uint32_t* maps, long words, MapHead* head, const int* used) {
+__global__ void __launch_bounds__(256) pages_clear_kernel(uint4* maps, long count, MapHead* head, const int* used) {
   const long t = long(blockIdx.x) * 256 + threadIdx.x;
-  for (long w = t; w < words; w += long(gridDim.x) * 256) maps[w] = 0;
-  if (t == 0) *head = {*used, 0, 0, 0, 0};
+  for (long w = t; w < count; w += long(gridDim.x) * 256) maps[w] = make_uint4(0, 0, 0, 0);
+  if (t == 0) *head = {*used, 0, 0, 0};
 }
 
 // The first map from kept places (and free pages), the second from those given back; compact: live pages, then free ones.
 template <bool COMPACT>
-__global__ void __launch_bounds__(256) pages_mark_kernel(const PagesArgs p, const int* keep, uint32_t* first, uint32_t* second, MapHead* head) {
-  const long t = long(blockIdx.x) * 256 + threadIdx.x, all = long(gridDim.x) * 256;
-  const int used = head->used;
+__global__ void __launch_bounds__(256) pages_mark_kernel(const PagesArgs p, const int* keep, uint8_t* first, uint8_t* second, MapHead* head) {
+  const long t = long(blockIdx.x) * 256 + threadIdx.x, all_threads = long(gridDim.x) * 256;
+  const int used = head->used, segs = (p.width + UNIT - 1) / UNIT;
   int bad = 0;
   if (used < 0 || used > p.pool_size) bad = 1;
-  else if (mark_pool(p, used, COMPACT ? second : first, t, all) && COMPACT) bad |= 2;
-  if (mark_rows(p, keep, first, second, t >> 6, all >> 6)) bad |= 1;
+  else if (mark_pool(p, used, ByteMap{COMPACT ? second : first}, t, all_threads) && COMPACT) bad = 2;
+  for (long u = t >> 6; u < long(p.n) * segs; u += all_threads >> 6) {
+    const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * UNIT;
+    int kept, all;
+    if (!places_of_row(p, keep, i, kept, all)) bad |= 1;
+    if (j0 >= all) continue;
+    RowUnit<ByteMap> unit;
+    unit.load(p, i, j0, kept, all);
+    unit.mark(p, {first}, {second});
+  }
   if (bad) atomicOr(&head->bad, bad);
 }
+
+// The same by one block in LDS. Lengths come first, for all rows at once, and four units of each wave are under way. bad: a length; none: a
+// free page.
+constexpr int SMALL_ROWS = 2048;
+__device__ inline void mark_small(const PagesArgs& p, const int* keep, int used, const BitMap& pool, const BitMap& held, const BitMap& gone, int2* places, bool& bad,
+                                  bool& none) {
+  const int tid = threadIdx.x, wave = tid >> 6, segs = (p.width + UNIT - 1) / UNIT, units = p.n * segs;
+  for (int i = tid; i < p.n; i += MAP_THREADS) bad |= !places_of_row(p, keep, i, places[i].x, places[i].y);
+  __syncthreads();  // the maps are empty, the places there
+  bad |= used < 0 || used > p.pool_size;
+  none = used >= 0 && mark_pool(p, used, pool, tid, MAP_THREADS);
+  constexpr int WAVES = MAP_THREADS / 64, AHEAD = 4;
+  for (int u0 = wave; u0 < units; u0 += AHEAD * WAVES) {
+    RowUnit<BitMap> unit[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int u = min(u0 + k * WAVES, units - 1), i = u / segs;  // the last one again changes nothing
+      unit[k].load(p, i, (u - i * segs) * UNIT, places[i].x, places[i].y);
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) unit[k].mark(p, held, gone);
+  }
+}
+
+// Four bytes of a map as four bits.
+__device__ inline uint32_t bits_of(uint32_t bytes) { return ((bytes & 0x01010101u) * 0x01020408u) >> 24 & 15u; }
 
 // Pages of a word that are given back; live and free pages (low and high half). A page that is both is bad.
 template <bool COMPACT> __device__ inline uint64_t count_word(uint32_t first, uint32_t second, bool& bad) {
@@ -189,12 +231,13 @@ template <bool COMPACT> __device__ inline uint64_t count_word(uint32_t first, ui
   return uint64_t(__popc(second)) << 32 | uint64_t(__popc(first));
 }
 
+// A thread four pages: the counts of each chunk of 4096.
 template <bool COMPACT>
 __global__ void __launch_bounds__(MAP_THREADS) pages_count_kernel(const uint32_t* first, const uint32_t* second, long words, uint64_t* counts, MapHead* head) {
   __shared__ uint64_t sums[MAP_THREADS / 64];
-  const long w = long(blockIdx.x) * PAGE_CHUNK + threadIdx.x;
+  const long w = long(blockIdx.x) * MAP_THREADS + threadIdx.x;
   bool bad = false;
-  const uint64_t v = w < words ? count_word<COMPACT>(first[w], second[w], bad) : 0;
+  const uint64_t v = w < words ? count_word<COMPACT>(bits_of(first[w]), bits_of(second[w]), bad) : 0;
   uint64_t total;
   scan_block<MAP_THREADS>(v, sums, total);
   if (threadIdx.x == 0) counts[blockIdx.x] = total;
@@ -205,8 +248,9 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_count_kernel(const uint32_t
 __device__ inline uint64_t sum_counts(const uint64_t* counts, long chunks, long chunk, uint64_t* sums, uint64_t& total) {
   uint64_t before = 0, all = 0, b, t;
   for (long c = threadIdx.x; c < chunks; c += MAP_THREADS) {
-    all += counts[c];
-    if (c < chunk) before += counts[c];
+    const uint64_t v = counts[c];
+    all += v;
+    if (c < chunk) before += v;
   }
   scan_block<MAP_THREADS>(before, sums, b);
   scan_block<MAP_THREADS>(all, sums, t);
@@ -214,12 +258,12 @@ __device__ inline uint64_t sum_counts(const uint64_t* counts, long chunks, long 
   return b;
 }
 
-// A chunk's pages that are given back, in their order, into the pool in front of the free ones.
-__device__ inline void write_freed(const FreeArgs& a, uint32_t bits, long word, uint64_t rank, uint64_t total, int used, int bad, long thread, long threads) {
+// The pages of a word (from `page` on) that are given back, in their order, into the pool in front of the free ones.
+__device__ inline void write_freed(const FreeArgs& a, uint32_t bits, int page, uint64_t rank, uint64_t total, int used, int bad, long thread, long threads) {
   const PagesArgs& p = a.at;
   const int status = bad & 1 ? TABLE_BAD_LENGTH : long(total) > used ? TABLE_BAD_PAGE : TABLE_OK;
   if (status == TABLE_OK)
-    for (long at = used - long(total) + long(rank); bits; bits &= bits - 1, ++at) p.pool[at] = int(word * 32) + __builtin_ctz(bits);
+    for (long at = used - long(total) + long(rank); bits; bits &= bits - 1, ++at) p.pool[at] = page + __builtin_ctz(bits);
   for (long i = thread; i < p.n; i += threads) a.lens_out[i] = status == TABLE_OK ? a.keep[i] : p.lens[i];
   if (thread == 0) {
     *a.used_out = status == TABLE_OK ? used - int(total) : used;
@@ -230,29 +274,28 @@ __device__ inline void write_freed(const FreeArgs& a, uint32_t bits, long word, 
 __global__ void __launch_bounds__(MAP_THREADS) pages_free_kernel(const FreeArgs a, const uint32_t* held, const uint32_t* gone, long words, const uint64_t* counts,
                                                                  const MapHead* head) {
   __shared__ uint64_t sums[MAP_THREADS / 64];
-  const long w = long(blockIdx.x) * PAGE_CHUNK + threadIdx.x;
-  const uint32_t bits = w < words ? gone[w] & ~held[w] : 0;
+  const long w = long(blockIdx.x) * MAP_THREADS + threadIdx.x;
+  const uint32_t bits = w < words ? bits_of(gone[w]) & ~bits_of(held[w]) : 0;
   uint64_t total;
   uint64_t rank = scan_block<MAP_THREADS>(__popc(bits), sums, total);
   if (gridDim.x > 1) rank += sum_counts(counts, gridDim.x, blockIdx.x, sums, total);
-  write_freed(a, bits, w, rank, total, head->used, head->bad, w, long(gridDim.x) * MAP_THREADS);
+  write_freed(a, bits, int(w * 4), rank, total, head->used, head->bad, w, long(gridDim.x) * MAP_THREADS);
 }
 
 // Few rows and pages: the maps in LDS and all of it in one launch.
 __global__ void __launch_bounds__(MAP_THREADS) pages_free_small_kernel(const FreeArgs a) {
   __shared__ uint64_t sums[MAP_THREADS / 64];
-  __shared__ uint32_t held[PAGE_CHUNK], gone[PAGE_CHUNK];
+  __shared__ uint32_t held[MAP_THREADS], gone[MAP_THREADS];
+  __shared__ int2 places[SMALL_ROWS];
   const int tid = threadIdx.x, used = *a.at.used;
   held[tid] = gone[tid] = 0;
-  __syncthreads();
-  bool bad = used < 0 || used > a.at.pool_size;
-  if (!bad) mark_pool(a.at, used, held, tid, MAP_THREADS);
-  bad |= mark_rows(a.at, a.keep, held, gone, tid >> 6, MAP_THREADS / 64);
+  bool bad = false, none;
+  mark_small(a.at, a.keep, used, {held}, {held}, {gone}, places, bad, none);
   bad = __syncthreads_or(bad);
   const uint32_t bits = gone[tid] & ~held[tid];
   uint64_t total;
   const uint64_t rank = scan_block<MAP_THREADS>(__popc(bits), sums, total);
-  write_freed(a, bits, tid, rank, total, used, bad, tid, MAP_THREADS);
+  write_freed(a, bits, tid * 32, rank, total, used, bad, tid, MAP_THREADS);
 }
 
 // --- compaction ---------------------------------------------------------------------------------
@@ -268,12 +311,12 @@ __device__ inline int holes_in(uint32_t live, uint32_t free, int need) {
   return holes;
 }
 
-// A word's part of the result. before: live (low half) and free pages before it.
-__device__ inline void write_moves(const CompactArgs& a, uint32_t live, uint32_t free, long word, uint64_t before, int used, long in_use, long moved) {
+// A word's part of the result, whose pages are those from page0 on. before: live (low half) and free pages before it.
+__device__ inline void write_moves(const CompactArgs& a, uint32_t live, uint32_t free, int page0, uint64_t before, int used, long in_use, long moved) {
   uint32_t both = live | free;
   long l = long(before & 0xffffffffu), f = long(before >> 32);
   for (; both; both &= both - 1) {
-    const int page = int(word * 32) + __builtin_ctz(both);
+    const int page = page0 + __builtin_ctz(both);
     const bool is_live = live & (both & -both);
     const long rank = l + f - in_use;  // among the pages that are to be free
     if (rank >= 0) a.pool_out[used + rank] = page;
@@ -295,8 +338,9 @@ __device__ inline void write_rest(const CompactArgs& a, int status, int used, lo
   }
 }
 
-// The rows' entries where their pages are now. before[w]: live pages before word w.
-__device__ inline void rewrite_rows(const CompactArgs& a, const uint32_t* live, const int* before, int status, int kept, long wave, long waves) {
+// The rows' entries where their pages are now. rank_of(page): how many live pages are before it.
+template <typename Rank>
+__device__ inline void rewrite_rows(const CompactArgs& a, int status, int kept, long wave, long waves, Rank&& rank_of) {
   const PagesArgs& p = a.at;
   const bool in_place = a.table_out == p.table;
   const int lane = threadIdx.x & 63, segs = (p.width + UNIT - 1) / UNIT;
@@ -304,24 +348,24 @@ __device__ inline void rewrite_rows(const CompactArgs& a, const uint32_t* live, 
   for (long u = wave; u < long(p.n) * segs; u += waves) {
     const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * UNIT;
     const int all = status == TABLE_OK ? places_of(p.lens[i], p.shift) : 0, end = in_place ? all : p.width;
+    if (j0 >= end) continue;
     const int* row = p.table + long(i) * p.width;
     int* out = a.table_out + long(i) * p.width;
-    int page[UNIT / 64];
+    int page[UNIT / 64], rank[UNIT / 64];
 #pragma unroll
     for (int k = 0; k < UNIT / 64; ++k) {
       const int j = j0 + 64 * k + lane;
       page[k] = j < end ? row[j] : -1;
     }
 #pragma unroll
+    for (int k = 0; k < UNIT / 64; ++k) rank[k] = j0 + 64 * k + lane < all && page_ok(page[k], p.pages) ? rank_of(page[k]) : -1;
+#pragma unroll
+    for (int k = 0; k < UNIT / 64; ++k)
+      if (rank[k] >= kept) page[k] = a.dst[rank[k] - kept];  // kept is not negative
+#pragma unroll
     for (int k = 0; k < UNIT / 64; ++k) {
       const int j = j0 + 64 * k + lane;
-      if (j >= end) continue;
-      int now = page[k];
-      if (j < all && page_ok(now, p.pages)) {
-        const int w = now >> 5, rank = before[w] + __popc(live[w] & ((1u << (now & 31)) - 1));
-        if (rank >= kept) now = a.dst[rank - kept];
-      }
-      out[j] = now;
+      if (j < end) out[j] = page[k];
     }
   }
 }
@@ -332,8 +376,8 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_move_kernel(const CompactAr
   __shared__ long at_chunk, at_count;
   __shared__ uint64_t at_before;
   const int tid = threadIdx.x;
-  const long w = long(blockIdx.x) * PAGE_CHUNK + tid, chunks = gridDim.x;
-  const uint32_t l = w < words ? live[w] : 0, f = w < words ? free[w] : 0;
+  const long w = long(blockIdx.x) * MAP_THREADS + tid, chunks = gridDim.x;
+  const uint32_t l = w < words ? bits_of(live[w]) : 0, f = w < words ? bits_of(free[w]) : 0;
   bool both = false;
   uint64_t total, ahead = scan_block<MAP_THREADS>(count_word<true>(l, f, both), sums, total);
   if (chunks > 1) ahead += sum_counts(counts, chunks, blockIdx.x, sums, total);
@@ -360,17 +404,18 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_move_kernel(const CompactAr
     }
     __syncthreads();
   }
-  const long w2 = at_chunk * PAGE_CHUNK + tid;
-  const uint32_t l2 = w2 < words ? live[w2] : 0, f2 = w2 < words ? free[w2] : 0;
+  const long w2 = at_chunk * MAP_THREADS + tid;
+  const uint32_t l2 = w2 < words ? bits_of(live[w2]) : 0, f2 = w2 < words ? bits_of(free[w2]) : 0;
   uint64_t sum2;
   const uint64_t v2 = count_word<true>(l2, f2, both), b2 = at_before + scan_block<MAP_THREADS>(v2, sums, sum2);
   if (pages_in(b2) < in_use && in_use <= pages_in(b2) + pages_in(v2)) at_count = long(b2 >> 32) + holes_in(l2, f2, int(in_use - pages_in(b2)));
   __syncthreads();
   const long moved = at_count;
-  const int used = head->used, bad = head->bad | (twice ? 2 : 0);
+  // a free page that is there twice leaves fewer of them than the pool has
+  const int used = head->used, bad = head->bad | (twice || (!(head->bad & 1) && long(total >> 32) != long(a.at.pool_size) - used) ? 2 : 0);
   const int status = bad & 1 ? TABLE_BAD_LENGTH : bad ? TABLE_BAD_PAGE : moved > a.cap ? TABLE_SLOTS_FULL : TABLE_OK;
   if (w < words) before[w] = int(ahead & 0xffffffffu);
-  if (status == TABLE_OK && w < words) write_moves(a, l, f, w, ahead, used, in_use, moved);
+  if (status == TABLE_OK && w < words) write_moves(a, l, f, int(w * 4), ahead, used, in_use, moved);
   write_rest(a, status, used, moved, w, chunks * MAP_THREADS);
   if (w == 0) {
     head->kept = int(in_use - moved);
@@ -380,26 +425,29 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_move_kernel(const CompactAr
 
 __global__ void __launch_bounds__(256) pages_rewrite_kernel(const CompactArgs a, const uint32_t* live, const int* before, const MapHead* head) {
   const long t = long(blockIdx.x) * 256 + threadIdx.x;
-  rewrite_rows(a, live, before, head->status, head->kept, t >> 6, long(gridDim.x) * 4);
+  rewrite_rows(a, head->status, head->kept, t >> 6, long(gridDim.x) * 4, [&](int page) {
+    const int w = page >> 2;
+    return before[w] + __popc(live[w] & 0x01010101u & ((1u << (8 * (page & 3))) - 1));
+  });
 }
 
 // Few rows and pages: the maps in LDS and all of it in one launch.
 __global__ void __launch_bounds__(MAP_THREADS) pages_compact_small_kernel(const CompactArgs a) {
   __shared__ uint64_t sums[MAP_THREADS / 64];
-  __shared__ uint32_t live[PAGE_CHUNK], free[PAGE_CHUNK];
-  __shared__ int before[PAGE_CHUNK];
+  __shared__ uint32_t live[MAP_THREADS], free[MAP_THREADS];
+  __shared__ int before[MAP_THREADS];
+  __shared__ int2 places[SMALL_ROWS];
   __shared__ long holes;
   const int tid = threadIdx.x, used = *a.at.used;
   live[tid] = free[tid] = 0;
   if (tid == 0) holes = 0;
-  __syncthreads();
-  bool bad = used < 0 || used > a.at.pool_size, none = false;
-  if (!bad) none = mark_pool(a.at, used, free, tid, MAP_THREADS);
-  bad |= mark_rows(a.at, nullptr, live, nullptr, tid >> 6, MAP_THREADS / 64);
+  bool bad = false, none;
+  mark_small(a.at, nullptr, used, {free}, {live}, {live}, places, bad, none);
   bad = __syncthreads_or(bad);
   const uint32_t l = live[tid], f = free[tid];
   uint64_t total;
   const uint64_t v = count_word<true>(l, f, none), ahead = scan_block<MAP_THREADS>(v, sums, total);
+  none |= !bad && long(total >> 32) != long(a.at.pool_size) - used;  // a free page that is there twice
   none = __syncthreads_or(none);
   const long in_use = long(total & 0xffffffffu), first = long(ahead & 0xffffffffu) + long(ahead >> 32), here = long(v & 0xffffffffu) + long(v >> 32);
   if (first < in_use && in_use <= first + here) holes = long(ahead >> 32) + holes_in(l, f, int(in_use - first));
@@ -407,10 +455,11 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_compact_small_kernel(const 
   __syncthreads();
   const long moved = holes;
   const int status = bad ? TABLE_BAD_LENGTH : none ? TABLE_BAD_PAGE : moved > a.cap ? TABLE_SLOTS_FULL : TABLE_OK;
-  if (status == TABLE_OK) write_moves(a, l, f, tid, ahead, used, in_use, moved);
+  if (status == TABLE_OK) write_moves(a, l, f, tid * 32, ahead, used, in_use, moved);
   write_rest(a, status, used, moved, tid, MAP_THREADS);
   __syncthreads();  // dst is there
-  rewrite_rows(a, live, before, status, int(in_use - moved), tid >> 6, MAP_THREADS / 64);
+  rewrite_rows(a, status, int(in_use - moved), tid >> 6, MAP_THREADS / 64,
+               [&](int page) { return before[page >> 5] + __popc(live[page >> 5] & ((1u << (page & 31)) - 1)); });
 }
 
 // --- copies -------------------------------------------------------------------------------------
@@ -453,32 +502,36 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyArgs
   }
 }
 
-// Places of all rows up to which one block marks them in LDS.
-constexpr long SMALL_PLACES = 65536;
+constexpr long FORK_BLOCKS = 256;  // each of which looks all rows over
 
-bool small(const PagesArgs& p) { return pages_plan(p.pages).chunks == 1 && long(p.n) * p.width <= SMALL_PLACES; }
+// Pages and places of all rows up to which one block takes them in LDS.
+constexpr int SMALL_PAGES = MAP_THREADS * 32;
+constexpr long SMALL_PLACES = 65536;
+bool small(const PagesArgs& p) { return p.pages <= SMALL_PAGES && p.n <= SMALL_ROWS && long(p.n) * p.width <= SMALL_PLACES; }
 
 // Waves that the rows' units fill, four a block, no more than the chip holds several times.
 int mark_blocks(const PagesArgs& p) { return int(std::max<long>(1, std::min<long>(2048, (long(p.n) * cdiv(p.width, UNIT) + 3) / 4))); }
 
 struct Maps {
-  uint32_t* first; uint32_t* second; int* before; uint64_t* counts; MapHead* head;
+  uint8_t* first; uint8_t* second; int* before; uint64_t* counts; MapHead* head;
   Maps(const PagesPlan& plan, void* workspace) {
     char* ws = static_cast<char*>(workspace);
-    first = reinterpret_cast<uint32_t*>(ws);
-    second = reinterpret_cast<uint32_t*>(ws + plan.second);
+    first = reinterpret_cast<uint8_t*>(ws);
+    second = reinterpret_cast<uint8_t*>(ws + plan.second);
     before = reinterpret_cast<int*>(ws + plan.before);
     counts = reinterpret_cast<uint64_t*>(ws + plan.counts);
     head = reinterpret_cast<MapHead*>(ws + plan.head);
   }
+  const uint32_t* first4() const { return reinterpret_cast<const uint32_t*>(first); }
+  const uint32_t* second4() const { return reinterpret_cast<const uint32_t*>(second); }
 };
 
 // The maps of a call's pages, and the counts of their chunks where there are several.
 template <bool COMPACT> void fill_maps(const Exec& ex, const PagesArgs& p, const int* keep, const PagesPlan& plan, const Maps& m) {
-  const long words = (plan.second + plan.words * 4) / 4;
-  pages_clear_kernel<<<std::max(1, std::min(cdiv(words, 256), 2048)), 256, 0, ex.stream>>>(m.first, words, m.head, p.used);
+  const long count = long(plan.before / 16);  // both maps
+  pages_clear_kernel<<<int(std::max<long>(1, std::min<long>((count + 255) / 256, 2048))), 256, 0, ex.stream>>>(reinterpret_cast<uint4*>(m.first), count, m.head, p.used);
   pages_mark_kernel<COMPACT><<<mark_blocks(p), 256, 0, ex.stream>>>(p, keep, m.first, m.second, m.head);
-  if (plan.chunks > 1) pages_count_kernel<COMPACT><<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(m.first, m.second, plan.words, m.counts, m.head);
+  if (plan.chunks > 1) pages_count_kernel<COMPACT><<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(m.first4(), m.second4(), plan.words, m.counts, m.head);
 }
 
 }  // namespace
@@ -491,8 +544,8 @@ void fork_pages(const Exec& ex, const ForkArgs& args) {
   ProfScope prof(ex, "fork_pages", 0, 8.0 * p.n * p.width + 32.0 * p.n);
   auto launch = [&](auto threads) {
     constexpr int N = decltype(threads)::value;
-    const dim3 grid(std::max(1, std::min(p.n, 1024)), std::max(1, std::min(cdiv(p.width, 4 * N), cdiv(1024, std::max(p.n, 1)))));
-    if ((grid.x == 1 && grid.y == 1) || (a.lens_out != p.lens && a.used_out != p.used)) {
+    const int grid = int(std::max<long>(1, std::min<long>(FORK_BLOCKS, (long(p.n) * cdiv(p.width, FORK_UNIT) + N / 64 - 1) / (N / 64))));
+    if (grid == 1 || (a.lens_out != p.lens && a.used_out != p.used)) {
       fork_pages_kernel<N, true, true><<<grid, N, 0, ex.stream>>>(a);
     } else {
       fork_pages_kernel<N, true, false><<<grid, N, 0, ex.stream>>>(a);
@@ -516,7 +569,7 @@ void free_pages(const Exec& ex, const FreeArgs& args, void* workspace, size_t by
     const PagesPlan plan = pages_plan(p.pages);
     const Maps m(plan, workspace);
     fill_maps<false>(ex, p, a.keep, plan, m);
-    pages_free_kernel<<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(a, m.first, m.second, plan.words, m.counts, m.head);
+    pages_free_kernel<<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(a, m.first4(), m.second4(), plan.words, m.counts, m.head);
   }
   SPLAT_HIP(hipGetLastError());
 }
@@ -533,8 +586,8 @@ void compact_pages(const Exec& ex, const CompactArgs& args, void* workspace, siz
     const PagesPlan plan = pages_plan(p.pages);
     const Maps m(plan, workspace);
     fill_maps<true>(ex, p, nullptr, plan, m);
-    pages_move_kernel<<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(a, m.first, m.second, plan.words, m.before, m.counts, m.head);
-    pages_rewrite_kernel<<<mark_blocks(p), 256, 0, ex.stream>>>(a, m.first, m.before, m.head);
+    pages_move_kernel<<<int(plan.chunks), MAP_THREADS, 0, ex.stream>>>(a, m.first4(), m.second4(), plan.words, m.before, m.counts, m.head);
+    pages_rewrite_kernel<<<mark_blocks(p), 256, 0, ex.stream>>>(a, m.first4(), m.before, m.head);
   }
   SPLAT_HIP(hipGetLastError());
 }
