@@ -549,7 +549,7 @@ size_t prefix_attention_bytes(const KvCache& c, int n, int heads, int groups, in
   if (n == 0 || groups == 0) return 0;
   const int G = heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;
   const size_t item = long(n) * heads + std::min<long>(groups, n) * c.kv_heads * WIDE_ROWS;
-  const size_t cut = std::min<size_t>(size_t(WIDE_BLOCKS) * 4 * WIDE_ROWS, item * ((max_shared + keys - 1L) / keys));
+  const size_t cut = std::min<size_t>(size_t(WIDE_BLOCKS) * 4 * WIDE_ROWS, item * ((long(max_shared) + keys - 1) / keys));
   // own parts: one a token and column group, or as many as there are blocks for
   const size_t cols = size_t(c.kv_heads) * ((G + 15) / 16);
   const size_t own = max_own == 0 ? 0 : std::max<size_t>(size_t(n) * heads, size_t(OWN_BLOCKS) / cols * heads);
