@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
 //
 // Bound by the matrix instructions and by the vector unit's work on the scores, about as much of either: so half a tile's products
 // with K and the half before the last one's with V are under way while the half between becomes weights, all in one wave's stream,
-// and three waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 113 us and the join's 14 (0.70 PFLOP/s).
+// and three waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 112 us and the join's 10 (0.70 PFLOP/s).
 // Of a SIMD's cycles 1024 go to the matrix instructions of a tile of 64 columns and 1250 to the vector unit (half of them
 // exponentials), and 60% of the former lie beside the latter. Two blocks a CU with a tile more under way took 130 us, waves of 64 columns 125, two teams
 // of waves that multiply and exponentiate in turn 140, the compiler's own order of the same instructions 6% more than this one.
@@ -896,48 +896,64 @@ __global__ void __launch_bounds__(WAVES * 64, WIDE_OCCUPANCY) prefix_wide_kernel
 
 // --- the join -----------------------------------------------------------------------------------
 
-// One wave a (token, head): 16 lanes a part, four channels each, so that four parts are one load and 4 AT_ONCE are under way. Bound by its
-// chain of loads (starts, the plan, the parts), and by the parts' bytes where there are many rows.
+// 16 lanes hold a part's column, four channels each. A wave takes one (token, head), four parts a load and 4 AT_ONCE under way, or four
+// (token, head)s, a part of each a load, where there are MANY_COLUMNS, so that all of them are on the chip at once. Bound by its chain of
+// loads (starts, the plan, the parts), and by the parts' bytes where there are many rows. Measured, one / four a wave: 768 of them 5.7 / 6.9 us,
+// 1536 7.4 / 8.9, 12444 (seven parts, 26 MB) 14.2 / 9.8; of whole calls 4800 65.3 / 65.9, 7200 80.0 / 78.9, 9600 99.6 / 97.4.
 constexpr int JOIN_WAVES = 4, AT_ONCE = 8;
-template <typename T>
+constexpr long MANY_COLUMNS = 6144;  // (token, head)s
+template <typename T, int COLUMNS>
 __global__ void __launch_bounds__(JOIN_WAVES * 64) prefix_join_kernel(const PrefixArgs a, int R, int own, size_t parts, size_t own_parts, char* workspace) {
+  constexpr int ACROSS = 4 / COLUMNS;  // parts of a load
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), quad = lane & 15, g = lane >> 4;
-  const int u = int(blockIdx.x) * JOIN_WAVES + wave;  // below 2^21
-  if (u >= a.n * a.heads) return;
+  const int u0 = (int(blockIdx.x) * JOIN_WAVES + wave) * COLUMNS, all_columns = a.n * a.heads;  // below 2^21
+  if (u0 >= all_columns) return;
   const GroupPlan* plans = reinterpret_cast<const GroupPlan*>(workspace + sizeof(PlanHead));
   // for up to 64 groups what is asked of them comes in one load, a group a lane
   const int near = min(lane, a.groups - 1), valid = reinterpret_cast<const PlanHead*>(workspace)->valid, begin = start_of(a, near), end = start_of(a, near + 1);
-  GroupPlan plan = plans[near];
+  const GroupPlan near_plan = plans[near];
   if (!valid) return;
-  const int i = u / a.heads, head = u % a.heads;
-  if (a.groups <= 64) {
-    const uint64_t in = __ballot(lane < a.groups && begin <= i && i < end);
-    if (!in) return;
-    const int l = 63 - __builtin_clzll(in);
-    plan = {__builtin_amdgcn_readlane(plan.block0, l), __builtin_amdgcn_readlane(plan.parts, l), __builtin_amdgcn_readlane(plan.items, l),
-            __builtin_amdgcn_readlane(plan.row0, l)};
-  } else {
-    const int group = group_of(a, i);
-    if (group < 0) return;
-    plan = plans[group];
+  const int u = u0 + (COLUMNS > 1 ? g : 0), i = u / a.heads, head = u - i * a.heads;
+  GroupPlan plan = {};
+  bool found = false;
+#pragma unroll
+  for (int x = 0; x < COLUMNS; ++x) {
+    const int token = COLUMNS > 1 ? __builtin_amdgcn_readlane(i, 16 * x) : i;
+    GroupPlan its;
+    if (a.groups <= 64) {
+      const uint64_t in = __ballot(lane < a.groups && begin <= token && token < end);
+      if (!in) continue;
+      const int l = 63 - __builtin_clzll(in);
+      its = {__builtin_amdgcn_readlane(near_plan.block0, l), __builtin_amdgcn_readlane(near_plan.parts, l), __builtin_amdgcn_readlane(near_plan.items, l),
+             __builtin_amdgcn_readlane(near_plan.row0, l)};
+    } else {
+      const int group = group_of(a, min(token, a.n - 1));
+      if (group < 0) continue;
+      its = plans[group];
+    }
+    if (COLUMNS == 1 || g == x) {
+      plan = its;
+      found = true;
+    }
   }
+  found &= u < all_columns;
   const KvCache& c = a.cache;
-  const int G = a.heads / c.kv_heads, kh = head / G, e = head % G;
-  const int r = (i - plan.row0) * G + e, item = r / R, column = r % R, columns = min(G, 16), cols = c.kv_heads * ((G + 15) / 16);
+  const int G = a.heads / c.kv_heads, kh = head / G, e = head - kh * G;
+  const int r = (i - plan.row0) * G + e, item = r / R, column = r - item * R, columns = min(G, 16), cols = c.kv_heads * ((G + 15) / 16);
   const long own0 = (long(i) * cols + kh * ((G + 15) / 16) + e / 16) * own;
-  const int count = plan.parts + own;
+  const int count = found ? plan.parts + own : 0;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f, m = -INFINITY;
   bool some = false;
-  for (int k0 = 0; k0 < count; k0 += 4 * AT_ONCE) {
+  for (int k0 = 0; k0 < count; k0 += ACROSS * AT_ONCE) {
     float2 ml[AT_ONCE];
     float4 o[AT_ONCE];
     float mx = m;
 #pragma unroll
     for (int x = 0; x < AT_ONCE; ++x) {
-      const int k = k0 + 4 * x + g;
+      const int k = k0 + ACROSS * x + (COLUMNS > 1 ? 0 : g);
       ml[x] = make_float2(0.f, -1.f);
-      if (k0 + 4 * x >= count || k >= count) continue;
+      if (k0 + ACROSS * x >= count || k >= count) continue;
       const bool mine = k >= plan.parts;
       const int width = mine ? columns : R, at = mine ? e % 16 : column;
       const float* p = mine ? part_at(workspace, own_parts, own0 + k - plan.parts, columns)
@@ -963,18 +979,22 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) prefix_join_kernel(const Pref
         sum += ml[x].y * f;
       }
   }
-  // the four groups of lanes; one without a key has zeros, whatever the others hold
-  const float top = max_groups(m), f = m == -INFINITY ? 0.f : exp_of(m - top);
-  const bool any = max_groups(some ? 1.f : 0.f) > 0.f;
-  auto all = [&](float v) { return sum_groups(some ? v * f : 0.f); };
-  const float inv = all(sum), v[4] = {all(acc.x), all(acc.y), all(acc.z), all(acc.w)};
-  if (g) return;
-  float w[4];
+  float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  if constexpr (COLUMNS == 1) {  // the four groups of lanes; one without a key has zeros, whatever the others hold
+    const float top = max_groups(m), f = m == -INFINITY ? 0.f : exp_of(m - top);
+    auto all = [&](float x) { return sum_groups(some ? x * f : 0.f); };
+    sum = all(sum);
 #pragma unroll
-  for (int x = 0; x < 4; ++x) w[x] = any ? v[x] / inv : 0.f;
+    for (int x = 0; x < 4; ++x) v[x] = all(v[x]);
+    some = max_groups(some ? 1.f : 0.f) > 0.f;
+    if (g) return;
+  }
+  if (!found) return;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) v[x] = some ? v[x] / sum : 0.f;
   T* out = static_cast<T*>(a.out) + long(i) * a.ldo + long(head) * 64 + quad * 4;
-  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(w[0], w[1], w[2], w[3]);
-  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(w[0], w[1]), pack2<T>(w[2], w[3]));
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+  else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
 }
 
 }  // namespace
@@ -1003,8 +1023,13 @@ void prefix_attention(const Exec& ex, const PrefixArgs& args, void* workspace, s
       if (own) prefix_own_kernel<T><<<int(own), WAVES * 64, 0, ex.stream>>>(a, plan.own, plan.own_parts, ws);
       prefix_wide_kernel<T><<<plan.blocks, WAVES * 64, 0, ex.stream>>>(a, plan.blocks, plan.join, plan.parts, ws);
     }
-    if (plan.join)
-      prefix_join_kernel<T><<<cdiv(long(a.n) * a.heads, JOIN_WAVES), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.rows, plan.own, plan.parts, plan.own_parts, ws);
+    auto join = [&](auto columns) {
+      constexpr int N = decltype(columns)::value;
+      prefix_join_kernel<T, N><<<cdiv(long(a.n) * a.heads, JOIN_WAVES * N), JOIN_WAVES * 64, 0, ex.stream>>>(a, plan.rows, plan.own, plan.parts, plan.own_parts, ws);
+    };
+    if (!plan.join) return;
+    if (long(a.n) * a.heads >= MANY_COLUMNS) join(std::integral_constant<int, 4>());
+    else join(std::integral_constant<int, 1>());
   });
   SPLAT_HIP(hipGetLastError());
 }

@@ -162,6 +162,22 @@ TOKENS = [([1], [1], 1, 1, 8), ([37], [500], 6, 6, 16), ([300, 1, 70], [1037, 0,
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("members,shared,own,heads,kv", [
+    ([90, 0, 91] * 35 + [0], [40 + 7 * i % 300 for i in range(106)], lambda i: i % 5 * 9, 1, 1), ([1, 70, 450], [0, 1500, 2000], lambda i: i % 40, 12, 2),
+    ([300] * 3, [3000, 700, 5], lambda i: 0, 7, 1),
+])
+def test_many_tokens_and_heads(ctx, dtype, members, shared, own, heads, kv):
+    """Parts of several groups' columns in a wave of the join."""
+    n = sum(members)
+    report("prefix.many", dtype=dtype, members=members[:4], heads=heads, kv=kv)
+    s = Shared(dtype, members, shared, [own(i) for i in range(n)], heads, kv, 16)
+    out = s.run(ctx)
+    ends = np.cumsum(members)
+    s.check(out, rows=sorted({i for e in [0, *ends.tolist()] for i in (e - 1, e, e + 1) if 0 <= i < n} | set(range(0, n, 97))))
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("members,shared,heads,kv,ps", TOKENS)
 def test_tokens_of_requests(ctx, dtype, causal, members, shared, heads, kv, ps):
