@@ -1,8 +1,8 @@
 // What happens to the pages of a cache: rows that become forks of others and share their pages, pages given back that no row
 // holds any more, pages moved so that those in use come first, and the copies that forks and moves ask for.
 //
-// Which pages are in use follows from the tables alone: no counts of holders are kept that a call could miss. Maps of one
-// bit a page are filled from the rows and read in the order of the pages, so that what is given back, and what moves where,
+// Which pages are in use follows from the tables alone: no counts of holders are kept that a call could miss. Maps of the
+// pages are filled from the rows and read in the order of the pages, so that what is given back, and what moves where,
 // does not hang on the order in which threads come. Entries outside [0, pages) are no pages.
 #include "paged.h"
 
@@ -161,10 +161,10 @@ template <typename Map> struct RowUnit {
   }
 };
 
-// The free pages; true where one is none.
-template <typename Map> __device__ inline bool mark_pool(const PagesArgs& p, int used, const Map& map, long thread, long threads) {
+// The free pages from the first-th on; true where one is none.
+template <typename Map> __device__ inline bool mark_pool(const PagesArgs& p, long first, const Map& map, long thread, long threads) {
   bool bad = false;
-  for (long k = used + thread; k < p.pool_size; k += threads) {
+  for (long k = first + thread; k < p.pool_size; k += threads) {
     const int page = p.pool[k];
     if (page_ok(page, p.pages)) map.set(page);
     else bad = true;
@@ -198,17 +198,23 @@ __global__ void __launch_bounds__(256) pages_mark_kernel(const PagesArgs p, cons
   if (bad) atomicOr(&head->bad, bad);
 }
 
-// The same by one block in LDS. Lengths come first, for all rows at once, and four units of each wave are under way. bad: a length; none: a
-// free page.
+// The same by one block in LDS. Lengths come first, for all rows at once, then POOL_AHEAD thousand free pages and four units of each wave
+// are under way. bad: a length; none: a free page.
 constexpr int SMALL_ROWS = 2048;
 __device__ inline void mark_small(const PagesArgs& p, const int* keep, int used, const BitMap& pool, const BitMap& held, const BitMap& gone, int2* places, bool& bad,
                                   bool& none) {
+  constexpr int WAVES = MAP_THREADS / 64, AHEAD = 4, POOL_AHEAD = 4;
   const int tid = threadIdx.x, wave = tid >> 6, segs = (p.width + UNIT - 1) / UNIT, units = p.n * segs;
   for (int i = tid; i < p.n; i += MAP_THREADS) bad |= !places_of_row(p, keep, i, places[i].x, places[i].y);
+  const bool inside = used >= 0 && used <= p.pool_size;
+  int free_page[POOL_AHEAD];
+  auto in_pool = [&](int k) { return inside && k * MAP_THREADS + tid < p.pool_size - used; };
+#pragma unroll
+  for (int k = 0; k < POOL_AHEAD; ++k)
+    if (in_pool(k)) free_page[k] = p.pool[used + k * MAP_THREADS + tid];
   __syncthreads();  // the maps are empty, the places there
-  bad |= used < 0 || used > p.pool_size;
-  none = used >= 0 && mark_pool(p, used, pool, tid, MAP_THREADS);
-  constexpr int WAVES = MAP_THREADS / 64, AHEAD = 4;
+  bad |= !inside;
+  none = false;
   for (int u0 = wave; u0 < units; u0 += AHEAD * WAVES) {
     RowUnit<BitMap> unit[AHEAD];
 #pragma unroll
@@ -219,6 +225,13 @@ __device__ inline void mark_small(const PagesArgs& p, const int* keep, int used,
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) unit[k].mark(p, held, gone);
   }
+#pragma unroll
+  for (int k = 0; k < POOL_AHEAD; ++k) {
+    if (!in_pool(k)) continue;
+    if (page_ok(free_page[k], p.pages)) pool.set(free_page[k]);
+    else none = true;
+  }
+  if (inside) none |= mark_pool(p, long(used) + POOL_AHEAD * MAP_THREADS, pool, tid, MAP_THREADS);
 }
 
 // Four bytes of a map as four bits.
@@ -244,18 +257,11 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_count_kernel(const uint32_t
   if (bad) atomicOr(&head->bad, 2);
 }
 
-// The sums of counts before chunk `chunk` and of all of them.
-__device__ inline uint64_t sum_counts(const uint64_t* counts, long chunks, long chunk, uint64_t* sums, uint64_t& total) {
-  uint64_t before = 0, all = 0, b, t;
-  for (long c = threadIdx.x; c < chunks; c += MAP_THREADS) {
-    const uint64_t v = counts[c];
-    all += v;
-    if (c < chunk) before += v;
-  }
-  scan_block<MAP_THREADS>(before, sums, b);
-  scan_block<MAP_THREADS>(all, sums, t);
-  total = t;
-  return b;
+// The counts' (below 2^32) sums before chunk `chunk`, in the high half, and of all of them: this thread's share.
+__device__ inline uint64_t share_of_counts(const uint64_t* counts, long chunks, long chunk) {
+  uint64_t v = 0;
+  for (long c = threadIdx.x; c < chunks; c += MAP_THREADS) v += counts[c] * (c < chunk ? 0x100000001u : 1u);
+  return v;
 }
 
 // The pages of a word (from `page` on) that are given back, in their order, into the pool in front of the free ones.
@@ -276,10 +282,17 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_free_kernel(const FreeArgs 
   __shared__ uint64_t sums[MAP_THREADS / 64];
   const long w = long(blockIdx.x) * MAP_THREADS + threadIdx.x;
   const uint32_t bits = w < words ? bits_of(gone[w]) & ~bits_of(held[w]) : 0;
+  const uint64_t share = gridDim.x > 1 ? share_of_counts(counts, gridDim.x, blockIdx.x) : 0;
+  const int used = head->used, bad = head->bad;
   uint64_t total;
   uint64_t rank = scan_block<MAP_THREADS>(__popc(bits), sums, total);
-  if (gridDim.x > 1) rank += sum_counts(counts, gridDim.x, blockIdx.x, sums, total);
-  write_freed(a, bits, int(w * 4), rank, total, head->used, head->bad, w, long(gridDim.x) * MAP_THREADS);
+  if (gridDim.x > 1) {
+    uint64_t both;
+    scan_block<MAP_THREADS>(share, sums, both);
+    rank += both >> 32;
+    total = both & 0xffffffffu;
+  }
+  write_freed(a, bits, int(w * 4), rank, total, used, bad, w, long(gridDim.x) * MAP_THREADS);
 }
 
 // Few rows and pages: the maps in LDS and all of it in one launch.
@@ -338,16 +351,16 @@ __device__ inline void write_rest(const CompactArgs& a, int status, int used, lo
   }
 }
 
-// The rows' entries where their pages are now. rank_of(page): how many live pages are before it.
-template <typename Rank>
-__device__ inline void rewrite_rows(const CompactArgs& a, int status, int kept, long wave, long waves, Rank&& rank_of) {
+// The rows' entries where their pages are now. rank_of(page): how many live pages are before it; places(i): the pages of row i.
+template <typename Rank, typename Places>
+__device__ inline void rewrite_rows(const CompactArgs& a, int status, int kept, long wave, long waves, Rank&& rank_of, Places&& places) {
   const PagesArgs& p = a.at;
   const bool in_place = a.table_out == p.table;
   const int lane = threadIdx.x & 63, segs = (p.width + UNIT - 1) / UNIT;
   if (status != TABLE_OK && in_place) return;
   for (long u = wave; u < long(p.n) * segs; u += waves) {
     const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * UNIT;
-    const int all = status == TABLE_OK ? places_of(p.lens[i], p.shift) : 0, end = in_place ? all : p.width;
+    const int all = status == TABLE_OK ? places(i) : 0, end = in_place ? all : p.width;
     if (j0 >= end) continue;
     const int* row = p.table + long(i) * p.width;
     int* out = a.table_out + long(i) * p.width;
@@ -374,35 +387,48 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_move_kernel(const CompactAr
                                                                  const uint64_t* counts, MapHead* head) {
   __shared__ uint64_t sums[MAP_THREADS / 64];
   __shared__ long at_chunk, at_count;
-  __shared__ uint64_t at_before;
-  const int tid = threadIdx.x;
+  __shared__ uint64_t at_before, at_mine;
+  const int tid = threadIdx.x, used = head->used, head_bad = head->bad;
   const long w = long(blockIdx.x) * MAP_THREADS + tid, chunks = gridDim.x;
   const uint32_t l = w < words ? bits_of(live[w]) : 0, f = w < words ? bits_of(free[w]) : 0;
+  // one chunk's counts are its block's, of which there is one
+  auto count_of = [&](long c) { return chunks > 1 && c < chunks ? counts[c] : 0; };
+  uint64_t v = count_of(tid), b = 0;
+  if (tid == 0) at_chunk = at_count = at_before = at_mine = 0;
   bool both = false;
   uint64_t total, ahead = scan_block<MAP_THREADS>(count_word<true>(l, f, both), sums, total);
-  if (chunks > 1) ahead += sum_counts(counts, chunks, blockIdx.x, sums, total);
   const bool twice = __syncthreads_or(both);  // with several chunks the count has looked at all of them
+  auto pages_in = [](uint64_t v) { return long(v & 0xffffffffu) + long(v >> 32); };
+  // the sums before each of MAP_THREADS chunks from c0 on, one a thread
+  auto sums_before = [&](long c0, uint64_t& base) {
+    if (c0) v = count_of(c0 + tid);
+    uint64_t sum;
+    b = base + scan_block<MAP_THREADS>(v, sums, sum);
+    base += sum;
+  };
+  if (chunks > 1) {
+    total = 0;
+    for (long c0 = 0; c0 < chunks; c0 += MAP_THREADS) {
+      sums_before(c0, total);
+      if (c0 + tid == long(blockIdx.x)) at_mine = b;
+    }
+  }
   const long in_use = long(total & 0xffffffffu);
   // the chunk that holds the last of the first `in_use` pages, then the word in it: the holes are the free pages before there
-  auto pages_in = [](uint64_t v) { return long(v & 0xffffffffu) + long(v >> 32); };
-  if (tid == 0) {
-    at_chunk = at_count = 0;
-    at_before = 0;
-  }
-  __syncthreads();
   if (chunks > 1) {
     uint64_t base = 0;
     for (long c0 = 0; c0 < chunks; c0 += MAP_THREADS) {
-      const uint64_t v = c0 + tid < chunks ? counts[c0 + tid] : 0;
-      uint64_t sum;
-      const uint64_t b = base + scan_block<MAP_THREADS>(v, sums, sum);
+      if (chunks > MAP_THREADS) {
+        v = count_of(c0 + tid);
+        sums_before(c0, base);
+      }
       if (pages_in(b) < in_use && in_use <= pages_in(b) + pages_in(v)) {
         at_chunk = c0 + tid;
         at_before = b;
       }
-      base += sum;
     }
     __syncthreads();
+    ahead += at_mine;
   }
   const long w2 = at_chunk * MAP_THREADS + tid;
   const uint32_t l2 = w2 < words ? bits_of(live[w2]) : 0, f2 = w2 < words ? bits_of(free[w2]) : 0;
@@ -412,7 +438,7 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_move_kernel(const CompactAr
   __syncthreads();
   const long moved = at_count;
   // a free page that is there twice leaves fewer of them than the pool has
-  const int used = head->used, bad = head->bad | (twice || (!(head->bad & 1) && long(total >> 32) != long(a.at.pool_size) - used) ? 2 : 0);
+  const int bad = head_bad | (twice || (!(head_bad & 1) && long(total >> 32) != long(a.at.pool_size) - used) ? 2 : 0);
   const int status = bad & 1 ? TABLE_BAD_LENGTH : bad ? TABLE_BAD_PAGE : moved > a.cap ? TABLE_SLOTS_FULL : TABLE_OK;
   if (w < words) before[w] = int(ahead & 0xffffffffu);
   if (status == TABLE_OK && w < words) write_moves(a, l, f, int(w * 4), ahead, used, in_use, moved);
@@ -428,7 +454,7 @@ __global__ void __launch_bounds__(256) pages_rewrite_kernel(const CompactArgs a,
   rewrite_rows(a, head->status, head->kept, t >> 6, long(gridDim.x) * 4, [&](int page) {
     const int w = page >> 2;
     return before[w] + __popc(live[w] & 0x01010101u & ((1u << (8 * (page & 3))) - 1));
-  });
+  }, [&](int i) { return places_of(a.at.lens[i], a.at.shift); });
 }
 
 // Few rows and pages: the maps in LDS and all of it in one launch.
@@ -459,7 +485,7 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_compact_small_kernel(const 
   write_rest(a, status, used, moved, tid, MAP_THREADS);
   __syncthreads();  // dst is there
   rewrite_rows(a, status, int(in_use - moved), tid >> 6, MAP_THREADS / 64,
-               [&](int page) { return before[page >> 5] + __popc(live[page >> 5] & ((1u << (page & 31)) - 1)); });
+               [&](int page) { return before[page >> 5] + __popc(live[page >> 5] & ((1u << (page & 31)) - 1)); }, [&](int i) { return places[i].y; });
 }
 
 // --- copies -------------------------------------------------------------------------------------

@@ -341,6 +341,23 @@ def test_compact_pages_does_all_or_nothing(ctx, pages, in_place):
 
 # --- copies -----------------------------------------------------------------------------------------
 
+def test_millions_of_pages(ctx):
+    """More chunks of the maps than a block has threads, with the rows' pages in the first, the last and ones between."""
+    pages, ps, rng = 4096 * 1024 + 50000, 8, np.random.default_rng(5)
+    report("pages.millions", pages=pages)
+    ids = rng.permutation(pages)
+    ids[:4] = [0, pages - 1, 4096 * 1024 - 1, 4096 * 1024]
+    ids = np.concatenate([ids[:4], rng.permutation(np.setdiff1d(np.arange(pages), ids[:4]))])
+    table = np.full((3, 2000), -1, np.int64)
+    table[0], table[1, :1500], table[2, :700] = ids[:2000], ids[1000:2500], ids[:700]
+    lens = [16000, 12000 - 3, 5600]
+    used, pool = 2500, [0] * 2500 + ids[2500:].tolist()
+    check_free(ctx, [4000, 0, 5600], lens, ps, pages, pool, used, table)
+    check_compact(ctx, lens, ps, pages, pool, used, table, 2500)
+    half = 2110000   # nearly all pages in use: the last of them lies in a chunk past the 1024th
+    check_compact(ctx, [half * ps - 3, half * ps], ps, pages, [0] * 7 + ids[2 * half:].tolist(), 7, ids[:2 * half].reshape(2, half), pages - 2 * half, in_place=True)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("kv,ps,layers,gap,bounds", [(1, 8, 1, 0, False), (3, 16, 2, 64, True), (12, 32, 5, 0, True), (8, 64, 64, 8, False), (2, 256, 3, 0, True)])
 def test_copy_pages(ctx, dtype, kv, ps, layers, gap, bounds):
