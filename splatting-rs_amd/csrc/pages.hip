@@ -264,17 +264,16 @@ __device__ inline uint64_t share_of_counts(const uint64_t* counts, long chunks, 
   return v;
 }
 
-// The pages of a word (from `page` on) that are given back, in their order, into the pool in front of the free ones.
-__device__ inline void write_freed(const FreeArgs& a, uint32_t bits, int page, uint64_t rank, uint64_t total, int used, int bad, long thread, long threads) {
+// What becomes of `total` pages that are to be given back; the rows' lengths.
+__device__ inline int write_lengths(const FreeArgs& a, uint64_t total, int used, int bad, long thread, long threads) {
   const PagesArgs& p = a.at;
   const int status = bad & 1 ? TABLE_BAD_LENGTH : long(total) > used ? TABLE_BAD_PAGE : TABLE_OK;
-  if (status == TABLE_OK)
-    for (long at = used - long(total) + long(rank); bits; bits &= bits - 1, ++at) p.pool[at] = page + __builtin_ctz(bits);
   for (long i = thread; i < p.n; i += threads) a.lens_out[i] = status == TABLE_OK ? a.keep[i] : p.lens[i];
   if (thread == 0) {
     *a.used_out = status == TABLE_OK ? used - int(total) : used;
     *p.status = status;
   }
+  return status;
 }
 
 __global__ void __launch_bounds__(MAP_THREADS) pages_free_kernel(const FreeArgs a, const uint32_t* held, const uint32_t* gone, long words, const uint64_t* counts,
@@ -292,13 +291,19 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_free_kernel(const FreeArgs 
     rank += both >> 32;
     total = both & 0xffffffffu;
   }
-  write_freed(a, bits, int(w * 4), rank, total, used, bad, w, long(gridDim.x) * MAP_THREADS);
+  if (write_lengths(a, total, used, bad, w, long(gridDim.x) * MAP_THREADS) != TABLE_OK) return;
+  // in their order in front of the free ones
+  int* to = a.at.pool + (used - long(total) + long(rank));
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (bits >> k & 1) *to++ = int(w * 4) + k;
 }
 
 // Few rows and pages: the maps in LDS and all of it in one launch.
 __global__ void __launch_bounds__(MAP_THREADS) pages_free_small_kernel(const FreeArgs a) {
   __shared__ uint64_t sums[MAP_THREADS / 64];
   __shared__ uint32_t held[MAP_THREADS], gone[MAP_THREADS];
+  __shared__ int before[MAP_THREADS];
   __shared__ int2 places[SMALL_ROWS];
   const int tid = threadIdx.x, used = *a.at.used;
   held[tid] = gone[tid] = 0;
@@ -307,8 +312,15 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_free_small_kernel(const Fre
   bad = __syncthreads_or(bad);
   const uint32_t bits = gone[tid] & ~held[tid];
   uint64_t total;
-  const uint64_t rank = scan_block<MAP_THREADS>(__popc(bits), sums, total);
-  write_freed(a, bits, tid * 32, rank, total, used, bad, tid, MAP_THREADS);
+  before[tid] = int(scan_block<MAP_THREADS>(__popc(bits), sums, total));
+  gone[tid] = bits;  // only this thread has read it since the marks
+  __syncthreads();
+  if (write_lengths(a, total, used, bad, tid, MAP_THREADS) != TABLE_OK) return;
+  int* to = a.at.pool + (used - long(total));
+  for (int page = tid; page < a.at.pages; page += MAP_THREADS) {
+    const uint32_t word = gone[page >> 5], bit = 1u << (page & 31);
+    if (word & bit) to[before[page >> 5] + __popc(word & (bit - 1))] = page;
+  }
 }
 
 // --- compaction ---------------------------------------------------------------------------------
@@ -316,28 +328,21 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_free_small_kernel(const Fre
 // Of the pages in use (L) and the free ones, in their order, the first L are to be in use. The free ones among those are the holes,
 // M of them, and the live ones behind them move there, both in their order: the first L - M live pages stay.
 
-// Free pages among the first `need` (at least one) of a word's pages.
+// Free pages among the first `need` (at least one, as many as there are at most) of a word's pages.
 __device__ inline int holes_in(uint32_t live, uint32_t free, int need) {
-  uint32_t both = live | free;
-  int holes = 0;
-  for (; need > 0; --need, both &= both - 1) holes += (free & (both & -both)) != 0;
-  return holes;
+  uint32_t last = 0;  // the bit of the need-th page
+#pragma unroll
+  for (uint32_t s = 16; s; s >>= 1)
+    if (__popc((live | free) & ((1u << (last + s)) - 1)) < need) last += s;
+  return __popc(free & ((2u << last) - 1));
 }
 
-// A word's part of the result, whose pages are those from page0 on. before: live (low half) and free pages before it.
-__device__ inline void write_moves(const CompactArgs& a, uint32_t live, uint32_t free, int page0, uint64_t before, int used, long in_use, long moved) {
-  uint32_t both = live | free;
-  long l = long(before & 0xffffffffu), f = long(before >> 32);
-  for (; both; both &= both - 1) {
-    const int page = page0 + __builtin_ctz(both);
-    const bool is_live = live & (both & -both);
-    const long rank = l + f - in_use;  // among the pages that are to be free
-    if (rank >= 0) a.pool_out[used + rank] = page;
-    if (is_live && rank >= 0) a.src[l - (in_use - moved)] = page;
-    if (!is_live && rank < 0) a.dst[f] = page;
-    if (is_live) ++l;
-    else ++f;
-  }
+// A page's part of the result. l, f: live and free pages before it.
+__device__ inline void write_move(const CompactArgs& a, int page, bool is_live, long l, long f, int used, long in_use, long moved) {
+  const long rank = l + f - in_use;  // among the pages that are to be free
+  if (rank >= 0) a.pool_out[used + rank] = page;
+  if (is_live && rank >= 0) a.src[l - (in_use - moved)] = page;
+  if (!is_live && rank < 0) a.dst[f] = page;
 }
 
 // What there is besides the moves: places of src and dst behind them, and the pool as it was where nothing is done.
@@ -441,7 +446,15 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_move_kernel(const CompactAr
   const int bad = head_bad | (twice || (!(head_bad & 1) && long(total >> 32) != long(a.at.pool_size) - used) ? 2 : 0);
   const int status = bad & 1 ? TABLE_BAD_LENGTH : bad ? TABLE_BAD_PAGE : moved > a.cap ? TABLE_SLOTS_FULL : TABLE_OK;
   if (w < words) before[w] = int(ahead & 0xffffffffu);
-  if (status == TABLE_OK && w < words) write_moves(a, l, f, int(w * 4), ahead, used, in_use, moved);
+  if (status == TABLE_OK && w < words) {
+    long lives = long(ahead & 0xffffffffu), frees = long(ahead >> 32);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (!((l | f) >> k & 1)) continue;
+      write_move(a, int(w * 4) + k, l >> k & 1, lives, frees, used, in_use, moved);
+      ++(l >> k & 1 ? lives : frees);
+    }
+  }
   write_rest(a, status, used, moved, w, chunks * MAP_THREADS);
   if (w == 0) {
     head->kept = int(in_use - moved);
@@ -461,7 +474,7 @@ __global__ void __launch_bounds__(256) pages_rewrite_kernel(const CompactArgs a,
 __global__ void __launch_bounds__(MAP_THREADS) pages_compact_small_kernel(const CompactArgs a) {
   __shared__ uint64_t sums[MAP_THREADS / 64];
   __shared__ uint32_t live[MAP_THREADS], free[MAP_THREADS];
-  __shared__ int before[MAP_THREADS];
+  __shared__ int before[MAP_THREADS], frees[MAP_THREADS];  // live and free pages before a word
   __shared__ int2 places[SMALL_ROWS];
   __shared__ long holes;
   const int tid = threadIdx.x, used = *a.at.used;
@@ -478,10 +491,17 @@ __global__ void __launch_bounds__(MAP_THREADS) pages_compact_small_kernel(const 
   const long in_use = long(total & 0xffffffffu), first = long(ahead & 0xffffffffu) + long(ahead >> 32), here = long(v & 0xffffffffu) + long(v >> 32);
   if (first < in_use && in_use <= first + here) holes = long(ahead >> 32) + holes_in(l, f, int(in_use - first));
   before[tid] = int(ahead & 0xffffffffu);
+  frees[tid] = int(ahead >> 32);
   __syncthreads();
   const long moved = holes;
   const int status = bad ? TABLE_BAD_LENGTH : none ? TABLE_BAD_PAGE : moved > a.cap ? TABLE_SLOTS_FULL : TABLE_OK;
-  if (status == TABLE_OK) write_moves(a, l, f, tid * 32, ahead, used, in_use, moved);
+  if (status == TABLE_OK) {
+    for (int page = tid; page < a.at.pages; page += MAP_THREADS) {
+      const int w = page >> 5;
+      const uint32_t lives = live[w], open = free[w], bit = 1u << (page & 31);
+      if ((lives | open) & bit) write_move(a, page, lives & bit, before[w] + __popc(lives & (bit - 1)), frees[w] + __popc(open & (bit - 1)), used, in_use, moved);
+    }
+  }
   write_rest(a, status, used, moved, tid, MAP_THREADS);
   __syncthreads();  // dst is there
   rewrite_rows(a, status, int(in_use - moved), tid >> 6, MAP_THREADS / 64,
