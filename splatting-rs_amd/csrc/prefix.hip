@@ -309,12 +309,14 @@ struct Mine {
 // (blocks - items) always fits.
 template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a, int blocks, char* workspace, bool join) {
   const int lane = threadIdx.x & 63, G = a.heads / a.cache.kv_heads, kv = a.cache.kv_heads, rounds = (a.groups + 63) / 64;
-  struct Group { int start, tokens, shared, items, tiles; };  // items of a key head
+  struct Group { int start, tokens, shared, items, tiles; bool descends; };  // items of a key head
   auto group_at = [&](int k) {
     const int g = 64 * k + lane, at = min(g, a.groups - 1);
     Group x;
     x.start = start_of(a, at);
-    x.tokens = g < a.groups ? max(0, start_of(a, at + 1) - x.start) : 0;
+    const int count = g < a.groups ? start_of(a, at + 1) - x.start : 0;
+    x.tokens = max(0, count);
+    x.descends = count < 0;
     x.shared = shared_of(a, at);
     x.items = (x.tokens * G + R - 1) / R;  // tokens times G are below 2^21
     x.tiles = (x.shared + KEYS - 1) / KEYS;
@@ -324,14 +326,14 @@ template <int KEYS, int R> __device__ inline Mine find_item(const PrefixArgs& a,
   auto group_of_round = [&](int k) { return k == 0 ? first : group_at(k); };
   const auto plus = [](uint64_t x, uint64_t y) { return x + y; };
   auto last = [&](uint64_t v) { return long(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), 63))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(v), 63))); };
-  long tokens = 0, items = 0, tiles = 0, total = 0, each = 1L << 40;
+  long items = 0, tiles = 0, total = 0, each = 1L << 40;
+  bool valid = true;  // starts ascend: no token is in two groups
   for (int k = 0; k < rounds; ++k) {
     const Group x = group_of_round(k);
-    tokens += last(scan_wave(uint64_t(x.tokens), uint64_t(0), plus));
+    valid &= !__ballot(x.descends);
     items += last(scan_wave(uint64_t(x.items) * kv, uint64_t(0), plus));
     tiles += last(scan_wave(uint64_t(x.items) * kv * x.tiles, uint64_t(0), plus));
   }
-  const bool valid = tokens <= a.n;  // more only where starts descend: nothing is done
   auto parts_of = [&](const Group& x) { return int(max(1L, quotient(x.tiles + each - 1, each))); };
   for (int attempt = 0; attempt < 2; ++attempt) {
     const long share = attempt == 0 ? blocks : blocks - items;

@@ -324,6 +324,16 @@ def test_offsets_past_32_bits(ctx):
         assert ((out[i].cpu().double() - ref).abs() <= 2 ** -8 * (ref.abs() + V.abs().max())).all()
 
 
+@pytest.mark.parametrize("starts", [[0, 5, 3, 4], [0, 5, 3, 8], [8, 0, 0, 0], [0, 8, 7, 7], [3, 2, 5, 8]])
+@pytest.mark.parametrize("shared,own", [(40, None), (40, 9), (6000, 9)])
+def test_starts_that_descend_write_nothing(ctx, starts, shared, own):
+    """Also where the groups' tokens are no more than there are: one of them would be in two groups."""
+    s = Shared("bf16", [3, 3, 2], [shared] * 3, own and [own] * 8, 6, 2, 16)
+    report("prefix.descends", starts=starts, shared=shared, own=own)
+    assert torch.isnan(s.run(ctx, starts=starts)).all()
+    s.check(s.run(ctx))
+
+
 def test_calls_without_tokens_or_groups(ctx):
     L = lib()
     cache = L.KvCache(L.BF16, 1 << 20, 1 << 30, 4, 16, 2)
