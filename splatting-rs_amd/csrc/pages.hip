@@ -36,13 +36,15 @@ __device__ inline int places_of(int len, int shift) { return int((long(len) + (1
 // effect whole or not at all without a launch before; then each wave takes its share of a row's full pages from the parent's, and
 // block 0 writes what there is one of for a row. FILL and COMMIT as in block_tables_kernel: two launches where lens_out lies over
 // lens or used_out over used and there are several blocks.
-// Bound by its chain of loads (parents, lengths, entries, the pool).
-constexpr int FORK_UNIT = 512;  // entries of a row that a wave takes at once
-template <int THREADS, bool FILL, bool COMMIT>
-__global__ void __launch_bounds__(THREADS) fork_pages_kernel(const ForkArgs a) {
-  __shared__ uint64_t sums[THREADS / 64];
+// Bound by its chain of loads (parents, lengths, entries, the pool): 28 of 64 rows 5.1 us, a call among others, a thousand (2.3 MB of entries
+// read and written) 5.8, where an empty call takes 3.9.
+constexpr int FORK_THREADS = 1024;  // a row each up to as many; blocks of 256 take 5.2 us for 64 rows, as these, and 8.4 for 1024, these 6.2
+constexpr int FORK_UNIT = 512;      // entries of a row that a wave takes at once
+template <bool FILL, bool COMMIT>
+__global__ void __launch_bounds__(FORK_THREADS) fork_pages_kernel(const ForkArgs a) {
+  __shared__ uint64_t sums[FORK_THREADS / 64];
   const PagesArgs& p = a.at;
-  const int tid = threadIdx.x, k = (p.n + THREADS - 1) / THREADS, ps = 1 << p.shift;
+  const int tid = threadIdx.x, k = (p.n + FORK_THREADS - 1) / FORK_THREADS, ps = 1 << p.shift;
   const int i0 = int(min(long(tid) * k, long(p.n))), i1 = int(min(long(i0) + k, long(p.n)));
   const long most = long(p.width) << p.shift;
   const int used = *p.used;
@@ -62,13 +64,13 @@ __global__ void __launch_bounds__(THREADS) fork_pages_kernel(const ForkArgs a) {
     else need += page_ok(begun(from, len), p.pages);
   }
   uint64_t total;
-  long rank = long(scan_block<THREADS>(uint64_t(need), sums, total));
+  long rank = long(scan_block<FORK_THREADS>(uint64_t(need), sums, total));
   const bool broken = __syncthreads_or(bad), stray = __syncthreads_or(no_row);
   const int status = broken ? TABLE_BAD_LENGTH : stray ? TABLE_BAD_ROW : long(total) > long(p.pool_size) - used ? TABLE_POOL_EMPTY : TABLE_OK;
   if constexpr (FILL) {
     if (status == TABLE_OK) {
       const int lane = tid & 63, segs = (p.width + FORK_UNIT - 1) / FORK_UNIT;
-      for (long u = long(blockIdx.x) * (THREADS / 64) + (tid >> 6); u < long(p.n) * segs; u += long(gridDim.x) * (THREADS / 64)) {
+      for (long u = long(blockIdx.x) * (FORK_THREADS / 64) + (tid >> 6); u < long(p.n) * segs; u += long(gridDim.x) * (FORK_THREADS / 64)) {
         const int i = int(quotient(u, segs)), j0 = int(u - long(i) * segs) * FORK_UNIT + lane;
         const int from = a.parents[i];
         if (from == -1) continue;
@@ -116,7 +118,12 @@ __global__ void __launch_bounds__(THREADS) fork_pages_kernel(const ForkArgs a) {
 //
 // Over many pages a map has a byte a page and the XCDs' caches store into it as they like: all of them store 1. (Bits, set with atomic
 // operations of the device, took 95 us for 320 thousand entries of a thousand rows that share their pages, where the bytes take 6.) Few
-// pages are bits in one block's LDS.
+// pages are bits in one block's LDS (bytes there, without atomics, took as long).
+//
+// Measured, a call among others: 64 rows of 8 thousand positions give pages back in 8.3 us, by one block, which its CU's loads of the
+// entries bound; a thousand rows of up to 25 thousand positions (320 thousand entries) in 15.3, by four launches (clear 2, marks 7, counts
+// 2, pages 4) that stores of a byte from each lane and the launches bound. 16 rows compact in 6.7 us by one block; 512 rows and a hundred
+// thousand pages in 24.4, by five launches (clear 2, marks 5, counts 2, moves 8, entries 8), each two to four dependent loads.
 
 constexpr int MAP_THREADS = PAGE_CHUNK;
 constexpr int UNIT = 256;  // places of a row that a wave takes at once
@@ -516,7 +523,8 @@ constexpr int COPY_PIECE = COPY_THREADS * COPY_AT_ONCE;  // pieces of 16 bytes a
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // 16 bytes a thread, four of them under way. A block takes (pair, array, part of a page) units in turn; arrays are the layers' keys,
-// values and bounds. Bound by HBM.
+// values and bounds. Bound by HBM: 1000 pages of 64 KB of two layers, 268 MB read and as many written, 111.6 us (4.8 TB/s); 32 begun pages of four
+// layers 5.9, where an empty call takes 3.9.
 __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyArgs a, int es, int parts, long units) {
   const KvCache& c = a.cache;
   const int arrays = a.layers * (a.has_bounds ? 3 : 2), row_shift = es == 4 ? 4 : 3;  // 16-byte pieces of a row
@@ -550,10 +558,12 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyArgs
 
 constexpr long FORK_BLOCKS = 256;  // each of which looks all rows over
 
-// Pages and places of all rows up to which one block takes them in LDS.
+// Pages, rows and places of all rows up to which one block takes them in LDS, where a CU reads alone. Measured, one block / several
+// launches, 520 places a row of 16 positions: 16 rows given back 5.4 / 10.6 us, 64 8.5 / 10.5, 128 13.3 / 10.5; 16 compacted 9.1 / 13.2, 64 20.5 /
+// 13.5 (each entry is read again and its page's new place looked up).
 constexpr int SMALL_PAGES = MAP_THREADS * 32;
-constexpr long SMALL_PLACES = 65536;
-bool small(const PagesArgs& p) { return p.pages <= SMALL_PAGES && p.n <= SMALL_ROWS && long(p.n) * p.width <= SMALL_PLACES; }
+constexpr long SMALL_FREE = 49152, SMALL_COMPACT = 16384;
+bool small(const PagesArgs& p, long places) { return p.pages <= SMALL_PAGES && p.n <= SMALL_ROWS && long(p.n) * p.width <= places; }
 
 // Waves that the rows' units fill, four a block, no more than the chip holds several times.
 int mark_blocks(const PagesArgs& p) { return int(std::max<long>(1, std::min<long>(2048, (long(p.n) * cdiv(p.width, UNIT) + 3) / 4))); }
@@ -588,18 +598,13 @@ void fork_pages(const Exec& ex, const ForkArgs& args) {
   if (ex.dry) return;
   const PagesArgs& p = a.at;
   ProfScope prof(ex, "fork_pages", 0, 8.0 * p.n * p.width + 32.0 * p.n);
-  auto launch = [&](auto threads) {
-    constexpr int N = decltype(threads)::value;
-    const int grid = int(std::max<long>(1, std::min<long>(FORK_BLOCKS, (long(p.n) * cdiv(p.width, FORK_UNIT) + N / 64 - 1) / (N / 64))));
-    if (grid == 1 || (a.lens_out != p.lens && a.used_out != p.used)) {
-      fork_pages_kernel<N, true, true><<<grid, N, 0, ex.stream>>>(a);
-    } else {
-      fork_pages_kernel<N, true, false><<<grid, N, 0, ex.stream>>>(a);
-      fork_pages_kernel<N, false, true><<<1, N, 0, ex.stream>>>(a);
-    }
-  };
-  if (p.n <= 256) launch(std::integral_constant<int, 256>());
-  else launch(std::integral_constant<int, 1024>());
+  const int grid = int(std::max<long>(1, std::min<long>(FORK_BLOCKS, (long(p.n) * cdiv(p.width, FORK_UNIT) + FORK_THREADS / 64 - 1) / (FORK_THREADS / 64))));
+  if (grid == 1 || (a.lens_out != p.lens && a.used_out != p.used)) {
+    fork_pages_kernel<true, true><<<grid, FORK_THREADS, 0, ex.stream>>>(a);
+  } else {
+    fork_pages_kernel<true, false><<<grid, FORK_THREADS, 0, ex.stream>>>(a);
+    fork_pages_kernel<false, true><<<1, FORK_THREADS, 0, ex.stream>>>(a);
+  }
   SPLAT_HIP(hipGetLastError());
 }
 
@@ -609,7 +614,7 @@ void free_pages(const Exec& ex, const FreeArgs& args, void* workspace, size_t by
   if (ex.dry) return;
   const PagesArgs& p = a.at;
   ProfScope prof(ex, "free_pages", 0, 4.0 * p.n * p.width + 12.0 * p.n);
-  if (small(p)) {
+  if (small(p, SMALL_FREE)) {
     pages_free_small_kernel<<<1, MAP_THREADS, 0, ex.stream>>>(a);
   } else {
     const PagesPlan plan = pages_plan(p.pages);
@@ -626,7 +631,7 @@ void compact_pages(const Exec& ex, const CompactArgs& args, void* workspace, siz
   if (ex.dry) return;
   const PagesArgs& p = a.at;
   ProfScope prof(ex, "compact_pages", 0, 8.0 * p.n * p.width + 8.0 * p.pages);
-  if (small(p)) {
+  if (small(p, SMALL_COMPACT)) {
     pages_compact_small_kernel<<<1, MAP_THREADS, 0, ex.stream>>>(a);
   } else {
     const PagesPlan plan = pages_plan(p.pages);

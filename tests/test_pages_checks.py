@@ -46,7 +46,7 @@ def test_bounds_past_the_rows_size_no_launch(lines):
 def test_kernels_keep_their_values_in_registers(kernels):  # noqa: F811
     """The wide form alone has scratch, for the sums that are taken again with care, whose registers three blocks a CU do not leave; and
     the fp32 form of 64 columns three values of its set-up."""
-    for want, count in (("prefix_parts_kernel", 3 + 2 + 2), ("prefix_wide_kernel", 2), ("prefix_own_kernel", 2), ("prefix_join_kernel", 6), ("fork_pages_kernel", 6),
+    for want, count in (("prefix_parts_kernel", 3 + 2 + 2), ("prefix_wide_kernel", 2), ("prefix_own_kernel", 2), ("prefix_join_kernel", 6), ("fork_pages_kernel", 3),
                         ("pages_mark_kernel", 2), ("pages_free_kernel", 1), ("pages_free_small_kernel", 1), ("pages_move_kernel", 1), ("pages_rewrite_kernel", 1),
                         ("pages_compact_small_kernel", 1), ("copy_pages_kernel", 1)):
         found = {k: v for k, v in kernels.items() if want in k}
