@@ -111,8 +111,9 @@ int splat_kernel_reconstruct(splat_ctx* ctx, int V, int H, int W, const float* d
  * For networks of the caller's in which a token's keys and values stay as they are when others come: they are kept in pages,
  * and in each call one token of each sequence attends to those of its sequence. The two networks of this library are none: in
  * their global blocks every token sees every other, so that a new view changes the keys of all of them behind the first such
- * block, and no forward here uses the cache. Many tokens of one view are many sequences to these calls, each of which reads the whole
- * cache; splat_kernel_attention is for whole views. No counterpart in the reference. Heads of 64 channels, as in
+ * block, and no forward here uses the cache. Tokens that see the same positions (a view's against a scene, many forks of one) are
+ * splat_kernel_prefix_attention's, which reads those once; to the other calls they are many sequences, each of which reads the whole
+ * cache. splat_kernel_attention is for whole views. No counterpart in the reference. Heads of 64 channels, as in
  * splat_kernel_attention.
  *
  * Position p of sequence i lies in row p % page_size of page table[i * width + p / page_size]; a slot is
@@ -233,7 +234,8 @@ int splat_kernel_fork_pages(splat_ctx* ctx, int n, const int32_t* parents, const
 
 /* Rows are cut to their first keep[i] of lens[i] positions (0: the row ends). Pages behind those that no row keeps and that are
  * not free already go back into the pool, ascending, in front of the free ones: into pool[*used_out .. *used). The table stays: what
- * it holds behind a row's pages means nothing. Every row that may hold a page has to be in the call. lens_out may also be
+ * it holds behind a row's pages means nothing. Every row that may hold a page has to be in the call. A row that is cut into a page
+ * that others hold too is not to grow in place: new tokens would go into their page; splat_kernel_fork_pages copies it. lens_out may also be
  * keep. workspace: splat_pages_workspace's bytes, 16-byte aligned; one for the most pages serves every smaller call. */
 int splat_pages_workspace(int pages, size_t* bytes);
 int splat_kernel_free_pages(splat_ctx* ctx, int n, const int32_t* keep, const int32_t* lens, int page_size, int pages,
