@@ -498,6 +498,9 @@ int own_parts(long n, long cols, int max_own, int keys) {
   const long tiles = (max_own + keys - 1) / keys + 1;
   return max_own == 0 ? 0 : int(std::max<long>(1, std::min<long>(tiles / 16, OWN_BLOCKS / std::max<long>(1, n * cols))));
 }
+// Of a token's own positions: groups of up to 16 query heads of a key head, each of which leaves a part of min(G, 16) columns, the last one too
+// where it has fewer heads.
+long own_groups(int kv_heads, int G) { return long(kv_heads) * ((G + 15) / 16); }
 }  // namespace
 
 // Measured, a call among others, 12 heads, one group and no own positions unless said so. Rows of an item: 16 / 32 / 128 at 16 tokens on 24889
@@ -514,7 +517,8 @@ PrefixPlan prefix_plan(const PrefixArgs& a) {
   plan.rows = each <= 16 ? 16 : c.dt == 0 ? (each <= 32 ? 32 : 64) : each <= (a.max_own ? 64 : 32) ? 32 : WIDE_ROWS;
   const bool wide = plan.rows == WIDE_ROWS;
   const int keys = wide ? 64 : small;
-  plan.own = own_parts(a.n, long(c.kv_heads) * ((G + 15) / 16), a.max_own, small);
+  const long cols = own_groups(c.kv_heads, G);
+  plan.own = own_parts(a.n, cols, a.max_own, small);
   // of an item that is cut, parts of eight tiles at least (two a wave), in the wide form of four
   const long items = most_items(a.n, G, a.groups, plan.rows) * c.kv_heads, tiles = (a.max_shared + keys - 1) / keys;
   const long most = std::max<long>(1, std::min<long>(MOST_PARTS, tiles / (wide ? 4 : 8))), round = wide ? WIDE_BLOCKS : NARROW_BLOCKS;
@@ -536,7 +540,7 @@ PrefixPlan prefix_plan(const PrefixArgs& a) {
   if (!plan.join) return plan;
   plan.parts = (16 + a.groups * 16L);
   plan.own_parts = plan.parts + size_t(plan.blocks) * plan.rows * PART_HEAD * 4;
-  plan.bytes = plan.own_parts + size_t(a.n) * a.heads * plan.own * PART_HEAD * 4;
+  plan.bytes = plan.own_parts + size_t(a.n) * cols * plan.own * std::min(G, 16) * PART_HEAD * 4;
   return plan;
 }
 
@@ -550,9 +554,8 @@ size_t prefix_attention_bytes(const KvCache& c, int n, int heads, int groups, in
   const int G = heads / c.kv_heads, keys = c.dt == 0 ? 16 : 32;
   const size_t item = long(n) * heads + std::min<long>(groups, n) * c.kv_heads * WIDE_ROWS;
   const size_t cut = std::min<size_t>(size_t(WIDE_BLOCKS) * 4 * WIDE_ROWS, item * ((long(max_shared) + keys - 1) / keys));
-  // own parts: one a token and column group, or as many as there are blocks for
-  const size_t cols = size_t(c.kv_heads) * ((G + 15) / 16);
-  const size_t own = max_own == 0 ? 0 : std::max<size_t>(size_t(n) * heads, size_t(OWN_BLOCKS) / cols * heads);
+  // own parts: one a token and group of heads, or as many as there are blocks for
+  const size_t own = max_own == 0 ? 0 : std::max<size_t>(size_t(n) * own_groups(c.kv_heads, G), OWN_BLOCKS) * std::min(G, 16);
   return 16 + groups * 16L + (item + cut + own) * PART_HEAD * 4;
 }
 
