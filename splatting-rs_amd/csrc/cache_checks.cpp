@@ -504,17 +504,18 @@ long own_groups(int kv_heads, int G) { return long(kv_heads) * ((G + 15) / 16); 
 }  // namespace
 
 // Measured, a call among others, 12 heads, one group and no own positions unless said so. Rows of an item: 16 / 32 / 128 at 16 tokens on 24889
-// positions (bf16) 24.0 / 26.3 / 32.6 us, at 32 28.9 / 26.5 / 31.8, at 48 34.9 / 35.3 / 31.9, at 64 43.8 / 36.1 / 31.6, at 128 92.6 / 56.4 /
-// 32.5; with own positions, which the narrow forms take in the same launch, 64 forks 46.7 / 48.1 (32 / 128 rows), 48 forks of four scenes (32
-// heads on 8) 43.6 / 46.9; in fp32 16 / 32 / 64 on 12000 positions at 16 tokens 24.8 / 31.0 / 43.6, at 32 33.1 / 31.5 / 44.0, at 64 52.8 /
-// 46.6 / 44.7, at 256 208 / 168 / 126. Blocks: 256 / 512 of the narrow forms at 16 tokens 24.0 / 26.5, 64 forks 44 / 52 (own positions run beside,
-// on each CU's second block); 512 / 768 / 1024 of the wide form at 128 tokens 36 / 39 / 48 (parts to join), at 1037 127 / 120 / 128.
+// positions (bf16) 23.9 / 26.3 / 39.6 us, at 32 29.6 / 27.0 / 39.6, at 48 35.7 / 36.4 / 40.0; 32 / 128 at 64 37.8 / 40.7, at 72 45.3 / 40.8, at 128
+// 57.3 / 43.6; with own positions, which the narrow forms take in the same launch, 64 forks with a view each 44.5 / 63.3, 128 71.4 / 86.6, 128 with
+// one position each 57.8 / 55.7, 48 forks of four scenes (32 heads on 8) 38.9 / 60.7; in fp32 16 / 32 / 64 on 12000 positions at 16
+// tokens 24.8 / 31.0 / 43.6, at 32 33.1 / 31.5 / 44.0, at 64 52.8 / 46.6 / 44.7, at 256 208 / 168 / 126. Blocks: 256 / 512 of the narrow forms at 16
+// tokens 24.0 / 26.5, 64 forks 44 / 52 (own positions run beside, on each CU's second block); 512 / 768 / 1024 of the wide form at 128
+// tokens 42.9 / 45.6 / 54.0 (parts to join), at 1037 180 / 165 / 170, at 2074 322 / 324 / 285.
 PrefixPlan prefix_plan(const PrefixArgs& a) {
   PrefixPlan plan;
   const KvCache& c = a.cache;
   const int G = a.heads / c.kv_heads, small = c.dt == 0 ? 16 : 32;
   const long each = (long(a.n) * G + a.groups - 1) / a.groups;  // rows of a group and key head, if all are alike
-  plan.rows = each <= 16 ? 16 : c.dt == 0 ? (each <= 32 ? 32 : 64) : each <= (a.max_own ? 64 : 32) ? 32 : WIDE_ROWS;
+  plan.rows = each <= 16 ? 16 : c.dt == 0 ? (each <= 32 ? 32 : 64) : each <= (a.max_own ? 128 : 64) ? 32 : WIDE_ROWS;
   const bool wide = plan.rows == WIDE_ROWS;
   const int keys = wide ? 64 : small;
   const long cols = own_groups(c.kv_heads, G);

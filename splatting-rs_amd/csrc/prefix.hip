@@ -501,16 +501,17 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
 //
 // Bound by the matrix instructions and by the vector unit's work on the scores, about as much of either: so half a tile's products
 // with K and the half before the last one's with V are under way while the half between becomes weights, all in one wave's stream,
-// and three waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 112 us and the join's 10 (0.70 PFLOP/s).
-// Of a SIMD's cycles 1024 go to the matrix instructions of a tile of 64 columns and 1250 to the vector unit (half of them
-// exponentials), and 60% of the former lie beside the latter. Two blocks a CU with a tile more under way took 130 us, waves of 64 columns 125, two teams
-// of waves that multiply and exponentiate in turn 140, the compiler's own order of the same instructions 6% more than this one.
+// and three waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 158 us, the join's 10 among them (0.50 PFLOP/s,
+// and half as many operations again for the weights' second terms: 0.8 PFLOP/s while the parts are formed). Of a SIMD's cycles 1536 go to the
+// matrix instructions of a tile of 64 columns and 1750 to the vector unit (a third of them exponentials). With weights of one term, when all of
+// it took 115 us: two blocks a CU with a tile more under way 130, waves of 64 columns 125, two teams of waves that multiply and exponentiate in
+// turn 140, the compiler's own order of the same instructions 6% more.
 //
 // The weights are 2^(c s - r), c = |scale| log2(e), in one fused multiply-add: its one rounding is of the difference, and what r was
 // rounded by is the same for all weights of a column. r is the largest score of the first half tile with a key; sums that overflow
-// with it (2^64, in f16 weights of 2^16) are taken again with care. The weights are rounded once to the values' type, where the two
-// terms of the other form would cost half the matrix instructions again; their sum is of the rounded ones, so that what a column's
-// weights have in common cancels.
+// with it (2^64, in f16 weights of 2^16) are taken again with care. A weight is two terms of the values' type, as in TileOps: 16 bits of it in
+// bf16, 22 in f16. Rounded to one (115 us for 158) a bf16 view is off by 1.9e-3 where the output's own rounding is 1.65e-3, and the same
+// token by as much between a call of few rows and one of many.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -520,14 +521,17 @@ template <typename T> __device__ inline f32x16 mma32(const uint4& a, const uint4
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_v, a), __builtin_bit_cast(f16x8_v, b), c, 0, 0, 0);
 }
-// acc + both values of a packed pair
+// What one value of a packed pair leaves of x, which it is x rounded to: exact, by a product with (-1, 0) or (0, -1). The factors stay in
+// registers: a 16-bit constant of an instruction's own is not in the half that it is in here.
 typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_v __attribute__((ext_vector_type(2)));
-template <typename T> __device__ inline float add_pair(uint32_t pair, float acc) {
+template <typename T, int WHICH> __device__ inline float rest_of(uint32_t pair, float x) {
+  uint32_t minus = (std::is_same<T, bf16>::value ? 0xbf80u : 0xbc00u) << (16 * WHICH);
+  asm("" : "+s"(minus));
   if constexpr (std::is_same<T, bf16>::value)
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pair), __builtin_bit_cast(bf16x2_v, 0x3f803f80u), acc, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pair), __builtin_bit_cast(bf16x2_v, minus), x, false);
   else
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_v, pair), __builtin_bit_cast(f16x2_v, 0x3c003c00u), acc, false);
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_v, pair), __builtin_bit_cast(f16x2_v, minus), x, false);
 }
 __device__ inline float most_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN stays
 // fn over lanes l and l ^ 32
@@ -635,7 +639,7 @@ template <typename T> struct WideWave {
   }
 
   // Half a tile: its operands, scores, weights, and what those add to the sums.
-  struct Weights { uint32_t p[8]; };
+  struct Weights { uint32_t p[8], rest[8]; };
   __device__ inline void load_keys(uint4 (&kf)[4], int b, int half) const {
 #pragma unroll
     for (int st = 0; st < 4; ++st) kf[st] = keys(b, half, st);
@@ -653,8 +657,10 @@ template <typename T> struct WideWave {
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w.p[e] = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[2 * e], scale, ref)), __builtin_amdgcn_exp2f(fmaf(s[2 * e + 1], scale, ref)));
-      sum = add_pair<T>(w.p[e], sum);
+      const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * e], scale, ref)), y = __builtin_amdgcn_exp2f(fmaf(s[2 * e + 1], scale, ref));
+      w.p[e] = pack2<T>(x, y);
+      w.rest[e] = pack2<T>(rest_of<T, 0>(w.p[e], x), rest_of<T, 1>(w.p[e], y));
+      sum += x + y;
     }
     l += sum;
   }
@@ -662,6 +668,11 @@ template <typename T> struct WideWave {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t* p = w.p + 4 * (k >> 1);
+      o[k & 1] = mma32<T>(vf[k], make_uint4(p[0], p[1], p[2], p[3]), o[k & 1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t* p = w.rest + 4 * (k >> 1);
       o[k & 1] = mma32<T>(vf[k], make_uint4(p[0], p[1], p[2], p[3]), o[k & 1]);
     }
   }
@@ -739,15 +750,18 @@ template <typename T> struct WideWave {
   __device__ inline void pin(Weights& w) {
     asm volatile("" : "+v"(l));
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) asm volatile("" : "+v"(w.p[e]), "+v"(w.p[e + 1]), "+v"(w.p[e + 2]), "+v"(w.p[e + 3]));
+    for (int e = 0; e < 8; e += 4) {
+      asm volatile("" : "+v"(w.p[e]), "+v"(w.p[e + 1]), "+v"(w.p[e + 2]), "+v"(w.p[e + 3]));
+      asm volatile("" : "+v"(w.rest[e]), "+v"(w.rest[e + 1]), "+v"(w.rest[e + 2]), "+v"(w.rest[e + 3]));
+    }
   }
-  // Beside the eight matrix instructions of half a tile: the vector unit's work, five of its instructions between each two (6 to 9 were
-  // slower).
+  // Beside the twelve matrix instructions of half a tile: the vector unit's work, six of its instructions between each two (4, 5, 7
+  // and 9 take as long, 8 are 6% slower).
   __device__ static inline void interleave() {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 12; ++k) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
     }
   }
 
