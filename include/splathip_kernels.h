@@ -225,8 +225,8 @@ int splat_kernel_sparse_attention(splat_ctx* ctx, const splat_kv_cache* cache, c
 /* Rows with a parent become forks: with parents[i] = p, the empty row i (lens[i] 0) gets the first keep[i] positions of row p
  * (keep NULL: all lens[p]), which is no fork in the same call; parents[i] -1: row i stays. Full pages are shared; a begun one is
  * the next of the pool instead, requests in order, for new tokens to go into, and its keys and values are to be copied: rows[i]
- * rows of page src[i] to page dst[i] (-1, -1 and 0: none). An entry that is no page stays one. keep is not
- * looked at where there is no parent. */
+ * rows of page src[i] to page dst[i] (-1, -1 and 0: none). An entry that is no page stays one; a free
+ * one that is to be taken and is none is SPLAT_TABLE_BAD_PAGE. keep is not looked at where there is no parent. */
 int splat_kernel_fork_pages(splat_ctx* ctx, int n, const int32_t* parents, const int32_t* keep, const int32_t* lens,
                             int page_size, int pages, const int32_t* pool, int pool_size, const int32_t* used,
                             int32_t* table, int width, int32_t* lens_out, int32_t* src, int32_t* dst, int32_t* rows,

@@ -49,6 +49,8 @@ __global__ void __launch_bounds__(FORK_THREADS) fork_pages_kernel(const ForkArgs
   const long most = long(p.width) << p.shift;
   const int used = *p.used;
   bool bad = used < 0 || used > p.pool_size, no_row = false;
+  auto in_pool = [&](long k) { return !bad && used + k < p.pool_size; };
+  const int next = in_pool(tid) ? p.pool[used + tid] : 0;  // asked for beside the rows
   int need = 0;
   // the entry of the page that the fork begins with a copy, -1: none
   auto begun = [&](int from, int len) { return len & (ps - 1) ? p.table[long(from) * p.width + (len >> p.shift)] : -1; };
@@ -63,10 +65,15 @@ __global__ void __launch_bounds__(FORK_THREADS) fork_pages_kernel(const ForkArgs
     if (have < 0 || have > most || len < 0 || len > have) bad = true;
     else need += page_ok(begun(from, len), p.pages);
   }
-  uint64_t total;
-  long rank = long(scan_block<FORK_THREADS>(uint64_t(need), sums, total));
-  const bool broken = __syncthreads_or(bad), stray = __syncthreads_or(no_row);
-  const int status = broken ? TABLE_BAD_LENGTH : stray ? TABLE_BAD_ROW : long(total) > long(p.pool_size) - used ? TABLE_POOL_EMPTY : TABLE_OK;
+  // pages (up to n) in the low half of a sum, threads with a bad length and with a bad row above
+  uint64_t sum;
+  long rank = long(uint32_t(scan_block<FORK_THREADS>(uint64_t(no_row) << 48 | uint64_t(bad) << 32 | uint32_t(need), sums, sum)));
+  const int total = int(uint32_t(sum));
+  bool none = false;  // a page that is to be taken
+  for (long k = tid; k < total && in_pool(k); k += FORK_THREADS) none |= !page_ok(k == tid ? next : p.pool[used + k], p.pages);
+  const bool no_page = __syncthreads_or(none);
+  const int status = sum >> 32 & 0xffff ? TABLE_BAD_LENGTH : sum >> 48 ? TABLE_BAD_ROW : total > long(p.pool_size) - used ? TABLE_POOL_EMPTY
+                     : no_page ? TABLE_BAD_PAGE : TABLE_OK;
   if constexpr (FILL) {
     if (status == TABLE_OK) {
       const int lane = tid & 63, segs = (p.width + FORK_UNIT - 1) / FORK_UNIT;
@@ -108,7 +115,7 @@ __global__ void __launch_bounds__(FORK_THREADS) fork_pages_kernel(const ForkArgs
       a.rows[i] = rows;
     }
     if (tid == 0) {
-      *a.used_out = status == TABLE_OK ? used + int(total) : used;
+      *a.used_out = status == TABLE_OK ? used + total : used;
       *p.status = status;
     }
   }
