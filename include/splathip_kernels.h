@@ -269,7 +269,7 @@ int splat_kernel_copy_pages(splat_ctx* ctx, const splat_kv_cache* caches, int la
  * table theirs, and the tokens of a view to a cache, or in causal order with lens = position + 1, with prefix the request's row.
  * out[i, h] = softmax(scale q[i, h] K^T) V over what it sees, with the keys and values of head h / (heads / kv_heads); zeros where
  * that is nothing. max_shared and max_own: upper bounds of shared[g] and of lens[i] - shared[g] that the host knows; what is
- * behind them is cut off. q, out, strides, and weights as in splat_kernel_paged_attention, infinities and NaN in
+ * behind them is cut off (own positions begin at shared[g] all the same). q, out, strides, and weights as in splat_kernel_paged_attention, infinities and NaN in
  * values that a token does not see leave its row alone. workspace: splat_prefix_attention_workspace's bytes, 16-byte aligned; one for the
  * largest n, groups, max_shared and max_own serves every smaller call. starts that descend: nothing is written. groups times
  * kv_heads up to 2^21. */

@@ -392,7 +392,7 @@ __device__ inline PrefixWave<T, 1> own_tiles(const PrefixArgs& a, int i, int gro
   w.ops[0].load_q(static_cast<const T*>(a.q) + long(i) * a.ldq + long(kh * G + h0 + (in ? col : 0)) * 64, g, in);
   // for up to 64 groups what is asked of them comes in one load, a group a lane
   const int near = min(lane, a.groups - 1), begin = start_of(a, near), end = start_of(a, near + 1);
-  int shared = shared_of(a, near), len = a.lens[i], at = -1;
+  int shared = a.shared[near], len = a.lens[i], at = -1;  // whole: where the prefix is cut, own positions begin behind it all the same
   if (a.groups <= 64) {
     const uint64_t of_token = __ballot(lane < a.groups && begin <= i && i < end);
     if (of_token) {
@@ -400,9 +400,9 @@ __device__ inline PrefixWave<T, 1> own_tiles(const PrefixArgs& a, int i, int gro
       shared = __builtin_amdgcn_readlane(shared, at);
     }
   } else if ((at = group_of(a, i)) >= 0) {
-    shared = shared_of(a, at);
+    shared = a.shared[at];
   }
-  w.lo = at < 0 ? 0 : uniform(shared);
+  w.lo = at < 0 ? 0 : uniform(max(shared, 0));
   w.end = at < 0 ? 0 : uniform(int(min(long(length_of(len, a.width, c.shift, 0x7fffffff)), long(w.lo) + a.max_own)));
   w.least = w.hi[0] = w.end;
   const int from = w.lo / KEYS, tiles = w.end > w.lo ? (w.end + KEYS - 1) / KEYS - from : 0;

@@ -16,3 +16,28 @@ def test_parts_of_heads_that_fill_no_group_of_16(ctx, dtype, n, G, shared, max_o
     own = [max_own // 8 if i % 13 == 1 else 37 * i % (1 + max_own // 60) for i in range(n)]
     s = Shared(dtype, [n - n // 3, n // 3], [shared, shared // 2], own, G, 1, 16)
     s.check(s.run(ctx, max_own=max_own), rows=sorted({0, 1, n - 1, *range(0, n, 7)}))
+
+
+class Cut(Shared):
+    """Of a group's shared positions the first `most` are seen; own ones begin behind all of them."""
+
+    def seen(self, i):
+        k, v = self.group[i], self.lens[i]
+        out = [(int(self.prefix[k, p // self.ps]), p % self.ps) for p in range(min(v, self.shared[k], self.most))]
+        out += [(int(self.table[i, p // self.ps]), p % self.ps) for p in range(self.shared[k], min(v, self.shared[k] + self.most_own))]
+        return [x for x in out if 0 <= x[0] < self.pages]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("members,shared,most,most_own", [([4], [100], 64, 1000), ([3, 150], [1037, 90], 70, 20), ([150, 2], [300, 5000], 0, 33), ([1] * 70, [40] * 70, 33, 50)])
+def test_own_positions_begin_behind_a_prefix_that_is_cut(ctx, dtype, members, shared, most, most_own):
+    """By max_shared, then by the width of the prefix's rows."""
+    report("prefix.cut", dtype=dtype, members=members[:4], shared=shared[:4], most=most, most_own=most_own)
+    s = Cut(dtype, members, shared, [(23 * i + 30) % 61 for i in range(sum(members))], 4, 2, 16)
+    s.most, s.most_own = most, most_own
+    rows = sorted({*range(0, s.n, 5), s.n - 1})
+    s.check(s.run(ctx, max_shared=most, max_own=most_own), rows=rows)
+    s.prefix_width = max(1, most // 16)
+    s.prefix = s.prefix[:, :s.prefix_width].contiguous()
+    s.most = s.prefix_width * 16
+    s.check(s.run(ctx, max_own=most_own), rows=rows)
