@@ -237,7 +237,8 @@ template <typename T, int NT> struct PrefixWave {
 
 // --- a block ------------------------------------------------------------------------------------
 
-// A part: `columns` times 64 sums, then (m, l) of each, the sums being of weights e^(x - m); l is -1 where no key was there.
+// A part: `columns` times 64 sums, then (m, l) of each, the sums being of weights e^(x - m), m the largest score as it is: a logarithm of the
+// forms' factors 2^TOP taken off it would round it, at scores of 8192 by up to 2^-11. l is -1 where no key was there.
 __device__ inline float* part_at(char* workspace, size_t offset, long index, int columns) {
   return reinterpret_cast<float*>(workspace + offset) + index * columns * long(PART_HEAD);
 }
@@ -290,8 +291,9 @@ __device__ inline void join_waves(const PrefixWave<T, NT>& w, char* smem, float 
       if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
       else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     } else {
-      *reinterpret_cast<float4*>(part + column * 64 + 16 * wave + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
-      if (wave == 0 && g == 0) *reinterpret_cast<float2*>(part + columns * 64 + column * 2) = make_float2(mn - TileOps<T>::TOP * 0.693147180559945309f, some ? sum : -1.f);
+      constexpr float f = 1.f / (1 << TileOps<T>::TOP);
+      *reinterpret_cast<float4*>(part + column * 64 + 16 * wave + 4 * g) = make_float4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+      if (wave == 0 && g == 0) *reinterpret_cast<float2*>(part + columns * 64 + column * 2) = make_float2(mn, some ? sum * f : -1.f);
     }
   }
 }
@@ -507,8 +509,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
 // it took 115 us: two blocks a CU with a tile more under way 130, waves of 64 columns 125, two teams of waves that multiply and exponentiate in
 // turn 140, the compiler's own order of the same instructions 6% more.
 //
-// The weights are 2^(c s - r), c = |scale| log2(e), in one fused multiply-add: its one rounding is of the difference, and what r was
-// rounded by is the same for all weights of a column. r is the largest score of the first half tile with a key; sums that overflow
+// The weights are 2^(c s + ref), c = |scale| log2(e), in one fused multiply-add: its one rounding is of the difference, and what ref =
+// -c r was rounded by is the same for all weights of a column: parts are freed of it. r is the largest product of the first half tile with a key; sums that overflow
 // with it (2^64, in f16 weights of 2^16) are taken again with care. A weight is two terms of the values' type, as in TileOps: 16 bits of it in
 // bf16, 22 in f16. Rounded to one (115 us for 158) a bf16 view is off by 1.9e-3 where the output's own rounding is 1.65e-3, and the same
 // token by as much between a call of few rows and one of many.
@@ -664,6 +666,11 @@ template <typename T> struct WideWave {
     }
     l += sum;
   }
+  __device__ inline void weigh_one(const Weights& w, int k, const uint4& v) {
+    const int p = 4 * (k >> 1);
+    o[k & 1] = mma32<T>(v, make_uint4(w.p[p], w.p[p + 1], w.p[p + 2], w.p[p + 3]), o[k & 1]);
+    o[k & 1] = mma32<T>(v, make_uint4(w.rest[p], w.rest[p + 1], w.rest[p + 2], w.rest[p + 3]), o[k & 1]);
+  }
   __device__ inline void weigh(const Weights& w, const uint4 (&vf)[4]) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -676,12 +683,14 @@ template <typename T> struct WideWave {
       o[k & 1] = mma32<T>(vf[k], make_uint4(p[0], p[1], p[2], p[3]), o[k & 1]);
     }
   }
-  // The largest score of the lane's column, times scale.
-  __device__ static inline float largest(const f32x16& s, float scale) {
+  // The weights are 2^(scale s + ref) of products s.
+  __device__ inline float ref_of(float scale) const { return r == -INFINITY ? TOP : fmaf(-r, scale, TOP); }
+  // The largest product of the lane's column.
+  __device__ static inline float largest(const f32x16& s) {
     float m = most_of(most_of(s[0], s[1]), s[2]);
 #pragma unroll
     for (int e = 3; e < 15; e += 2) m = most_of(most_of(m, s[e]), s[e + 1]);
-    return over_two(most_of(m, s[15]), most_of) * scale;
+    return over_two(most_of(m, s[15]), most_of);
   }
   // Of half a tile from position `first` on (a multiple of 32), in the group of 8 keys in one page: how many from the lane's own first
   // one on its column sees.
@@ -706,9 +715,11 @@ template <typename T> struct WideWave {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[4 * x4 + e] = e < below ? s[4 * x4 + e] : -INFINITY;
     }
-    const float mx = largest(s, scale), top = r == -INFINITY || (CAREFUL && mx > r) ? mx : r;
+    const float mx = largest(s), old = r, was = ref;
+    r = r == -INFINITY || (CAREFUL && mx > r) ? mx : r;
+    ref = ref_of(scale);
     if (CAREFUL) {  // where there was none, the sums are zeros
-      const float keep = r == top ? 1.f : __builtin_amdgcn_exp2f(r - top);
+      const float keep = r == old ? 1.f : old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - was);
       l *= keep;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -716,15 +727,13 @@ template <typename T> struct WideWave {
         o[1][e] *= keep;
       }
     }
-    r = top;
-    ref = TOP - (top == -INFINITY ? 0.f : top);
     weights(w, s, scale, ref);
     if constexpr (CAREFUL) {
       const f32x16 zero = {};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint4 raw = vf[k];
-        vf[k] = map_pairs(raw, [](float y) { return fabsf(y) < INFINITY ? y : 0.f; });
+        weigh_one(w, k, map_pairs(raw, [](float y) { return fabsf(y) < INFINITY ? y : 0.f; }));
         uint32_t one[4];  // how many of each other kind the column sees
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -732,18 +741,18 @@ template <typename T> struct WideWave {
           one[e] = pack2<T>(below > 0 ? 1.f : 0.f, below > 1 ? 1.f : 0.f);
         }
         const uint4 sees = make_uint4(one[0], one[1], one[2], one[3]);
-        const f32x16 none = mma32<T>(map_pairs(raw, [](float y) { return y != y ? 1.f : 0.f; }), sees, zero);
-        const f32x16 up = mma32<T>(map_pairs(raw, [](float y) { return y == INFINITY ? 1.f : 0.f; }), sees, zero);
-        const f32x16 down = mma32<T>(map_pairs(raw, [](float y) { return y == -INFINITY ? 1.f : 0.f; }), sees, zero);
+        auto add = [&](auto&& kind, float what) {
+          const f32x16 count = mma32<T>(map_pairs(raw, [&](float y) { return kind(y) ? 1.f : 0.f; }), sees, zero);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (none[e] > 0.f) o[k & 1][e] = NAN;
-          if (up[e] > 0.f) o[k & 1][e] += INFINITY;
-          if (down[e] > 0.f) o[k & 1][e] -= INFINITY;
-        }
+          for (int e = 0; e < 16; ++e) o[k & 1][e] += count[e] > 0.f ? what : 0.f;
+        };
+        add([](float y) { return y != y; }, NAN);
+        add([](float y) { return y == INFINITY; }, INFINITY);
+        add([](float y) { return y == -INFINITY; }, -INFINITY);
       }
+    } else {
+      weigh(w, vf);
     }
-    weigh(w, vf);
   }
 
   // Weights are taken here, not where they are used first: that is behind the next barrier.
@@ -767,7 +776,7 @@ template <typename T> struct WideWave {
 
   // Tiles t0 up to t1. True where the sums are not to be taken: a NaN, an infinity, or weights beyond 2^64.
   template <bool CAREFUL> __device__ inline bool pass(int t0, int t1, float scale) {
-    float ref = 0.f;
+    float ref = TOP;
 #pragma unroll
     for (int x = 0; x < 16; ++x) o[0][x] = o[1][x] = 0.f;
     r = -INFINITY;
@@ -888,13 +897,16 @@ __global__ void __launch_bounds__(WAVES * 64, WIDE_OCCUPANCY) prefix_wide_kernel
   const bool some = w.hi > w.key0;
   if (join) {
     float* part = part_at(workspace, parts, uniform(mine.id), R);
+    // the largest score as it is: what its weight is other than 1 goes into the sums, 2^TOP and what rounding ref left of scale r
+    const bool none = w.r == -INFINITY;
+    const float f = none ? 1.f : __builtin_amdgcn_exp2f(-fmaf(w.r, scale, w.ref_of(scale))), m = none ? w.r : w.r * fabsf(a.scale);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         *reinterpret_cast<float4*>(part + column * 64 + dt * 32 + 8 * k + 4 * g) =
-            make_float4(w.o[dt][4 * k], w.o[dt][4 * k + 1], w.o[dt][4 * k + 2], w.o[dt][4 * k + 3]);
-    if (g == 0) *reinterpret_cast<float2*>(part + R * 64 + column * 2) = make_float2((w.r - w.TOP) * 0.693147180559945309f, some ? sum : -1.f);
+            make_float4(w.o[dt][4 * k] * f, w.o[dt][4 * k + 1] * f, w.o[dt][4 * k + 2] * f, w.o[dt][4 * k + 3] * f);
+    if (g == 0) *reinterpret_cast<float2*>(part + R * 64 + column * 2) = make_float2(m, some ? sum * f : -1.f);
   } else if (in) {
     const float inv = 1.f / sum;
     T* out = static_cast<T*>(a.out) + long(token) * a.ldo + long(head) * 64 + 4 * g;

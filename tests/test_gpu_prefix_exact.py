@@ -54,3 +54,54 @@ def test_weights_keep_more_than_their_type_holds(ctx, dtype, members, shared, ow
         worst = max(worst, float(((out[i].double().view(ref.shape) - ref).abs() / tol).max()))
     report("prefix.weights.err", of_tolerance=f"{worst:.3f}")
     assert worst <= 1, worst
+
+
+class Whole(Shared):
+    """Whole numbers whose products and sums hold no rounding: scores of 8196 and some units more or less, in eighths; values of 1 and -1."""
+
+    def __init__(self, *args, **named):
+        super().__init__(*args, **named)
+        g = torch.Generator().manual_seed(self.n)
+        q = torch.randint(-2, 3, (self.n, self.heads, 64), generator=g).float()
+        q[..., 0], q[..., 1] = 256.0, 8.0
+        self.q = q.view(self.n, -1).to(self.q.dtype)
+
+    def fill(self, page, first, end, g):
+        at = [p[page, :self.kv * self.ps * 64].view(self.kv, self.ps, 64) for p in (self.k, self.v)]
+        k = torch.randint(-2, 3, (self.kv, end - first, 64), generator=g).float()
+        k[..., 0], k[..., 1] = 256.0, 4.0
+        at[0][:, first:end] = k.to(self.k.dtype)
+        at[1][:, first:end] = (torch.randint(0, 2, (self.kv, end - first, 64), generator=g) * 2.0 - 1).to(self.v.dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.125, -0.125])
+@pytest.mark.parametrize("members,shared,own,heads,kv", [
+    ([3], [300], lambda i: 20 * i, 2, 2), ([7], [1037], None, 2, 1), ([20, 9], [600, 90], lambda i: 13 * i % 60, 6, 3), ([90], [1200], None, 4, 2),
+    ([150, 5], [520, 700], lambda i: i % 70, 2, 1), ([200], [64], lambda i: 64, 1, 1),
+])
+def test_large_scores_lose_nothing_where_parts_join(ctx, dtype, scale, members, shared, own, heads, kv):
+    """A score s that holds no rounding gives the weight e^d, d = s - max, which is off by 2 u |d| (log2(e) and its product) and 3 u
+    (exp2 and a product); each later tile or part that moves the largest score adds 3 u, L u in all; and the sums L u, the
+    weights of 16-bit types h^2: |out - ref| <= h |ref| + sum w (|v| + |ref|) (2 |d| + 3 + 2 L + 8) u / sum w + h^2 A."""
+    report("prefix.large", dtype=dtype, scale=scale, members=members, shared=shared, heads=heads, kv=kv)
+    n = sum(members)
+    s = Whole(dtype, members, shared, own and [own(i) for i in range(n)], heads, kv, 16)
+    out, worst, h = s.run(ctx, scale=scale), 0.0, torch.finfo(TDT[dtype]).eps / 2
+    for i in sorted({0, n - 1, *range(0, n, 3)}):
+        at = s.seen(i)
+        page, row = (torch.tensor(x) for x in zip(*at))
+        k, v = (p[:, :kv * 16 * 64].view(s.pages, kv, 16, 64)[page, :, row].double().transpose(0, 1) for p in (s.k, s.v))
+        x = s.q[i].double().view(kv, -1, 64) @ k.transpose(1, 2) * scale
+        assert x.abs().min() > 8000
+        d = x - x.amax(-1, keepdim=True)
+        w = torch.softmax(x, -1)
+        ref, of = w @ v, 2 * d.abs() + 3 + 2 * len(at) + 8
+        tol = h * ref.abs() + U * ((w * of) @ v.abs() + (w * of).sum(-1, keepdim=True) * ref.abs())
+        if dtype != "f32":
+            tol = tol + h * h * (w @ v.abs())
+        if dtype == "f16":
+            tol = tol + len(at) * 2.0 ** -29 + 2.0 ** -25
+        worst = max(worst, float(((out[i].double().view(ref.shape) - ref).abs() / tol).max()))
+    report("prefix.large.err", of_tolerance=f"{worst:.3f}")
+    assert worst <= 1, worst
