@@ -36,9 +36,9 @@ __device__ inline int places_of(int len, int shift) { return int((long(len) + (1
 // effect whole or not at all without a launch before; then each wave takes its share of a row's full pages from the parent's, and
 // block 0 writes what there is one of for a row. FILL and COMMIT as in block_tables_kernel: two launches where lens_out lies over
 // lens or used_out over used and there are several blocks.
-// Bound by its chain of loads (parents, lengths, entries, the pool): 28 of 64 rows 5.1 us, a call among others, a thousand (2.3 MB of entries
-// read and written) 5.8, where an empty call takes 3.9.
-constexpr int FORK_THREADS = 1024;  // a row each up to as many; blocks of 256 take 5.2 us for 64 rows, as these, and 8.4 for 1024, these 6.2
+// Bound by its chain of loads (parents, lengths, entries, the pool): 28 of 64 rows 5.0 us, a call among others, a thousand (2.3 MB of entries
+// read and written) 5.6, where an empty call takes 3.9.
+constexpr int FORK_THREADS = 1024;  // a row each up to as many; blocks of 256 take as long for 64 rows and 12.7 us for 1024, these 5.6
 constexpr int FORK_UNIT = 512;      // entries of a row that a wave takes at once
 template <bool FILL, bool COMMIT>
 __global__ void __launch_bounds__(FORK_THREADS) fork_pages_kernel(const ForkArgs a) {
@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(FORK_THREADS) fork_pages_kernel(const ForkArgs
 // operations of the device, took 95 us for 320 thousand entries of a thousand rows that share their pages, where the bytes take 6.) Few
 // pages are bits in one block's LDS (bytes there, without atomics, took as long).
 //
-// Measured, a call among others: 64 rows of 8 thousand positions give pages back in 8.3 us, by one block, which its CU's loads of the
-// entries bound; a thousand rows of up to 25 thousand positions (320 thousand entries) in 15.3, by four launches (clear 2, marks 7, counts
+// Measured, a call among others: 64 rows of 8 thousand positions give pages back in 8.4 us, by one block, which its CU's loads of the
+// entries bound; a thousand rows of up to 25 thousand positions (320 thousand entries) in 15.1, by four launches (clear 2, marks 7, counts
 // 2, pages 4) that stores of a byte from each lane and the launches bound. 16 rows compact in 6.7 us by one block; 512 rows and a hundred
 // thousand pages in 24.4, by five launches (clear 2, marks 5, counts 2, moves 8, entries 8), each two to four dependent loads.
 
@@ -530,8 +530,8 @@ constexpr int COPY_PIECE = COPY_THREADS * COPY_AT_ONCE;  // pieces of 16 bytes a
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // 16 bytes a thread, four of them under way. A block takes (pair, array, part of a page) units in turn; arrays are the layers' keys,
-// values and bounds. Bound by HBM: 1000 pages of 64 KB of two layers, 268 MB read and as many written, 111.6 us (4.8 TB/s); 32 begun pages of four
-// layers 5.9, where an empty call takes 3.9.
+// values and bounds. Bound by HBM: 1000 pages of 64 KB of two layers, 268 MB read and as many written, 112.0 us (4.8 TB/s); 32 begun pages of four
+// layers 5.7, where an empty call takes 3.9.
 __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyArgs a, int es, int parts, long units) {
   const KvCache& c = a.cache;
   const int arrays = a.layers * (a.has_bounds ? 3 : 2), row_shift = es == 4 ? 4 : 3;  // 16-byte pieces of a row

@@ -504,8 +504,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefix_parts_kernel(const Prefi
 // Bound by the matrix instructions and by the vector unit's work on the scores, about as much of either: so half a tile's products
 // with K and the half before the last one's with V are under way while the half between becomes weights, all in one wave's stream,
 // and three waves share a SIMD. 1037 tokens of 12 heads on 24889 positions (bf16, 79 GFLOP): 158 us, the join's 10 among them (0.50 PFLOP/s,
-// and half as many operations again for the weights' second terms: 0.8 PFLOP/s while the parts are formed). Of a SIMD's cycles 1536 go to the
-// matrix instructions of a tile of 64 columns and 1750 to the vector unit (a third of them exponentials). With weights of one term, when all of
+// and half as many operations again for the weights' second terms: 0.8 PFLOP/s while the parts are formed). Of the 3600 cycles that a tile
+// of 64 columns takes a SIMD 1550 go to the matrix instructions and 2000 to the vector unit (by their counters). With weights of one term, when all of
 // it took 115 us: two blocks a CU with a tile more under way 130, waves of 64 columns 125, two teams of waves that multiply and exponentiate in
 // turn 140, the compiler's own order of the same instructions 6% more.
 //

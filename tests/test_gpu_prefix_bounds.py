@@ -41,3 +41,13 @@ def test_own_positions_begin_behind_a_prefix_that_is_cut(ctx, dtype, members, sh
     s.prefix = s.prefix[:, :s.prefix_width].contiguous()
     s.most = s.prefix_width * 16
     s.check(s.run(ctx, max_own=most_own), rows=rows)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("members", [4, 150])
+def test_a_shared_length_past_every_token(ctx, dtype, members):
+    """No position of a token's own lies behind it, up to the largest number there is."""
+    s = Cut(dtype, [members], [100], [(23 * i + 30) % 61 for i in range(members)], 4, 2, 16)
+    s.most, s.most_own = 64, 0
+    for shared in (161, 2 ** 30, 2 ** 31 - 1):
+        s.check(s.run(ctx, shared=[shared], max_shared=64, max_own=2 ** 31 - 1), rows=range(0, members, 3))
